@@ -222,6 +222,80 @@ int l2_attention_decode_noalloc(int n_heads, int n_kv_heads, int pos, const floa
                                 float* key_cache, float* value_cache, const float* rope_cos, const float* rope_sin,
                                 float* out, void* cuda_stream);
 
+/* ---- paged KV cache and its attention on device buffers (no counterpart in the reference, whose cache is one sequence's, in f32) ----
+ *
+ * One layer's cache of many sequences, in pages of page_size positions: K and V in f16, bf16, or int8 with one f32 scale per position
+ * and kv head.  Position j of sequence b is in page page_table[b][j / page_size], at j % page_size.  All arrays belong to the caller
+ * and are device memory of the current device; every call is enqueued on cuda_stream (NULL: the default stream) and does not wait.
+ *
+ * The lengths are read on the device, so a step's record serves all layers and may be captured in a graph.  What only the device can
+ * see to be wrong it reports in the batch's status word (L2_KV_*); the entry concerned is left out, nothing is read or written
+ * outside the caller's arrays. */
+#define L2_F32 0
+#define L2_F16 1
+#define L2_BF16 2
+#define L2_I8 3
+
+typedef struct l2_kv_pages {
+    void* k;                /* element d of (page, position, kv head): page * page_stride + position * position_stride + head * head_stride + d */
+    void* v;
+    float* k_scale;         /* L2_I8: [n_pages][n_kv_heads][page_size], value = stored * scale; else NULL */
+    float* v_scale;
+    int64_t page_stride, position_stride, head_stride;  /* in elements; multiples of 16 bytes, the same for k and v */
+    int32_t type;           /* L2_F16, L2_BF16 or L2_I8 */
+    int32_t n_pages;
+    int32_t page_size;      /* 8, 16, 32, 64, 128 or 256 */
+    int32_t n_kv_heads;
+    int32_t head_size;      /* 64 or 128 */
+} l2_kv_pages;
+
+/* One step of a batch.  Sequence b holds kv_len[b] positions and brings the rows row_start[b] .. row_start[b + 1] - 1 of the row arrays: they
+ * are its last positions, kv_len[b] - n .. kv_len[b] - 1 for n rows.  Rows of a negative position, and rows that belong to no sequence, are left out
+ * (l2_kv_attend: a row of a negative position sees nothing and gives 0). */
+typedef struct l2_kv_batch {
+    const int32_t* page_table; /* [n_seqs][table_width]; entries that no call needs may hold anything */
+    const int32_t* kv_len;     /* [n_seqs] */
+    const int32_t* row_start;  /* [n_seqs + 1], ascending, within 0 .. n_rows */
+    int32_t* status;           /* device word that gets L2_KV_* bits or'ed in, or NULL */
+    int32_t n_seqs, table_width;
+    int32_t n_rows;            /* rows of the row arrays */
+    int32_t max_rows;          /* no sequence brings more rows than this */
+} l2_kv_batch;
+
+#define L2_KV_BAD_PAGE 1   /* a page that is needed is outside 0 .. n_pages - 1: taken as zeros, not written */
+#define L2_KV_BAD_LENGTH 2 /* kv_len outside 0 .. table_width * page_size: taken as the nearest of them */
+#define L2_KV_BAD_ROWS 4   /* row_start not ascending, outside 0 .. n_rows or more than max_rows apart: that sequence brings no rows */
+#define L2_KV_BAD_ROPE 8   /* a position beyond the rope table: its rows are left out */
+#define L2_KV_TIMEOUT 16   /* a bounded wait inside a kernel gave up: the call's results are not valid */
+
+/* An array [row][head][head_size]: element d of (row, head) at row * row_stride + head * head_stride + d; strides multiples of 16 bytes. */
+typedef struct l2_kv_rows {
+    void* data;
+    int64_t row_stride, head_stride;  /* in elements */
+    int32_t type;                     /* L2_F32, L2_F16 or L2_BF16 */
+    int32_t heads;
+} l2_kv_rows;
+
+/* K and V of the batch's rows into their pages.  With rope tables ([rope_len][head_size / 2] each, f32, see l2_rope_table) k is rotated at its
+ * position first (element d with d + head_size / 2, as src/models.rs:100-135 does), and so is q into q_out where q is not NULL; without them
+ * q is rounded to q_out's type only.  int8: a row and head is scaled by 127 / its largest magnitude and rounded to nearest even.  One that holds a
+ * NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros. */
+int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
+                 const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, void* cuda_stream);
+/* The other way: the cached positions of the batch's rows as rows of f32, f16 or bf16 (all of a sequence where it brings kv_len[b] rows). */
+int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, void* cuda_stream);
+/* Attention of the batch's rows over the cache (their own K and V appended before).  A row at position p sees position j when j <= p and,
+ * where window > 0, p - j < window or j < sinks.  out = softmax(scale * q k) v over what it sees; 0 where it sees nothing.  What a row does not see
+ * does not reach its result, NaN and infinities included.  heads of q a multiple of n_kv_heads (at most 64 times).  q: f16 or bf16, the
+ * cache's type or either with an int8 cache; out: q's type or f32.  Products of q and k are exact and all sums are f32; the probabilities
+ * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16).
+ * Pages that no row of the call sees are not read: with a window they can be given back. */
+int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* q, const l2_kv_rows* out, float scale, int window, int sinks,
+                 void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* Bytes of device scratch that l2_kv_attend needs for such a batch (contents need not be kept between calls; calls that may overlap
+ * need one each), 0 where the arguments are not valid. */
+size_t l2_kv_attend_workspace_bytes(const l2_kv_pages* pages, const l2_kv_batch* batch, int n_heads);
+
 /* ---- measurement hooks (no counterpart in the reference, which times whole runs only,
  *      src/main.rs:61-65) --------------------------------------------------------------- */
 /* Enqueue `count` launches of one projection kernel of the token forward, cycling through the

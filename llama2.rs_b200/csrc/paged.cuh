@@ -1,0 +1,145 @@
+// Paged KV cache: parameter records and device helpers shared by paged.cu and the attention kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/llama2_b200.h"
+
+namespace l2 {
+
+struct KvPool {  // l2_kv_pages as the kernels take it
+    char* k; char* v;
+    float* ks; float* vs;
+    int64_t page_stride, pos_stride, head_stride;  // elements
+    int n_pages, page_shift, n_kv_heads;
+};
+struct KvStep {  // l2_kv_batch
+    const int* table; const int* kv_len; const int* row_start;
+    int* status;
+    int n_seqs, width, n_rows, max_rows;
+};
+struct KvRows {
+    char* data;
+    int64_t row_stride, head_stride;
+    int type, heads;
+};
+
+struct KvAttendParams {
+    KvPool pool;
+    KvStep step;
+    KvRows q, out;
+    float scale_log2;   // scale * log2(e): scores in powers of two
+    int window, sinks;  // window 0: all
+    int group;          // query heads per kv head
+    void* work;
+};
+
+// One sequence of a step, with what is out of range put right (and reported once, by the caller's choice).
+struct KvSeq { int row0, n, kv; };
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void kv_report(int* status, int bit) { if (status) atomicOr(status, bit); }
+
+__device__ __forceinline__ KvSeq kv_seq(const KvStep& s, int page_shift, int b) {
+    KvSeq q;
+    q.row0 = s.row_start[b];
+    const int64_t n = (int64_t)s.row_start[b + 1] - q.row0;
+    q.n = (int)n;
+    if (q.row0 < 0 || n < 0 || n > s.max_rows || q.row0 + n > s.n_rows) { kv_report(s.status, L2_KV_BAD_ROWS); q.row0 = 0; q.n = 0; }
+    q.kv = s.kv_len[b];
+    const int64_t most = (int64_t)s.width << page_shift;
+    if (q.kv < 0 || q.kv > most) { kv_report(s.status, L2_KV_BAD_LENGTH); q.kv = q.kv < 0 ? 0 : (int)most; }
+    return q;
+}
+
+// The page of position j of sequence b, or -1 where the table's entry is none.
+__device__ __forceinline__ int kv_page(const KvStep& s, const KvPool& p, int b, int j) {
+    const int page = __ldg(s.table + (size_t)b * s.width + (j >> p.page_shift));
+    if ((unsigned)page >= (unsigned)p.n_pages) { kv_report(s.status, L2_KV_BAD_PAGE); return -1; }
+    return page;
+}
+
+// The sequence that row r belongs to, by the whole warp: the last b with row_start[b] <= r (the caller checks r against kv_seq(b)).
+__device__ __forceinline__ int kv_find_seq(const KvStep& s, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = s.n_seqs;  // the answer is in lo .. lo + n - 1
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(s.row_start + at) <= r);
+        const int k = below ? 31 - __clz(below) : 0;
+        n = min(step, n - k * step);
+        lo += k * step;
+    }
+    return lo;
+}
+
+// Type codes as template arguments: how 8 elements are loaded as f32 and stored.
+template <int T> struct KvElem;
+template <> struct KvElem<L2_F32> { using type = float; };
+template <> struct KvElem<L2_F16> { using type = __half; };
+template <> struct KvElem<L2_BF16> { using type = __nv_bfloat16; };
+
+__device__ __forceinline__ void kv_load8(const float* p, float (&x)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void kv_load8(const __half* p, float (&x)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void kv_load8(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void kv_load8(const int8_t* p, float (&x)[8]) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
+}
+__device__ __forceinline__ void kv_store8(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void kv_store8(__half* p, const float (&x)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+}
+__device__ __forceinline__ void kv_store8(__nv_bfloat16* p, const float (&x)[8]) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+}
+// by a type known at run time (row arrays)
+__device__ __forceinline__ void kv_load8(const KvRows& r, int64_t row, int head, int d, float (&x)[8]) {
+    const int64_t e = row * r.row_stride + head * r.head_stride + d;
+    if (r.type == L2_F32) kv_load8(reinterpret_cast<const float*>(r.data) + e, x);
+    else if (r.type == L2_F16) kv_load8(reinterpret_cast<const __half*>(r.data) + e, x);
+    else kv_load8(reinterpret_cast<const __nv_bfloat16*>(r.data) + e, x);
+}
+__device__ __forceinline__ void kv_store8(const KvRows& r, int64_t row, int head, int d, const float (&x)[8]) {
+    const int64_t e = row * r.row_stride + head * r.head_stride + d;
+    if (r.type == L2_F32) kv_store8(reinterpret_cast<float*>(r.data) + e, x);
+    else if (r.type == L2_F16) kv_store8(reinterpret_cast<__half*>(r.data) + e, x);
+    else kv_store8(reinterpret_cast<__nv_bfloat16*>(r.data) + e, x);
+}
+#endif
+
+cudaError_t launch_kv_attend(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
+size_t kv_attend_work(const KvStep& s, const KvPool& p, int n_heads, int type, int head_size, int sms);
+
+}  // namespace l2

@@ -32,6 +32,24 @@ class Options(C.Structure):
                 ("tp_rank", C.c_int32), ("tp_world", C.c_int32), ("poll_limit_log2", C.c_int32)]
 
 
+class KvPagesArgs(C.Structure):
+    """l2_kv_pages."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_stride", C.c_int64), ("position_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("type", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_size", C.c_int32)]
+
+
+class KvBatchArgs(C.Structure):
+    """l2_kv_batch."""
+    _fields_ = [("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("row_start", C.c_void_p), ("status", C.c_void_p),
+                ("n_seqs", C.c_int32), ("table_width", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32)]
+
+
+class KvRowsArgs(C.Structure):
+    """l2_kv_rows."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("type", C.c_int32), ("heads", C.c_int32)]
+
+
 FLAG_NO_GRAPH = 1
 FLAG_NO_PDL = 2
 
@@ -83,6 +101,10 @@ SIGNATURES = {
     "l2_attention_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "l2_attention_decode_dev": (C.c_int, [C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "l2_attention_decode_noalloc": (C.c_int, [C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "l2_kv_append": (C.c_int, [_vp] * 8 + [C.c_int, _vp]),
+    "l2_kv_read": (C.c_int, [_vp] * 5),
+    "l2_kv_attend": (C.c_int, [_vp] * 4 + [C.c_float, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
+    "l2_kv_attend_workspace_bytes": (C.c_size_t, [_vp, _vp, C.c_int]),
     "l2_bench_projection": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int]),
     "l2_projection_bytes": (C.c_uint64, [_vp, C.c_int]),
     "l2_debug_trace": (C.c_int, [C.c_int, _p(C.c_uint64), C.c_int]),
