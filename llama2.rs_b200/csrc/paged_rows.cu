@@ -1,0 +1,682 @@
+// l2_kv_attend for sequences with few rows (tokens x query heads of a kv head: single tokens, drafted tokens).
+//
+// For one kv head of one sequence, with the rows' queries Q (8 NT rows at most), keys K and values V:
+//   S^T = K Q^T,  P^T = 2^(scale S^T - m),  O^T += V^T P^T,  l += sum P,   out = O / l
+// m is the running maximum of a row; when it moves, O and l are scaled.  The products are taken transposed: positions (S^T) and head
+// elements (O^T) are the 16 rows of an mma.sync.m16n8k16, the few query rows its 8 columns, so that one row wastes 7 of 8, not 15 of 16.
+// The kernel is bound by reading the cache: it is read once, by TMA, while the matrix work of a tile hides behind the copies of the next.
+//
+// Work.  The tiles of 64 positions of all (sequence, kv head) pairs form one line, cut evenly over the CTAs whatever the lengths are; a pair
+// that a cut goes through leaves a partial (m, l, O) in each piece, which kv_combine_kernel adds in order.  The cuts are found on the device: the host
+// does not know the lengths.
+//
+// Roles: warps 0-3 take 16 positions of a tile each, with a softmax of their own, and meet at the end of a piece; warp 4 fills a ring of
+// tiles with TMA copies, one a page run (and the scales of an int8 cache, one bulk copy a run).
+//
+// An int8 cache is multiplied as it is stored: K as q's type and V as bf16, both exact; the scale of a position is applied to its score and to
+// its probability.  (The probabilities times scales are rounded to bf16 even where q is f16: they can leave f16's range.)
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.cuh"
+#include "paged_device.cuh"
+#include "paged_attend.h"
+
+namespace l2 {
+
+namespace {
+
+constexpr int KR_TILE = 64, KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
+constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
+
+// Shared memory of a variant: Q, the buffer in which the warps' results meet, the ring.
+template <int CT, int HD, int NT>
+struct KrShape {
+    static constexpr bool I8 = CT == L2_I8;
+    static constexpr int ROWS = 8 * NT, ROW_BYTES = HD * (I8 ? 1 : 2);
+    static constexpr int Q_PITCH = HD * 2 + 16;                                 // bytes between rows of Q: no bank conflicts
+    static constexpr int KV_BYTES = KR_TILE * ROW_BYTES;                        // K or V of a tile
+    static constexpr int SCALE_BYTES = I8 ? KR_TILE * 4 : 0;
+    static constexpr int STAGE = (2 * (KV_BYTES + SCALE_BYTES) + 1023) / 1024 * 1024;
+    static constexpr int MEET = ROWS * HD * 4;
+    static constexpr int FIXED = 1024 + MEET + ROWS * Q_PITCH;
+    static constexpr int STAGES = (KR_SMEM - FIXED) / STAGE < KR_MAX_STAGES ? (KR_SMEM - FIXED) / STAGE : KR_MAX_STAGES;
+    static constexpr int SMEM = FIXED + STAGES * STAGE;
+    static_assert(STAGES >= 2, "ring");
+};
+
+// Where byte `c16` (a 16-byte chunk) of row r of a tile is: rows of 128 bytes (two halves of a tile one after the other) or 64, as the TMA swizzles them.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint32_t kr_offset(int r, int c16) {
+    if constexpr (ROW_BYTES == 64) return r * 64 + ((c16 ^ ((r >> 1) & 3)) << 4);
+    else return (c16 >> 3) * (KR_TILE * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// The 16-bit numbers of bytes SEL & 3 and SEL >> 4 & 3 of w (two's complement), exact.
+template <bool BF, uint32_t SEL>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+    uint32_t r;
+    constexpr uint32_t sel = 0x4040u | (SEL & 15u) | ((SEL >> 4) & 15u) << 8;
+    if constexpr (BF) {  // 0x4300 | x is 128 + x for x < 128: 128 + (low seven bits) minus 128 or, for a negative byte, 256
+        const uint32_t t = __byte_perm(w, 0, sel);
+        const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    } else {             // 0x6400 | x is 1024 + x: with the sign bit turned over, 1024 + 128 + byte
+        const uint32_t t = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));
+    }
+    return r;
+}
+template <bool BF> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {  // non-zero where one of the two is NaN or infinite
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    return ((v & E) == E) | ((v & (E << 16)) == (E << 16));
+}
+template <bool BF> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    if ((v & E) == E) v &= 0xffff0000u;
+    if ((v & (E << 16)) == (E << 16)) v &= 0x0000ffffu;
+    return v;
+}
+
+// The line of tiles: sequence by sequence, kv head by kv head, tile by tile.
+struct KrSeq {
+    KvSeq s;
+    KvView<KR_TILE> view;
+    int rows;  // tokens x group, 0: not this kernel's
+};
+__device__ __forceinline__ KrSeq kr_seq(const KvAttendParams& P, int lim, int b) {
+    KrSeq q;
+    q.s = kv_seq(P.step, P.pool.page_shift, b);
+    const int64_t rows = (int64_t)q.s.n * P.group;
+    q.rows = rows <= lim ? (int)rows : 0;
+    q.view = KvView<KR_TILE>(q.s.kv - q.s.n, q.s.kv - 1, P.window, P.sinks);
+    return q;
+}
+__device__ __forceinline__ int64_t kr_length(const KvAttendParams& P, int lim, int b) {
+    const KrSeq q = kr_seq(P, lim, b);
+    return q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0;
+}
+
+struct KrSpot { int64_t total, start; int b; };  // length of the line; the sequence that a position is in, and where that begins
+
+// By all threads of a CTA of THREADS: the line's length, and where position cta * (length / ctas) is.  Scratch: shared memory.
+template <int THREADS>
+__device__ KrSpot kr_locate(const KvAttendParams& P, int lim, int cta, int ctas, int64_t* scratch) {
+    constexpr int WARPS = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = P.step.n_seqs;
+    auto scan = [&](int64_t v) {  // inclusive, over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        return v;
+    };
+    const int64_t mine = tid < n ? kr_length(P, lim, tid) : 0;  // (most steps have no more sequences than threads)
+    int64_t sum = mine;
+    for (int b = tid + THREADS; b < n; b += THREADS) sum += kr_length(P, lim, b);
+    sum = scan(sum);
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    KrSpot spot{0, -1, n};
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) spot.total += scratch[w];
+    const int64_t at = (spot.total + ctas - 1) / ctas * cta;
+    if (at >= spot.total) return spot;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < n; b0 += THREADS) {
+        const int64_t v = b0 == 0 ? mine : b0 + tid < n ? kr_length(P, lim, b0 + tid) : 0;
+        const int64_t inc = scan(v);
+        __syncthreads();
+        if (lane == 31) scratch[warp] = inc;
+        if (tid == 0) scratch[WARPS] = -1;
+        __syncthreads();
+        int64_t base = before, chunk = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            if (w < warp) base += scratch[w];
+            chunk += scratch[w];
+        }
+        const int64_t from = base + inc - v;
+        if (from <= at && at < from + v) { scratch[WARPS] = b0 + tid; scratch[WARPS + 1] = from; }
+        __syncthreads();
+        if (scratch[WARPS] >= 0) { spot.b = (int)scratch[WARPS]; spot.start = scratch[WARPS + 1]; break; }
+        before += chunk;
+    }
+    return spot;
+}
+
+// A CTA's piece of the line, one (sequence, kv head) at a time.
+struct KrWalk {
+    int64_t w, w1, start;
+    int b;
+    KrSeq q;
+    int head, t0, t1;
+    bool first;  // the piece is the CTA's first
+    __device__ __forceinline__ KrWalk(const KvAttendParams& P, int lim, const KrSpot& spot) {
+        const int64_t per = (spot.total + gridDim.x - 1) / gridDim.x;
+        w = per * blockIdx.x;
+        w1 = min(spot.total, w + per);
+        start = spot.start; b = spot.b;
+        first = true;
+        t0 = -1;
+        if (w < w1) q = kr_seq(P, lim, b);
+    }
+    __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
+        if (t0 >= 0) first = false;
+        if (w >= w1) return false;
+        while (w >= start + (q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0)) {
+            if (q.rows) start += (int64_t)q.view.tiles * P.pool.n_kv_heads;
+            q = kr_seq(P, lim, ++b);
+        }
+        const int in = (int)(w - start);
+        head = in / q.view.tiles;
+        t0 = in - head * q.view.tiles;
+        t1 = (int)min((int64_t)q.view.tiles, t0 + (w1 - w));
+        w += t1 - t0;
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == q.view.tiles; }
+};
+
+// Partial results: [CTA][first or last piece] of ROWS x (HD floats), then ROWS x (m, l).
+__device__ __forceinline__ float* kr_part(void* work, int rows, int hd, int64_t cta, int slot) { return static_cast<float*>(work) + (cta * 2 + slot) * rows * (hd + 2); }
+
+__device__ __forceinline__ void store2(const KvRows& o, int64_t e, float x) {
+    if (o.type == L2_F32) reinterpret_cast<float*>(o.data)[e] = x;
+    else if (o.type == L2_F16) reinterpret_cast<__half*>(o.data)[e] = __float2half_rn(x);
+    else reinterpret_cast<__nv_bfloat16*>(o.data)[e] = __float2bfloat16_rn(x);
+}
+
+// CT: cache type; QB: q is bf16, else f16
+template <int CT, bool QB, int HD, int NT>
+__global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
+                                                               const __grid_constant__ CUtensorMap map_v) {
+    using S = KrShape<CT, HD, NT>;
+    constexpr bool I8 = S::I8, PB = I8 || QB;       // probabilities and V in bf16
+    constexpr int KS = HD / 16, MT = HD / 16, RB = S::ROW_BYTES;
+    extern __shared__ __align__(1024) uint8_t kr_smem[];
+    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES];
+    __shared__ int64_t scratch[KR_THREADS / 32 + 2];
+    __shared__ float meet_ml[KR_WARPS][S::ROWS][2];
+    __shared__ volatile int failed;
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kr_smem) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sq = ring + S::STAGES * S::STAGE;
+    float* meet = reinterpret_cast<float*>(sq + S::ROWS * S::Q_PITCH);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; i++) { kv_bar_init(&full[i], 1); kv_bar_init(&empty[i], KR_WARPS); }
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const KrSpot spot = kr_locate<KR_THREADS>(P, lim, blockIdx.x, gridDim.x, scratch);  // (ends behind a barrier)
+    __syncthreads();
+    KrWalk walk(P, lim, spot);
+    KvWait wait{&failed};
+
+    if (warp == KR_WARPS) {
+        // ================= copies: lane l brings run l of a tile ==============================================================
+        const int R = min(KR_TILE, 1 << P.pool.page_shift), runs = KR_TILE / R;
+        uint32_t st = 0, ph = 1;
+        while (walk.next(P, lim)) {
+            const KvView<KR_TILE>& view = walk.q.view;
+            for (int t = walk.t0; t < walk.t1; t++) {
+                const int j = view.base(t) + lane * R;
+                int page = P.pool.n_pages;  // (outside the pool: the copy gives zeros)
+                if (lane < runs && view.any(j, R, P.window, P.sinks)) {
+                    const int x = kv_page(P.step, P.pool, walk.b, j);
+                    if (x >= 0) page = x;
+                }
+                wait(&empty[st], ph);
+                if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                uint8_t* stage = ring + st * S::STAGE;
+                const bool there = lane < runs && page < P.pool.n_pages;
+                uint32_t bytes = 2 * S::KV_BYTES;
+                if constexpr (I8) {
+                    if (lane < runs && !there)
+                        for (int i = 0; i < R; i++)
+                            for (int x = 0; x < 2; x++) reinterpret_cast<float*>(stage + 2 * S::KV_BYTES + x * S::SCALE_BYTES)[lane * R + i] = 0.0f;
+                    bytes += __popc(__ballot_sync(0xffffffffu, there)) * R * 8;
+                }
+                __syncwarp();
+                if (lane == 0) kv_bar_expect(&full[st], bytes);
+                __syncwarp();
+                if (lane < runs) {
+                    const int at = j & ((1 << P.pool.page_shift) - 1);
+                    const uint32_t k = kv_smem(stage), v = k + S::KV_BYTES;
+#pragma unroll
+                    for (int h = 0; h < (RB + 127) / 128; h++) {
+                        const uint32_t to = h * (KR_TILE * 128) + lane * R * min(RB, 128);
+                        kv_tma4(k + to, &map_k, h * 64, at, walk.head, page, &full[st]);
+                        kv_tma4(v + to, &map_v, h * 64, at, walk.head, page, &full[st]);
+                    }
+                    if constexpr (I8) {
+                        if (there) {
+                            const int64_t e = ((int64_t)page * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + at;
+                            const uint32_t s = v + S::KV_BYTES + lane * R * 4;
+                            kv_bulk(s, P.pool.ks + e, R * 4, &full[st]);
+                            kv_bulk(s + S::SCALE_BYTES, P.pool.vs + e, R * 4, &full[st]);
+                        }
+                    }
+                }
+                if (++st == S::STAGES) { st = 0; ph ^= 1u; }
+            }
+            if (wait.dead) break;
+        }
+    } else {
+        // ================= matrix work ========================================================================================
+        const int c = lane & 3, g8 = lane >> 2;
+        uint32_t st = 0, ph = 0;
+        while (walk.next(P, lim)) {
+            const KrSeq& seq = walk.q;
+            const int rows = seq.rows, G = P.group;
+            // Q into shared memory: rows beyond the last are zeros
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // (everybody has read the piece before's)
+            for (int i = tid; i < S::ROWS * (HD / 8); i += KR_WARPS * 32) {
+                const int r = i / (HD / 8), ch = i % (HD / 8);
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < rows) {
+                    const int tok = r / G;
+                    x = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((seq.s.row0 + tok) * P.q.row_stride + (int64_t)(walk.head * G + r - tok * G) * P.q.head_stride + ch * 8));
+                }
+                *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = x;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            auto q_frag = [&](int nt, int ks, uint32_t& b0, uint32_t& b1) {  // columns 8 nt .., elements 16 ks .. of Q^T
+                const uint8_t* p = sq + (8 * nt + g8) * S::Q_PITCH + ks * 32;
+                if constexpr (I8) { const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * c); b0 = x.x; b1 = x.y; }
+                else { b0 = *reinterpret_cast<const uint32_t*>(p + 4 * c); b1 = *reinterpret_cast<const uint32_t*>(p + 16 + 4 * c); }
+            };
+            uint32_t qr[NT][KS][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) q_frag(nt, ks, qr[nt][ks][0], qr[nt][ks][1]);
+            int pos[NT][2];  // positions of this thread's two rows of each eight
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) pos[nt][e] = seq.view.lo_pos + (8 * nt + 2 * c + e) / G;
+
+            float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.0f;
+            }
+#pragma unroll 1
+            for (int t = walk.t0; t < walk.t1; t++) {
+                const int base = seq.view.base(t);
+                const bool whole = seq.view.whole(base, P.window, P.sinks);
+                wait(&full[st], ph);
+                __syncwarp();
+                const uint8_t* stage = ring + st * S::STAGE;
+                const uint32_t k_at = kv_smem(stage), v_at = k_at + S::KV_BYTES;
+                // ---- scores of this warp's 16 positions: rows g8 and g8 + 8, columns 2 c and 2 c + 1
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                const int kr = 16 * warp + (lane & 15);
+                auto by_k = [&](int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[nt], a0, a1, a2, a3, qr[nt][ks][0], qr[nt][ks][1]);
+                };
+                if constexpr (I8) {
+#pragma unroll
+                    for (int c2 = 0; c2 < KS / 2; c2++) {  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
+                        uint32_t a[4];
+                        ldsm4(a, k_at + kr_offset<RB>(kr, 2 * c2 + (lane >> 4)));
+                        by_k(2 * c2, widen<QB, 0x10>(a[0]), widen<QB, 0x10>(a[1]), widen<QB, 0x32>(a[0]), widen<QB, 0x32>(a[1]));
+                        by_k(2 * c2 + 1, widen<QB, 0x10>(a[2]), widen<QB, 0x10>(a[3]), widen<QB, 0x32>(a[2]), widen<QB, 0x32>(a[3]));
+                    }
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        uint32_t a[4];
+                        ldsm4(a, k_at + kr_offset<RB>(kr, 2 * ks + (lane >> 4)));
+                        by_k(ks, a[0], a[1], a[2], a[3]);
+                    }
+                }
+                // ---- softmax
+                float f0 = P.scale_log2, f1 = P.scale_log2, v0 = 1.0f, v1 = 1.0f;
+                const int j0 = base + 16 * warp + g8;
+                if constexpr (I8) {
+                    const float* sc = reinterpret_cast<const float*>(stage + 2 * S::KV_BYTES) + 16 * warp + g8;
+                    f0 *= sc[0]; f1 *= sc[8];
+                    v0 = sc[KR_TILE]; v1 = sc[KR_TILE + 8];
+                }
+                bool moved = false;
+                float m1[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    s[nt][0] *= f0; s[nt][1] *= f0; s[nt][2] *= f1; s[nt][3] *= f1;
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (!kv_sees(pos[nt][i & 1], j0 + 8 * (i >> 1), P.window, P.sinks)) s[nt][i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float x = fmaxf(s[nt][e], s[nt][e + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        // f16: probabilities up to 2^15, so that those 2^-29 times the largest are still normal numbers
+                        m1[nt][e] = fmaxf(m[nt][e], PB ? x : x - 15.0f);
+                        moved |= m1[nt][e] != m[nt][e];
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float f = m1[nt][e] == -INFINITY ? 1.0f : kv_exp2(m[nt][e] - m1[nt][e]);
+                            m[nt][e] = m1[nt][e];
+                            l[nt][e] *= f;
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] *= f; o[mt][nt][e + 2] *= f; }
+                        }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float ref = m[nt][i & 1] == -INFINITY ? 0.0f : m[nt][i & 1];
+                        p[i] = kv_exp2(s[nt][i] - ref);
+                        l[nt][i & 1] += p[i];
+                        if constexpr (I8) p[i] = !whole && !kv_sees(pos[nt][i & 1], j0 + 8 * (i >> 1), P.window, P.sinks) ? 0.0f : p[i] * (i < 2 ? v0 : v1);
+                    }
+                    pb[nt][0] = transpose8(pack16<PB>(p[0], p[1]));
+                    pb[nt][1] = transpose8(pack16<PB>(p[2], p[3]));
+                }
+                // ---- O^T += V^T P^T
+                const int vr = 16 * warp + (lane & 7) + 8 * (lane >> 4);
+                uint32_t odd = 0;
+                if constexpr (I8) {
+#pragma unroll
+                    for (int m2 = 0; m2 < (MT + 1) / 2; m2++) {  // 32 elements; row i of a product is element 2 i, row 8 + i element 2 i + 1
+                        uint32_t a[4];
+                        ldsm4_t(a, v_at + kr_offset<RB>(vr, 2 * m2 + ((lane >> 3) & 1)));
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t x0 = widen<true, 0x20>(a[h]), x1 = widen<true, 0x31>(a[h]), x2 = widen<true, 0x20>(a[h + 2]), x3 = widen<true, 0x31>(a[h + 2]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma<true>(o[2 * m2 + h][nt], x0, x1, x2, x3, pb[nt][0], pb[nt][1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        uint32_t a[4];
+                        ldsm4_t(a, v_at + kr_offset<RB>(vr, 2 * mt + ((lane >> 3) & 1)));
+                        if (!whole) {  // 0 x NaN is NaN: a value that some row does not see may only be multiplied where it is finite
+                            if (__any_sync(0xffffffffu, not_finite<PB>(a[0]) | not_finite<PB>(a[1]) | not_finite<PB>(a[2]) | not_finite<PB>(a[3]))) {
+                                odd = 1;
+#pragma unroll
+                                for (int i = 0; i < 4; i++) a[i] = only_finite<PB>(a[i]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) mma<PB>(o[mt][nt], a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
+                    }
+                    if (odd) {  // rare: the values that are not finite, one by one, to the rows that see them
+#pragma unroll 1
+                        for (int i = 0; i < 16; i++) {
+                            const int r = 16 * warp + i;
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                                for (int h = 0; h < 2; h++) {
+                                    const uint16_t bits = *reinterpret_cast<const uint16_t*>(stage + S::KV_BYTES + kr_offset<RB>(r, 2 * mt + h) + 2 * g8);
+                                    if (not_finite<PB>(bits)) {
+                                        const float x = PB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+#pragma unroll
+                                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                            for (int e = 0; e < 2; e++)
+                                                if (kv_sees(pos[nt][e], base + r, P.window, P.sinks)) o[mt][nt][2 * h + e] += x;
+                                    }
+                                }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) kv_bar_arrive(&empty[st]);
+                if (++st == S::STAGES) { st = 0; ph ^= 1u; }
+            }
+            // ---- the four warps' results meet: a common maximum, then sums in a fixed order (warp 3's into 2's into 1's into 0's)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x = l[nt][e];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    l[nt][e] = x;
+                    if (g8 == 0) { meet_ml[warp][8 * nt + 2 * c + e][0] = m[nt][e]; meet_ml[warp][8 * nt + 2 * c + e][1] = x; }
+                }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            float lsum[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = 8 * nt + 2 * c + e;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < KR_WARPS; w++) top = fmaxf(top, meet_ml[w][r][0]);
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    lsum[nt][e] = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < KR_WARPS; w++) lsum[nt][e] += kv_exp2(meet_ml[w][r][0] - ref) * meet_ml[w][r][1];
+                    const float f = kv_exp2(m[nt][e] - ref);
+                    m[nt][e] = top;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] *= f; o[mt][nt][e + 2] *= f; }
+                }
+#pragma unroll
+            for (int from = KR_WARPS - 1; from > 0; from--) {
+                if (warp == from) {
+#pragma unroll
+                    for (int i = 0; i < MT * NT; i++) *reinterpret_cast<float4*>(meet + (i * 32 + lane) * 4) = *reinterpret_cast<float4*>(o[i / NT][i % NT]);
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (warp == from - 1) {
+#pragma unroll
+                    for (int i = 0; i < MT * NT; i++) {
+                        const float4 x = *reinterpret_cast<const float4*>(meet + (i * 32 + lane) * 4);
+                        float* y = o[i / NT][i % NT];
+                        y[0] += x.x; y[1] += x.y; y[2] += x.z; y[3] += x.w;
+                    }
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            if (warp == 0) {
+                const bool done = walk.whole();
+                float* part = kr_part(P.work, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = 8 * nt + 2 * c + e;
+                        if (r >= rows) continue;
+                        const int tok = r / G;
+                        const int64_t at = (seq.s.row0 + tok) * P.out.row_stride + (int64_t)(walk.head * G + r - tok * G) * P.out.head_stride;
+                        const float inv = pos[nt][e] < 0 ? 0.0f : 1.0f / lsum[nt][e];
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int d = I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
+                                const float x = o[mt][nt][2 * h + e];
+                                if (done) store2(P.out, at + d, pos[nt][e] < 0 ? 0.0f : x * inv);
+                                else part[r * HD + d] = x;
+                            }
+                        if (!done && g8 == 0) *reinterpret_cast<float2*>(part + S::ROWS * HD + 2 * r) = make_float2(m[nt][e], lsum[nt][e]);
+                    }
+            }
+        }
+    }
+    __syncthreads();
+    if (failed) {  // copies may still be on their way into this CTA's shared memory: a bounded time to land
+        if (tid < S::STAGES)
+            for (int i = 0; i < 64; i++) { kv_bar_try(&full[tid], 0); kv_bar_try(&full[tid], 1); }
+        if (tid == 0) kv_report(P.step.status, L2_KV_TIMEOUT);
+    }
+}
+
+// Adds the pieces of the pairs that cuts go through: CTA x looks at cut x + 1 and takes the pair in it if that is the pair's first cut.
+// HD / 4 threads for a row; with fewer than eight rows the others take pieces of the same row, and meet in order.
+template <int HD>
+__global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int ctas, const int part_rows) {
+    constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
+    __shared__ int64_t scratch[256 / 32 + 2];
+    __shared__ float4 sums[256];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int cut = blockIdx.x + 1;
+    const KrSpot spot = kr_locate<256>(P, lim, cut, ctas, scratch);
+    if (spot.start < 0) return;
+    const int64_t per = (spot.total + ctas - 1) / ctas, at = per * cut;
+    const KrSeq q = kr_seq(P, lim, spot.b);
+    const int T = q.view.tiles, head = (int)((at - spot.start) / T);
+    const int64_t from = spot.start + (int64_t)head * T, to = from + T;
+    if (from == at || from / per != cut - 1) return;
+    const int c0 = cut - 1, n = (int)((to - 1) / per) - c0 + 1;
+    auto piece = [&](int i) { return kr_part(P.work, part_rows, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
+    int width = 1;  // rows side by side
+    while (width < q.rows && width < SLOTS) width <<= 1;
+    const int share = SLOTS / width, slot = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES), mine = slot / width;
+    for (int r0 = 0; r0 < q.rows; r0 += width) {
+        const int r = r0 + slot % width;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.0f;
+        if (r < q.rows) {
+            float top = -INFINITY;
+            for (int i = 0; i < n; i++) top = fmaxf(top, piece(i)[part_rows * HD + 2 * r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            for (int i = 0; i < n; i++) sum += kv_exp2(piece(i)[part_rows * HD + 2 * r] - ref) * piece(i)[part_rows * HD + 2 * r + 1];
+#pragma unroll 4
+            for (int i = mine; i < n; i += share) {
+                const float* p = piece(i);
+                const float f = kv_exp2(p[part_rows * HD + 2 * r] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
+                acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+            }
+        }
+        if (share > 1) {
+            sums[threadIdx.x] = acc;
+            __syncthreads();
+            for (int i = 1; i < share && mine == 0; i++) {
+                const float4 x = sums[threadIdx.x + i * width * LANES];
+                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+            }
+            __syncthreads();
+        }
+        if (r < q.rows && mine == 0) {
+            const int tok = r / P.group, pos = q.view.lo_pos + tok;
+            const int64_t e = (q.s.row0 + tok) * P.out.row_stride + (int64_t)(head * P.group + r - tok * P.group) * P.out.head_stride + d;
+            const float inv = 1.0f / sum;
+            const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+            for (int i = 0; i < 4; i++) store2(P.out, e + i, pos < 0 ? 0.0f : y[i]);
+        }
+    }
+}
+
+template <class F>
+cudaError_t kr_by_variant(int type, bool qb, int hd, int nt, F f) {
+    auto by_nt = [&](auto t, auto b, auto h) {
+        return nt == 1 ? f(t, b, h, std::integral_constant<int, 1>()) : f(t, b, h, std::integral_constant<int, 2>());
+    };
+    auto by_hd = [&](auto t, auto b) { return hd == 128 ? by_nt(t, b, std::integral_constant<int, 128>()) : by_nt(t, b, std::integral_constant<int, 64>()); };
+    if (type == L2_F16) return by_hd(std::integral_constant<int, L2_F16>(), std::false_type());
+    if (type == L2_BF16) return by_hd(std::integral_constant<int, L2_BF16>(), std::true_type());
+    return qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
+}
+
+int kr_nt(int lim) { return lim <= 8 ? 1 : 2; }
+// CTAs of a launch: two an SM, no more than there can be tiles
+int kr_grid(const KvStep& s, const KvPool& p, int sms) {
+    const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KR_TILE - 1) / KR_TILE + 1);
+    return (int)std::min<int64_t>(2 * sms, tiles);
+}
+
+}  // namespace
+
+int kv_rows_limit(const KvStep& s, int group) {
+    const int64_t most = (int64_t)s.max_rows * group;
+    return most <= 16 ? (int)most : group <= 16 ? group : 0;
+}
+
+size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
+    const int lim = kv_rows_limit(s, group);
+    return lim ? (size_t)kr_grid(s, p, sms) * 2 * 8 * kr_nt(lim) * (head_size + 2) * sizeof(float) : 0;
+}
+
+cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
+    const int lim = kv_rows_limit(p.step, p.group);
+    if (!lim) return cudaSuccess;
+    CUtensorMap mk, mv;
+    if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, KR_TILE)) return e;
+    if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, KR_TILE)) return e;
+    const int nt = kr_nt(lim), grid = kr_grid(p.step, p.pool, sms);
+    cudaError_t e = kr_by_variant(type, p.q.type == L2_BF16, head_size, nt, [&](auto t, auto b, auto h, auto n) {
+        constexpr int T = decltype(t)::value, HD = decltype(h)::value, NT = decltype(n)::value;
+        auto kernel = kv_rows_kernel<T, decltype(b)::value, HD, NT>;
+        static KvOnce once;
+        if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KrShape<T, HD, NT>::SMEM)) return x;
+        kernel<<<grid, KR_THREADS, KrShape<T, HD, NT>::SMEM, st>>>(p, lim, mk, mv);
+        return cudaGetLastError();
+    });
+    g_launches++;
+    if (e != cudaSuccess || grid < 2) return e;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(grid - 1);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    g_launches++;
+    return head_size == 128 ? cudaLaunchKernelEx(&cfg, kv_rows_combine_kernel<128>, p, lim, grid, 8 * nt) : cudaLaunchKernelEx(&cfg, kv_rows_combine_kernel<64>, p, lim, grid, 8 * nt);
+}
+
+}  // namespace l2
