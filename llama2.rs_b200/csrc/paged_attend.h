@@ -32,4 +32,8 @@ int kv_rows_limit(const KvStep& s, int group);
 size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms);
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
 
+// The others: tcgen05.
+size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms);
+cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
+
 }  // namespace l2

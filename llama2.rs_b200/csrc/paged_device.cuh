@@ -56,6 +56,12 @@ __device__ __forceinline__ float kv_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// x 2^d for d <= 0 (d = -inf: 0), in two steps: 2^d alone may be too small for a normal number where the product is none too small
+struct KvScale {
+    float h;
+    __device__ __forceinline__ explicit KvScale(float d) : h(kv_exp2(0.5f * d)) {}
+    __device__ __forceinline__ float operator()(float x) const { return x * h * h; }
+};
 
 // ---- what a block of rows sees -----------------------------------------------------------------------------------------
 // Rows at positions lo_pos .. hi_pos of a sequence see positions in tiles of TS: the tiles of the sinks (first `sink_tiles`), then those from
@@ -83,6 +89,100 @@ struct KvView {
 };
 __device__ __forceinline__ bool kv_sees(int pos, int j, int window, int sinks) {
     return j <= pos && (!window || pos - j < window || j < sinks);
+}
+
+// ---- the line of tiles -----------------------------------------------------------------------------------------------------
+// The tiles of all sequences one after the other; CTA c of `ctas` takes positions c * per .. of it, per = total / ctas rounded up.
+struct KvSpot { int64_t total, start; int b; };  // its length; the sequence that a CTA's first position is in and where that begins (-1: there is none)
+
+// By all threads of a CTA of THREADS.  len(b): tiles of sequence b, called by whole warps, 0 for b >= n.  Scratch: THREADS / 32 + 2 words of shared memory.
+template <int THREADS, class Len>
+__device__ KvSpot kv_locate(int n, int cta, int ctas, int64_t* scratch, Len len) {
+    constexpr int WARPS = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto scan = [&](int64_t v) {  // inclusive, over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        return v;
+    };
+    const int64_t mine = len(tid);  // (most steps have no more sequences than threads)
+    int64_t sum = mine;
+    for (int b0 = THREADS; b0 < n; b0 += THREADS) sum += len(b0 + tid);
+    sum = scan(sum);
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    KvSpot spot{0, -1, n};
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) spot.total += scratch[w];
+    const int64_t at = (spot.total + ctas - 1) / ctas * cta;
+    if (at >= spot.total) return spot;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < n; b0 += THREADS) {
+        const int64_t v = b0 == 0 ? mine : len(b0 + tid);
+        const int64_t inc = scan(v);
+        __syncthreads();
+        if (lane == 31) scratch[warp] = inc;
+        if (tid == 0) scratch[WARPS] = -1;
+        __syncthreads();
+        int64_t base = before, chunk = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            if (w < warp) base += scratch[w];
+            chunk += scratch[w];
+        }
+        const int64_t from = base + inc - v;
+        if (from <= at && at < from + v) { scratch[WARPS] = b0 + tid; scratch[WARPS + 1] = from; }
+        __syncthreads();
+        if (scratch[WARPS] >= 0) { spot.b = (int)scratch[WARPS]; spot.start = scratch[WARPS + 1]; break; }
+        before += chunk;
+    }
+    return spot;
+}
+
+// Partial results of a CTA's first (slot 0) and last piece: `rows` times hd floats, then `rows` times (m, l).
+__device__ __forceinline__ float* kv_part(void* work, int rows, int hd, int64_t cta, int slot) { return static_cast<float*>(work) + (cta * 2 + slot) * rows * (hd + 2); }
+
+__device__ __forceinline__ void kv_store1(const KvRows& o, int64_t e, float x) {
+    if (o.type == L2_F32) reinterpret_cast<float*>(o.data)[e] = x;
+    else if (o.type == L2_F16) reinterpret_cast<__half*>(o.data)[e] = __float2half_rn(x);
+    else reinterpret_cast<__nv_bfloat16*>(o.data)[e] = __float2bfloat16_rn(x);
+}
+
+// ---- bytes as 16-bit numbers -------------------------------------------------------------------------------------------------
+// The 16-bit numbers of bytes SEL & 3 and SEL >> 4 & 3 of w (two's complement), exact.
+template <bool BF, uint32_t SEL>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+    uint32_t r;
+    constexpr uint32_t sel = 0x4040u | (SEL & 15u) | ((SEL >> 4) & 15u) << 8;
+    if constexpr (BF) {  // 0x4300 | x is 128 + x for x < 128: 128 + (low seven bits) minus 128 or, for a negative byte, 256
+        const uint32_t t = __byte_perm(w, 0, sel);
+        const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    } else {             // 0x6400 | x is 1024 + x: with the sign bit turned over, 1024 + 128 + byte
+        const uint32_t t = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));
+    }
+    return r;
+}
+template <bool BF> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {  // non-zero where one of the two is NaN or infinite
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    return ((v & E) == E) | ((v & (E << 16)) == (E << 16));
+}
+template <bool BF> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    if ((v & E) == E) v &= 0xffff0000u;
+    if ((v & (E << 16)) == (E << 16)) v &= 0x0000ffffu;
+    return v;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 }  // namespace l2

@@ -73,39 +73,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-    uint32_t r;
-    if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-// The 16-bit numbers of bytes SEL & 3 and SEL >> 4 & 3 of w (two's complement), exact.
-template <bool BF, uint32_t SEL>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-    uint32_t r;
-    constexpr uint32_t sel = 0x4040u | (SEL & 15u) | ((SEL >> 4) & 15u) << 8;
-    if constexpr (BF) {  // 0x4300 | x is 128 + x for x < 128: 128 + (low seven bits) minus 128 or, for a negative byte, 256
-        const uint32_t t = __byte_perm(w, 0, sel);
-        const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    } else {             // 0x6400 | x is 1024 + x: with the sign bit turned over, 1024 + 128 + byte
-        const uint32_t t = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));
-    }
-    return r;
-}
-template <bool BF> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {  // non-zero where one of the two is NaN or infinite
-    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-    return ((v & E) == E) | ((v & (E << 16)) == (E << 16));
-}
-template <bool BF> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
-    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-    if ((v & E) == E) v &= 0xffff0000u;
-    if ((v & (E << 16)) == (E << 16)) v &= 0x0000ffffu;
-    return v;
-}
-
 // The line of tiles: sequence by sequence, kv head by kv head, tile by tile.
 struct KrSeq {
     KvSeq s;
@@ -121,57 +88,9 @@ __device__ __forceinline__ KrSeq kr_seq(const KvAttendParams& P, int lim, int b)
     return q;
 }
 __device__ __forceinline__ int64_t kr_length(const KvAttendParams& P, int lim, int b) {
+    if (b >= P.step.n_seqs) return 0;
     const KrSeq q = kr_seq(P, lim, b);
     return q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0;
-}
-
-struct KrSpot { int64_t total, start; int b; };  // length of the line; the sequence that a position is in, and where that begins
-
-// By all threads of a CTA of THREADS: the line's length, and where position cta * (length / ctas) is.  Scratch: shared memory.
-template <int THREADS>
-__device__ KrSpot kr_locate(const KvAttendParams& P, int lim, int cta, int ctas, int64_t* scratch) {
-    constexpr int WARPS = THREADS / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = P.step.n_seqs;
-    auto scan = [&](int64_t v) {  // inclusive, over the warp
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        return v;
-    };
-    const int64_t mine = tid < n ? kr_length(P, lim, tid) : 0;  // (most steps have no more sequences than threads)
-    int64_t sum = mine;
-    for (int b = tid + THREADS; b < n; b += THREADS) sum += kr_length(P, lim, b);
-    sum = scan(sum);
-    if (lane == 31) scratch[warp] = sum;
-    __syncthreads();
-    KrSpot spot{0, -1, n};
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) spot.total += scratch[w];
-    const int64_t at = (spot.total + ctas - 1) / ctas * cta;
-    if (at >= spot.total) return spot;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < n; b0 += THREADS) {
-        const int64_t v = b0 == 0 ? mine : b0 + tid < n ? kr_length(P, lim, b0 + tid) : 0;
-        const int64_t inc = scan(v);
-        __syncthreads();
-        if (lane == 31) scratch[warp] = inc;
-        if (tid == 0) scratch[WARPS] = -1;
-        __syncthreads();
-        int64_t base = before, chunk = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            if (w < warp) base += scratch[w];
-            chunk += scratch[w];
-        }
-        const int64_t from = base + inc - v;
-        if (from <= at && at < from + v) { scratch[WARPS] = b0 + tid; scratch[WARPS + 1] = from; }
-        __syncthreads();
-        if (scratch[WARPS] >= 0) { spot.b = (int)scratch[WARPS]; spot.start = scratch[WARPS + 1]; break; }
-        before += chunk;
-    }
-    return spot;
 }
 
 // A CTA's piece of the line, one (sequence, kv head) at a time.
@@ -181,7 +100,7 @@ struct KrWalk {
     KrSeq q;
     int head, t0, t1;
     bool first;  // the piece is the CTA's first
-    __device__ __forceinline__ KrWalk(const KvAttendParams& P, int lim, const KrSpot& spot) {
+    __device__ __forceinline__ KrWalk(const KvAttendParams& P, int lim, const KvSpot& spot) {
         const int64_t per = (spot.total + gridDim.x - 1) / gridDim.x;
         w = per * blockIdx.x;
         w1 = min(spot.total, w + per);
@@ -207,15 +126,6 @@ struct KrWalk {
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == q.view.tiles; }
 };
 
-// Partial results: [CTA][first or last piece] of ROWS x (HD floats), then ROWS x (m, l).
-__device__ __forceinline__ float* kr_part(void* work, int rows, int hd, int64_t cta, int slot) { return static_cast<float*>(work) + (cta * 2 + slot) * rows * (hd + 2); }
-
-__device__ __forceinline__ void store2(const KvRows& o, int64_t e, float x) {
-    if (o.type == L2_F32) reinterpret_cast<float*>(o.data)[e] = x;
-    else if (o.type == L2_F16) reinterpret_cast<__half*>(o.data)[e] = __float2half_rn(x);
-    else reinterpret_cast<__nv_bfloat16*>(o.data)[e] = __float2bfloat16_rn(x);
-}
-
 // CT: cache type; QB: q is bf16, else f16
 template <int CT, bool QB, int HD, int NT>
 __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
@@ -239,7 +149,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const KrSpot spot = kr_locate<KR_THREADS>(P, lim, blockIdx.x, gridDim.x, scratch);  // (ends behind a barrier)
+    const KvSpot spot = kv_locate<KR_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kr_length(P, lim, b); });  // (ends behind a barrier)
     __syncthreads();
     KrWalk walk(P, lim, spot);
     KvWait wait{&failed};
@@ -393,8 +303,8 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        // f16: probabilities up to 2^15, so that those 2^-29 times the largest are still normal numbers
-                        m1[nt][e] = fmaxf(m[nt][e], PB ? x : x - 15.0f);
+                        // probabilities carry a factor of 2^15 or, in bf16, 2^24, so that small ones are normal numbers
+                        m1[nt][e] = fmaxf(m[nt][e], x - (PB ? 24.0f : 15.0f));
                         moved |= m1[nt][e] != m[nt][e];
                     }
                 }
@@ -403,11 +313,11 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const float f = m1[nt][e] == -INFINITY ? 1.0f : kv_exp2(m[nt][e] - m1[nt][e]);
+                            const KvScale f(m1[nt][e] == -INFINITY ? 0.0f : m[nt][e] - m1[nt][e]);
                             m[nt][e] = m1[nt][e];
-                            l[nt][e] *= f;
+                            l[nt][e] = f(l[nt][e]);
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] *= f; o[mt][nt][e + 2] *= f; }
+                            for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
                         }
                 }
                 uint32_t pb[NT][2];
@@ -504,11 +414,11 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     const float ref = top == -INFINITY ? 0.0f : top;
                     lsum[nt][e] = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < KR_WARPS; w++) lsum[nt][e] += kv_exp2(meet_ml[w][r][0] - ref) * meet_ml[w][r][1];
-                    const float f = kv_exp2(m[nt][e] - ref);
+                    for (int w = 0; w < KR_WARPS; w++) lsum[nt][e] += KvScale(meet_ml[w][r][0] - ref)(meet_ml[w][r][1]);
+                    const KvScale f(m[nt][e] - ref);
                     m[nt][e] = top;
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] *= f; o[mt][nt][e + 2] *= f; }
+                    for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
                 }
 #pragma unroll
             for (int from = KR_WARPS - 1; from > 0; from--) {
@@ -529,7 +439,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
             }
             if (warp == 0) {
                 const bool done = walk.whole();
-                float* part = kr_part(P.work, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
+                float* part = kv_part(P.work, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -545,7 +455,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                             for (int h = 0; h < 2; h++) {
                                 const int d = I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
                                 const float x = o[mt][nt][2 * h + e];
-                                if (done) store2(P.out, at + d, pos[nt][e] < 0 ? 0.0f : x * inv);
+                                if (done) kv_store1(P.out, at + d, pos[nt][e] < 0 ? 0.0f : x * inv);
                                 else part[r * HD + d] = x;
                             }
                         if (!done && g8 == 0) *reinterpret_cast<float2*>(part + S::ROWS * HD + 2 * r) = make_float2(m[nt][e], lsum[nt][e]);
@@ -570,7 +480,7 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
     __shared__ float4 sums[256];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int cut = blockIdx.x + 1;
-    const KrSpot spot = kr_locate<256>(P, lim, cut, ctas, scratch);
+    const KvSpot spot = kv_locate<256>(P.step.n_seqs, cut, ctas, scratch, [&](int b) { return kr_length(P, lim, b); });
     if (spot.start < 0) return;
     const int64_t per = (spot.total + ctas - 1) / ctas, at = per * cut;
     const KrSeq q = kr_seq(P, lim, spot.b);
@@ -578,7 +488,7 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
     const int64_t from = spot.start + (int64_t)head * T, to = from + T;
     if (from == at || from / per != cut - 1) return;
     const int c0 = cut - 1, n = (int)((to - 1) / per) - c0 + 1;
-    auto piece = [&](int i) { return kr_part(P.work, part_rows, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
+    auto piece = [&](int i) { return kv_part(P.work, part_rows, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
     int width = 1;  // rows side by side
     while (width < q.rows && width < SLOTS) width <<= 1;
     const int share = SLOTS / width, slot = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES), mine = slot / width;
@@ -590,13 +500,13 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
             float top = -INFINITY;
             for (int i = 0; i < n; i++) top = fmaxf(top, piece(i)[part_rows * HD + 2 * r]);
             const float ref = top == -INFINITY ? 0.0f : top;
-            for (int i = 0; i < n; i++) sum += kv_exp2(piece(i)[part_rows * HD + 2 * r] - ref) * piece(i)[part_rows * HD + 2 * r + 1];
+            for (int i = 0; i < n; i++) sum += KvScale(piece(i)[part_rows * HD + 2 * r] - ref)(piece(i)[part_rows * HD + 2 * r + 1]);
 #pragma unroll 4
             for (int i = mine; i < n; i += share) {
                 const float* p = piece(i);
-                const float f = kv_exp2(p[part_rows * HD + 2 * r] - ref);
+                const KvScale f(p[part_rows * HD + 2 * r] - ref);
                 const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
-                acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+                acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
             }
         }
         if (share > 1) {
@@ -614,7 +524,7 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
             const float inv = 1.0f / sum;
             const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
-            for (int i = 0; i < 4; i++) store2(P.out, e + i, pos < 0 ? 0.0f : y[i]);
+            for (int i = 0; i < 4; i++) kv_store1(P.out, e + i, pos < 0 ? 0.0f : y[i]);
         }
     }
 }

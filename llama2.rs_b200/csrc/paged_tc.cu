@@ -1,0 +1,777 @@
+// l2_kv_attend for sequences with many rows (chunks of a prompt, whole prompts): tcgen05 matrix products, softmax in registers.
+//
+// A block of up to 256 rows (tokens x query heads of one kv head) of one sequence, as two tiles Q0, Q1 of 128, walks tiles of 128 positions:
+//   S = Q K^T (tensor memory),  P = 2^(scale S - m) (over S, 16 bits),  O += P V (tensor memory),  l += sum P,   out = O / l
+// m is a row's maximum of some earlier tile: it is raised, and O and l scaled, only when a score exceeds it by more than 2^8 (the sums
+// are f32: a common factor costs nothing).
+//
+// The products take 4 x 256 clocks a tile of positions (two tiles of rows, 128 x 128 x 128 each); the exponentials 2 x 1024 if the special function
+// unit (16 a clock) did them all.
+//
+// Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs; a block that a cut goes
+// through leaves a partial (m, l, O) in each piece, which kv_tc_combine_kernel adds in order.  Causal blocks of different lengths, windows
+// and ragged sequences need no other balance.
+//
+// Roles (they meet only through mbarriers):
+//   warps 0-3, 4-7  softmax of Q0 and Q1, a row a thread; they bring Q, and the result out
+//   warp 8          one thread issues the products: O0 += P0 V, S0 = Q0 K', O1 += P1 V, S1 = Q1 K': while one tile's softmax runs, the other's
+//                   products do
+//   warp 9          K and V tiles by TMA into one ring, a copy a page run
+//   warps 12-15     16-bit caches: tiles that some row sees in part are searched for values that are not finite: 0 x NaN is NaN, and a row must not be
+//                   reached by what it does not see.  They are taken out before the product and added to the rows that see them at the end.
+//                   int8 caches: they turn the bytes into 16-bit numbers (K q's type, V bf16, exact); scales are applied to the scores and to the
+//                   probabilities.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.cuh"
+#include "paged_attend.h"
+#include "paged_device.cuh"
+
+namespace l2 {
+
+namespace {
+
+constexpr int KT_TILE = 128, KT_ROWS = 256, KT_THREADS = 512;
+constexpr int KT_MMA_WARP = 8, KT_COPY_WARP = 9, KT_HELP_WARP = 12;
+constexpr int KT_SCALE_SLOTS = 4;
+constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
+
+template <int CT, int HD>
+struct KtShape {
+    static constexpr bool I8 = CT == L2_I8;
+    static constexpr int SLOT = KT_TILE * HD * 2;                     // K or V of a tile in 16 bits
+    static constexpr int RAW = I8 ? KT_TILE * HD : 0;                 // ... in 8
+    static constexpr int SLOTS = HD == 64 ? 6 : I8 ? 3 : 5, RAWS = I8 ? (HD == 64 ? 4 : 3) : 0;
+    static constexpr int SCALES = I8 ? KT_SCALE_SLOTS * 2 * KT_TILE * 4 : 0;
+    static constexpr int Q_BYTES = 2 * SLOT;
+    // (always more than half of an SM's shared memory: one CTA, one owner of the tensor memory, per SM)
+    static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + SCALES > 120 * 1024 ? 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + SCALES : 120 * 1024;
+    static_assert(SMEM <= 226 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_units) { return ((saddr >> 4) & 0x3FFFu) | (lbo_units << 16); }
+constexpr uint32_t KT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8 rows of 128 bytes 1024 bytes apart, 128-byte swizzle
+// D (+)= A B: A and B in shared memory, or A in tensor memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 da, {%1, %3};\nmov.b64 db, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 db, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(kv_smem(bar)) : "memory");
+}
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+#define KT_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define KT_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t* v, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : KT_R8(v, 0), KT_R8(v, 8), KT_R8(v, 16), KT_R8(v, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::KT_W8(v, 0), KT_W8(v, 8), KT_W8(v, 16), KT_W8(v, 24), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::KT_W8(v, 0), KT_W8(v, 8), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(unsigned long long d) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(d));
+    return v;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// byte offset of 16-byte chunk c of row r in a tile of 128 rows: halves of 128 bytes one after the other, 128-byte swizzle (rows of 64 bytes: 64-byte swizzle)
+__device__ __forceinline__ uint32_t kt_offset(int r, int c) { return (c >> 3) * (KT_TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t kt_offset64(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
+
+// ---- the line: sequence by sequence, kv head by kv head, block by block, tile by tile ---------------------------------------
+struct KtBlocks { KvSeq s; int tokens, n; };  // blocks of a sequence, of `tokens` tokens; n = 0: not this kernel's
+__device__ __forceinline__ KtBlocks kt_blocks(const KvAttendParams& P, int lim, int b) {
+    KtBlocks k;
+    k.tokens = KT_ROWS / P.group;
+    k.n = 0;
+    if (b >= P.step.n_seqs) { k.s = KvSeq{0, 0, 0}; return k; }
+    k.s = kv_seq(P.step, P.pool.page_shift, b);
+    if ((int64_t)k.s.n * P.group > lim) k.n = (k.s.n + k.tokens - 1) / k.tokens;
+    return k;
+}
+__device__ __forceinline__ KvView<KT_TILE> kt_view(const KvAttendParams& P, const KtBlocks& k, int block) {
+    const int t0 = block * k.tokens, t1 = min(k.s.n, t0 + k.tokens), p = k.s.kv - k.s.n;
+    return KvView<KT_TILE>(p + t0, p + t1 - 1, P.window, P.sinks);
+}
+// Tiles of one kv head of the lane's sequence, by the whole warp (each lane its own sequence).
+__device__ __forceinline__ int64_t kt_tiles(const KvAttendParams& P, KtBlocks k) {
+    const int lane = threadIdx.x & 31;
+    int64_t sum = 0;
+    if (k.n <= 4)
+        for (int i = 0; i < k.n; i++) sum += kt_view(P, k, i).tiles;
+    unsigned many = __ballot_sync(0xffffffffu, k.n > 4);
+    while (many) {  // the warp's lanes share the blocks of a long one
+        const int src = __ffs(many) - 1;
+        many &= many - 1;
+        KtBlocks q = k;
+        q.s.n = __shfl_sync(0xffffffffu, k.s.n, src);
+        q.s.kv = __shfl_sync(0xffffffffu, k.s.kv, src);
+        q.n = __shfl_sync(0xffffffffu, k.n, src);
+        int64_t x = 0;
+        for (int i = lane; i < q.n; i += 32) x += kt_view(P, q, i).tiles;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (lane == src) sum = x;
+    }
+    return sum;
+}
+// The block that tile `at` of a head of the sequence is in, and the tiles in front of it; by the whole warp, all lanes with the same arguments.
+__device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBlocks& k, int64_t at, int64_t* before) {
+    const int lane = threadIdx.x & 31;
+    int64_t base = 0;
+    for (int i0 = 0; i0 < k.n; i0 += 32) {
+        int64_t v = i0 + lane < k.n ? kt_view(P, k, i0 + lane).tiles : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, base + v > at);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const int64_t upto = __shfl_sync(0xffffffffu, v, max(l - 1, 0));
+            *before = l ? base + upto : base;
+            return i0 + l;
+        }
+        base += __shfl_sync(0xffffffffu, v, 31);
+    }
+    *before = base;
+    return k.n - 1;
+}
+
+struct KtWalk {
+    int64_t w, w1;
+    int b, head, block, skip;  // skip: tiles of the first block that belong to the CTA in front
+    KtBlocks k;
+    KvView<KT_TILE> view;
+    int t0, t1, rows, index;   // rows of the block; pieces before this one
+    __device__ __forceinline__ KtWalk(const KvAttendParams& P, int lim, const KvSpot& spot) {
+        const int64_t per = (spot.total + gridDim.x - 1) / gridDim.x;
+        w = per * blockIdx.x;
+        w1 = min(spot.total, w + per);
+        b = spot.b; index = -1; head = block = skip = 0;
+        if (w >= w1) return;
+        k = kt_blocks(P, lim, b);
+        const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = w - spot.start;
+        head = (int)(in / tiles);
+        int64_t before;
+        block = kt_find_block(P, k, in - head * tiles, &before);
+        skip = (int)(in - head * tiles - before);
+        block--;  // (next() goes on to it)
+    }
+    __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
+        if (w >= w1) return false;
+        index++;
+        if (++block >= k.n) {
+            block = 0;
+            if (++head == P.pool.n_kv_heads) {
+                head = 0;
+                do k = kt_blocks(P, lim, ++b); while (!k.n && b < P.step.n_seqs);
+            }
+        }
+        view = kt_view(P, k, block);
+        rows = min(k.tokens, k.s.n - block * k.tokens) * P.group;
+        t0 = skip;
+        skip = 0;
+        t1 = (int)min((int64_t)view.tiles, t0 + (w1 - w));
+        w += t1 - t0;
+        return true;
+    }
+    // what tile i of the block's rows sees (its rows: 128 i and on); without rows it sees nothing
+    __device__ __forceinline__ KvView<KT_TILE> part(const KvAttendParams& P, int i) const {
+        KvView<KT_TILE> v = view;
+        const int lo = 128 * i, hi = min(rows, lo + 128) - 1;
+        v.lo_pos = view.lo_pos + lo / P.group;
+        v.hi_pos = hi < lo ? -1 : view.lo_pos + hi / P.group;
+        return v;
+    }
+};
+
+template <int CT, bool QB, int HD>
+__global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
+                                                              const __grid_constant__ CUtensorMap map_v) {
+    using S = KtShape<CT, HD>;
+    constexpr bool I8 = S::I8, PB = I8 || QB;
+    constexpr uint32_t S_COL = 0, O_COL = 256;                   // tensor memory: S0 S1 O0 O1, 128 columns each; P over S
+    // Probabilities carry a factor of 2^BIAS, so that small ones are normal numbers: f16 at most 2^(7 + KT_RAISE); f32 and bf16 have room (2^95 for a V).
+    constexpr float BIAS = PB ? 24.0f : 7.0f;
+    extern __shared__ __align__(1024) uint8_t kt_smem[];
+    __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[I8 ? S::RAWS : 1], raw_empty[I8 ? S::RAWS : 1],
+        sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ int64_t scratch[KT_THREADS / 32 + 2];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int failed;
+    __shared__ volatile int odd[8];  // by piece: values that are not finite have been taken out of a V tile
+    uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem) + 1023) & ~(uintptr_t)1023);  // Q0, Q1
+    uint8_t* ring = sq + S::Q_BYTES;
+    uint8_t* raw = ring + S::SLOTS * S::SLOT;
+    float* scales = reinterpret_cast<float*>(raw + S::RAWS * S::RAW);  // [slot][k, v][position]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::SLOTS; i++) { kv_bar_init(&full[i], I8 ? 4 : 1); kv_bar_init(&empty[i], I8 ? 1 : 5); kv_bar_init(&ready[i], 4); }
+        for (int i = 0; i < (I8 ? S::RAWS : 1); i++) { kv_bar_init(&raw_full[i], 1); kv_bar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 1); kv_bar_init(&sc_empty[i], 8); }
+        for (int i = 0; i < 2; i++) { kv_bar_init(&q_full[i], 128); kv_bar_init(&s_full[i], 1); kv_bar_init(&p_full[i], 4); kv_bar_init(&o_full[i], 1); }
+        kv_bar_init(&drained, 1);
+        for (int i = 0; i < 8; i++) odd[i] = 0;
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == KT_MMA_WARP) {  // all 512 columns of tensor memory
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const KvSpot spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch,
+                                              [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_s;
+    KtWalk walk(P, lim, spot);
+    KvWait wait{&failed};
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        // ================= softmax: a row a thread ============================================================================
+        const int i = warp >> 2, row = 128 * i + (tid & 127);
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + S_COL + 128 * i, o_at = tmem + lanes + O_COL + 128 * i;
+        uint32_t s_ph = 0, o_ph = 0, sc = 0, sc_ph = 0;
+        while (walk.next(P, lim)) {
+            const KvView<KT_TILE> mine = walk.part(P, i);
+            const bool there = row < walk.rows;
+            const int tok = min(row, walk.rows - 1) / P.group, head = walk.head * P.group + (there ? row - tok * P.group : 0);
+            const int pos = walk.view.lo_pos + tok;
+            const int64_t at = walk.k.s.row0 + walk.block * walk.k.tokens + tok;
+            int first = walk.t0;
+            while (first < walk.t1 && !mine.any(walk.view.base(first), KT_TILE, P.window, P.sinks)) first++;
+            if (first < walk.t1) {  // Q, swizzled as the products want it; rows that there are not: zeros
+                uint8_t* to = sq + i * S::SLOT;
+                const char* from = P.q.data + 2 * (at * P.q.row_stride + (int64_t)head * P.q.head_stride);
+#pragma unroll 8
+                for (int c = 0; c < HD / 8; c++)
+                    *reinterpret_cast<uint4*>(to + kt_offset(tid & 127, c)) = there ? *reinterpret_cast<const uint4*>(from + 16 * c) : make_uint4(0, 0, 0, 0);
+                fence_async();
+                kv_bar_arrive(&q_full[i]);
+            }
+            float m = -INFINITY, l = 0.0f;
+            bool started = false;
+#pragma unroll 1
+            for (int t = walk.t0; t < walk.t1; t++) {
+                const int base = walk.view.base(t);
+                if (!mine.any(base, KT_TILE, P.window, P.sinks)) {
+                    if constexpr (I8) {
+                        wait(&sc_full[sc], sc_ph);
+                        __syncwarp();
+                        if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
+                        if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
+                    }
+                    continue;
+                }
+                const bool whole = mine.whole(base, P.window, P.sinks);
+                uint32_t x[128];
+                wait(&s_full[i], s_ph);
+                s_ph ^= 1u;
+                __syncwarp();
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32(x + 32 * c, s_at + 32 * c);
+                wait_ld();
+                const float* ks = scales + sc * 2 * KT_TILE;
+                if constexpr (I8) {
+                    wait(&sc_full[sc], sc_ph);
+#pragma unroll
+                    for (int j = 0; j < 128; j += 4) {
+                        const float4 k = *reinterpret_cast<const float4*>(ks + j);
+                        x[j] = __float_as_uint(__uint_as_float(x[j]) * k.x);
+                        x[j + 1] = __float_as_uint(__uint_as_float(x[j + 1]) * k.y);
+                        x[j + 2] = __float_as_uint(__uint_as_float(x[j + 2]) * k.z);
+                        x[j + 3] = __float_as_uint(__uint_as_float(x[j + 3]) * k.w);
+                    }
+                }
+                if (!whole) {
+                    const int hi = pos - base, lo = P.window ? pos - P.window - base : -1, sinks = P.sinks - base;  // seen: j <= hi and (j > lo or j < sinks)
+#pragma unroll
+                    for (int j = 0; j < 128; j++)
+                        if (!(j <= hi && (j > lo || j < sinks))) x[j] = 0xff800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 128; j += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c])));
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale_log2 - BIAS;
+                if (__any_sync(0xffffffffu, most > m + KT_RAISE)) {
+                    const float m1 = fmaxf(m, most);
+                    const KvScale f(m1 == -INFINITY ? 0.0f : m - m1);
+                    m = m1;
+                    l = f(l);
+                    if (started) {  // (the products that wrote O are done: those that wrote S came behind them)
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o, o_at + c);
+                            wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(f(__uint_as_float(o[j])));
+                            tmem_st32(o_at + c, o);
+                        }
+                    }
+                }
+                started = true;
+                const float ref = m == -INFINITY ? 0.0f : m;
+                const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
+                unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t p16[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 e = unpair(fma2(pair(__uint_as_float(x[c + j]), __uint_as_float(x[c + j + 1])), f2, r2));
+                        float2 p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
+                        sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(p.x, p.y));
+                        if constexpr (I8) {
+                            const float2 v = *reinterpret_cast<const float2*>(ks + KT_TILE + c + j);
+                            if (whole) p = make_float2(p.x * v.x, p.y * v.y);
+                            else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
+                        }
+                        p16[j / 2] = pack16<PB>(p.x, p.y);
+                    }
+                    tmem_st16(s_at + c / 2, p16);
+                }
+                const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
+                l += (s0.x + s0.y) + (s1.x + s1.y);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    kv_bar_arrive(&p_full[i]);
+                    if constexpr (I8) kv_bar_arrive(&sc_empty[sc]);
+                }
+                if constexpr (I8) { if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; } }
+            }
+            // ---- the result of the piece
+            const bool done = walk.t0 == 0 && walk.t1 == walk.view.tiles;
+            if (started) {
+                wait(&o_full[i], o_ph);
+                o_ph ^= 1u;
+                __syncwarp();
+                fence_after();
+            }
+            if (128 * i >= walk.rows) continue;  // (whole warps: this tile has no rows)
+            const bool fix = !I8 && started && odd[walk.index & 7];
+            float* part = kv_part(P.work, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
+            const float inv = pos < 0 ? 0.0f : done ? 1.0f / l : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) o[j] = 0u;
+                if (started) { tmem_ld32(o, o_at + c); wait_ld(); }
+                if constexpr (!I8) {
+                    if (fix) {  // rare: the values that were taken out, one by one, to the rows that see them
+#pragma unroll 1
+                        for (int t = walk.t0; t < walk.t1; t++) {
+                            const int base = walk.view.base(t);
+                            if (!mine.any(base, KT_TILE, P.window, P.sinks) || mine.whole(base, P.window, P.sinks)) {
+                                const KvView<KT_TILE> other = walk.part(P, i ^ 1);  // (taken out for the other tile's rows)
+                                if (!mine.any(base, KT_TILE, P.window, P.sinks) || !other.any(base, KT_TILE, P.window, P.sinks) || other.whole(base, P.window, P.sinks)) continue;
+                            }
+#pragma unroll 1
+                            for (int j = base; j < base + KT_TILE; j++) {
+                                if (!kv_sees(pos, j, P.window, P.sinks)) continue;
+                                const int page = kv_page(P.step, P.pool, walk.b, j);
+                                if (page < 0) continue;
+                                const uint16_t* v = reinterpret_cast<const uint16_t*>(P.pool.v) + (int64_t)page * P.pool.page_stride +
+                                                    (j & ((1 << P.pool.page_shift) - 1)) * P.pool.pos_stride + walk.head * P.pool.head_stride + c;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    const uint16_t bits = v[e];
+                                    if (not_finite<QB>(bits)) o[e] = __float_as_uint(__uint_as_float(o[e]) + (QB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits))));
+                                }
+                            }
+                        }
+                    }
+                }
+                if (!there) continue;
+                if (!done) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + row * HD + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = pos < 0 ? 0.0f : __uint_as_float(o[j + e]) * inv;
+                    kv_store8(P.out, at, head, c + j, y);
+                }
+            }
+            if (!done && there) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
+            fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == KT_MMA_WARP) {
+            // ================= products ========================================================================================
+            const bool leader = elect();
+            constexpr uint32_t fmt = QB ? 1u : 0u, fmt_p = PB ? 1u : 0u;
+            constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | (fmt_p << 7) | (fmt_p << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);  // V: elements contiguous
+            const uint32_t q_lo = desc_lo(kv_smem(sq), 1), k_lo = desc_lo(kv_smem(ring), 1), v_lo = desc_lo(kv_smem(ring), KT_TILE * 128 / 16);
+            uint32_t slot = 0, ph = 0, ready_ph = 0, q_ph = 0, p_ph = 0;  // q_ph, p_ph: a bit for each tile; ready_ph: one for each slot
+            auto step = [&]() { if (++slot == S::SLOTS) { slot = 0; ph ^= 1u; } };
+            while (walk.next(P, lim)) {
+                const KvView<KT_TILE> see[2] = {walk.part(P, 0), walk.part(P, 1)};
+                uint32_t begun = 0;  // tiles whose Q has been waited for, and (bits 2, 3) whose O has been written
+                // S of tile i from the K tile in the current slot
+                auto scores = [&](int i) {
+                    if (!(begun & (1u << i))) { wait(&q_full[i], (q_ph >> i) & 1u); q_ph ^= 1u << i; begun |= 1u << i; }
+                    wait(&full[slot], ph);
+                    __syncwarp();
+                    fence_after();
+                    if (leader && !wait.dead) {
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++) {
+                            const uint32_t off = (k / 4) * (KT_TILE * 128 / 16) + (k % 4) * 2;
+                            mma_ss(tmem + S_COL + 128 * i, q_lo + i * (S::SLOT / 16) + off, k_lo + slot * (S::SLOT / 16) + off, idesc_s, k > 0);
+                        }
+                        commit(&s_full[i]);
+                    }
+                    __syncwarp();
+                };
+                auto active = [&](int i, int t) { return see[i].any(walk.view.base(t), KT_TILE, P.window, P.sinks); };
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if (active(i, walk.t0)) scores(i);
+                wait(&full[slot], ph);  // (a slot is given back only when it has been filled)
+                if (leader) commit(&empty[slot]);
+                __syncwarp();
+                step();
+#pragma unroll 1
+                for (int t = walk.t0; t < walk.t1; t++) {
+                    const int base = walk.view.base(t);
+                    const uint32_t v_slot = slot, v_ph = ph;
+                    step();
+                    const bool more = t + 1 < walk.t1;
+                    bool part = false;
+                    if constexpr (!I8)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) part |= active(i, t) && !see[i].whole(base, P.window, P.sinks);
+                    bool v_here = false;
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (active(i, t)) {
+                            if (!v_here) {
+                                wait(&full[v_slot], v_ph);
+                                if (part) { wait(&ready[v_slot], (ready_ph >> v_slot) & 1u); ready_ph ^= 1u << v_slot; }
+                                v_here = true;
+                            }
+                            wait(&p_full[i], (p_ph >> i) & 1u);
+                            p_ph ^= 1u << i;
+                            __syncwarp();
+                            fence_after();
+                            if (leader && !wait.dead) {
+#pragma unroll
+                                for (int k = 0; k < KT_TILE / 16; k++)
+                                    mma_ts(tmem + O_COL + 128 * i, tmem + S_COL + 128 * i + 8 * k, v_lo + v_slot * (S::SLOT / 16) + k * (16 * 128 / 16), idesc_o, k > 0 || (begun & (4u << i)));
+                            }
+                            begun |= 4u << i;
+                            __syncwarp();
+                        }
+                        if (i == 1) {
+                            if (!v_here) wait(&full[v_slot], v_ph);
+                            if (leader) commit(&empty[v_slot]);
+                            __syncwarp();
+                        }
+                        if (more && active(i, t + 1)) scores(i);
+                    }
+                    if (more) {
+                        wait(&full[slot], ph);
+                        if (leader) commit(&empty[slot]);
+                        __syncwarp();
+                        step();
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if ((begun & (1u << i)) && leader) commit(&o_full[i]);
+                __syncwarp();
+            }
+            if (failed) {  // products still under way read shared memory: a bounded time to end
+                if (leader) commit(&drained);
+                __syncwarp();
+                for (int i = 0; i < 1024 && !kv_bar_try(&drained, 0); i++) {}
+            }
+        } else if (warp == KT_COPY_WARP) {
+            // ================= copies: lane l brings run l of a tile ==============================================================
+            const int R = min(KT_TILE, 1 << P.pool.page_shift), runs = KT_TILE / R;
+            constexpr int RB = HD * (I8 ? 1 : 2), W = RB < 128 ? RB : 128;  // bytes of a row, of a copy's row
+            uint32_t slot = 0, ph = 1, sc = 0, sc_ph = 1;
+            while (walk.next(P, lim) && !wait.dead) {
+                auto page_of = [&](int t) {  // the page of this lane's run of tile t, n_pages (zeros) where no row sees it or there is none
+                    const int j = walk.view.base(t) + lane * R;
+                    if (lane >= runs || !walk.view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
+                    const int x = kv_page(P.step, P.pool, walk.b, j);
+                    return x >= 0 ? x : P.pool.n_pages;
+                };
+                int page = page_of(walk.t0);
+                for (int t = walk.t0; t < walk.t1; t++) {
+                    const int j = walk.view.base(t) + lane * R, at = j & ((1 << P.pool.page_shift) - 1);
+                    const int ahead = t + 1 < walk.t1 ? page_of(t + 1) : P.pool.n_pages;
+                    if constexpr (I8) {
+                        wait(&sc_empty[sc], sc_ph);
+                        if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                        float* s = scales + sc * 2 * KT_TILE + lane * R;
+                        const bool there = lane < runs && page < P.pool.n_pages;
+                        if (lane < runs && !there)
+                            for (int i = 0; i < R; i++) s[i] = s[KT_TILE + i] = 0.0f;
+                        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * R * 8;
+                        __syncwarp();
+                        if (lane == 0) kv_bar_expect(&sc_full[sc], bytes);
+                        __syncwarp();
+                        if (there) {
+                            const int64_t e = ((int64_t)page * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + at;
+                            kv_bulk(kv_smem(s), P.pool.ks + e, R * 4, &sc_full[sc]);
+                            kv_bulk(kv_smem(s + KT_TILE), P.pool.vs + e, R * 4, &sc_full[sc]);
+                        }
+                        if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
+                    }
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        uint64_t *f = I8 ? &raw_full[slot] : &full[slot], *e = I8 ? &raw_empty[slot] : &empty[slot];
+                        wait(e, ph);
+                        if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                        if (lane == 0) kv_bar_expect(f, KT_TILE * RB);
+                        __syncwarp();
+                        if (lane < runs) {
+                            const uint32_t to = kv_smem(I8 ? raw + slot * S::RAW : ring + slot * S::SLOT) + lane * R * W;
+#pragma unroll
+                            for (int h = 0; h < RB / W; h++) kv_tma4(to + h * (KT_TILE * 128), kv ? &map_v : &map_k, h * 64, at, walk.head, page, f);
+                        }
+                        if (++slot == (I8 ? S::RAWS : S::SLOTS)) { slot = 0; ph ^= 1u; }
+                    }
+                    if (wait.dead) break;
+                    page = ahead;
+                }
+            }
+        } else if (warp >= KT_HELP_WARP) {
+            const int r = tid & 127;
+            if constexpr (I8) {
+                // ================= bytes to 16-bit numbers: a position a thread ==================================================
+                uint32_t rs = 0, rph = 0, slot = 0, ph = 1;
+                while (walk.next(P, lim)) {
+#pragma unroll 1
+                    for (int n = 2 * (walk.t1 - walk.t0), kv = 0; n > 0; n--, kv ^= 1) {
+                        wait(&raw_full[rs], rph);
+                        wait(&empty[slot], ph);
+                        __syncwarp();
+                        const uint8_t* from = raw + rs * S::RAW;
+                        uint8_t* to = ring + slot * S::SLOT;
+                        auto turn = [&](auto bf) {
+                            constexpr bool BF = decltype(bf)::value;
+#pragma unroll
+                            for (int c = 0; c < HD / 16; c++) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(from + (HD == 64 ? kt_offset64(r, c) : kt_offset(r, c)));
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 2 * c)) = make_uint4(widen<BF, 0x10>(w.x), widen<BF, 0x32>(w.x), widen<BF, 0x10>(w.y), widen<BF, 0x32>(w.y));
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 2 * c + 1)) = make_uint4(widen<BF, 0x10>(w.z), widen<BF, 0x32>(w.z), widen<BF, 0x10>(w.w), widen<BF, 0x32>(w.w));
+                            }
+                        };
+                        if (kv || QB) turn(std::true_type());
+                        else turn(std::false_type());
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) { kv_bar_arrive(&raw_empty[rs]); kv_bar_arrive(&full[slot]); }
+                        if (++rs == (uint32_t)S::RAWS) { rs = 0; rph ^= 1u; }
+                        if (++slot == (uint32_t)S::SLOTS) { slot = 0; ph ^= 1u; }
+                    }
+                }
+            } else {
+                // ================= V tiles that some row sees in part: only finite values stay ===================================
+                // (they see every slot of the ring and give it back with the products: neither can be a round ahead of the other)
+                uint32_t slot = 0, ph = 0;
+                auto step = [&]() {
+                    __syncwarp();
+                    if (lane == 0) kv_bar_arrive(&empty[slot]);
+                    if (++slot == S::SLOTS) { slot = 0; ph ^= 1u; }
+                };
+                while (walk.next(P, lim)) {
+                    const KvView<KT_TILE> see[2] = {walk.part(P, 0), walk.part(P, 1)};
+                    if (tid == KT_HELP_WARP * 32) odd[(walk.index + 4) & 7] = 0;  // (a piece to come)
+#pragma unroll 1
+                    for (int t = walk.t0; t < walk.t1; t++) {
+                        const int base = walk.view.base(t);
+                        wait(&full[slot], ph);
+                        step();
+                        bool part = false;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) part |= see[i].any(base, KT_TILE, P.window, P.sinks) && !see[i].whole(base, P.window, P.sinks);
+                        wait(&full[slot], ph);
+                        if (part) {
+                            uint8_t* v = ring + slot * S::SLOT;
+                            uint32_t found = 0;
+#pragma unroll
+                            for (int c = 0; c < HD / 8; c++) {
+                                uint4* at = reinterpret_cast<uint4*>(v + kt_offset(r, c));
+                                uint4 w = *at;
+                                if (not_finite<QB>(w.x) | not_finite<QB>(w.y) | not_finite<QB>(w.z) | not_finite<QB>(w.w)) {
+                                    found = 1;
+                                    *at = make_uint4(only_finite<QB>(w.x), only_finite<QB>(w.y), only_finite<QB>(w.z), only_finite<QB>(w.w));
+                                }
+                            }
+                            if (found) { odd[walk.index & 7] = 1; __threadfence_block(); }
+                            fence_async();
+                            __syncwarp();
+                            if (lane == 0) kv_bar_arrive(&ready[slot]);
+                        }
+                        step();
+                    }
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (failed) {  // copies may still be on their way into this CTA's shared memory: a bounded time to land
+        uint64_t* bar = tid < S::SLOTS ? &full[tid] : tid < S::SLOTS + S::RAWS ? &raw_full[tid - S::SLOTS] : tid < S::SLOTS + S::RAWS + KT_SCALE_SLOTS && I8 ? &sc_full[tid - S::SLOTS - S::RAWS] : nullptr;
+        if (bar)
+            for (int i = 0; i < 64; i++) { kv_bar_try(bar, 0); kv_bar_try(bar, 1); }
+        if (tid == 0) kv_report(P.step.status, L2_KV_TIMEOUT);
+    }
+    if (warp == KT_MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+constexpr int KT_COMBINE_SPLIT = 8;  // CTAs that share the rows of a block
+
+// Adds the pieces of the blocks that cuts go through: CTA x looks at cut x + 1 and takes the block in it if that is the block's first cut.
+template <int HD>
+__global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int ctas) {
+    constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
+    __shared__ int64_t scratch[256 / 32 + 2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int cut = blockIdx.x + 1;
+    const KvSpot spot = kv_locate<256>(P.step.n_seqs, cut, ctas, scratch, [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
+    if (spot.start < 0) return;
+    const int64_t per = (spot.total + ctas - 1) / ctas, at = per * cut;
+    const KtBlocks k = kt_blocks(P, lim, spot.b);
+    const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = at - spot.start;
+    const int head = (int)(in / tiles);
+    int64_t before;
+    const int block = kt_find_block(P, k, in - head * tiles, &before);
+    const KvView<KT_TILE> view = kt_view(P, k, block);
+    const int64_t from = spot.start + head * tiles + before, to = from + view.tiles;
+    if (from == at || from / per != cut - 1) return;
+    const int c0 = cut - 1, n = (int)((to - 1) / per) - c0 + 1;
+    auto piece = [&](int i) { return kv_part(P.work, KT_ROWS, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
+    const int rows = min(k.tokens, k.s.n - block * k.tokens) * P.group, d = 4 * (threadIdx.x % LANES);
+    for (int r = blockIdx.y * SLOTS + threadIdx.x / LANES; r < rows; r += KT_COMBINE_SPLIT * SLOTS) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int i = 0; i < n; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float* p = piece(i);
+            const float2 ml = *reinterpret_cast<const float2*>(p + KT_ROWS * HD + 2 * r);
+            const KvScale f(ml.x - ref);
+            const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
+            sum += f(ml.y);
+            acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
+        }
+        const int tok = r / P.group, pos = view.lo_pos + tok;
+        const int64_t e = ((int64_t)k.s.row0 + block * k.tokens + tok) * P.out.row_stride + (int64_t)(head * P.group + r - tok * P.group) * P.out.head_stride + d;
+        const float inv = 1.0f / sum;
+        const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+        for (int i = 0; i < 4; i++) kv_store1(P.out, e + i, pos < 0 ? 0.0f : y[i]);
+    }
+}
+
+// CTAs of a launch: one an SM, no more than there can be tiles
+int kt_grid(const KvStep& s, const KvPool& p, int group, int sms) {
+    const int64_t blocks = s.n_rows / (KT_ROWS / group) + s.n_seqs;
+    return (int)std::min<int64_t>(sms, blocks * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KT_TILE - 1) / KT_TILE + 1));
+}
+
+bool kt_needed(const KvStep& s, int group) { return (int64_t)s.max_rows * group > kv_rows_limit(s, group); }
+
+}  // namespace
+
+size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
+    return kt_needed(s, group) ? (size_t)kt_grid(s, p, group, sms) * 2 * KT_ROWS * (head_size + 2) * sizeof(float) : 0;
+}
+
+cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
+    if (!kt_needed(p.step, p.group)) return cudaSuccess;
+    const int lim = kv_rows_limit(p.step, p.group), grid = kt_grid(p.step, p.pool, p.group, sms);
+    CUtensorMap mk, mv;
+    if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, KT_TILE)) return e;
+    if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, KT_TILE)) return e;
+    auto go = [&](auto t, auto b, auto h) {
+        constexpr int T = decltype(t)::value, HD = decltype(h)::value;
+        auto kernel = kv_tc_kernel<T, decltype(b)::value, HD>;
+        static KvOnce once;
+        if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KtShape<T, HD>::SMEM)) return x;
+        kernel<<<grid, KT_THREADS, KtShape<T, HD>::SMEM, st>>>(p, lim, mk, mv);
+        return cudaGetLastError();
+    };
+    auto by_hd = [&](auto t, auto b) { return head_size == 128 ? go(t, b, std::integral_constant<int, 128>()) : go(t, b, std::integral_constant<int, 64>()); };
+    const bool qb = p.q.type == L2_BF16;
+    const cudaError_t e = type == L2_F16 ? by_hd(std::integral_constant<int, L2_F16>(), std::false_type())
+                        : type == L2_BF16 ? by_hd(std::integral_constant<int, L2_BF16>(), std::true_type())
+                        : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
+    g_launches++;
+    if (e != cudaSuccess || grid < 2) return e;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(grid - 1, KT_COMBINE_SPLIT);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    g_launches++;
+    return head_size == 128 ? cudaLaunchKernelEx(&cfg, kv_tc_combine_kernel<128>, p, lim, grid) : cudaLaunchKernelEx(&cfg, kv_tc_combine_kernel<64>, p, lim, grid);
+}
+
+}  // namespace l2
