@@ -28,20 +28,16 @@ __device__ __forceinline__ bool kv_bar_try(uint64_t* bar, uint32_t parity) {
                  : "=r"(ok) : "r"(kv_smem(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
-// A wait that ends: after KV_WAIT_LIMIT polls, or soon after another thread has given up, it fails, and later ones return at once.
+// A wait that ends: after KV_WAIT_LIMIT polls, or soon after another thread has given up; *failed is set then.
 struct KvWait {
     volatile int* failed;
-    bool dead = false;
-    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (dead) return;
+    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) const {
+        if (kv_bar_try(bar, parity)) return;
 #pragma unroll 1
-        for (uint32_t i = 0; i < KV_WAIT_LIMIT; i++) {
-            if (kv_bar_try(bar, parity)) return;
-            if ((i & 63) == 63 && *failed) break;
-        }
-        dead = true;
-        *failed = 1;
+        for (uint32_t i = 0; !kv_bar_try(bar, parity); i++)
+            if (i == KV_WAIT_LIMIT || ((i & 15) == 0 && *failed)) { *failed = 1; return; }
     }
+    __device__ __forceinline__ bool over() const { return __any_sync(0xffffffffu, *failed); }  // (by whole warps)
 };
 __device__ __forceinline__ void kv_tma4(uint32_t dst, const CUtensorMap* map, int x, int pos, int head, int page, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"

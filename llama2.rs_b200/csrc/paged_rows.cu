@@ -152,13 +152,14 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     const KvSpot spot = kv_locate<KR_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kr_length(P, lim, b); });  // (ends behind a barrier)
     __syncthreads();
     KrWalk walk(P, lim, spot);
-    KvWait wait{&failed};
+    const KvWait wait{&failed};
 
     if (warp == KR_WARPS) {
         // ================= copies: lane l brings run l of a tile ==============================================================
         const int R = min(KR_TILE, 1 << P.pool.page_shift), runs = KR_TILE / R;
         uint32_t st = 0, ph = 1;
-        while (walk.next(P, lim)) {
+        bool over = false;
+        while (!over && walk.next(P, lim)) {
             const KvView<KR_TILE>& view = walk.q.view;
             for (int t = walk.t0; t < walk.t1; t++) {
                 const int j = view.base(t) + lane * R;
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     if (x >= 0) page = x;
                 }
                 wait(&empty[st], ph);
-                if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                if ((over = wait.over())) break;
                 uint8_t* stage = ring + st * S::STAGE;
                 const bool there = lane < runs && page < P.pool.n_pages;
                 uint32_t bytes = 2 * S::KV_BYTES;
@@ -201,7 +202,6 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 }
                 if (++st == S::STAGES) { st = 0; ph ^= 1u; }
             }
-            if (wait.dead) break;
         }
     } else {
         // ================= matrix work ========================================================================================

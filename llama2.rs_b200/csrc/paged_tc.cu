@@ -13,10 +13,11 @@
 // and ragged sequences need no other balance.
 //
 // Roles (they meet only through mbarriers):
-//   warps 0-3, 4-7  softmax of Q0 and Q1, a row a thread; they bring Q, and the result out
-//   warp 8          one thread issues the products: O0 += P0 V, S0 = Q0 K', O1 += P1 V, S1 = Q1 K': while one tile's softmax runs, the other's
-//                   products do
-//   warp 9          K and V tiles by TMA into one ring, a copy a page run
+//   warps 0, 2      one thread each issues the products of Q0 and of Q1, for 64 positions at a time, S in two halves of its room in turn: O += P V of one half,
+//                   S = Q K of the same half of the next tile, and so on; the softmax finds the next scores ready.  (One warp for both was the bound: the issue of a product
+//                   takes 80 clocks, and every wait adds a few hundred.)
+//   warp 1          K and V tiles by TMA into one ring, a copy a page run
+//   warps 4-7, 8-11 softmax of Q0 and Q1, a row a thread; they bring Q, and the result out
 //   warps 12-15     16-bit caches: tiles that some row sees in part are searched for values that are not finite: 0 x NaN is NaN, and a row must not be
 //                   reached by what it does not see.  They are taken out before the product and added to the rows that see them at the end.
 //                   int8 caches: they turn the bytes into 16-bit numbers (K q's type, V bf16, exact); scales are applied to the scores and to the
@@ -34,8 +35,8 @@ namespace l2 {
 
 namespace {
 
-constexpr int KT_TILE = 128, KT_ROWS = 256, KT_THREADS = 512;
-constexpr int KT_MMA_WARP = 8, KT_COPY_WARP = 9, KT_HELP_WARP = 12;
+constexpr int KT_TILE = 128, KT_SUB = 64, KT_ROWS = 256, KT_THREADS = 512;
+constexpr int KT_MMA_WARP = 0, KT_COPY_WARP = 1, KT_ROW_WARP = 4, KT_HELP_WARP = 12;
 constexpr int KT_SCALE_SLOTS = 4;
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
@@ -55,15 +56,17 @@ struct KtShape {
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_units) { return ((saddr >> 4) & 0x3FFFu) | (lbo_units << 16); }
 constexpr uint32_t KT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8 rows of 128 bytes 1024 bytes apart, 128-byte swizzle
 // D (+)= A B: A and B in shared memory, or A in tensor memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
     asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 da, {%1, %3};\nmov.b64 db, {%2, %3};\n"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}"
-                 ::"r"(d), "r"(a_lo), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "r"(acc) : "memory");
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+template <bool ACC>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
     asm volatile("{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 db, {%2, %3};\n"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "r"(acc) : "memory");
+                 ::"r"(d), "r"(a), "r"(b_lo), "n"(KT_DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(kv_smem(bar)) : "memory");
@@ -78,6 +81,10 @@ __device__ __forceinline__ bool elect() {
 __device__ __forceinline__ void tmem_ld32(uint32_t* v, uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : KT_R8(v, 0), KT_R8(v, 8), KT_R8(v, 16), KT_R8(v, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t* v, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : KT_R8(v, 0), KT_R8(v, 8) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
@@ -215,6 +222,12 @@ struct KtWalk {
         w += t1 - t0;
         return true;
     }
+    // A bit for each of the tiles t .. t + 31 of positions (of this piece) of which f(first position) holds; by the whole warp.  What is decided once for 32
+    // tiles, and by a vote, is in uniform registers, and so is all that follows from it.
+    template <class F> __device__ __forceinline__ uint32_t bits(int t, F f) const {
+        const int mine = t + (threadIdx.x & 31);
+        return __ballot_sync(0xffffffffu, mine >= t0 && mine < t1 && f(view.base(mine)));
+    }
     // what tile i of the block's rows sees (its rows: 128 i and on); without rows it sees nothing
     __device__ __forceinline__ KvView<KT_TILE> part(const KvAttendParams& P, int i) const {
         KvView<KT_TILE> v = view;
@@ -230,12 +243,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                                                               const __grid_constant__ CUtensorMap map_v) {
     using S = KtShape<CT, HD>;
     constexpr bool I8 = S::I8, PB = I8 || QB;
+    constexpr int LANES = HD / 8;
     constexpr uint32_t S_COL = 0, O_COL = 256;                   // tensor memory: S0 S1 O0 O1, 128 columns each; P over S
     // Probabilities carry a factor of 2^BIAS, so that small ones are normal numbers: f16 at most 2^(7 + KT_RAISE); f32 and bf16 have room (2^95 for a V).
     constexpr float BIAS = PB ? 24.0f : 7.0f;
     extern __shared__ __align__(1024) uint8_t kt_smem[];
     __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[I8 ? S::RAWS : 1], raw_empty[I8 ? S::RAWS : 1],
-        sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+        sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
     __shared__ int64_t scratch[KT_THREADS / 32 + 2];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
@@ -247,11 +261,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < S::SLOTS; i++) { kv_bar_init(&full[i], I8 ? 4 : 1); kv_bar_init(&empty[i], I8 ? 1 : 5); kv_bar_init(&ready[i], 4); }
+        for (int i = 0; i < S::SLOTS; i++) { kv_bar_init(&full[i], I8 ? 4 : 1); kv_bar_init(&empty[i], I8 ? 2 : 6); kv_bar_init(&ready[i], 4); }
         for (int i = 0; i < (I8 ? S::RAWS : 1); i++) { kv_bar_init(&raw_full[i], 1); kv_bar_init(&raw_empty[i], 4); }
         for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 1); kv_bar_init(&sc_empty[i], 8); }
-        for (int i = 0; i < 2; i++) { kv_bar_init(&q_full[i], 128); kv_bar_init(&s_full[i], 1); kv_bar_init(&p_full[i], 4); kv_bar_init(&o_full[i], 1); }
-        kv_bar_init(&drained, 1);
+        for (int i = 0; i < 2; i++) {
+            kv_bar_init(&q_full[i], 128); kv_bar_init(&drained[i], 1);
+            for (int h = 0; h < 2; h++) { kv_bar_init(&s_full[i][h], 1); kv_bar_init(&p_full[i][h], 4); kv_bar_init(&pv_done[i][h], 1); }
+        }
         for (int i = 0; i < 8; i++) odd[i] = 0;
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -268,37 +284,46 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     fence_after();
     const uint32_t tmem = tmem_s;
     KtWalk walk(P, lim, spot);
-    KvWait wait{&failed};
+    const KvWait wait{&failed};
 
-    if (warp < 8) {
+    if (warp >= KT_ROW_WARP && warp < KT_HELP_WARP) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ================= softmax: a row a thread ============================================================================
-        const int i = warp >> 2, row = 128 * i + (tid & 127);
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + S_COL + 128 * i, o_at = tmem + lanes + O_COL + 128 * i;
-        uint32_t s_ph = 0, o_ph = 0, sc = 0, sc_ph = 0;
+        const int i = (warp - KT_ROW_WARP) >> 2, row = 128 * i + (tid & 127);
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_row = tmem + lanes + S_COL + 128 * i, o_at = tmem + lanes + O_COL + 128 * i;
+        uint32_t s_ph = 0, sc = 0, sc_ph = 0;
         while (walk.next(P, lim)) {
             const KvView<KT_TILE> mine = walk.part(P, i);
-            const bool there = row < walk.rows;
-            const int tok = min(row, walk.rows - 1) / P.group, head = walk.head * P.group + (there ? row - tok * P.group : 0);
+            const int tok = min(row, walk.rows - 1) / P.group;
             const int pos = walk.view.lo_pos + tok;
-            const int64_t at = walk.k.s.row0 + walk.block * walk.k.tokens + tok;
-            int first = walk.t0;
-            while (first < walk.t1 && !mine.any(walk.view.base(first), KT_TILE, P.window, P.sinks)) first++;
-            if (first < walk.t1) {  // Q, swizzled as the products want it; rows that there are not: zeros
+            auto any = [&](int base) { return mine.any(base, KT_TILE, P.window, P.sinks); };
+            uint32_t some = 0;
+            for (int t = walk.t0; t < walk.t1 && !some; t += 32) some = walk.bits(t, any);
+            if (some) {  // Q, swizzled as the products want it, HD / 8 threads a row; rows that there are not: zeros
                 uint8_t* to = sq + i * S::SLOT;
-                const char* from = P.q.data + 2 * (at * P.q.row_stride + (int64_t)head * P.q.head_stride);
+                const int c = tid % LANES;
+                const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
 #pragma unroll 8
-                for (int c = 0; c < HD / 8; c++)
-                    *reinterpret_cast<uint4*>(to + kt_offset(tid & 127, c)) = there ? *reinterpret_cast<const uint4*>(from + 16 * c) : make_uint4(0, 0, 0, 0);
+                for (int r = (tid & 127) / LANES; r < 128; r += 128 / LANES) {
+                    const int f = 128 * i + r, k = f / P.group;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (f < walk.rows)
+                        x = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((block_at + k) * P.q.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.q.head_stride + 8 * c));
+                    *reinterpret_cast<uint4*>(to + kt_offset(r, c)) = x;
+                }
                 fence_async();
                 kv_bar_arrive(&q_full[i]);
             }
             float m = -INFINITY, l = 0.0f;
-            bool started = false;
+            int seen = 0;      // halves of tiles seen
+            uint32_t on = 0, all = 0;  // by tile of positions: seen by some row; by every row
 #pragma unroll 1
-            for (int t = walk.t0; t < walk.t1; t++) {
-                const int base = walk.view.base(t);
-                if (!mine.any(base, KT_TILE, P.window, P.sinks)) {
+            for (int t = walk.t0; t < walk.t1; t++, on >>= 1, all >>= 1) {
+                if ((t - walk.t0) % 32 == 0) {
+                    on = walk.bits(t, any);
+                    all = walk.bits(t, [&](int base) { return mine.whole(base, P.window, P.sinks); });
+                }
+                if (!(on & 1u)) {
                     if constexpr (I8) {
                         wait(&sc_full[sc], sc_ph);
                         __syncwarp();
@@ -307,100 +332,108 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     }
                     continue;
                 }
-                const bool whole = mine.whole(base, P.window, P.sinks);
-                uint32_t x[128];
-                wait(&s_full[i], s_ph);
-                s_ph ^= 1u;
-                __syncwarp();
-                fence_after();
+                const bool whole = all & 1u;
+                if constexpr (I8) wait(&sc_full[sc], sc_ph);
+#pragma unroll 1
+                for (int h = 0; h < 2; h++, seen++) {
+                    const float* ks = scales + sc * 2 * KT_TILE + KT_SUB * h;
+                    const uint32_t s_at = s_row + KT_SUB * h;
+                    uint32_t x[KT_SUB];
+                    wait(&s_full[i][h], s_ph);
+                    __syncwarp();
+                    fence_after();
+                    tmem_ld32(x, s_at);
+                    tmem_ld32(x + 32, s_at + 32);
+                    wait_ld();
+                    if constexpr (I8) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32(x + 32 * c, s_at + 32 * c);
-                wait_ld();
-                const float* ks = scales + sc * 2 * KT_TILE;
-                if constexpr (I8) {
-                    wait(&sc_full[sc], sc_ph);
-#pragma unroll
-                    for (int j = 0; j < 128; j += 4) {
-                        const float4 k = *reinterpret_cast<const float4*>(ks + j);
-                        x[j] = __float_as_uint(__uint_as_float(x[j]) * k.x);
-                        x[j + 1] = __float_as_uint(__uint_as_float(x[j + 1]) * k.y);
-                        x[j + 2] = __float_as_uint(__uint_as_float(x[j + 2]) * k.z);
-                        x[j + 3] = __float_as_uint(__uint_as_float(x[j + 3]) * k.w);
-                    }
-                }
-                if (!whole) {
-                    const int hi = pos - base, lo = P.window ? pos - P.window - base : -1, sinks = P.sinks - base;  // seen: j <= hi and (j > lo or j < sinks)
-#pragma unroll
-                    for (int j = 0; j < 128; j++)
-                        if (!(j <= hi && (j > lo || j < sinks))) x[j] = 0xff800000u;
-                }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < 128; j += 8)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c])));
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale_log2 - BIAS;
-                if (__any_sync(0xffffffffu, most > m + KT_RAISE)) {
-                    const float m1 = fmaxf(m, most);
-                    const KvScale f(m1 == -INFINITY ? 0.0f : m - m1);
-                    m = m1;
-                    l = f(l);
-                    if (started) {  // (the products that wrote O are done: those that wrote S came behind them)
-#pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o, o_at + c);
-                            wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(f(__uint_as_float(o[j])));
-                            tmem_st32(o_at + c, o);
+                        for (int j = 0; j < KT_SUB; j += 4) {
+                            const float4 k = *reinterpret_cast<const float4*>(ks + j);
+                            x[j] = __float_as_uint(__uint_as_float(x[j]) * k.x);
+                            x[j + 1] = __float_as_uint(__uint_as_float(x[j + 1]) * k.y);
+                            x[j + 2] = __float_as_uint(__uint_as_float(x[j + 2]) * k.z);
+                            x[j + 3] = __float_as_uint(__uint_as_float(x[j + 3]) * k.w);
                         }
                     }
-                }
-                started = true;
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
-                unsigned long long sum[2] = {0ull, 0ull};
+                    if (!whole) {
+                        const int base = walk.view.base(t) + KT_SUB * h;
+                        const int hi = pos - base, lo = P.window ? pos - P.window - base : -1, sinks = P.sinks - base;  // seen: j <= hi and (j > lo or j < sinks)
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t p16[16];
+                        for (int j = 0; j < KT_SUB; j++)
+                            if (!(j <= hi && (j > lo || j < sinks))) x[j] = 0xff800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 e = unpair(fma2(pair(__uint_as_float(x[c + j]), __uint_as_float(x[c + j + 1])), f2, r2));
+                    for (int j = 0; j < KT_SUB; j += 8)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c])));
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale_log2 - BIAS;
+                    const bool raise = most > m + KT_RAISE;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float m1 = raise ? most : m;  // (a row's result does not depend on the others of its warp)
+                        const KvScale f(m1 == -INFINITY ? 0.0f : m - m1);
+                        m = m1;
+                        l = f(l);
+                        if (seen) {  // O is this thread's when the product in front has written it
+                            wait(&pv_done[i][h ^ 1], h ? s_ph : s_ph ^ 1u);
+                            __syncwarp();
+                            fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(o, o_at + c);
+                                wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; j++) o[j] = __float_as_uint(f(__uint_as_float(o[j])));
+                                tmem_st16(o_at + c, o);
+                            }
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
+                    unsigned long long sum[2] = {0ull, 0ull};
+                    uint32_t p16[KT_SUB / 2];
+#pragma unroll
+                    for (int j = 0; j < KT_SUB; j += 2) {
+                        const float2 e = unpair(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, r2));
                         float2 p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
                         sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(p.x, p.y));
                         if constexpr (I8) {
-                            const float2 v = *reinterpret_cast<const float2*>(ks + KT_TILE + c + j);
+                            const float2 v = *reinterpret_cast<const float2*>(ks + KT_TILE + j);
                             if (whole) p = make_float2(p.x * v.x, p.y * v.y);
                             else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
                         }
                         p16[j / 2] = pack16<PB>(p.x, p.y);
                     }
-                    tmem_st16(s_at + c / 2, p16);
+                    tmem_st32(s_at, p16);
+                    const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
+                    l += (s0.x + s0.y) + (s1.x + s1.y);
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) kv_bar_arrive(&p_full[i][h]);
                 }
-                const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
-                l += (s0.x + s0.y) + (s1.x + s1.y);
-                wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    kv_bar_arrive(&p_full[i]);
-                    if constexpr (I8) kv_bar_arrive(&sc_empty[sc]);
+                s_ph ^= 1u;
+                if constexpr (I8) {
+                    if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
+                    if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
                 }
-                if constexpr (I8) { if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; } }
             }
             // ---- the result of the piece
             const bool done = walk.t0 == 0 && walk.t1 == walk.view.tiles;
+            const bool started = seen > 0;
             if (started) {
-                wait(&o_full[i], o_ph);
-                o_ph ^= 1u;
+                wait(&pv_done[i][1], s_ph ^ 1u);
                 __syncwarp();
                 fence_after();
             }
             if (128 * i >= walk.rows) continue;  // (whole warps: this tile has no rows)
             const bool fix = !I8 && started && odd[walk.index & 7];
             float* part = kv_part(P.work, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
-            const float inv = pos < 0 ? 0.0f : done ? 1.0f / l : 1.0f;
+            const float inv = done && pos >= 0 ? 1.0f / l : 1.0f;
+            // A whole block's result goes through this tile's room of Q (its products are done), so that rows leave in whole lines.
+            uint8_t* stage = sq + i * S::SLOT;
+            const int wide = P.out.type == L2_F32 ? 4 : 2, cols = HD * 2 / wide;  // bytes of an element, columns at a time
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
@@ -432,122 +465,138 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         }
                     }
                 }
-                if (!there) continue;
-                if (!done) {
+                if (!done) {  // partial results: [4 columns][row][4], so that a warp's rows are side by side
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + row * HD + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * KT_ROWS + row) * 4) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     continue;
                 }
+                float y[32];
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    float y[8];
+                for (int j = 0; j < 32; j++) y[j] = pos < 0 ? 0.0f : __uint_as_float(o[j]) * inv;
+                const int in = c % cols;
+                if (wide == 4) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = pos < 0 ? 0.0f : __uint_as_float(o[j + e]) * inv;
-                    kv_store8(P.out, at, head, c + j, y);
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(stage + kt_offset(tid & 127, (in + j) / 4)) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint4 w = QB ? make_uint4(pack16<true>(y[j], y[j + 1]), pack16<true>(y[j + 2], y[j + 3]), pack16<true>(y[j + 4], y[j + 5]), pack16<true>(y[j + 6], y[j + 7]))
+                                     : make_uint4(pack16<false>(y[j], y[j + 1]), pack16<false>(y[j + 2], y[j + 3]), pack16<false>(y[j + 4], y[j + 5]), pack16<false>(y[j + 6], y[j + 7]));
+                        *reinterpret_cast<uint4*>(stage + kt_offset(tid & 127, (in + j) / 8)) = w;
+                    }
                 }
+                if (in + 32 < cols) continue;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
+                const int ch = tid % LANES;
+                for (int r = (tid & 127) / LANES; r < 128; r += 128 / LANES) {
+                    const int f = 128 * i + r, k = f / P.group;
+                    if (f >= walk.rows) break;
+                    const int64_t e = (block_at + k) * P.out.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.out.head_stride + (c + 32 - cols);
+                    *reinterpret_cast<uint4*>(P.out.data + e * wide + 16 * ch) = *reinterpret_cast<const uint4*>(stage + kt_offset(r, ch));
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
             }
-            if (!done && there) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
+            if (!done) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
             fence_before();
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == KT_MMA_WARP) {
-            // ================= products ========================================================================================
+        if (warp == KT_MMA_WARP || warp == KT_MMA_WARP + 2) {
+            // ================= products of one tile of rows =====================================================================
+            // (All of the tensor memory is this CTA's: it starts at 0.  The operands are uniform registers: the whole warp walks, one elected lane issues.)
+            const int i = warp == KT_MMA_WARP ? 0 : 1;
             const bool leader = elect();
             constexpr uint32_t fmt = QB ? 1u : 0u, fmt_p = PB ? 1u : 0u;
-            constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (((uint32_t)KT_SUB >> 3) << 17) | ((128u >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | (fmt_p << 7) | (fmt_p << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);  // V: elements contiguous
-            const uint32_t q_lo = desc_lo(kv_smem(sq), 1), k_lo = desc_lo(kv_smem(ring), 1), v_lo = desc_lo(kv_smem(ring), KT_TILE * 128 / 16);
-            uint32_t slot = 0, ph = 0, ready_ph = 0, q_ph = 0, p_ph = 0;  // q_ph, p_ph: a bit for each tile; ready_ph: one for each slot
+            const uint32_t s_col = S_COL + 128 * i, o_col = O_COL + 128 * i, q_lo = desc_lo(kv_smem(sq + i * S::SLOT), 1), k_lo = desc_lo(kv_smem(ring), 1),
+                           v_lo = desc_lo(kv_smem(ring), KT_TILE * 128 / 16);
+            uint32_t slot = 0, ph = 0, ready_ph = 0, q_ph = 0, p_ph = 0;  // ready_ph: a bit for each slot
             auto step = [&]() { if (++slot == S::SLOTS) { slot = 0; ph ^= 1u; } };
-            while (walk.next(P, lim)) {
-                const KvView<KT_TILE> see[2] = {walk.part(P, 0), walk.part(P, 1)};
-                uint32_t begun = 0;  // tiles whose Q has been waited for, and (bits 2, 3) whose O has been written
-                // S of tile i from the K tile in the current slot
-                auto scores = [&](int i) {
-                    if (!(begun & (1u << i))) { wait(&q_full[i], (q_ph >> i) & 1u); q_ph ^= 1u << i; begun |= 1u << i; }
-                    wait(&full[slot], ph);
+            while (__any_sync(0xffffffffu, walk.next(P, lim))) {
+                const KvView<KT_TILE> mine = walk.part(P, i), other = walk.part(P, i ^ 1);
+                auto any = [&](int base) { return mine.any(base, KT_TILE, P.window, P.sinks); };
+                const int t0 = __reduce_max_sync(0xffffffffu, walk.t0), t1 = __reduce_max_sync(0xffffffffu, walk.t1);
+                uint32_t begun = 0;  // S has been computed (1), O has been written (2)
+                auto scores = [&](int h) {  // S of half a tile, from the K tile in the current slot
+                    if (!(begun & 1u)) { wait(&q_full[i], q_ph); q_ph ^= 1u; begun |= 1u; }
                     __syncwarp();
                     fence_after();
-                    if (leader && !wait.dead) {
+                    const uint32_t k_at = k_lo + slot * (S::SLOT / 16) + h * (KT_SUB * 128 / 16), d = s_col + KT_SUB * h;
+                    if (leader) {
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++) {
                             const uint32_t off = (k / 4) * (KT_TILE * 128 / 16) + (k % 4) * 2;
-                            mma_ss(tmem + S_COL + 128 * i, q_lo + i * (S::SLOT / 16) + off, k_lo + slot * (S::SLOT / 16) + off, idesc_s, k > 0);
+                            if (k == 0) mma_ss<false>(d, q_lo + off, k_at + off, idesc_s);
+                            else mma_ss<true>(d, q_lo + off, k_at + off, idesc_s);
                         }
-                        commit(&s_full[i]);
+                        commit(&s_full[i][h]);
                     }
                     __syncwarp();
                 };
-                auto active = [&](int i, int t) { return see[i].any(walk.view.base(t), KT_TILE, P.window, P.sinks); };
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    if (active(i, walk.t0)) scores(i);
-                wait(&full[slot], ph);  // (a slot is given back only when it has been filled)
+                uint32_t on = walk.bits(t0, any);
+                wait(&full[slot], ph);
+                if (on & 1u) { scores(0); scores(1); }
                 if (leader) commit(&empty[slot]);
                 __syncwarp();
                 step();
 #pragma unroll 1
-                for (int t = walk.t0; t < walk.t1; t++) {
-                    const int base = walk.view.base(t);
-                    const uint32_t v_slot = slot, v_ph = ph;
-                    step();
-                    const bool more = t + 1 < walk.t1;
-                    bool part = false;
-                    if constexpr (!I8)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) part |= active(i, t) && !see[i].whole(base, P.window, P.sinks);
-                    bool v_here = false;
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        if (active(i, t)) {
-                            if (!v_here) {
-                                wait(&full[v_slot], v_ph);
-                                if (part) { wait(&ready[v_slot], (ready_ph >> v_slot) & 1u); ready_ph ^= 1u << v_slot; }
-                                v_here = true;
-                            }
-                            wait(&p_full[i], (p_ph >> i) & 1u);
-                            p_ph ^= 1u << i;
-                            __syncwarp();
-                            fence_after();
-                            if (leader && !wait.dead) {
-#pragma unroll
-                                for (int k = 0; k < KT_TILE / 16; k++)
-                                    mma_ts(tmem + O_COL + 128 * i, tmem + S_COL + 128 * i + 8 * k, v_lo + v_slot * (S::SLOT / 16) + k * (16 * 128 / 16), idesc_o, k > 0 || (begun & (4u << i)));
-                            }
-                            begun |= 4u << i;
-                            __syncwarp();
-                        }
-                        if (i == 1) {
-                            if (!v_here) wait(&full[v_slot], v_ph);
-                            if (leader) commit(&empty[v_slot]);
-                            __syncwarp();
-                        }
-                        if (more && active(i, t + 1)) scores(i);
-                    }
-                    if (more) {
-                        wait(&full[slot], ph);
-                        if (leader) commit(&empty[slot]);
-                        __syncwarp();
+                for (int tc = t0; tc < t1; tc += 32) {
+                    const uint32_t part = I8 ? 0u : walk.bits(tc, [&](int base) {
+                        return (any(base) && !mine.whole(base, P.window, P.sinks)) || (other.any(base, KT_TILE, P.window, P.sinks) && !other.whole(base, P.window, P.sinks)); });
+                    on = walk.bits(tc, any);
+                    const uint32_t next = walk.bits(tc + 1, any);
+                    const int n = min(32, t1 - tc);
+#pragma unroll 1
+                    for (int b = 0; b < n; b++) {
+                        const uint32_t v_slot = slot, v_ph = ph;
                         step();
+                        const bool more = tc + b + 1 < t1;
+                        wait(&full[v_slot], v_ph);
+                        if (part >> b & 1u) { wait(&ready[v_slot], ready_ph >> v_slot & 1u); ready_ph ^= 1u << v_slot; }
+                        if (more) wait(&full[slot], ph);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            if (on >> b & 1u) {
+                                wait(&p_full[i][h], p_ph);
+                                __syncwarp();
+                                fence_after();
+                                const uint32_t v_at = v_lo + v_slot * (S::SLOT / 16) + h * (KT_SUB * 128 / 16), a = s_col + KT_SUB * h;
+                                if (leader) {
+                                    if (begun & 2u) mma_ts<true>(o_col, a, v_at, idesc_o);
+                                    else mma_ts<false>(o_col, a, v_at, idesc_o);
+#pragma unroll
+                                    for (int k = 1; k < KT_SUB / 16; k++) mma_ts<true>(o_col, a + 8 * k, v_at + k * (16 * 128 / 16), idesc_o);
+                                    commit(&pv_done[i][h]);
+                                }
+                                begun |= 2u;
+                                __syncwarp();
+                            }
+                            if (next >> b & 1u) scores(h);
+                        }
+                        p_ph ^= on >> b & 1u;
+                        if (leader) {
+                            commit(&empty[v_slot]);
+                            if (more) commit(&empty[slot]);
+                        }
+                        __syncwarp();
+                        if (more) step();
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    if ((begun & (1u << i)) && leader) commit(&o_full[i]);
-                __syncwarp();
             }
             if (failed) {  // products still under way read shared memory: a bounded time to end
-                if (leader) commit(&drained);
+                if (leader) commit(&drained[i]);
                 __syncwarp();
-                for (int i = 0; i < 1024 && !kv_bar_try(&drained, 0); i++) {}
+                for (int n = 0; n < 1024 && !kv_bar_try(&drained[i], 0); n++) {}
             }
         } else if (warp == KT_COPY_WARP) {
             // ================= copies: lane l brings run l of a tile ==============================================================
             const int R = min(KT_TILE, 1 << P.pool.page_shift), runs = KT_TILE / R;
             constexpr int RB = HD * (I8 ? 1 : 2), W = RB < 128 ? RB : 128;  // bytes of a row, of a copy's row
             uint32_t slot = 0, ph = 1, sc = 0, sc_ph = 1;
-            while (walk.next(P, lim) && !wait.dead) {
+            bool over = false;
+            while (!over && walk.next(P, lim)) {
                 auto page_of = [&](int t) {  // the page of this lane's run of tile t, n_pages (zeros) where no row sees it or there is none
                     const int j = walk.view.base(t) + lane * R;
                     if (lane >= runs || !walk.view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
@@ -560,7 +609,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     const int ahead = t + 1 < walk.t1 ? page_of(t + 1) : P.pool.n_pages;
                     if constexpr (I8) {
                         wait(&sc_empty[sc], sc_ph);
-                        if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                        if ((over = wait.over())) break;
                         float* s = scales + sc * 2 * KT_TILE + lane * R;
                         const bool there = lane < runs && page < P.pool.n_pages;
                         if (lane < runs && !there)
@@ -580,7 +629,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     for (int kv = 0; kv < 2; kv++) {
                         uint64_t *f = I8 ? &raw_full[slot] : &full[slot], *e = I8 ? &raw_empty[slot] : &empty[slot];
                         wait(e, ph);
-                        if (__any_sync(0xffffffffu, wait.dead)) { wait.dead = true; break; }
+                        if ((over = wait.over())) break;
                         if (lane == 0) kv_bar_expect(f, KT_TILE * RB);
                         __syncwarp();
                         if (lane < runs) {
@@ -590,7 +639,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         }
                         if (++slot == (I8 ? S::RAWS : S::SLOTS)) { slot = 0; ph ^= 1u; }
                     }
-                    if (wait.dead) break;
+                    if (over) break;
                     page = ahead;
                 }
             }
@@ -713,7 +762,7 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
             const float* p = piece(i);
             const float2 ml = *reinterpret_cast<const float2*>(p + KT_ROWS * HD + 2 * r);
             const KvScale f(ml.x - ref);
-            const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
+            const float4 x = *reinterpret_cast<const float4*>(p + (d / 4 * KT_ROWS + r) * 4);
             sum += f(ml.y);
             acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
         }
