@@ -309,6 +309,7 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     P.scale_log2 = scale * 1.4426950408889634f;
     P.window = window; P.sinks = window ? sinks : 0;
     P.group = q->heads / pages->n_kv_heads;
+    P.group_inv = (65536 + P.group - 1) / P.group;
     P.work = workspace;
     L2_CUDA(launch_kv_attend(P, pages->type, pages->head_size, sms, static_cast<cudaStream_t>(cuda_stream)));
     return L2_OK;

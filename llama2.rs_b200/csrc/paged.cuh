@@ -35,6 +35,7 @@ struct KvAttendParams {
     float scale_log2;   // scale * log2(e): scores in powers of two
     int window, sinks;  // window 0: all
     int group;          // query heads per kv head
+    int group_inv;      // 2^16 / group, rounded up
     void* work;
 };
 

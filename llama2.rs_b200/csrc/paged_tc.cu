@@ -184,6 +184,9 @@ __device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBl
     return k.n - 1;
 }
 
+// row / group for the rows of a block: exact for rows below 256, groups up to 64 (the error of the rounded-up reciprocal stays below 1 / group)
+__device__ __forceinline__ int kt_token(const KvAttendParams& P, int row) { return row * P.group_inv >> 16; }
+
 struct KtWalk {
     int64_t w, w1;
     int b, head, block, skip;  // skip: tiles of the first block that belong to the CTA in front
@@ -232,8 +235,8 @@ struct KtWalk {
     __device__ __forceinline__ KvView<KT_TILE> part(const KvAttendParams& P, int i) const {
         KvView<KT_TILE> v = view;
         const int lo = 128 * i, hi = min(rows, lo + 128) - 1;
-        v.lo_pos = view.lo_pos + lo / P.group;
-        v.hi_pos = hi < lo ? -1 : view.lo_pos + hi / P.group;
+        v.lo_pos = view.lo_pos + kt_token(P, lo);
+        v.hi_pos = hi < lo ? -1 : view.lo_pos + kt_token(P, hi);
         return v;
     }
 };
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         uint32_t s_ph = 0, sc = 0, sc_ph = 0;
         while (walk.next(P, lim)) {
             const KvView<KT_TILE> mine = walk.part(P, i);
-            const int tok = min(row, walk.rows - 1) / P.group;
+            const int tok = kt_token(P, min(row, walk.rows - 1));
             const int pos = walk.view.lo_pos + tok;
             auto any = [&](int base) { return mine.any(base, KT_TILE, P.window, P.sinks); };
             uint32_t some = 0;
@@ -303,13 +306,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 uint8_t* to = sq + i * S::SLOT;
                 const int c = tid % LANES;
                 const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
-#pragma unroll 8
-                for (int r = (tid & 127) / LANES; r < 128; r += 128 / LANES) {
-                    const int f = 128 * i + r, k = f / P.group;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (f < walk.rows)
-                        x = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((block_at + k) * P.q.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.q.head_stride + 8 * c));
-                    *reinterpret_cast<uint4*>(to + kt_offset(r, c)) = x;
+                constexpr int AT_ONCE = 8, ROWS_ONCE = 128 / LANES;
+#pragma unroll 1
+                for (int r0 = (tid & 127) / LANES; r0 < 128; r0 += AT_ONCE * ROWS_ONCE) {
+                    uint4 x[AT_ONCE];  // (requested together: the compiler keeps a load behind the store in front of it)
+#pragma unroll
+                    for (int n = 0; n < AT_ONCE; n++) {
+                        const int f = 128 * i + r0 + n * ROWS_ONCE, k = kt_token(P, f);
+                        x[n] = make_uint4(0, 0, 0, 0);
+                        if (f < walk.rows)
+                            x[n] = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((block_at + k) * P.q.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.q.head_stride + 8 * c));
+                    }
+#pragma unroll
+                    for (int n = 0; n < AT_ONCE; n++) *reinterpret_cast<uint4*>(to + kt_offset(r0 + n * ROWS_ONCE, c)) = x[n];
                 }
                 fence_async();
                 kv_bar_arrive(&q_full[i]);
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
                 const int ch = tid % LANES;
                 for (int r = (tid & 127) / LANES; r < 128; r += 128 / LANES) {
-                    const int f = 128 * i + r, k = f / P.group;
+                    const int f = 128 * i + r, k = kt_token(P, f);
                     if (f >= walk.rows) break;
                     const int64_t e = (block_at + k) * P.out.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.out.head_stride + (c + 32 - cols);
                     *reinterpret_cast<uint4*>(P.out.data + e * wide + 16 * ch) = *reinterpret_cast<const uint4*>(stage + kt_offset(r, ch));
