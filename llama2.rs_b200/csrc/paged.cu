@@ -12,13 +12,14 @@
 #include "host_common.h"
 #include "kernels.cuh"
 #include "model.h"
-#include "paged.cuh"
+#include "paged_attend.h"
 
 namespace l2 {
 
 namespace {
 
-constexpr int KV_THREADS = 256;
+constexpr int KV_THREADS = 256, KV_WARPS = KV_THREADS / 32, KV_MAX_ROWS = 16;
+constexpr int KV_AT_ONCE = 4;  // heads that a group of threads has under way
 
 struct KvCopyParams {
     KvPool pool;
@@ -26,102 +27,207 @@ struct KvCopyParams {
     KvRows k, v, q, q_out;
     const float* cos; const float* sin;
     int rope_len;
+    int rows;  // of a CTA
 };
 
-// One row a CTA (blockIdx.y strides over the rows), LANES = hd / 8 threads for a head, 8 elements each.
+// Where a row's position is; by one warp a row, the rows of a CTA side by side: three or four loads that depend on one another, once a row.
+struct KvPlace { int64_t at, scale; int pos; bool there, page; };  // elements of the pool, of the scales; there: a row of a sequence; page: it has one
+__device__ __forceinline__ KvPlace kv_place(const KvCopyParams& P, int r) {
+    KvPlace w{0, 0, 0, false, false};
+    if (r >= P.step.n_rows) return w;
+    const int b = kv_find_seq(P.step, r);
+    const KvSeq s = kv_seq(P.step, P.pool.page_shift, b);
+    w.pos = s.kv - s.n + (r - s.row0);
+    w.there = r >= s.row0 && r < s.row0 + s.n && w.pos >= 0;
+    if (w.there && P.cos && w.pos >= P.rope_len) { kv_report(P.step.status, L2_KV_BAD_ROPE); w.there = false; }
+    if (!w.there) return w;
+    const int page = kv_page(P.step, P.pool, b, w.pos), in = w.pos & ((1 << P.pool.page_shift) - 1);
+    w.page = page >= 0;
+    w.at = (int64_t)page * P.pool.page_stride + in * P.pool.pos_stride;
+    w.scale = ((int64_t)page * P.pool.n_kv_heads << P.pool.page_shift) + in;
+    return w;
+}
+__device__ __forceinline__ void kv_places(const KvCopyParams& P, int r0, KvPlace* place) {
+    for (int i = threadIdx.x >> 5; i < P.rows; i += KV_WARPS) {
+        const KvPlace w = kv_place(P, r0 + i);
+        if ((threadIdx.x & 31) == 0) place[i] = w;
+    }
+    __syncthreads();
+}
+
+// The N elements of a thread as they lie in memory, as f32, and back (8 at a time).
+template <int T, int N> struct KvRaw { uint4 w[N * (T == L2_F32 ? 4 : 2) / 16]; };
+template <int T, int N>
+__device__ __forceinline__ KvRaw<T, N> load_raw(const char* base, int64_t e) {
+    KvRaw<T, N> r;
+    const uint4* p = reinterpret_cast<const uint4*>(base + e * (T == L2_F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(r.w) / 16); i++) r.w[i] = p[i];
+    return r;
+}
+template <int T, int N>
+__device__ __forceinline__ void to_f32(const KvRaw<T, N>& r, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+        if constexpr (T == L2_F32) x[i] = __uint_as_float(w[i]);
+        else if constexpr (T == L2_F16) x[i] = __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i % 2)))));
+        else x[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+}
+template <int T, int N>
+__device__ __forceinline__ void store_n(char* base, int64_t e, const float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[i + j];
+        if constexpr (T == L2_F32) kv_store8(reinterpret_cast<float*>(base) + e + i, y);
+        else if constexpr (T == L2_F16) kv_store8(reinterpret_cast<__half*>(base) + e + i, y);
+        else kv_store8(reinterpret_cast<__nv_bfloat16*>(base) + e + i, y);
+    }
+}
+
+// A CTA has a few rows (blockIdx.y) of k, v or q (blockIdx.x modulo their number), or a part of one row's heads.  HD / N threads have a head, N elements each: 16 bytes of the cache.
+// Every group requests the next KV_AT_ONCE heads together; nothing is used twice, so bytes under way are what counts.
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_constant__ KvCopyParams P) {
-    constexpr int LANES = HD / 8, GROUPS = KV_THREADS / LANES;
-    const int sub = threadIdx.x % LANES, grp = threadIdx.x / LANES, d = 8 * sub, half = HD / 2;
-    const int kvh = P.pool.n_kv_heads, units = 2 * kvh + (P.q.data ? P.q.heads : 0);
-    for (int r = blockIdx.y; r < P.step.n_rows; r += gridDim.y) {
-        const int b = kv_find_seq(P.step, r);
-        const KvSeq s = kv_seq(P.step, P.pool.page_shift, b);
-        const int pos = s.kv - s.n + (r - s.row0);
-        if (r < s.row0 || r >= s.row0 + s.n || pos < 0) continue;
-        if (P.cos && pos >= P.rope_len) { kv_report(P.step.status, L2_KV_BAD_ROPE); continue; }
-        const int page = kv_page(P.step, P.pool, b, pos), at = pos & ((1 << P.pool.page_shift) - 1);
-        for (int u0 = blockIdx.x * GROUPS; u0 < units; u0 += gridDim.x * GROUPS) {  // (whole warps stay together for the shuffles)
-            const int u = min(u0 + grp, units - 1);
-            const bool mine = u0 + grp < units;
-            const int what = u < kvh ? 0 : u < 2 * kvh ? 1 : 2, head = u - what * kvh;
-            float x[8];
-            kv_load8(what == 0 ? P.k : what == 1 ? P.v : P.q, r, head, d, x);
-            if (P.cos) {  // products and their sum are rounded one by one, as written
-                float y[8];
+    constexpr bool I8 = T == L2_I8;
+    constexpr int N = I8 ? 16 : 8, LANES = HD / N, GROUPS = KV_THREADS / LANES, HALF = HD / 2;
+    __shared__ KvPlace place[KV_MAX_ROWS];
+    const int sub = threadIdx.x % LANES, grp = threadIdx.x / LANES, d = N * sub;
+    const int arrays = P.q.data ? 3 : 2, what = blockIdx.x % arrays, part = blockIdx.x / arrays, parts = gridDim.x / arrays;  // what: 0 k, 1 v, 2 q
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int r0 = blockIdx.y * P.rows; r0 < P.step.n_rows; r0 += gridDim.y * P.rows) {
+        kv_places(P, r0, place);
+        auto heads_of = [&](const KvRows& from, auto type) {
+            constexpr int IN = decltype(type)::value;
+            const int heads = from.heads, units = P.rows * heads;
+            const bool turn = P.cos && what != 1;
+#pragma unroll 1
+            for (int u0 = part * GROUPS; u0 < units; u0 += parts * GROUPS * KV_AT_ONCE) {  // (whole warps stay together for the shuffles)
+                KvRaw<IN, N> raw[KV_AT_ONCE];
+                int row[KV_AT_ONCE], head[KV_AT_ONCE];
+                bool mine[KV_AT_ONCE];
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = __shfl_xor_sync(0xffffffffu, x[i], LANES / 2);
-                if (what != 1) {
-                    const int e = d & (half - 1);
-                    float c[8], w[8];
-                    kv_load8(P.cos + (size_t)pos * half + e, c);
-                    kv_load8(P.sin + (size_t)pos * half + e, w);
+                for (int a = 0; a < KV_AT_ONCE; a++) {
+                    const int u = u0 + a * parts * GROUPS + grp;
+                    row[a] = u / heads;
+                    head[a] = u - row[a] * heads;
+                    mine[a] = u < units && place[row[a]].there;
+                    raw[a] = {};
+                    if (mine[a]) raw[a] = load_raw<IN, N>(from.data, (int64_t)(r0 + row[a]) * from.row_stride + head[a] * from.head_stride + d);
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        x[i] = d < half ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], w[i])) : __fadd_rn(__fmul_rn(y[i], w[i]), __fmul_rn(x[i], c[i]));
+                for (int a = 0; a < KV_AT_ONCE; a++) {
+                    if (u0 + a * parts * GROUPS >= units) break;  // (whole CTAs)
+                    const KvPlace w = mine[a] ? place[row[a]] : KvPlace{0, 0, 0, false, false};
+                    float x[N];
+                    to_f32(raw[a], x);
+                    if (turn) {  // products and their sum are rounded one by one, as written
+                        float y[N], c[N], s[N];
+#pragma unroll
+                        for (int i = 0; i < N; i++) y[i] = __shfl_xor_sync(0xffffffffu, x[i], LANES / 2);
+                        const int64_t e = (int64_t)w.pos * HALF + (d & (HALF - 1));
+                        to_f32(load_raw<L2_F32, N>(reinterpret_cast<const char*>(P.cos), e), c);
+                        to_f32(load_raw<L2_F32, N>(reinterpret_cast<const char*>(P.sin), e), s);
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            x[i] = d < HALF ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i])) : __fadd_rn(__fmul_rn(y[i], s[i]), __fmul_rn(x[i], c[i]));
+                    }
+                    if (what == 2) {
+                        if (!mine[a]) continue;
+                        const int64_t e = (int64_t)(r0 + row[a]) * P.q_out.row_stride + head[a] * P.q_out.head_stride + d;
+                        if (P.q_out.type == L2_F32) store_n<L2_F32, N>(P.q_out.data, e, x);
+                        else if (P.q_out.type == L2_F16) store_n<L2_F16, N>(P.q_out.data, e, x);
+                        else store_n<L2_BF16, N>(P.q_out.data, e, x);
+                        continue;
+                    }
+                    const int64_t e = w.at + head[a] * P.pool.head_stride + d;
+                    char* to = what == 1 ? P.pool.v : P.pool.k;
+                    if constexpr (I8) {
+                        // the row's largest magnitude, as bits: of non-negative floats the order of the bits is that of the values, NaN above all
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int i = 0; i < N; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+                        for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        const float m = __uint_as_float(most);
+                        const bool finite = most < 0x7f800000u, zero = m < 0x1p-100f;
+                        const float inv = finite && !zero ? __fmul_rn(__frcp_rn(m), 127.0f) : 0.0f;
+                        // (|x| inv is at most 127 and a few units in the last place.  Added to 1.5 x 2^23 it is rounded to a whole number, to nearest even, whose
+                        // two's complement is the low byte: a conversion instruction takes four times as long.)
+                        uint32_t b[N];
+#pragma unroll
+                        for (int i = 0; i < N; i++) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(finite ? x[i] : 0.0f, inv), 12582912.0f));
+#pragma unroll
+                        for (int i = 0; i < N; i += 4) b[i / 4] = __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
+                        if (!w.page) continue;
+                        *reinterpret_cast<uint4*>(to + e) = make_uint4(b[0], b[1], b[2], b[3]);
+                        if (sub == 0) (what == 1 ? P.pool.vs : P.pool.ks)[w.scale + ((int64_t)head[a] << P.pool.page_shift)] =
+                            !finite ? __int_as_float(0x7fc00000) : zero ? 0.0f : __fmul_rn(m, 1.0f / 127.0f);
+                    } else if (w.page) {
+                        store_n<T, N>(to, e, x);
+                    }
                 }
             }
-            if (what == 2) {
-                if (mine) kv_store8(P.q_out, r, head, d, x);
-                if constexpr (T != L2_I8) continue;
-            }
-            const int64_t e = (int64_t)page * P.pool.page_stride + at * P.pool.pos_stride + head * P.pool.head_stride + d;
-            char* to = what == 1 ? P.pool.v : P.pool.k;
-            if constexpr (T == L2_I8) {
-                // the row's largest magnitude, as bits: of non-negative floats the order of the bits is that of the values, NaN above all
-                uint32_t most = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-                for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float a = __uint_as_float(most);
-                const bool finite = most < 0x7f800000u, zero = a < 0x1p-100f;
-                const float inv = finite && !zero ? __fmul_rn(__frcp_rn(a), 127.0f) : 0.0f;
-                uint32_t w[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int v = finite ? max(-127, min(127, __float2int_rn(__fmul_rn(x[i], inv)))) : 0;
-                    w[i / 4] |= (uint32_t)(v & 255) << (8 * (i % 4));
-                }
-                if (!mine || page < 0 || what == 2) continue;
-                *reinterpret_cast<uint2*>(to + e) = make_uint2(w[0], w[1]);
-                if (sub == 0) (what == 1 ? P.pool.vs : P.pool.ks)[((int64_t)page * kvh + head << P.pool.page_shift) + at] =
-                    !finite ? __int_as_float(0x7fc00000) : zero ? 0.0f : __fmul_rn(a, 1.0f / 127.0f);
-            } else {
-                using E = typename KvElem<T>::type;
-                if (mine && page >= 0) kv_store8(reinterpret_cast<E*>(to) + e, x);
-            }
-        }
+        };
+        const KvRows& from = what == 0 ? P.k : what == 1 ? P.v : P.q;
+        if (from.type == L2_F32) heads_of(from, std::integral_constant<int, L2_F32>());
+        else if (from.type == L2_F16) heads_of(from, std::integral_constant<int, L2_F16>());
+        else heads_of(from, std::integral_constant<int, L2_BF16>());
+        __syncthreads();
     }
 }
 
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvCopyParams P) {
-    constexpr int LANES = HD / 8, GROUPS = KV_THREADS / LANES;
-    const int d = 8 * (threadIdx.x % LANES), grp = threadIdx.x / LANES, kvh = P.pool.n_kv_heads;
-    for (int r = blockIdx.y; r < P.step.n_rows; r += gridDim.y) {
-        const int b = kv_find_seq(P.step, r);
-        const KvSeq s = kv_seq(P.step, P.pool.page_shift, b);
-        const int pos = s.kv - s.n + (r - s.row0);
-        if (r < s.row0 || r >= s.row0 + s.n || pos < 0) continue;
-        const int page = kv_page(P.step, P.pool, b, pos), at = pos & ((1 << P.pool.page_shift) - 1);
-        for (int u = blockIdx.x * GROUPS + grp; u < 2 * kvh; u += gridDim.x * GROUPS) {
-            const int what = u >= kvh, head = u - what * kvh;
-            float x[8] = {};
-            if (page >= 0) {
-                const int64_t e = (int64_t)page * P.pool.page_stride + at * P.pool.pos_stride + head * P.pool.head_stride + d;
-                const char* from = what ? P.pool.v : P.pool.k;
-                if constexpr (T == L2_I8) {
-                    const float f = (what ? P.pool.vs : P.pool.ks)[((int64_t)page * kvh + head << P.pool.page_shift) + at];
-                    kv_load8(reinterpret_cast<const int8_t*>(from) + e, x);
+    constexpr bool I8 = T == L2_I8;
+    constexpr int N = I8 ? 16 : 8, LANES = HD / N, GROUPS = KV_THREADS / LANES;
+    __shared__ KvPlace place[KV_MAX_ROWS];
+    const int d = N * (threadIdx.x % LANES), grp = threadIdx.x / LANES, heads = P.pool.n_kv_heads, units = 2 * P.rows * heads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int r0 = blockIdx.y * P.rows; r0 < P.step.n_rows; r0 += gridDim.y * P.rows) {
+        kv_places(P, r0, place);
+#pragma unroll 1
+        for (int u0 = blockIdx.x * GROUPS + grp; u0 < units; u0 += gridDim.x * GROUPS * KV_AT_ONCE) {
+            uint4 x[KV_AT_ONCE];
+            float f[KV_AT_ONCE];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= f;
-                } else {
-                    kv_load8(reinterpret_cast<const typename KvElem<T>::type*>(from) + e, x);
+            for (int a = 0; a < KV_AT_ONCE; a++) {
+                const int u = u0 + a * gridDim.x * GROUPS, r = u / (2 * heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
+                x[a] = make_uint4(0, 0, 0, 0);
+                f[a] = 0.0f;
+                if (u < units && place[r].page) {
+                    const char* from = h < heads ? P.pool.k : P.pool.v;
+                    x[a] = __ldcs(reinterpret_cast<const uint4*>(from + (place[r].at + head * P.pool.head_stride + d) * (I8 ? 1 : 2)));
+                    if constexpr (I8) f[a] = (h < heads ? P.pool.ks : P.pool.vs)[place[r].scale + ((int64_t)head << P.pool.page_shift)];
                 }
             }
-            kv_store8(what ? P.v : P.k, r, head, d, x);
+#pragma unroll
+            for (int a = 0; a < KV_AT_ONCE; a++) {
+                const int u = u0 + a * gridDim.x * GROUPS, r = u / (2 * heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
+                if (u >= units || !place[r].there) continue;
+                const KvRows& to = h < heads ? P.k : P.v;
+                float y[N];
+                const uint32_t w[4] = {x[a].x, x[a].y, x[a].z, x[a].w};
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    // 2^23 + 128 + byte, less 2^23 + 128: exact, and no conversion instruction
+                    if constexpr (I8) y[i] = (__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (i % 4))) - 8388736.0f) * f[a];
+                    else if constexpr (T == L2_F16) y[i] = __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i % 2)))));
+                    else y[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+                }
+                const int64_t e = (int64_t)(r0 + r) * to.row_stride + head * to.head_stride + d;
+                if (to.type == T) *reinterpret_cast<uint4*>(to.data + 2 * e) = x[a];
+                else if (to.type == L2_F32) store_n<L2_F32, N>(to.data, e, y);
+                else if (to.type == L2_F16) store_n<L2_F16, N>(to.data, e, y);
+                else store_n<L2_BF16, N>(to.data, e, y);
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -198,7 +304,7 @@ int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_
 }
 
 template <class F>
-int by_type(int type, int head_size, F f) {
+cudaError_t by_type(int type, int head_size, F f) {
     if (head_size == 128) {
         if (type == L2_F16) return f(std::integral_constant<int, L2_F16>(), std::integral_constant<int, 128>());
         if (type == L2_BF16) return f(std::integral_constant<int, L2_BF16>(), std::integral_constant<int, 128>());
@@ -209,11 +315,13 @@ int by_type(int type, int head_size, F f) {
     return f(std::integral_constant<int, L2_I8>(), std::integral_constant<int, 64>());
 }
 
-// CTAs of a copy: a row's heads in one CTA where the rows fill the device, spread over several where they do not.
-dim3 copy_grid(int rows, int units, int head_size, int sms) {
-    const int groups = KV_THREADS / (head_size / 8), blocks = (units + groups - 1) / groups;
-    const int x = std::min(blocks, std::max(1, 4 * sms / std::max(1, rows)));
-    return dim3(x, std::min(rows, 65535));
+// Rows of a CTA and CTAs of a copy: as many rows as give every group of threads some KV_AT_ONCE heads, where that leaves four CTAs an SM; a row's heads
+// in several CTAs where the rows alone do not fill the device.
+dim3 copy_grid(KvCopyParams& P, int heads, int arrays, int head_size, int type, int sms) {
+    const int groups = KV_THREADS / (head_size / (type == L2_I8 ? 16 : 8)), n = P.step.n_rows;
+    P.rows = std::max(1, std::min({KV_MAX_ROWS, 2 * KV_AT_ONCE * groups / heads, n * arrays / (4 * sms)}));
+    const int y = (n + P.rows - 1) / P.rows, x = std::min((P.rows * heads + groups - 1) / groups, std::max(1, 4 * sms / (y * arrays)));
+    return dim3(x * arrays, std::min(y, 65535));
 }
 
 }  // namespace
@@ -243,14 +351,10 @@ extern "C" int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
-    const dim3 grid = copy_grid(batch->n_rows, 2 * pages->n_kv_heads + (q ? q->heads : 0), pages->head_size, sms);
-    cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
-        kv_append_kernel<decltype(t)::value, decltype(hd)::value><<<grid, KV_THREADS, 0, st>>>(P);
-        return 0;
-    });
-    g_launches++;
-    L2_CUDA(cudaGetLastError());
+    const dim3 grid = copy_grid(P, std::max(pages->n_kv_heads, q ? q->heads : 0), q ? 3 : 2, pages->head_size, pages->type, sms);
+    L2_CUDA(by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
+        return kv_launch(kv_append_kernel<decltype(t)::value, decltype(hd)::value>, grid, KV_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), P);
+    }));
     return L2_OK;
 }
 
@@ -265,14 +369,10 @@ extern "C" int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, co
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
-    const dim3 grid = copy_grid(batch->n_rows, 2 * pages->n_kv_heads, pages->head_size, sms);
-    cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
-        kv_read_kernel<decltype(t)::value, decltype(hd)::value><<<grid, KV_THREADS, 0, st>>>(P);
-        return 0;
-    });
-    g_launches++;
-    L2_CUDA(cudaGetLastError());
+    const dim3 grid = copy_grid(P, 2 * pages->n_kv_heads, 1, pages->head_size, pages->type, sms);
+    L2_CUDA(by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
+        return kv_launch(kv_read_kernel<decltype(t)::value, decltype(hd)::value>, grid, KV_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), P);
+    }));
     return L2_OK;
 }
 

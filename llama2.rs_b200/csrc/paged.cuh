@@ -43,6 +43,8 @@ struct KvAttendParams {
 struct KvSeq { int row0, n, kv; };
 
 #ifdef __CUDACC__
+// (The kernels are launched programmatically: lengths and tables may be written by the kernel in front, for whose end they wait, so nothing here is read through
+// the read-only path.)
 __device__ __forceinline__ void kv_report(int* status, int bit) { if (status) atomicOr(status, bit); }
 
 __device__ __forceinline__ KvSeq kv_seq(const KvStep& s, int page_shift, int b) {
@@ -59,7 +61,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvStep& s, int page_shift, int b) 
 
 // The page of position j of sequence b, or -1 where the table's entry is none.
 __device__ __forceinline__ int kv_page(const KvStep& s, const KvPool& p, int b, int j) {
-    const int page = __ldg(s.table + (size_t)b * s.width + (j >> p.page_shift));
+    const int page = s.table[(size_t)b * s.width + (j >> p.page_shift)];
     if ((unsigned)page >= (unsigned)p.n_pages) { kv_report(s.status, L2_KV_BAD_PAGE); return -1; }
     return page;
 }
@@ -70,7 +72,7 @@ __device__ __forceinline__ int kv_find_seq(const KvStep& s, int r) {
     int lo = 0, n = s.n_seqs;  // the answer is in lo .. lo + n - 1
     while (n > 1) {
         const int step = (n + 31) / 32, at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(s.row_start + at) <= r);
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && s.row_start[at] <= r);
         const int k = below ? 31 - __clz(below) : 0;
         n = min(step, n - k * step);
         lo += k * step;

@@ -6,6 +6,7 @@
 
 #include <atomic>
 
+#include "kernels.cuh"
 #include "paged.cuh"
 
 namespace l2 {
@@ -21,6 +22,23 @@ struct KvOnce {
         return e;
     }
 };
+
+// Launched programmatically: a kernel's launch overlaps the one in front of it, for whose end it waits before it reads anything.
+template <class... A>
+cudaError_t kv_launch(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    g_launches++;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // The pool as a TMA tensor (element, position in the page, kv head, page); a copy brings up to `tile` positions of one page and head, 128 bytes wide (or a
 // row, where that is less), swizzled accordingly.

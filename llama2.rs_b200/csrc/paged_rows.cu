@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const KvSpot spot = kv_locate<KR_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kr_length(P, lim, b); });  // (ends behind a barrier)
     __syncthreads();
@@ -571,22 +572,11 @@ cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int
         auto kernel = kv_rows_kernel<T, decltype(b)::value, HD, NT>;
         static KvOnce once;
         if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KrShape<T, HD, NT>::SMEM)) return x;
-        kernel<<<grid, KR_THREADS, KrShape<T, HD, NT>::SMEM, st>>>(p, lim, mk, mv);
-        return cudaGetLastError();
+        return kv_launch(kernel, dim3(grid), KR_THREADS, KrShape<T, HD, NT>::SMEM, st, p, lim, mk, mv);
     });
-    g_launches++;
     if (e != cudaSuccess || grid < 2) return e;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(grid - 1);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    g_launches++;
-    return head_size == 128 ? cudaLaunchKernelEx(&cfg, kv_rows_combine_kernel<128>, p, lim, grid, 8 * nt) : cudaLaunchKernelEx(&cfg, kv_rows_combine_kernel<64>, p, lim, grid, 8 * nt);
+    auto combine = head_size == 128 ? kv_rows_combine_kernel<128> : kv_rows_combine_kernel<64>;
+    return kv_launch(combine, dim3(grid - 1), 256, 0, st, p, lim, grid, 8 * nt);
 }
 
 }  // namespace l2

@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const KvSpot spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch,
                                               [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
@@ -809,27 +810,16 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
         auto kernel = kv_tc_kernel<T, decltype(b)::value, HD>;
         static KvOnce once;
         if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KtShape<T, HD>::SMEM)) return x;
-        kernel<<<grid, KT_THREADS, KtShape<T, HD>::SMEM, st>>>(p, lim, mk, mv);
-        return cudaGetLastError();
+        return kv_launch(kernel, dim3(grid), KT_THREADS, KtShape<T, HD>::SMEM, st, p, lim, mk, mv);
     };
     auto by_hd = [&](auto t, auto b) { return head_size == 128 ? go(t, b, std::integral_constant<int, 128>()) : go(t, b, std::integral_constant<int, 64>()); };
     const bool qb = p.q.type == L2_BF16;
     const cudaError_t e = type == L2_F16 ? by_hd(std::integral_constant<int, L2_F16>(), std::false_type())
                         : type == L2_BF16 ? by_hd(std::integral_constant<int, L2_BF16>(), std::true_type())
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
-    g_launches++;
     if (e != cudaSuccess || grid < 2) return e;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(grid - 1, KT_COMBINE_SPLIT);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    g_launches++;
-    return head_size == 128 ? cudaLaunchKernelEx(&cfg, kv_tc_combine_kernel<128>, p, lim, grid) : cudaLaunchKernelEx(&cfg, kv_tc_combine_kernel<64>, p, lim, grid);
+    auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;
+    return kv_launch(combine, dim3(grid - 1, KT_COMBINE_SPLIT), 256, 0, st, p, lim, grid);
 }
 
 }  // namespace l2

@@ -7,18 +7,21 @@
     pages.attend(batch, q16, out, window=4096, sinks=4)
     pages.read(batch, k_back, v_back)
 
-Tensors are anything with torch's `data_ptr`, `dtype`, `shape` and `stride`; the objects keep those they are made of.  Work is enqueued
-on the current torch stream unless `stream` (a cudaStream_t) is given.
+The objects keep the tensors they are made of.  Work is enqueued on the current torch stream unless `stream` (a cudaStream_t) is given; a call
+does not wait for it.  One host thread at a time uses a KvPages.
 """
 import ctypes as C
+import struct
 import sys
 
 from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, check, lib
 
-F32, F16, BF16, I8 = 0, 1, 2, 3
+F32, F16, BF16, I8, I32 = 0, 1, 2, 3, 4
 BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
-_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8}
+_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.int32": I32}
 _types = {}  # the same by dtype object, filled as they are seen
+_ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
+assert _ROWS2.size == 2 * C.sizeof(KvRowsArgs) and _ROWS4.size == 4 * C.sizeof(KvRowsArgs)
 
 
 def _type(t):
@@ -34,21 +37,13 @@ def _stream(stream, device):
     torch = sys.modules["torch"]
     if torch.cuda.current_device() != device:
         raise ValueError("the tensors are on device %d, which is not the current one" % device)
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _tensor(t, what, device, dims, dtype=None):
-    if not t.is_cuda or (device is not None and t.get_device() != device):
-        raise ValueError("%s: not a tensor of the device" % what)
-    if t.dim() != dims or (dtype is not None and str(t.dtype) != dtype):
-        raise ValueError("%s: %d dimensions%s expected" % (what, dims, "" if dtype is None else " of " + dtype))
-    return t
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (without making a Stream object, which takes longer than the launch)
+    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
 
 
 def _packed(t, what, device, shape, dtype):
-    _tensor(t, what, device, len(shape), dtype)
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError("%s: contiguous %s expected, got %s" % (what, tuple(shape), tuple(t.shape)))
+    if t.get_device() != device or tuple(t.shape) != shape or _type(t) != dtype or not t.is_contiguous():  # (-1: not on a CUDA device)
+        raise ValueError("%s: contiguous %s of type code %d on device %d expected, got %s of %s" % (what, shape, dtype, device, tuple(t.shape), t.dtype))
     return t.data_ptr()
 
 
@@ -57,13 +52,14 @@ class KvBatch:
     at most max_rows of one sequence.  `status` (one int32 on the device, optional) gets the BAD_* bits of what only the device can see."""
 
     def __init__(self, page_table, kv_len, row_start, n_rows, max_rows, status=None):
-        _tensor(page_table, "page_table", None, 2, "torch.int32")
+        if page_table.dim() != 2 or not page_table.is_cuda:
+            raise ValueError("page_table: [n_seqs, width] on a CUDA device expected")
         self.device = page_table.get_device()
         n_seqs, width = page_table.shape
-        self._args = KvBatchArgs(_packed(page_table, "page_table", self.device, (n_seqs, width), "torch.int32"),
-                                 _packed(kv_len, "kv_len", self.device, (n_seqs,), "torch.int32"),
-                                 _packed(row_start, "row_start", self.device, (n_seqs + 1,), "torch.int32"),
-                                 _packed(status, "status", self.device, (1,), "torch.int32") if status is not None else None,
+        self._args = KvBatchArgs(_packed(page_table, "page_table", self.device, (n_seqs, width), I32),
+                                 _packed(kv_len, "kv_len", self.device, (n_seqs,), I32),
+                                 _packed(row_start, "row_start", self.device, (n_seqs + 1,), I32),
+                                 _packed(status, "status", self.device, (1,), I32) if status is not None else None,
                                  n_seqs, width, n_rows, max_rows)
         self._ref = C.byref(self._args)
         self._keep = (page_table, kv_len, row_start, status)
@@ -77,9 +73,9 @@ class KvPages:
     def __init__(self, k, v, k_scale=None, v_scale=None, layout="NHD"):
         if layout not in ("NHD", "HND"):
             raise ValueError("layout: NHD or HND")
-        _tensor(k, "k", None, 4)
         self.device = k.get_device()
-        _tensor(v, "v", self.device, 4)
+        if k.dim() != 4 or self.device < 0 or v.get_device() != self.device:
+            raise ValueError("k and v: four dimensions on a CUDA device expected")
         if v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride() or k.stride(3) != 1:
             raise ValueError("k and v: the same shape, type and strides, the last dimension contiguous")
         at, head = (1, 2) if layout == "NHD" else (2, 1)
@@ -90,40 +86,58 @@ class KvPages:
             if k_scale is None or v_scale is None:
                 raise ValueError("an int8 cache needs k_scale and v_scale")
             shape = (self.n_pages, self.n_kv_heads, self.page_size)
-            scales = [_packed(s, "scales", self.device, shape, "torch.float32") for s in (k_scale, v_scale)]
+            scales = [_packed(s, "scales", self.device, shape, F32) for s in (k_scale, v_scale)]
         elif k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to an int8 cache")
         self._args = KvPagesArgs(k.data_ptr(), v.data_ptr(), scales[0], scales[1], k.stride(0), k.stride(at), k.stride(head), kind,
                                  self.n_pages, self.page_size, self.n_kv_heads, self.head_size)
         self._ref = C.byref(self._args)
         self._keep = (k, v, k_scale, v_scale)
+        # the row records of a call, filled in place: making ctypes structures takes longer than the rest of it
+        self._rows = (KvRowsArgs * 4)()
+        self._at = tuple(C.addressof(self._rows) + i * C.sizeof(KvRowsArgs) for i in range(4))
 
-    def _rows(self, t, what, batch, heads=None):
-        if t.get_device() != self.device or t.dim() != 3:  # (-1: not on a CUDA device)
-            raise ValueError("%s: [rows, heads, head_size] on the cache's device expected" % what)
-        n, h, hd = t.shape
-        a, b, c = t.stride()
-        if n != batch.n_rows or hd != self.head_size or c != 1 or (heads is not None and h != heads):
-            raise ValueError("%s: [%d, %s, %d] with its last dimension contiguous expected, got %s" % (what, batch.n_rows, heads or "heads", self.head_size, tuple(t.shape)))
-        return C.byref(KvRowsArgs(t.data_ptr(), a, b, _type(t), h))
+    def _row(self, t, what, n, heads):
+        """The fields of an l2_kv_rows for t; heads 0: as many as it has."""
+        try:
+            m, h, size = t.shape
+            row, head, one = t.stride()
+        except ValueError:
+            m = h = size = one = -1
+        kind = _types.get(t.dtype)
+        if kind is None:
+            kind = _type(t)
+        if m != n or size != self.head_size or one != 1 or (heads and h != heads) or t.get_device() != self.device:
+            raise ValueError("%s: [%d, %s, %d] on device %d with its last dimension contiguous expected, got %s" % (what, n, heads or "heads", self.head_size, self.device, tuple(t.shape)))
+        return t.data_ptr(), row, head, kind, h
 
     def append(self, batch, k, v, rope=None, q=None, q_out=None, stream=None):
         """K and V rows of the step into their pages; rope = (cos, sin), [positions, head_size / 2] f32, rotates k and, into q_out, q."""
-        if (q is None) != (q_out is None):
-            raise ValueError("q and q_out go together")
+        n, heads = batch.n_rows, self.n_kv_heads
+        a = self._at
+        if q is None and q_out is None:
+            _ROWS2.pack_into(self._rows, 0, *self._row(k, "k", n, heads), *self._row(v, "v", n, heads))
+            q_at = q_out_at = None
+        else:
+            if q is None or q_out is None:
+                raise ValueError("q and q_out go together")
+            _ROWS4.pack_into(self._rows, 0, *self._row(k, "k", n, heads), *self._row(v, "v", n, heads),
+                             *self._row(q, "q", n, 0), *self._row(q_out, "q_out", n, q.shape[1]))
+            q_at, q_out_at = a[2], a[3]
         cos = sin = None
         positions = 0
         if rope is not None:
-            positions = rope[0].shape[0]
-            cos, sin = (_packed(t, "rope", self.device, (positions, self.head_size // 2), "torch.float32") for t in rope)
-        check(lib.l2_kv_append(self._ref, batch._ref, self._rows(k, "k", batch, self.n_kv_heads), self._rows(v, "v", batch, self.n_kv_heads),
-                               self._rows(q, "q", batch) if q is not None else None, self._rows(q_out, "q_out", batch, q.shape[1]) if q is not None else None,
-                               cos, sin, positions, _stream(stream, self.device)))
+            cos, sin = rope
+            positions = cos.shape[0]
+            shape = (positions, self.head_size // 2)
+            cos, sin = _packed(cos, "rope", self.device, shape, F32), _packed(sin, "rope", self.device, shape, F32)
+        check(lib.l2_kv_append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(stream, self.device)))
 
     def read(self, batch, k, v, stream=None):
         """The cached positions of the step's rows into k and v ([rows, kv_heads, head_size], f32, f16 or bf16)."""
-        check(lib.l2_kv_read(self._ref, batch._ref, self._rows(k, "k", batch, self.n_kv_heads), self._rows(v, "v", batch, self.n_kv_heads),
-                             _stream(stream, self.device)))
+        n, heads = batch.n_rows, self.n_kv_heads
+        _ROWS2.pack_into(self._rows, 0, *self._row(k, "k", n, heads), *self._row(v, "v", n, heads))
+        check(lib.l2_kv_read(self._ref, batch._ref, self._at[0], self._at[1], _stream(stream, self.device)))
 
     def workspace_bytes(self, batch, n_heads):
         return int(lib.l2_kv_attend_workspace_bytes(self._ref, batch._ref, n_heads))
@@ -131,14 +145,15 @@ class KvPages:
     def attend(self, batch, q, out, scale=None, window=0, sinks=0, workspace=None, stream=None):
         """Attention of the step's rows q [rows, heads, head_size] over the cache into out; scale defaults to head_size ** -0.5.
         `workspace`: a uint8 tensor of workspace_bytes(); one is made where none is given."""
-        heads = q.shape[1]
+        n = batch.n_rows
+        row = self._row(q, "q", n, 0)
+        _ROWS2.pack_into(self._rows, 0, *row, *self._row(out, "out", n, row[4]))
         if workspace is None:
             if stream is not None:
                 raise ValueError("a stream of your own needs a workspace of your own: one made here is handed out again in the order of torch's stream")
-            workspace = q.new_empty(self.workspace_bytes(batch, heads), dtype=sys.modules["torch"].uint8)
+            workspace = q.new_empty(self.workspace_bytes(batch, row[4]), dtype=sys.modules["torch"].uint8)
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("workspace: a contiguous tensor on the cache's device expected")
-        check(lib.l2_kv_attend(self._ref, batch._ref, self._rows(q, "q", batch), self._rows(out, "out", batch, heads),
-                               self.head_size ** -0.5 if scale is None else scale, window, sinks,
-                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream, self.device)))
+        check(lib.l2_kv_attend(self._ref, batch._ref, self._at[0], self._at[1], self.head_size ** -0.5 if scale is None else scale, window, sinks,
+                               workspace.data_ptr(), workspace.nbytes, _stream(stream, self.device)))
         return out
