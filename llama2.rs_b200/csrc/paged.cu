@@ -19,7 +19,7 @@ namespace l2 {
 namespace {
 
 constexpr int KV_THREADS = 256, KV_WARPS = KV_THREADS / 32, KV_MAX_ROWS = 16;
-constexpr int KV_AT_ONCE = 4;  // heads that a group of threads has under way
+constexpr int KV_AT_ONCE = 2, KV_READ_AT_ONCE = 4;  // heads that a group of threads has under way
 
 struct KvCopyParams {
     KvPool pool;
@@ -28,25 +28,28 @@ struct KvCopyParams {
     const float* cos; const float* sin;
     int rope_len;
     int rows;  // of a CTA
+    uint32_t by_heads, by_q_heads;  // reciprocals of the kv heads (kv_read_kernel: twice as many) and of q's
 };
 
 // Where a row's position is; by one warp a row, the rows of a CTA side by side: three or four loads that depend on one another, once a row.
-struct KvPlace { int64_t at, scale; int pos; bool there, page; };  // elements of the pool, of the scales; there: a row of a sequence; page: it has one
+struct KvPlace { int64_t at, scale; int pos; };  // elements of the pool (-1: no page), of the scales; position, -1: a row that is left out
 __device__ __forceinline__ KvPlace kv_place(const KvCopyParams& P, int r) {
-    KvPlace w{0, 0, 0, false, false};
+    KvPlace w{-1, 0, -1};
     if (r >= P.step.n_rows) return w;
     const int b = kv_find_seq(P.step, r);
     const KvSeq s = kv_seq(P.step, P.pool.page_shift, b);
-    w.pos = s.kv - s.n + (r - s.row0);
-    w.there = r >= s.row0 && r < s.row0 + s.n && w.pos >= 0;
-    if (w.there && P.cos && w.pos >= P.rope_len) { kv_report(P.step.status, L2_KV_BAD_ROPE); w.there = false; }
-    if (!w.there) return w;
-    const int page = kv_page(P.step, P.pool, b, w.pos), in = w.pos & ((1 << P.pool.page_shift) - 1);
-    w.page = page >= 0;
+    const int pos = s.kv - s.n + (r - s.row0);
+    if (r < s.row0 || r >= s.row0 + s.n || pos < 0) return w;
+    if (P.cos && pos >= P.rope_len) { kv_report(P.step.status, L2_KV_BAD_ROPE); return w; }
+    w.pos = pos;
+    const int page = kv_page(P.step, P.pool, b, pos), in = pos & ((1 << P.pool.page_shift) - 1);
+    if (page < 0) return w;
     w.at = (int64_t)page * P.pool.page_stride + in * P.pool.pos_stride;
     w.scale = ((int64_t)page * P.pool.n_kv_heads << P.pool.page_shift) + in;
     return w;
 }
+// u / n by n's reciprocal, 2^32 / n rounded up: exact for u n < 2^32, and u and n stay below 2^13 (n = 1: the reciprocal is taken as 0)
+__device__ __forceinline__ int kv_div(int u, uint32_t by) { return by ? (int)__umulhi((uint32_t)u, by) : u; }
 __device__ __forceinline__ void kv_places(const KvCopyParams& P, int r0, KvPlace* place) {
     for (int i = threadIdx.x >> 5; i < P.rows; i += KV_WARPS) {
         const KvPlace w = kv_place(P, r0 + i);
@@ -55,128 +58,141 @@ __device__ __forceinline__ void kv_places(const KvCopyParams& P, int r0, KvPlace
     __syncthreads();
 }
 
-// The N elements of a thread as they lie in memory, as f32, and back (8 at a time).
-template <int T, int N> struct KvRaw { uint4 w[N * (T == L2_F32 ? 4 : 2) / 16]; };
-template <int T, int N>
-__device__ __forceinline__ KvRaw<T, N> load_raw(const char* base, int64_t e) {
-    KvRaw<T, N> r;
-    const uint4* p = reinterpret_cast<const uint4*>(base + e * (T == L2_F32 ? 4 : 2));
+// Eight elements as they lie in memory, as f32, and back.
+template <int T> struct KvRaw { uint4 w[T == L2_F32 ? 2 : 1]; };
+template <int T>
+__device__ __forceinline__ KvRaw<T> load_raw(const char* p) {
+    KvRaw<T> r;
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(r.w) / 16); i++) r.w[i] = p[i];
+    for (int i = 0; i < (int)(sizeof(r.w) / 16); i++) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
     return r;
 }
-template <int T, int N>
-__device__ __forceinline__ void to_f32(const KvRaw<T, N>& r, float (&x)[N]) {
+template <int T>
+__device__ __forceinline__ void to_f32(const KvRaw<T>& r, float* x) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+    for (int i = 0; i < 8; i++) {
         if constexpr (T == L2_F32) x[i] = __uint_as_float(w[i]);
         else if constexpr (T == L2_F16) x[i] = __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i % 2)))));
         else x[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
 }
-template <int T, int N>
-__device__ __forceinline__ void store_n(char* base, int64_t e, const float (&x)[N]) {
+template <int T>
+__device__ __forceinline__ void store8(char* base, int64_t e, const float* x) {
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < N; i += 8) {
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = x[i + j];
-        if constexpr (T == L2_F32) kv_store8(reinterpret_cast<float*>(base) + e + i, y);
-        else if constexpr (T == L2_F16) kv_store8(reinterpret_cast<__half*>(base) + e + i, y);
-        else kv_store8(reinterpret_cast<__nv_bfloat16*>(base) + e + i, y);
-    }
+    for (int j = 0; j < 8; j++) y[j] = x[j];
+    if constexpr (T == L2_F32) kv_store8(reinterpret_cast<float*>(base) + e, y);
+    else if constexpr (T == L2_F16) kv_store8(reinterpret_cast<__half*>(base) + e, y);
+    else kv_store8(reinterpret_cast<__nv_bfloat16*>(base) + e, y);
+}
+__device__ __forceinline__ float max_abs(float a, float x) {  // NaN if one of them is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(fabsf(x)));
+    return y;
 }
 
-// A CTA has a few rows (blockIdx.y) of k, v or q (blockIdx.x modulo their number), or a part of one row's heads.  HD / N threads have a head, N elements each: 16 bytes of the cache.
-// Every group requests the next KV_AT_ONCE heads together; nothing is used twice, so bytes under way are what counts.
+// A CTA has a few rows (blockIdx.y) of k, v or q (blockIdx.x modulo their number), or a part of one row's heads.  HD / 16 threads have a head, eight
+// elements each of its first half and the same of its second: whole lines, and the pairs that RoPE turns in one thread.
+// Latency of loads and instructions, then bandwidth, bound it: 7900 rows of 2 x 40 heads of 128, bf16 to int8 (242 MB), take 51 us (4.8 TB/s).  A row a CTA,
+// whose look-ups nothing hid, took 76; so did 16 elements of one run a thread with conversion instructions and 110 registers (18 instructions an element).
 template <int T, int HD>
-__global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_constant__ KvCopyParams P) {
+__global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_constant__ KvCopyParams P) {
     constexpr bool I8 = T == L2_I8;
-    constexpr int N = I8 ? 16 : 8, LANES = HD / N, GROUPS = KV_THREADS / LANES, HALF = HD / 2;
+    constexpr int LANES = HD / 16, GROUPS = KV_THREADS / LANES, HALF = HD / 2;
     __shared__ KvPlace place[KV_MAX_ROWS];
-    const int sub = threadIdx.x % LANES, grp = threadIdx.x / LANES, d = N * sub;
+    const int sub = threadIdx.x % LANES, grp = threadIdx.x / LANES, d = 8 * sub;
     const int arrays = P.q.data ? 3 : 2, what = blockIdx.x % arrays, part = blockIdx.x / arrays, parts = gridDim.x / arrays;  // what: 0 k, 1 v, 2 q
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const KvRows& from = what == 0 ? P.k : what == 1 ? P.v : P.q;
+    const int heads = from.heads, units = P.rows * heads;
+    const uint32_t by_heads = what == 2 ? P.by_q_heads : P.by_heads;
+    const bool turn = P.cos && what != 1;
+    char* const to = what == 1 ? P.pool.v : P.pool.k;
+    float* const scales = what == 1 ? P.pool.vs : P.pool.ks;
     for (int r0 = blockIdx.y * P.rows; r0 < P.step.n_rows; r0 += gridDim.y * P.rows) {
         kv_places(P, r0, place);
-        auto heads_of = [&](const KvRows& from, auto type) {
-            constexpr int IN = decltype(type)::value;
-            const int heads = from.heads, units = P.rows * heads;
-            const bool turn = P.cos && what != 1;
+        auto run = [&](auto type) {
+            constexpr int IN = decltype(type)::value, SIZE = IN == L2_F32 ? 4 : 2;
 #pragma unroll 1
             for (int u0 = part * GROUPS; u0 < units; u0 += parts * GROUPS * KV_AT_ONCE) {  // (whole warps stay together for the shuffles)
-                KvRaw<IN, N> raw[KV_AT_ONCE];
+                KvRaw<IN> raw[KV_AT_ONCE][2];
                 int row[KV_AT_ONCE], head[KV_AT_ONCE];
                 bool mine[KV_AT_ONCE];
 #pragma unroll
                 for (int a = 0; a < KV_AT_ONCE; a++) {
                     const int u = u0 + a * parts * GROUPS + grp;
-                    row[a] = u / heads;
+                    row[a] = kv_div(u, by_heads);
                     head[a] = u - row[a] * heads;
-                    mine[a] = u < units && place[row[a]].there;
-                    raw[a] = {};
-                    if (mine[a]) raw[a] = load_raw<IN, N>(from.data, (int64_t)(r0 + row[a]) * from.row_stride + head[a] * from.head_stride + d);
+                    mine[a] = u < units && place[row[a]].pos >= 0;
+                    raw[a][0] = raw[a][1] = {};
+                    if (mine[a]) {
+                        const char* p = from.data + ((int64_t)(r0 + row[a]) * from.row_stride + head[a] * from.head_stride + d) * SIZE;
+                        raw[a][0] = load_raw<IN>(p);
+                        raw[a][1] = load_raw<IN>(p + HALF * SIZE);
+                    }
                 }
 #pragma unroll
                 for (int a = 0; a < KV_AT_ONCE; a++) {
                     if (u0 + a * parts * GROUPS >= units) break;  // (whole CTAs)
-                    const KvPlace w = mine[a] ? place[row[a]] : KvPlace{0, 0, 0, false, false};
-                    float x[N];
-                    to_f32(raw[a], x);
+                    float x[16];
+                    to_f32(raw[a][0], x);
+                    to_f32(raw[a][1], x + 8);
+                    const int at_row = mine[a] ? row[a] : 0;
                     if (turn) {  // products and their sum are rounded one by one, as written
-                        float y[N], c[N], s[N];
+                        const int64_t e = (int64_t)max(place[at_row].pos, 0) * HALF + d;
+                        float c[8], s[8];
+                        to_f32(load_raw<L2_F32>(reinterpret_cast<const char*>(P.cos + e)), c);
+                        to_f32(load_raw<L2_F32>(reinterpret_cast<const char*>(P.sin + e)), s);
 #pragma unroll
-                        for (int i = 0; i < N; i++) y[i] = __shfl_xor_sync(0xffffffffu, x[i], LANES / 2);
-                        const int64_t e = (int64_t)w.pos * HALF + (d & (HALF - 1));
-                        to_f32(load_raw<L2_F32, N>(reinterpret_cast<const char*>(P.cos), e), c);
-                        to_f32(load_raw<L2_F32, N>(reinterpret_cast<const char*>(P.sin), e), s);
-#pragma unroll
-                        for (int i = 0; i < N; i++)
-                            x[i] = d < HALF ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i])) : __fadd_rn(__fmul_rn(y[i], s[i]), __fmul_rn(x[i], c[i]));
+                        for (int i = 0; i < 8; i++) {
+                            const float y = x[i], z = x[i + 8];
+                            x[i] = __fsub_rn(__fmul_rn(y, c[i]), __fmul_rn(z, s[i]));
+                            x[i + 8] = __fadd_rn(__fmul_rn(y, s[i]), __fmul_rn(z, c[i]));
+                        }
                     }
                     if (what == 2) {
                         if (!mine[a]) continue;
                         const int64_t e = (int64_t)(r0 + row[a]) * P.q_out.row_stride + head[a] * P.q_out.head_stride + d;
-                        if (P.q_out.type == L2_F32) store_n<L2_F32, N>(P.q_out.data, e, x);
-                        else if (P.q_out.type == L2_F16) store_n<L2_F16, N>(P.q_out.data, e, x);
-                        else store_n<L2_BF16, N>(P.q_out.data, e, x);
+                        auto out = [&](auto t) { store8<decltype(t)::value>(P.q_out.data, e, x); store8<decltype(t)::value>(P.q_out.data, e + HALF, x + 8); };
+                        if (P.q_out.type == L2_F32) out(std::integral_constant<int, L2_F32>());
+                        else if (P.q_out.type == L2_F16) out(std::integral_constant<int, L2_F16>());
+                        else out(std::integral_constant<int, L2_BF16>());
                         continue;
                     }
-                    const int64_t e = w.at + head[a] * P.pool.head_stride + d;
-                    char* to = what == 1 ? P.pool.v : P.pool.k;
+                    const int64_t e = place[at_row].at + head[a] * P.pool.head_stride + d;
+                    const bool store = mine[a] && place[at_row].at >= 0;
                     if constexpr (I8) {
-                        // the row's largest magnitude, as bits: of non-negative floats the order of the bits is that of the values, NaN above all
-                        uint32_t most = 0;
+                        float m = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < N; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+                        for (int i = 0; i < 16; i++) m = max_abs(m, x[i]);
 #pragma unroll
-                        for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        const float m = __uint_as_float(most);
-                        const bool finite = most < 0x7f800000u, zero = m < 0x1p-100f;
-                        const float inv = finite && !zero ? __fmul_rn(__frcp_rn(m), 127.0f) : 0.0f;
+                        for (int o = LANES / 2; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const bool finite = m < INFINITY, zero = m < 0x1p-100f;
+                        const float inv = zero ? 0.0f : __fmul_rn(__frcp_rn(m), 127.0f);
                         // (|x| inv is at most 127 and a few units in the last place.  Added to 1.5 x 2^23 it is rounded to a whole number, to nearest even, whose
-                        // two's complement is the low byte: a conversion instruction takes four times as long.)
-                        uint32_t b[N];
+                        // two's complement is the low byte: a conversion instruction takes four times as long.  What is not finite gives any byte: the scale is NaN.)
+                        uint32_t b[16];
 #pragma unroll
-                        for (int i = 0; i < N; i++) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(finite ? x[i] : 0.0f, inv), 12582912.0f));
+                        for (int i = 0; i < 16; i++) b[i] = __float_as_uint(__fmaf_rn(x[i], inv, 12582912.0f));
 #pragma unroll
-                        for (int i = 0; i < N; i += 4) b[i / 4] = __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
-                        if (!w.page) continue;
-                        *reinterpret_cast<uint4*>(to + e) = make_uint4(b[0], b[1], b[2], b[3]);
-                        if (sub == 0) (what == 1 ? P.pool.vs : P.pool.ks)[w.scale + ((int64_t)head[a] << P.pool.page_shift)] =
+                        for (int i = 0; i < 16; i += 4) b[i / 4] = __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
+                        if (!store) continue;
+                        *reinterpret_cast<uint2*>(to + e) = make_uint2(b[0], b[1]);
+                        *reinterpret_cast<uint2*>(to + e + HALF) = make_uint2(b[2], b[3]);
+                        if (sub == 0) scales[place[at_row].scale + ((int64_t)head[a] << P.pool.page_shift)] =
                             !finite ? __int_as_float(0x7fc00000) : zero ? 0.0f : __fmul_rn(m, 1.0f / 127.0f);
-                    } else if (w.page) {
-                        store_n<T, N>(to, e, x);
+                    } else if (store) {
+                        store8<T>(to, e, x);
+                        store8<T>(to, e + HALF, x + 8);
                     }
                 }
             }
         };
-        const KvRows& from = what == 0 ? P.k : what == 1 ? P.v : P.q;
-        if (from.type == L2_F32) heads_of(from, std::integral_constant<int, L2_F32>());
-        else if (from.type == L2_F16) heads_of(from, std::integral_constant<int, L2_F16>());
-        else heads_of(from, std::integral_constant<int, L2_BF16>());
+        if (from.type == L2_F32) run(std::integral_constant<int, L2_F32>());
+        else if (from.type == L2_F16) run(std::integral_constant<int, L2_F16>());
+        else run(std::integral_constant<int, L2_BF16>());
         __syncthreads();
     }
 }
@@ -192,24 +208,24 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
     for (int r0 = blockIdx.y * P.rows; r0 < P.step.n_rows; r0 += gridDim.y * P.rows) {
         kv_places(P, r0, place);
 #pragma unroll 1
-        for (int u0 = blockIdx.x * GROUPS + grp; u0 < units; u0 += gridDim.x * GROUPS * KV_AT_ONCE) {
-            uint4 x[KV_AT_ONCE];
-            float f[KV_AT_ONCE];
+        for (int u0 = blockIdx.x * GROUPS + grp; u0 < units; u0 += gridDim.x * GROUPS * KV_READ_AT_ONCE) {
+            uint4 x[KV_READ_AT_ONCE];
+            float f[KV_READ_AT_ONCE];
 #pragma unroll
-            for (int a = 0; a < KV_AT_ONCE; a++) {
-                const int u = u0 + a * gridDim.x * GROUPS, r = u / (2 * heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
+            for (int a = 0; a < KV_READ_AT_ONCE; a++) {
+                const int u = u0 + a * gridDim.x * GROUPS, r = kv_div(u, P.by_heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
                 x[a] = make_uint4(0, 0, 0, 0);
                 f[a] = 0.0f;
-                if (u < units && place[r].page) {
+                if (u < units && place[r].at >= 0) {
                     const char* from = h < heads ? P.pool.k : P.pool.v;
                     x[a] = __ldcs(reinterpret_cast<const uint4*>(from + (place[r].at + head * P.pool.head_stride + d) * (I8 ? 1 : 2)));
                     if constexpr (I8) f[a] = (h < heads ? P.pool.ks : P.pool.vs)[place[r].scale + ((int64_t)head << P.pool.page_shift)];
                 }
             }
 #pragma unroll
-            for (int a = 0; a < KV_AT_ONCE; a++) {
-                const int u = u0 + a * gridDim.x * GROUPS, r = u / (2 * heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
-                if (u >= units || !place[r].there) continue;
+            for (int a = 0; a < KV_READ_AT_ONCE; a++) {
+                const int u = u0 + a * gridDim.x * GROUPS, r = kv_div(u, P.by_heads), h = u - r * 2 * heads, head = h < heads ? h : h - heads;
+                if (u >= units || place[r].pos < 0) continue;
                 const KvRows& to = h < heads ? P.k : P.v;
                 float y[N];
                 const uint32_t w[4] = {x[a].x, x[a].y, x[a].z, x[a].w};
@@ -221,10 +237,14 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
                     else y[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
                 }
                 const int64_t e = (int64_t)(r0 + r) * to.row_stride + head * to.head_stride + d;
+                auto put = [&](auto t) {
+#pragma unroll
+                    for (int i = 0; i < N; i += 8) store8<decltype(t)::value>(to.data, e + i, y + i);
+                };
                 if (to.type == T) *reinterpret_cast<uint4*>(to.data + 2 * e) = x[a];
-                else if (to.type == L2_F32) store_n<L2_F32, N>(to.data, e, y);
-                else if (to.type == L2_F16) store_n<L2_F16, N>(to.data, e, y);
-                else store_n<L2_BF16, N>(to.data, e, y);
+                else if (to.type == L2_F32) put(std::integral_constant<int, L2_F32>());
+                else if (to.type == L2_F16) put(std::integral_constant<int, L2_F16>());
+                else put(std::integral_constant<int, L2_BF16>());
             }
         }
         __syncthreads();
@@ -315,14 +335,15 @@ cudaError_t by_type(int type, int head_size, F f) {
     return f(std::integral_constant<int, L2_I8>(), std::integral_constant<int, 64>());
 }
 
-// Rows of a CTA and CTAs of a copy: as many rows as give every group of threads some KV_AT_ONCE heads, where that leaves four CTAs an SM; a row's heads
-// in several CTAs where the rows alone do not fill the device.
-dim3 copy_grid(KvCopyParams& P, int heads, int arrays, int head_size, int type, int sms) {
-    const int groups = KV_THREADS / (head_size / (type == L2_I8 ? 16 : 8)), n = P.step.n_rows;
-    P.rows = std::max(1, std::min({KV_MAX_ROWS, 2 * KV_AT_ONCE * groups / heads, n * arrays / (4 * sms)}));
+// Rows of a CTA and CTAs of a copy: `rounds` rounds of a CTA's groups of threads, where that leaves four CTAs an SM (a CTA's look-ups are a chain of loads, which
+// few rows would not pay for); a row's heads in several CTAs where the rows alone do not fill the device.
+dim3 copy_grid(KvCopyParams& P, int heads, int arrays, int groups, int rounds, int sms) {
+    const int n = P.step.n_rows;
+    P.rows = std::max(1, std::min({KV_MAX_ROWS, rounds * groups / heads, (int)((int64_t)n * arrays / (4 * sms))}));
     const int y = (n + P.rows - 1) / P.rows, x = std::min((P.rows * heads + groups - 1) / groups, std::max(1, 4 * sms / (y * arrays)));
     return dim3(x * arrays, std::min(y, 65535));
 }
+uint32_t reciprocal(int n) { return n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0; }
 
 }  // namespace
 
@@ -341,7 +362,7 @@ extern "C" int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (int rc = check_rows(who, "v", v, batch, pages->head_size, pages->n_kv_heads, &P.v)) return rc;
     if (!q != !q_out) return fail(L2_EINVAL, "%s: q and q_out go together", who);
     if (q) {
-        if (q->heads < 1) return fail(L2_EINVAL, "%s: q has %d heads", who, q->heads);
+        if (q->heads < 1 || q->heads > 4096) return fail(L2_EINVAL, "%s: q has %d heads", who, q->heads);
         if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, &P.q)) return rc;
         if (int rc = check_rows(who, "q_out", q_out, batch, pages->head_size, q->heads, &P.q_out)) return rc;
     }
@@ -351,7 +372,9 @@ extern "C" int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
-    const dim3 grid = copy_grid(P, std::max(pages->n_kv_heads, q ? q->heads : 0), q ? 3 : 2, pages->head_size, pages->type, sms);
+    const dim3 grid = copy_grid(P, std::max(pages->n_kv_heads, q ? q->heads : 0), q ? 3 : 2, KV_THREADS / (pages->head_size / 16), 8, sms);
+    P.by_heads = reciprocal(pages->n_kv_heads);
+    P.by_q_heads = reciprocal(q ? q->heads : 1);
     L2_CUDA(by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
         return kv_launch(kv_append_kernel<decltype(t)::value, decltype(hd)::value>, grid, KV_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), P);
     }));
@@ -369,7 +392,8 @@ extern "C" int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, co
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
-    const dim3 grid = copy_grid(P, 2 * pages->n_kv_heads, 1, pages->head_size, pages->type, sms);
+    const dim3 grid = copy_grid(P, 2 * pages->n_kv_heads, 1, KV_THREADS / (pages->head_size / (pages->type == L2_I8 ? 16 : 8)), 8, sms);
+    P.by_heads = reciprocal(2 * pages->n_kv_heads);
     L2_CUDA(by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
         return kv_launch(kv_read_kernel<decltype(t)::value, decltype(hd)::value>, grid, KV_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), P);
     }));
