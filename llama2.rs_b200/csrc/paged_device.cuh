@@ -43,9 +43,12 @@ __device__ __forceinline__ void kv_tma4(uint32_t dst, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(pos), "r"(head), "r"(page), "r"(kv_smem(bar)) : "memory");
 }
-__device__ __forceinline__ void kv_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(kv_smem(bar)) : "memory");
+// 16 bytes by a thread, zeros where there is nothing to bring; its arrival at `bar` follows when it has landed (one of those the barrier counts).
+__device__ __forceinline__ void kv_copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void kv_copy16_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(kv_smem(bar)) : "memory");
 }
 __device__ __forceinline__ float kv_exp2(float x) {
     float y;

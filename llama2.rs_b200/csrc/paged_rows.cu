@@ -11,7 +11,7 @@
 // does not know the lengths.
 //
 // Roles: warps 0-3 take 16 positions of a tile each, with a softmax of their own, and meet at the end of a piece; warp 4 fills a ring of
-// tiles with TMA copies, one a page run (and the scales of an int8 cache, one bulk copy a run).
+// tiles with TMA copies, one a page run (and the scales of an int8 cache, 16 bytes a lane).
 //
 // An int8 cache is multiplied as it is stored: K as q's type and V as bf16, both exact; the scale of a position is applied to its score and to
 // its probability.  (The probabilities times scales are rounded to bf16 even where q is f16: they can leave f16's range.)
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < S::STAGES; i++) { kv_bar_init(&full[i], 1); kv_bar_init(&empty[i], KR_WARPS); }
+        for (int i = 0; i < S::STAGES; i++) { kv_bar_init(&full[i], I8 ? 33 : 1); kv_bar_init(&empty[i], KR_WARPS); }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -157,49 +157,43 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
 
     if (warp == KR_WARPS) {
         // ================= copies: lane l brings run l of a tile ==============================================================
-        const int R = min(KR_TILE, 1 << P.pool.page_shift), runs = KR_TILE / R;
+        // Pages are looked up for 32 runs at once, and for the next 32 while these are copied: a look-up takes as long as a tile's arithmetic.
+        const int R = min(KR_TILE, 1 << P.pool.page_shift), runs = KR_TILE / R, ahead = 32 / runs;
         uint32_t st = 0, ph = 1;
         bool over = false;
         while (!over && walk.next(P, lim)) {
             const KvView<KR_TILE>& view = walk.q.view;
-            for (int t = walk.t0; t < walk.t1; t++) {
-                const int j = view.base(t) + lane * R;
-                int page = P.pool.n_pages;  // (outside the pool: the copy gives zeros)
-                if (lane < runs && view.any(j, R, P.window, P.sinks)) {
-                    const int x = kv_page(P.step, P.pool, walk.b, j);
-                    if (x >= 0) page = x;
-                }
+            auto look_up = [&](int t) {  // lane l: run l % runs of tile t + l / runs; n_pages (a copy from there gives zeros) where no row sees it or there is none
+                const int mine = t + lane / runs, j = view.base(mine) + lane % runs * R;
+                if (mine >= walk.t1 || !view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
+                const int x = kv_page(P.step, P.pool, walk.b, j);
+                return x >= 0 ? x : P.pool.n_pages;
+            };
+            int pages = 0, next = look_up(walk.t0);
+            for (int t = walk.t0, k = 0; t < walk.t1; t++, k = k + 1 == ahead ? 0 : k + 1) {
+                if (k == 0) { pages = next; next = look_up(t + ahead); }
+                const int j = view.base(t), page = __shfl_sync(0xffffffffu, pages, k * runs + lane % runs);
                 wait(&empty[st], ph);
                 if ((over = wait.over())) break;
                 uint8_t* stage = ring + st * S::STAGE;
-                const bool there = lane < runs && page < P.pool.n_pages;
-                uint32_t bytes = 2 * S::KV_BYTES;
-                if constexpr (I8) {
-                    if (lane < runs && !there)
-                        for (int i = 0; i < R; i++)
-                            for (int x = 0; x < 2; x++) reinterpret_cast<float*>(stage + 2 * S::KV_BYTES + x * S::SCALE_BYTES)[lane * R + i] = 0.0f;
-                    bytes += __popc(__ballot_sync(0xffffffffu, there)) * R * 8;
-                }
-                __syncwarp();
-                if (lane == 0) kv_bar_expect(&full[st], bytes);
+                if (lane == 0) kv_bar_expect(&full[st], 2 * S::KV_BYTES);
                 __syncwarp();
                 if (lane < runs) {
-                    const int at = j & ((1 << P.pool.page_shift) - 1);
-                    const uint32_t k = kv_smem(stage), v = k + S::KV_BYTES;
+                    const int at = (j + lane * R) & ((1 << P.pool.page_shift) - 1);
+                    const uint32_t k_to = kv_smem(stage), v_to = k_to + S::KV_BYTES;
 #pragma unroll
                     for (int h = 0; h < (RB + 127) / 128; h++) {
                         const uint32_t to = h * (KR_TILE * 128) + lane * R * min(RB, 128);
-                        kv_tma4(k + to, &map_k, h * 64, at, walk.head, page, &full[st]);
-                        kv_tma4(v + to, &map_v, h * 64, at, walk.head, page, &full[st]);
+                        kv_tma4(k_to + to, &map_k, h * 64, at, walk.head, page, &full[st]);
+                        kv_tma4(v_to + to, &map_v, h * 64, at, walk.head, page, &full[st]);
                     }
-                    if constexpr (I8) {
-                        if (there) {
-                            const int64_t e = ((int64_t)page * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + at;
-                            const uint32_t s = v + S::KV_BYTES + lane * R * 4;
-                            kv_bulk(s, P.pool.ks + e, R * 4, &full[st]);
-                            kv_bulk(s + S::SCALE_BYTES, P.pool.vs + e, R * 4, &full[st]);
-                        }
-                    }
+                }
+                if constexpr (I8) {  // the scales: four positions a lane, of K by the first half of the warp, of V by the other
+                    const int pos = 4 * (lane & 15), of = __shfl_sync(0xffffffffu, pages, k * runs + pos / R);
+                    const bool there = of < P.pool.n_pages;
+                    const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((j + pos) & ((1 << P.pool.page_shift) - 1));
+                    kv_copy16(kv_smem(stage + 2 * S::KV_BYTES) + 16 * lane, (lane < 16 ? P.pool.ks : P.pool.vs) + e, there);
+                    kv_copy16_arrive(&full[st]);
                 }
                 if (++st == S::STAGES) { st = 0; ph ^= 1u; }
             }

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     if (tid == 0) {
         for (int i = 0; i < S::SLOTS; i++) { kv_bar_init(&full[i], I8 ? 4 : 1); kv_bar_init(&empty[i], I8 ? 2 : 6); kv_bar_init(&ready[i], 4); }
         for (int i = 0; i < (I8 ? S::RAWS : 1); i++) { kv_bar_init(&raw_full[i], 1); kv_bar_init(&raw_empty[i], 4); }
-        for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 1); kv_bar_init(&sc_empty[i], 8); }
+        for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 32); kv_bar_init(&sc_empty[i], 8); }
         for (int i = 0; i < 2; i++) {
             kv_bar_init(&q_full[i], 128); kv_bar_init(&drained[i], 1);
             for (int h = 0; h < 2; h++) { kv_bar_init(&s_full[i][h], 1); kv_bar_init(&p_full[i][h], 4); kv_bar_init(&pv_done[i][h], 1); }
@@ -620,19 +620,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     if constexpr (I8) {
                         wait(&sc_empty[sc], sc_ph);
                         if ((over = wait.over())) break;
-                        float* s = scales + sc * 2 * KT_TILE + lane * R;
-                        const bool there = lane < runs && page < P.pool.n_pages;
-                        if (lane < runs && !there)
-                            for (int i = 0; i < R; i++) s[i] = s[KT_TILE + i] = 0.0f;
-                        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * R * 8;
-                        __syncwarp();
-                        if (lane == 0) kv_bar_expect(&sc_full[sc], bytes);
-                        __syncwarp();
-                        if (there) {
-                            const int64_t e = ((int64_t)page * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + at;
-                            kv_bulk(kv_smem(s), P.pool.ks + e, R * 4, &sc_full[sc]);
-                            kv_bulk(kv_smem(s + KT_TILE), P.pool.vs + e, R * 4, &sc_full[sc]);
-                        }
+                        // four positions a lane, of K and of V
+                        const int x = 4 * lane, of = __shfl_sync(0xffffffffu, page, x / R);
+                        const bool there = of < P.pool.n_pages;
+                        const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((walk.view.base(t) + x) & ((1 << P.pool.page_shift) - 1));
+                        const uint32_t to = kv_smem(scales + sc * 2 * KT_TILE + x);
+                        kv_copy16(to, P.pool.ks + e, there);
+                        kv_copy16(to + 4 * KT_TILE, P.pool.vs + e, there);
+                        kv_copy16_arrive(&sc_full[sc]);
                         if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
                     }
 #pragma unroll
