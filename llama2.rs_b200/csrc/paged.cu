@@ -408,7 +408,7 @@ extern "C" size_t l2_kv_attend_workspace_bytes(const l2_kv_pages* pages, const l
     int sms;
     if (check_pages(who, pages, &pool) || check_batch(who, batch, pages->page_size, &step) || kv_device(&sms)) return 0;
     if (n_heads < 1 || n_heads % pool.n_kv_heads) { fail(L2_EINVAL, "%s: %d heads, %d kv heads", who, n_heads, pool.n_kv_heads); return 0; }
-    return kv_attend_work(step, pool, n_heads, pages->head_size, sms);
+    return kv_attend_work(step, pool, n_heads, pages->type, pages->head_size, sms);
 }
 
 extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* q, const l2_kv_rows* out, float scale, int window, int sinks,
@@ -427,7 +427,7 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);
     int sms;
     if (int rc = kv_device(&sms)) return rc;
-    const size_t need = kv_attend_work(P.step, P.pool, q->heads, pages->head_size, sms);
+    const size_t need = kv_attend_work(P.step, P.pool, q->heads, pages->type, pages->head_size, sms);
     if (workspace_bytes < need || (need && (!workspace || !aligned16(workspace)))) return fail(L2_EINVAL, "%s: a workspace of %zu bytes on a 16-byte boundary needed", who, need);
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
     P.scale_log2 = scale * 1.4426950408889634f;

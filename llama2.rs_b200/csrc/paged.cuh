@@ -143,6 +143,6 @@ __device__ __forceinline__ void kv_store8(const KvRows& r, int64_t row, int head
 #endif
 
 cudaError_t launch_kv_attend(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
-size_t kv_attend_work(const KvStep& s, const KvPool& p, int n_heads, int head_size, int sms);
+size_t kv_attend_work(const KvStep& s, const KvPool& p, int n_heads, int type, int head_size, int sms);
 
 }  // namespace l2

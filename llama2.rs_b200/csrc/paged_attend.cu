@@ -31,9 +31,9 @@ cudaError_t kv_map(CUtensorMap* map, const KvPool& p, const void* base, int type
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-size_t kv_attend_work(const KvStep& s, const KvPool& p, int n_heads, int head_size, int sms) {  // the kernels run one after the other
+size_t kv_attend_work(const KvStep& s, const KvPool& p, int n_heads, int type, int head_size, int sms) {  // the kernels run one after the other
     const int group = n_heads / p.n_kv_heads;
-    return std::max<size_t>(16, std::max(kv_rows_work(s, p, group, head_size, sms), kv_tc_work(s, p, group, head_size, sms)));
+    return std::max<size_t>(16, std::max(kv_rows_work(s, p, group, type, head_size, sms), kv_tc_work(s, p, group, head_size, sms)));
 }
 
 cudaError_t launch_kv_attend(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {

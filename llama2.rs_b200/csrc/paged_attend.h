@@ -47,7 +47,7 @@ cudaError_t kv_map(CUtensorMap* map, const KvPool& p, const void* base, int type
 // Sequences with at most this many rows (tokens x query heads per kv head) are taken by the kernel for few rows: all of a batch whose largest
 // sequence is that small, the single tokens of another; 0: none.
 int kv_rows_limit(const KvStep& s, int group);
-size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms);
+size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms);
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
 
 // The others: tcgen05.

@@ -92,36 +92,54 @@ __device__ __forceinline__ bool kv_sees(int pos, int j, int window, int sinks) {
 
 // ---- the line of tiles -----------------------------------------------------------------------------------------------------
 // The tiles of all sequences one after the other; CTA c of `ctas` takes positions c * per .. of it, per = total / ctas rounded up.
-struct KvSpot { int64_t total, start; int b; };  // its length; the sequence that a CTA's first position is in and where that begins (-1: there is none)
+struct KvSpot { int64_t per, total, start; int b; };  // its length; the sequence that a CTA's first position is in and where that begins (-1: there is none)
+
+__device__ __forceinline__ int64_t kv_quotient(int64_t a, int64_t b) {  // of numbers that are hardly ever beyond 32 bits
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int64_t kv_scan(int64_t v) {  // inclusive sum over the warp
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
 
 // By all threads of a CTA of THREADS.  len(b): tiles of sequence b, called by whole warps, 0 for b >= n.  Scratch: THREADS / 32 + 2 words of shared memory.
+// Up to 32 sequences: every warp by itself (with barriers between, the search took 3100 clocks of a kernel that takes 13000 for one token of one sequence).
 template <int THREADS, class Len>
-__device__ KvSpot kv_locate(int n, int cta, int ctas, int64_t* scratch, Len len) {
+__device__ __forceinline__ KvSpot kv_locate(int n, int cta, int ctas, int64_t* scratch, Len len) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto scan = [&](int64_t v) {  // inclusive, over the warp
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        return v;
-    };
-    const int64_t mine = len(tid);  // (most steps have no more sequences than threads)
+    KvSpot spot{0, 0, -1, n};
+    if (n <= 32) {
+        const int64_t v = len(lane), inc = kv_scan(v);
+        spot.total = __shfl_sync(0xffffffffu, inc, 31);
+        spot.per = kv_quotient(spot.total + ctas - 1, ctas);
+        const int64_t at = spot.per * cta;
+        if (at >= spot.total) return spot;
+        const int src = __ffs(__ballot_sync(0xffffffffu, inc > at)) - 1;
+        spot.b = src;
+        spot.start = __shfl_sync(0xffffffffu, inc - v, src);
+        return spot;
+    }
+    const int64_t mine = len(tid);
     int64_t sum = mine;
     for (int b0 = THREADS; b0 < n; b0 += THREADS) sum += len(b0 + tid);
-    sum = scan(sum);
+    sum = kv_scan(sum);
     if (lane == 31) scratch[warp] = sum;
     __syncthreads();
-    KvSpot spot{0, -1, n};
 #pragma unroll
     for (int w = 0; w < WARPS; w++) spot.total += scratch[w];
-    const int64_t at = (spot.total + ctas - 1) / ctas * cta;
+    spot.per = kv_quotient(spot.total + ctas - 1, ctas);
+    const int64_t at = spot.per * cta;
     if (at >= spot.total) return spot;
     int64_t before = 0;
     for (int b0 = 0; b0 < n; b0 += THREADS) {
         const int64_t v = b0 == 0 ? mine : len(b0 + tid);
-        const int64_t inc = scan(v);
+        const int64_t inc = kv_scan(v);
         __syncthreads();
         if (lane == 31) scratch[warp] = inc;
         if (tid == 0) scratch[WARPS] = -1;
@@ -141,8 +159,21 @@ __device__ KvSpot kv_locate(int n, int cta, int ctas, int64_t* scratch, Len len)
     return spot;
 }
 
-// Partial results of a CTA's first (slot 0) and last piece: `rows` times hd floats, then `rows` times (m, l).
-__device__ __forceinline__ float* kv_part(void* work, int rows, int hd, int64_t cta, int slot) { return static_cast<float*>(work) + (cta * 2 + slot) * rows * (hd + 2); }
+// What a CTA leaves for the kernel that adds the pieces of a block of rows: the block that begins in it and goes on in the next CTAs.
+struct alignas(16) KvCut {
+    int pieces;     // CTAs that have a piece; 0: no block begins here and goes on
+    int slot;       // of this CTA's piece: 0 its first, 1 its last
+    int rows, head; // of the block
+    int64_t row0;   // of the row arrays
+    int lo_pos, pad;
+};
+__device__ __forceinline__ KvCut* kv_cuts(void* work) { return static_cast<KvCut*>(work); }
+__host__ __device__ constexpr size_t kv_cut_bytes(int ctas) { return (size_t)ctas * sizeof(KvCut); }
+
+// Behind the cuts: partial results of a CTA's first (slot 0) and last piece: `rows` times hd floats, then `rows` times (m, l).
+__device__ __forceinline__ float* kv_part(void* work, int ctas, int rows, int hd, int64_t cta, int slot) {
+    return reinterpret_cast<float*>(static_cast<char*>(work) + kv_cut_bytes(ctas)) + (cta * 2 + slot) * rows * (hd + 2);
+}
 
 __device__ __forceinline__ void kv_store1(const KvRows& o, int64_t e, float x) {
     if (o.type == L2_F32) reinterpret_cast<float*>(o.data)[e] = x;

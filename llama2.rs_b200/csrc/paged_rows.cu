@@ -28,30 +28,33 @@ namespace l2 {
 
 namespace {
 
-constexpr int KR_TILE = 64, KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
+constexpr int KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
+constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
-// Shared memory of a variant: Q, the buffer in which the warps' results meet, the ring.
+// A variant: 16 KB of K and as much of V in a tile, 64 or 128 positions, of which a warp has 16 or 32 (an int8 cache with tiles of 64 positions was bound by the
+// chain of a warp's step, 2000 clocks whatever the bytes: 194 us where the same step over bf16, twice the bytes, takes 197).
+// Shared memory: Q and the ring; the warps' results meet in the slot of a piece's last tile.
 template <int CT, int HD, int NT>
 struct KrShape {
     static constexpr bool I8 = CT == L2_I8;
     static constexpr int ROWS = 8 * NT, ROW_BYTES = HD * (I8 ? 1 : 2);
+    static constexpr int TILE = ROW_BYTES == 256 ? 64 : 128, PER_WARP = TILE / KR_WARPS, MB = PER_WARP / 16;
     static constexpr int Q_PITCH = HD * 2 + 16;                                 // bytes between rows of Q: no bank conflicts
-    static constexpr int KV_BYTES = KR_TILE * ROW_BYTES;                        // K or V of a tile
-    static constexpr int SCALE_BYTES = I8 ? KR_TILE * 4 : 0;
+    static constexpr int KV_BYTES = TILE * ROW_BYTES;                           // K or V of a tile
+    static constexpr int SCALE_BYTES = I8 ? TILE * 4 : 0;
     static constexpr int STAGE = (2 * (KV_BYTES + SCALE_BYTES) + 1023) / 1024 * 1024;
-    static constexpr int MEET = ROWS * HD * 4;
-    static constexpr int FIXED = 1024 + MEET + ROWS * Q_PITCH;
+    static constexpr int FIXED = 1024 + ROWS * Q_PITCH;
     static constexpr int STAGES = (KR_SMEM - FIXED) / STAGE < KR_MAX_STAGES ? (KR_SMEM - FIXED) / STAGE : KR_MAX_STAGES;
     static constexpr int SMEM = FIXED + STAGES * STAGE;
-    static_assert(STAGES >= 2, "ring");
+    static_assert(STAGES >= 2 && KR_WARPS * ROWS * HD * 4 <= STAGE, "ring");
 };
 
-// Where byte `c16` (a 16-byte chunk) of row r of a tile is: rows of 128 bytes (two halves of a tile one after the other) or 64, as the TMA swizzles them.
-template <int ROW_BYTES>
+// Where 16-byte chunk c16 of row r of a tile is: rows of 128 bytes (two halves of a tile one after the other) or 64, as the TMA swizzles them.
+template <int ROW_BYTES, int TILE>
 __device__ __forceinline__ uint32_t kr_offset(int r, int c16) {
     if constexpr (ROW_BYTES == 64) return r * 64 + ((c16 ^ ((r >> 1) & 3)) << 4);
-    else return (c16 >> 3) * (KR_TILE * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
+    else return (c16 >> 3) * (TILE * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -74,51 +77,53 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // The line of tiles: sequence by sequence, kv head by kv head, tile by tile.
+template <int TILE>
 struct KrSeq {
     KvSeq s;
-    KvView<KR_TILE> view;
+    KvView<TILE> view;
     int rows;  // tokens x group, 0: not this kernel's
+    __device__ __forceinline__ KrSeq() {}
+    __device__ __forceinline__ KrSeq(const KvAttendParams& P, int lim, int b) {
+        s = kv_seq(P.step, P.pool.page_shift, b);
+        const int64_t n = (int64_t)s.n * P.group;
+        rows = n <= lim ? (int)n : 0;
+        view = KvView<TILE>(s.kv - s.n, s.kv - 1, P.window, P.sinks);
+    }
 };
-__device__ __forceinline__ KrSeq kr_seq(const KvAttendParams& P, int lim, int b) {
-    KrSeq q;
-    q.s = kv_seq(P.step, P.pool.page_shift, b);
-    const int64_t rows = (int64_t)q.s.n * P.group;
-    q.rows = rows <= lim ? (int)rows : 0;
-    q.view = KvView<KR_TILE>(q.s.kv - q.s.n, q.s.kv - 1, P.window, P.sinks);
-    return q;
-}
+template <int TILE>
 __device__ __forceinline__ int64_t kr_length(const KvAttendParams& P, int lim, int b) {
     if (b >= P.step.n_seqs) return 0;
-    const KrSeq q = kr_seq(P, lim, b);
+    const KrSeq<TILE> q(P, lim, b);
     return q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0;
 }
 
 // A CTA's piece of the line, one (sequence, kv head) at a time.
+template <int TILE>
 struct KrWalk {
-    int64_t w, w1, start;
+    int64_t w, w1, start, per;
     int b;
-    KrSeq q;
+    KrSeq<TILE> q;
     int head, t0, t1;
     bool first;  // the piece is the CTA's first
     __device__ __forceinline__ KrWalk(const KvAttendParams& P, int lim, const KvSpot& spot) {
-        const int64_t per = (spot.total + gridDim.x - 1) / gridDim.x;
+        per = spot.per;
         w = per * blockIdx.x;
         w1 = min(spot.total, w + per);
         start = spot.start; b = spot.b;
         first = true;
         t0 = -1;
-        if (w < w1) q = kr_seq(P, lim, b);
+        if (w < w1) q = KrSeq<TILE>(P, lim, b);
     }
     __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
         if (t0 >= 0) first = false;
         if (w >= w1) return false;
         while (w >= start + (q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0)) {
             if (q.rows) start += (int64_t)q.view.tiles * P.pool.n_kv_heads;
-            q = kr_seq(P, lim, ++b);
+            q = KrSeq<TILE>(P, lim, ++b);
         }
-        const int in = (int)(w - start);
-        head = in / q.view.tiles;
-        t0 = in - head * q.view.tiles;
+        const int64_t in = w - start;
+        head = (int)kv_quotient(in, q.view.tiles);
+        t0 = (int)(in - (int64_t)head * q.view.tiles);
         t1 = (int)min((int64_t)q.view.tiles, t0 + (w1 - w));
         w += t1 - t0;
         return true;
@@ -132,7 +137,8 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                                                                const __grid_constant__ CUtensorMap map_v) {
     using S = KrShape<CT, HD, NT>;
     constexpr bool I8 = S::I8, PB = I8 || QB;       // probabilities and V in bf16
-    constexpr int KS = HD / 16, MT = HD / 16, RB = S::ROW_BYTES;
+    constexpr int KS = HD / 16, MT = HD / 16, RB = S::ROW_BYTES, TILE = S::TILE, MB = S::MB;
+    constexpr float BIAS = PB ? 24.0f : 7.0f;       // probabilities carry a factor of 2^BIAS, so that small ones are normal numbers; f16 at most 2^(7 + KR_RAISE)
     extern __shared__ __align__(1024) uint8_t kr_smem[];
     __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES];
     __shared__ int64_t scratch[KR_THREADS / 32 + 2];
@@ -140,7 +146,6 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     __shared__ volatile int failed;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kr_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t* sq = ring + S::STAGES * S::STAGE;
-    float* meet = reinterpret_cast<float*>(sq + S::ROWS * S::Q_PITCH);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -150,19 +155,19 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const KvSpot spot = kv_locate<KR_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kr_length(P, lim, b); });  // (ends behind a barrier)
+    const KvSpot spot = kv_locate<KR_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kr_length<TILE>(P, lim, b); });
     __syncthreads();
-    KrWalk walk(P, lim, spot);
+    KrWalk<TILE> walk(P, lim, spot);
     const KvWait wait{&failed};
 
     if (warp == KR_WARPS) {
         // ================= copies: lane l brings run l of a tile ==============================================================
         // Pages are looked up for 32 runs at once, and for the next 32 while these are copied: a look-up takes as long as a tile's arithmetic.
-        const int R = min(KR_TILE, 1 << P.pool.page_shift), runs = KR_TILE / R, ahead = 32 / runs;
+        const int R = min(TILE, 1 << P.pool.page_shift), runs = TILE / R, ahead = 32 / runs;
         uint32_t st = 0, ph = 1;
         bool over = false;
         while (!over && walk.next(P, lim)) {
-            const KvView<KR_TILE>& view = walk.q.view;
+            const KvView<TILE>& view = walk.q.view;
             auto look_up = [&](int t) {  // lane l: run l % runs of tile t + l / runs; n_pages (a copy from there gives zeros) where no row sees it or there is none
                 const int mine = t + lane / runs, j = view.base(mine) + lane % runs * R;
                 if (mine >= walk.t1 || !view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
@@ -183,16 +188,18 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     const uint32_t k_to = kv_smem(stage), v_to = k_to + S::KV_BYTES;
 #pragma unroll
                     for (int h = 0; h < (RB + 127) / 128; h++) {
-                        const uint32_t to = h * (KR_TILE * 128) + lane * R * min(RB, 128);
+                        const uint32_t to = h * (TILE * 128) + lane * R * min(RB, 128);
                         kv_tma4(k_to + to, &map_k, h * 64, at, walk.head, page, &full[st]);
                         kv_tma4(v_to + to, &map_v, h * 64, at, walk.head, page, &full[st]);
                     }
                 }
-                if constexpr (I8) {  // the scales: four positions a lane, of K by the first half of the warp, of V by the other
-                    const int pos = 4 * (lane & 15), of = __shfl_sync(0xffffffffu, pages, k * runs + pos / R);
+                if constexpr (I8) {  // the scales: four positions a lane, of K and of V
+                    const int pos = 4 * lane, of = __shfl_sync(0xffffffffu, pages, k * runs + pos / R);
                     const bool there = of < P.pool.n_pages;
                     const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((j + pos) & ((1 << P.pool.page_shift) - 1));
-                    kv_copy16(kv_smem(stage + 2 * S::KV_BYTES) + 16 * lane, (lane < 16 ? P.pool.ks : P.pool.vs) + e, there);
+                    const uint32_t to = kv_smem(stage + 2 * S::KV_BYTES) + 16 * lane;
+                    kv_copy16(to, P.pool.ks + e, there);
+                    kv_copy16(to + S::SCALE_BYTES, P.pool.vs + e, there);
                     kv_copy16_arrive(&full[st]);
                 }
                 if (++st == S::STAGES) { st = 0; ph ^= 1u; }
@@ -203,7 +210,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
         const int c = lane & 3, g8 = lane >> 2;
         uint32_t st = 0, ph = 0;
         while (walk.next(P, lim)) {
-            const KrSeq& seq = walk.q;
+            const KrSeq<TILE>& seq = walk.q;
             const int rows = seq.rows, G = P.group;
             // Q into shared memory: rows beyond the last are zeros
             asm volatile("bar.sync 1, 128;" ::: "memory");  // (everybody has read the piece before's)
@@ -249,142 +256,161 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 __syncwarp();
                 const uint8_t* stage = ring + st * S::STAGE;
                 const uint32_t k_at = kv_smem(stage), v_at = k_at + S::KV_BYTES;
-                // ---- scores of this warp's 16 positions: rows g8 and g8 + 8, columns 2 c and 2 c + 1
-                float s[NT][4];
+                // ---- scores of this warp's positions, 16 at a time: rows g8 and g8 + 8, columns 2 c and 2 c + 1
+                float s[MB][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-                const int kr = 16 * warp + (lane & 15);
-                auto by_k = [&](int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[nt], a0, a1, a2, a3, qr[nt][ks][0], qr[nt][ks][1]);
+                    for (int nt = 0; nt < NT; nt++) s[mb][nt][0] = s[mb][nt][1] = s[mb][nt][2] = s[mb][nt][3] = 0.0f;
+                const int kr = S::PER_WARP * warp + (lane & 15);
+                auto by_k = [&](int mb, int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[mb][nt], a0, a1, a2, a3, qr[nt][ks][0], qr[nt][ks][1]);
                 };
                 if constexpr (I8) {
 #pragma unroll
-                    for (int c2 = 0; c2 < KS / 2; c2++) {  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
-                        uint32_t a[4];
-                        ldsm4(a, k_at + kr_offset<RB>(kr, 2 * c2 + (lane >> 4)));
-                        by_k(2 * c2, widen<QB, 0x10>(a[0]), widen<QB, 0x10>(a[1]), widen<QB, 0x32>(a[0]), widen<QB, 0x32>(a[1]));
-                        by_k(2 * c2 + 1, widen<QB, 0x10>(a[2]), widen<QB, 0x10>(a[3]), widen<QB, 0x32>(a[2]), widen<QB, 0x32>(a[3]));
-                    }
+                    for (int c2 = 0; c2 < KS / 2; c2++)  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
+#pragma unroll
+                        for (int mb = 0; mb < MB; mb++) {
+                            uint32_t a[4];
+                            ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
+                            by_k(mb, 2 * c2, widen<QB, 0x10>(a[0]), widen<QB, 0x10>(a[1]), widen<QB, 0x32>(a[0]), widen<QB, 0x32>(a[1]));
+                            by_k(mb, 2 * c2 + 1, widen<QB, 0x10>(a[2]), widen<QB, 0x10>(a[3]), widen<QB, 0x32>(a[2]), widen<QB, 0x32>(a[3]));
+                        }
                 } else {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        uint32_t a[4];
-                        ldsm4(a, k_at + kr_offset<RB>(kr, 2 * ks + (lane >> 4)));
-                        by_k(ks, a[0], a[1], a[2], a[3]);
-                    }
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int mb = 0; mb < MB; mb++) {
+                            uint32_t a[4];
+                            ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * ks + (lane >> 4)));
+                            by_k(mb, ks, a[0], a[1], a[2], a[3]);
+                        }
                 }
                 // ---- softmax
-                float f0 = P.scale_log2, f1 = P.scale_log2, v0 = 1.0f, v1 = 1.0f;
-                const int j0 = base + 16 * warp + g8;
-                if constexpr (I8) {
-                    const float* sc = reinterpret_cast<const float*>(stage + 2 * S::KV_BYTES) + 16 * warp + g8;
-                    f0 *= sc[0]; f1 *= sc[8];
-                    v0 = sc[KR_TILE]; v1 = sc[KR_TILE + 8];
-                }
-                bool moved = false;
-                float m1[NT][2];
+                const int j0 = base + S::PER_WARP * warp + g8;  // this thread's positions: j0 + 16 mb, and 8 more
+                auto sees = [&](int nt, int mb, int i) { return kv_sees(pos[nt][i & 1], j0 + 16 * mb + 8 * (i >> 1), P.window, P.sinks); };
+                float v_scale[MB][2], most[NT][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    s[nt][0] *= f0; s[nt][1] *= f0; s[nt][2] *= f1; s[nt][3] *= f1;
-                    if (!whole) {
+                for (int nt = 0; nt < NT; nt++) most[nt][0] = most[nt][1] = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (!kv_sees(pos[nt][i & 1], j0 + 8 * (i >> 1), P.window, P.sinks)) s[nt][i] = -INFINITY;
+                for (int mb = 0; mb < MB; mb++) {
+                    float f0 = P.scale_log2, f1 = P.scale_log2;
+                    if constexpr (I8) {
+                        const float* sc = reinterpret_cast<const float*>(stage + 2 * S::KV_BYTES) + S::PER_WARP * warp + 16 * mb + g8;
+                        f0 *= sc[0]; f1 *= sc[8];
+                        v_scale[mb][0] = sc[TILE]; v_scale[mb][1] = sc[TILE + 8];
                     }
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float x = fmaxf(s[nt][e], s[nt][e + 2]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        // probabilities carry a factor of 2^15 or, in bf16, 2^24, so that small ones are normal numbers
-                        m1[nt][e] = fmaxf(m[nt][e], x - (PB ? 24.0f : 15.0f));
-                        moved |= m1[nt][e] != m[nt][e];
+                    for (int nt = 0; nt < NT; nt++) {
+                        s[mb][nt][0] *= f0; s[mb][nt][1] *= f0; s[mb][nt][2] *= f1; s[mb][nt][3] *= f1;
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (!sees(nt, mb, i)) s[mb][nt][i] = -INFINITY;
+                        }
+                        most[nt][0] = fmaxf(most[nt][0], fmaxf(s[mb][nt][0], s[mb][nt][2]));
+                        most[nt][1] = fmaxf(most[nt][1], fmaxf(s[mb][nt][1], s[mb][nt][3]));
                     }
                 }
-                if (__any_sync(0xffffffffu, moved)) {
+                bool raise = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) raise |= most[nt][0] - BIAS > m[nt][0] + KR_RAISE || most[nt][1] - BIAS > m[nt][1] + KR_RAISE;
+                if (__any_sync(0xffffffffu, raise)) {  // seldom: only then do the lanes of a row need their common maximum
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const KvScale f(m1[nt][e] == -INFINITY ? 0.0f : m[nt][e] - m1[nt][e]);
-                            m[nt][e] = m1[nt][e];
+                            float x = most[nt][e] - BIAS;
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            const float m1 = x > m[nt][e] + KR_RAISE ? x : m[nt][e];  // (a row's result does not depend on the others)
+                            const KvScale f(m1 == -INFINITY ? 0.0f : m[nt][e] - m1);
+                            m[nt][e] = m1;
                             l[nt][e] = f(l[nt][e]);
 #pragma unroll
                             for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
                         }
                 }
-                uint32_t pb[NT][2];
+                uint32_t pb[MB][NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    float p[4];
+                    const float ref[2] = {m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m[nt][1] == -INFINITY ? 0.0f : m[nt][1]};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float ref = m[nt][i & 1] == -INFINITY ? 0.0f : m[nt][i & 1];
-                        p[i] = kv_exp2(s[nt][i] - ref);
-                        l[nt][i & 1] += p[i];
-                        if constexpr (I8) p[i] = !whole && !kv_sees(pos[nt][i & 1], j0 + 8 * (i >> 1), P.window, P.sinks) ? 0.0f : p[i] * (i < 2 ? v0 : v1);
+                    for (int mb = 0; mb < MB; mb++) {
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            p[i] = kv_exp2(s[mb][nt][i] - ref[i & 1]);
+                            l[nt][i & 1] += p[i];
+                            if constexpr (I8) p[i] = !whole && !sees(nt, mb, i) ? 0.0f : p[i] * v_scale[mb][i >> 1];
+                        }
+                        pb[mb][nt][0] = transpose8(pack16<PB>(p[0], p[1]));
+                        pb[mb][nt][1] = transpose8(pack16<PB>(p[2], p[3]));
                     }
-                    pb[nt][0] = transpose8(pack16<PB>(p[0], p[1]));
-                    pb[nt][1] = transpose8(pack16<PB>(p[2], p[3]));
                 }
                 // ---- O^T += V^T P^T
-                const int vr = 16 * warp + (lane & 7) + 8 * (lane >> 4);
-                uint32_t odd = 0;
-                if constexpr (I8) {
+                const int vr = S::PER_WARP * warp + (lane & 7) + 8 * (lane >> 4);
 #pragma unroll
-                    for (int m2 = 0; m2 < (MT + 1) / 2; m2++) {  // 32 elements; row i of a product is element 2 i, row 8 + i element 2 i + 1
-                        uint32_t a[4];
-                        ldsm4_t(a, v_at + kr_offset<RB>(vr, 2 * m2 + ((lane >> 3) & 1)));
+                for (int mb = 0; mb < MB; mb++) {
+                    if constexpr (I8) {
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t x0 = widen<true, 0x20>(a[h]), x1 = widen<true, 0x31>(a[h]), x2 = widen<true, 0x20>(a[h + 2]), x3 = widen<true, 0x31>(a[h + 2]);
+                        for (int m2 = 0; m2 < (MT + 1) / 2; m2++) {  // 32 elements; row i of a product is element 2 i, row 8 + i element 2 i + 1
+                            uint32_t a[4];
+                            ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * m2 + ((lane >> 3) & 1)));
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) mma<true>(o[2 * m2 + h][nt], x0, x1, x2, x3, pb[nt][0], pb[nt][1]);
-                        }
-                    }
-                } else {
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t x0 = widen<true, 0x20>(a[h]), x1 = widen<true, 0x31>(a[h]), x2 = widen<true, 0x20>(a[h + 2]), x3 = widen<true, 0x31>(a[h + 2]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        uint32_t a[4];
-                        ldsm4_t(a, v_at + kr_offset<RB>(vr, 2 * mt + ((lane >> 3) & 1)));
-                        if (!whole) {  // 0 x NaN is NaN: a value that some row does not see may only be multiplied where it is finite
-                            if (__any_sync(0xffffffffu, not_finite<PB>(a[0]) | not_finite<PB>(a[1]) | not_finite<PB>(a[2]) | not_finite<PB>(a[3]))) {
-                                odd = 1;
-#pragma unroll
-                                for (int i = 0; i < 4; i++) a[i] = only_finite<PB>(a[i]);
+                                for (int nt = 0; nt < NT; nt++) mma<true>(o[2 * m2 + h][nt], x0, x1, x2, x3, pb[mb][nt][0], pb[mb][nt][1]);
                             }
                         }
+                    } else {
+                        bool odd = false;
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma<PB>(o[mt][nt], a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
-                    }
-                    if (odd) {  // rare: the values that are not finite, one by one, to the rows that see them
-#pragma unroll 1
-                        for (int i = 0; i < 16; i++) {
-                            const int r = 16 * warp + i;
+                        for (int mt = 0; mt < MT; mt++) {
+                            uint32_t a[4];
+                            ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * mt + ((lane >> 3) & 1)));
+                            if (!whole) {  // 0 x NaN is NaN: a value that some row does not see may only be multiplied where it is finite
+                                if (__any_sync(0xffffffffu, not_finite<PB>(a[0]) | not_finite<PB>(a[1]) | not_finite<PB>(a[2]) | not_finite<PB>(a[3]))) {
+                                    odd = true;
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                                for (int h = 0; h < 2; h++) {
-                                    const uint16_t bits = *reinterpret_cast<const uint16_t*>(stage + S::KV_BYTES + kr_offset<RB>(r, 2 * mt + h) + 2 * g8);
-                                    if (not_finite<PB>(bits)) {
-                                        const float x = PB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
-#pragma unroll
-                                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                                            for (int e = 0; e < 2; e++)
-                                                if (kv_sees(pos[nt][e], base + r, P.window, P.sinks)) o[mt][nt][2 * h + e] += x;
-                                    }
+                                    for (int i = 0; i < 4; i++) a[i] = only_finite<PB>(a[i]);
                                 }
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma<PB>(o[mt][nt], a[0], a[1], a[2], a[3], pb[mb][nt][0], pb[mb][nt][1]);
+                        }
+                        if (odd) {  // rare: the values that are not finite, one by one, to the rows that see them
+#pragma unroll 1
+                            for (int i = 0; i < 16; i++) {
+                                const int r = S::PER_WARP * warp + 16 * mb + i;
+#pragma unroll
+                                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                                    for (int h = 0; h < 2; h++) {
+                                        const uint16_t bits = *reinterpret_cast<const uint16_t*>(stage + S::KV_BYTES + kr_offset<RB, TILE>(r, 2 * mt + h) + 2 * g8);
+                                        if (not_finite<PB>(bits)) {
+                                            const float x = PB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+#pragma unroll
+                                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                                for (int e = 0; e < 2; e++)
+                                                    if (kv_sees(pos[nt][e], base + r, P.window, P.sinks)) o[mt][nt][2 * h + e] += x;
+                                        }
+                                    }
+                            }
                         }
                     }
                 }
-                __syncwarp();
-                if (lane == 0) kv_bar_arrive(&empty[st]);
-                if (++st == S::STAGES) { st = 0; ph ^= 1u; }
+                if (t + 1 < walk.t1) {  // (the last tile's slot is kept for the meeting)
+                    __syncwarp();
+                    if (lane == 0) kv_bar_arrive(&empty[st]);
+                    if (++st == S::STAGES) { st = 0; ph ^= 1u; }
+                }
             }
-            // ---- the four warps' results meet: a common maximum, then sums in a fixed order (warp 3's into 2's into 1's into 0's)
+            // ---- the four warps' results meet: a common maximum, then each warp adds a quarter of the elements, in the order of the warps
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -393,10 +419,10 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     x += __shfl_xor_sync(0xffffffffu, x, 4);
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    l[nt][e] = x;
                     if (g8 == 0) { meet_ml[warp][8 * nt + 2 * c + e][0] = m[nt][e]; meet_ml[warp][8 * nt + 2 * c + e][1] = x; }
                 }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // (and everybody is done with the last tile)
+            float4* meet = reinterpret_cast<float4*>(ring + st * S::STAGE);  // [warp][product][lane]
             float lsum[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -416,47 +442,52 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                     for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
                 }
 #pragma unroll
-            for (int from = KR_WARPS - 1; from > 0; from--) {
-                if (warp == from) {
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int i = 0; i < MT * NT; i++) *reinterpret_cast<float4*>(meet + (i * 32 + lane) * 4) = *reinterpret_cast<float4*>(o[i / NT][i % NT]);
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (warp == from - 1) {
+                for (int nt = 0; nt < NT; nt++) meet[(warp * MT * NT + mt * NT + nt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            constexpr int SHARE = MT / KR_WARPS;  // products of a warp
+            const bool done = walk.whole();
+            float* part = kv_part(P.work, gridDim.x, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
 #pragma unroll
-                    for (int i = 0; i < MT * NT; i++) {
-                        const float4 x = *reinterpret_cast<const float4*>(meet + (i * 32 + lane) * 4);
-                        float* y = o[i / NT][i % NT];
-                        y[0] += x.x; y[1] += x.y; y[2] += x.z; y[3] += x.w;
+            for (int x = 0; x < SHARE; x++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const int mt = SHARE * warp + x;
+                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int w = 0; w < KR_WARPS; w++) {
+                        const float4 z = meet[(w * MT * NT + mt * NT + nt) * 32 + lane];
+                        y[0] += z.x; y[1] += z.y; y[2] += z.z; y[3] += z.w;
                     }
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-            }
-            if (warp == 0) {
-                const bool done = walk.whole();
-                float* part = kv_part(P.work, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int r = 8 * nt + 2 * c + e;
                         if (r >= rows) continue;
                         const int tok = r / G;
                         const int64_t at = (seq.s.row0 + tok) * P.out.row_stride + (int64_t)(walk.head * G + r - tok * G) * P.out.head_stride;
-                        const float inv = pos[nt][e] < 0 ? 0.0f : 1.0f / lsum[nt][e];
+                        const float inv = 1.0f / lsum[nt][e];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const int d = I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
-                                const float x = o[mt][nt][2 * h + e];
-                                if (done) kv_store1(P.out, at + d, pos[nt][e] < 0 ? 0.0f : x * inv);
-                                else part[r * HD + d] = x;
-                            }
-                        if (!done && g8 == 0) *reinterpret_cast<float2*>(part + S::ROWS * HD + 2 * r) = make_float2(m[nt][e], lsum[nt][e]);
+                        for (int h = 0; h < 2; h++) {
+                            const int d = I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
+                            if (done) kv_store1(P.out, at + d, pos[nt][e] < 0 ? 0.0f : y[2 * h + e] * inv);
+                            else part[r * HD + d] = y[2 * h + e];
+                        }
+                        if (!done && warp == 0 && x == 0 && g8 == 0) *reinterpret_cast<float2*>(part + S::ROWS * HD + 2 * r) = make_float2(m[nt][e], lsum[nt][e]);
                     }
+                }
+            if (warp == 0 && lane == 0 && walk.w >= walk.w1) {  // what the kernel behind this one has to know
+                KvCut cut{0, 0, 0, 0, 0, 0, 0};
+                if (walk.t0 == 0 && !done)
+                    cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + seq.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, rows, walk.head, seq.s.row0, seq.view.lo_pos, 0};
+                kv_cuts(P.work)[blockIdx.x] = cut;
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the slot goes back to the copies)
+            __syncwarp();
+            if (lane == 0) kv_bar_arrive(&empty[st]);
+            if (++st == S::STAGES) { st = 0; ph ^= 1u; }
         }
+        if (tid == 0 && walk.t0 < 0) kv_cuts(P.work)[blockIdx.x].pieces = 0;  // (a CTA without work)
     }
     __syncthreads();
     if (failed) {  // copies may still be on their way into this CTA's shared memory: a bounded time to land
@@ -466,38 +497,33 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     }
 }
 
-// Adds the pieces of the pairs that cuts go through: CTA x looks at cut x + 1 and takes the pair in it if that is the pair's first cut.
+// Adds the pieces of the pair that begins in CTA x of the launch in front and goes on in the next.
 // HD / 4 threads for a row; with fewer than eight rows the others take pieces of the same row, and meet in order.
 template <int HD>
-__global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int ctas, const int part_rows) {
+__global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_constant__ KvAttendParams P, const int ctas, const int part_rows) {
     constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
-    __shared__ int64_t scratch[256 / 32 + 2];
     __shared__ float4 sums[256];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int cut = blockIdx.x + 1;
-    const KvSpot spot = kv_locate<256>(P.step.n_seqs, cut, ctas, scratch, [&](int b) { return kr_length(P, lim, b); });
-    if (spot.start < 0) return;
-    const int64_t per = (spot.total + ctas - 1) / ctas, at = per * cut;
-    const KrSeq q = kr_seq(P, lim, spot.b);
-    const int T = q.view.tiles, head = (int)((at - spot.start) / T);
-    const int64_t from = spot.start + (int64_t)head * T, to = from + T;
-    if (from == at || from / per != cut - 1) return;
-    const int c0 = cut - 1, n = (int)((to - 1) / per) - c0 + 1;
-    auto piece = [&](int i) { return kv_part(P.work, part_rows, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const KvCut cut = kv_cuts(P.work)[blockIdx.x];
+    if (!cut.pieces) return;
+    auto piece = [&](int i) { return kv_part(P.work, ctas, part_rows, HD, blockIdx.x + i, i == 0 ? cut.slot : 0); };
     int width = 1;  // rows side by side
-    while (width < q.rows && width < SLOTS) width <<= 1;
+    while (width < cut.rows && width < SLOTS) width <<= 1;
     const int share = SLOTS / width, slot = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES), mine = slot / width;
-    for (int r0 = 0; r0 < q.rows; r0 += width) {
+    for (int r0 = 0; r0 < cut.rows; r0 += width) {
         const int r = r0 + slot % width;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.0f;
-        if (r < q.rows) {
+        if (r < cut.rows) {
             float top = -INFINITY;
-            for (int i = 0; i < n; i++) top = fmaxf(top, piece(i)[part_rows * HD + 2 * r]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            for (int i = 0; i < n; i++) sum += KvScale(piece(i)[part_rows * HD + 2 * r] - ref)(piece(i)[part_rows * HD + 2 * r + 1]);
 #pragma unroll 4
-            for (int i = mine; i < n; i += share) {
+            for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[part_rows * HD + 2 * r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+            for (int i = 0; i < cut.pieces; i++) sum += KvScale(piece(i)[part_rows * HD + 2 * r] - ref)(piece(i)[part_rows * HD + 2 * r + 1]);
+#pragma unroll 4
+            for (int i = mine; i < cut.pieces; i += share) {
                 const float* p = piece(i);
                 const KvScale f(p[part_rows * HD + 2 * r] - ref);
                 const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
@@ -513,9 +539,9 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
             }
             __syncthreads();
         }
-        if (r < q.rows && mine == 0) {
-            const int tok = r / P.group, pos = q.view.lo_pos + tok;
-            const int64_t e = (q.s.row0 + tok) * P.out.row_stride + (int64_t)(head * P.group + r - tok * P.group) * P.out.head_stride + d;
+        if (r < cut.rows && mine == 0) {
+            const int tok = r / P.group, pos = cut.lo_pos + tok;
+            const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride + d;
             const float inv = 1.0f / sum;
             const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
@@ -536,9 +562,10 @@ cudaError_t kr_by_variant(int type, bool qb, int hd, int nt, F f) {
 }
 
 int kr_nt(int lim) { return lim <= 8 ? 1 : 2; }
+int kr_tile(int type, int head_size) { return head_size * (type == L2_I8 ? 1 : 2) == 256 ? 64 : 128; }
 // CTAs of a launch: two an SM, no more than there can be tiles
-int kr_grid(const KvStep& s, const KvPool& p, int sms) {
-    const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KR_TILE - 1) / KR_TILE + 1);
+int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
+    const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + tile - 1) / tile + 1);
     return (int)std::min<int64_t>(2 * sms, tiles);
 }
 
@@ -549,18 +576,21 @@ int kv_rows_limit(const KvStep& s, int group) {
     return most <= 16 ? (int)most : group <= 16 ? group : 0;
 }
 
-size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
+size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms) {
     const int lim = kv_rows_limit(s, group);
-    return lim ? (size_t)kr_grid(s, p, sms) * 2 * 8 * kr_nt(lim) * (head_size + 2) * sizeof(float) : 0;
+    if (!lim) return 0;
+    const int grid = kr_grid(s, p, kr_tile(type, head_size), sms);
+    return kv_cut_bytes(grid) + (size_t)grid * 2 * 8 * kr_nt(lim) * (head_size + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
     const int lim = kv_rows_limit(p.step, p.group);
     if (!lim) return cudaSuccess;
+    const int tile = kr_tile(type, head_size);
     CUtensorMap mk, mv;
-    if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, KR_TILE)) return e;
-    if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, KR_TILE)) return e;
-    const int nt = kr_nt(lim), grid = kr_grid(p.step, p.pool, sms);
+    if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, tile)) return e;
+    if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, tile)) return e;
+    const int nt = kr_nt(lim), grid = kr_grid(p.step, p.pool, tile, sms);
     cudaError_t e = kr_by_variant(type, p.q.type == L2_BF16, head_size, nt, [&](auto t, auto b, auto h, auto n) {
         constexpr int T = decltype(t)::value, HD = decltype(h)::value, NT = decltype(n)::value;
         auto kernel = kv_rows_kernel<T, decltype(b)::value, HD, NT>;
@@ -570,7 +600,7 @@ cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int
     });
     if (e != cudaSuccess || grid < 2) return e;
     auto combine = head_size == 128 ? kv_rows_combine_kernel<128> : kv_rows_combine_kernel<64>;
-    return kv_launch(combine, dim3(grid - 1), 256, 0, st, p, lim, grid, 8 * nt);
+    return kv_launch(combine, dim3(grid - 1), 256, 0, st, p, grid, 8 * nt);
 }
 
 }  // namespace l2

@@ -17,6 +17,7 @@
 //                   S = Q K of the same half of the next tile, and so on; the softmax finds the next scores ready.  (One warp for both was the bound: the issue of a product
 //                   takes 80 clocks, and every wait adds a few hundred.)
 //   warp 1          K and V tiles by TMA into one ring, a copy a page run
+//   warp 3          leaves the kernel behind this one a record of the block that the CTA's end cuts
 //   warps 4-7, 8-11 softmax of Q0 and Q1, a row a thread; they bring Q, and the result out
 //   warps 12-15     16-bit caches: tiles that some row sees in part are searched for values that are not finite: 0 x NaN is NaN, and a row must not be
 //                   reached by what it does not see.  They are taken out before the product and added to the rows that see them at the end.
@@ -188,20 +189,20 @@ __device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBl
 __device__ __forceinline__ int kt_token(const KvAttendParams& P, int row) { return row * P.group_inv >> 16; }
 
 struct KtWalk {
-    int64_t w, w1;
+    int64_t w, w1, per;
     int b, head, block, skip;  // skip: tiles of the first block that belong to the CTA in front
     KtBlocks k;
     KvView<KT_TILE> view;
     int t0, t1, rows, index;   // rows of the block; pieces before this one
     __device__ __forceinline__ KtWalk(const KvAttendParams& P, int lim, const KvSpot& spot) {
-        const int64_t per = (spot.total + gridDim.x - 1) / gridDim.x;
+        per = spot.per;
         w = per * blockIdx.x;
         w1 = min(spot.total, w + per);
         b = spot.b; index = -1; head = block = skip = 0;
         if (w >= w1) return;
         k = kt_blocks(P, lim, b);
         const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = w - spot.start;
-        head = (int)(in / tiles);
+        head = (int)kv_quotient(in, tiles);
         int64_t before;
         block = kt_find_block(P, k, in - head * tiles, &before);
         skip = (int)(in - head * tiles - before);
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             }
             if (128 * i >= walk.rows) continue;  // (whole warps: this tile has no rows)
             const bool fix = !I8 && started && odd[walk.index & 7];
-            float* part = kv_part(P.work, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
+            float* part = kv_part(P.work, gridDim.x, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
             const float inv = done && pos >= 0 ? 1.0f / l : 1.0f;
             // A whole block's result goes through this tile's room of Q (its products are done), so that rows leave in whole lines.
             uint8_t* stage = sq + i * S::SLOT;
@@ -648,6 +649,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     page = ahead;
                 }
             }
+        } else if (warp == KT_COPY_WARP + 2) {
+            // ================= what the next kernel has to know ======================================================================
+            KvCut cut{0, 0, 0, 0, 0, 0, 0};
+            while (walk.next(P, lim))
+                if (walk.t0 == 0 && walk.t1 < walk.view.tiles)
+                    cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + walk.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.index ? 1 : 0, walk.rows, walk.head,
+                                (int64_t)walk.k.s.row0 + walk.block * walk.k.tokens, walk.view.lo_pos, 0};
+            if (lane == 0) kv_cuts(P.work)[blockIdx.x] = cut;
         } else if (warp >= KT_HELP_WARP) {
             const int r = tid & 127;
             if constexpr (I8) {
@@ -736,34 +745,23 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 
 constexpr int KT_COMBINE_SPLIT = 8;  // CTAs that share the rows of a block
 
-// Adds the pieces of the blocks that cuts go through: CTA x looks at cut x + 1 and takes the block in it if that is the block's first cut.
+// Adds the pieces of the block of rows that begins in CTA x of the launch in front and goes on in the next.
 template <int HD>
-__global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int ctas) {
+__global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constant__ KvAttendParams P, const int ctas) {
     constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
-    __shared__ int64_t scratch[256 / 32 + 2];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int cut = blockIdx.x + 1;
-    const KvSpot spot = kv_locate<256>(P.step.n_seqs, cut, ctas, scratch, [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
-    if (spot.start < 0) return;
-    const int64_t per = (spot.total + ctas - 1) / ctas, at = per * cut;
-    const KtBlocks k = kt_blocks(P, lim, spot.b);
-    const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = at - spot.start;
-    const int head = (int)(in / tiles);
-    int64_t before;
-    const int block = kt_find_block(P, k, in - head * tiles, &before);
-    const KvView<KT_TILE> view = kt_view(P, k, block);
-    const int64_t from = spot.start + head * tiles + before, to = from + view.tiles;
-    if (from == at || from / per != cut - 1) return;
-    const int c0 = cut - 1, n = (int)((to - 1) / per) - c0 + 1;
-    auto piece = [&](int i) { return kv_part(P.work, KT_ROWS, HD, c0 + i, i == 0 && from > c0 * per ? 1 : 0); };
-    const int rows = min(k.tokens, k.s.n - block * k.tokens) * P.group, d = 4 * (threadIdx.x % LANES);
-    for (int r = blockIdx.y * SLOTS + threadIdx.x / LANES; r < rows; r += KT_COMBINE_SPLIT * SLOTS) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const KvCut cut = kv_cuts(P.work)[blockIdx.x];
+    const int d = 4 * (threadIdx.x % LANES);
+    auto piece = [&](int i) { return kv_part(P.work, ctas, KT_ROWS, HD, blockIdx.x + i, i == 0 ? cut.slot : 0); };
+    if (!cut.pieces) return;
+    for (int r = blockIdx.y * SLOTS + threadIdx.x / LANES; r < cut.rows; r += KT_COMBINE_SPLIT * SLOTS) {
         float top = -INFINITY, sum = 0.0f;
-        for (int i = 0; i < n; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
+        for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int i = 0; i < n; i++) {
+        for (int i = 0; i < cut.pieces; i++) {
             const float* p = piece(i);
             const float2 ml = *reinterpret_cast<const float2*>(p + KT_ROWS * HD + 2 * r);
             const KvScale f(ml.x - ref);
@@ -771,8 +769,8 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
             sum += f(ml.y);
             acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
         }
-        const int tok = r / P.group, pos = view.lo_pos + tok;
-        const int64_t e = ((int64_t)k.s.row0 + block * k.tokens + tok) * P.out.row_stride + (int64_t)(head * P.group + r - tok * P.group) * P.out.head_stride + d;
+        const int tok = r / P.group, pos = cut.lo_pos + tok;
+        const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride + d;
         const float inv = 1.0f / sum;
         const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
@@ -791,7 +789,9 @@ bool kt_needed(const KvStep& s, int group) { return (int64_t)s.max_rows * group 
 }  // namespace
 
 size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
-    return kt_needed(s, group) ? (size_t)kt_grid(s, p, group, sms) * 2 * KT_ROWS * (head_size + 2) * sizeof(float) : 0;
+    if (!kt_needed(s, group)) return 0;
+    const int grid = kt_grid(s, p, group, sms);
+    return kv_cut_bytes(grid) + (size_t)grid * 2 * KT_ROWS * (head_size + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
@@ -814,7 +814,7 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
     if (e != cudaSuccess || grid < 2) return e;
     auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;
-    return kv_launch(combine, dim3(grid - 1, KT_COMBINE_SPLIT), 256, 0, st, p, lim, grid);
+    return kv_launch(combine, dim3(grid - 1, KT_COMBINE_SPLIT), 256, 0, st, p, grid);
 }
 
 }  // namespace l2
