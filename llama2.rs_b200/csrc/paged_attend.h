@@ -44,8 +44,9 @@ cudaError_t kv_launch(void (*kernel)(A...), dim3 grid, int threads, size_t smem,
 // row, where that is less), swizzled accordingly.
 cudaError_t kv_map(CUtensorMap* map, const KvPool& p, const void* base, int type, int head_size, int tile);
 
-// Sequences with at most this many rows (tokens x query heads per kv head) are taken by the kernel for few rows: all of a batch whose largest
-// sequence is that small, the single tokens of another; 0: none.
+// Sequences with at most this many rows (tokens x query heads per kv head) are taken by the kernel for few rows, the others by the tcgen05 kernel: all of a
+// batch whose largest sequence is that small, the single tokens of another; 0: none (there is room for as many rows as the largest sequence has for
+// every one: a batch of one kind, which one kernel takes whole).
 int kv_rows_limit(const KvStep& s, int group);
 size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms);
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);

@@ -189,7 +189,9 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
     constexpr uint32_t sel = 0x4040u | (SEL & 15u) | ((SEL >> 4) & 15u) << 8;
     if constexpr (BF) {  // 0x4300 | x is 128 + x for x < 128: 128 + (low seven bits) minus 128 or, for a negative byte, 256
         const uint32_t t = __byte_perm(w, 0, sel);
-        const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
+        uint32_t a, b;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(a) : "r"(t), "r"(0x007f007fu), "r"(0x43004300u));
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(b) : "r"(t), "r"(0x00800080u), "r"(0x43004300u));
         asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     } else {             // 0x6400 | x is 1024 + x: with the sign bit turned over, 1024 + 128 + byte
         const uint32_t t = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);

@@ -573,7 +573,8 @@ int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
 
 int kv_rows_limit(const KvStep& s, int group) {
     const int64_t most = (int64_t)s.max_rows * group;
-    return most <= 16 ? (int)most : group <= 16 ? group : 0;
+    if (most <= 16) return (int)most;
+    return group <= 16 && (int64_t)s.n_seqs * s.max_rows > s.n_rows ? group : 0;
 }
 
 size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms) {

@@ -17,7 +17,7 @@
 //                   S = Q K of the same half of the next tile, and so on; the softmax finds the next scores ready.  (One warp for both was the bound: the issue of a product
 //                   takes 80 clocks, and every wait adds a few hundred.)
 //   warp 1          K and V tiles by TMA into one ring, a copy a page run
-//   warp 3          leaves the kernel behind this one a record of the block that the CTA's end cuts
+//   warp 3          plans the pieces of the CTA, a few ahead, and leaves the kernel behind this one a record of the block that the CTA's end cuts
 //   warps 4-7, 8-11 softmax of Q0 and Q1, a row a thread; they bring Q, and the result out
 //   warps 12-15     16-bit caches: tiles that some row sees in part are searched for values that are not finite: 0 x NaN is NaN, and a row must not be
 //                   reached by what it does not see.  They are taken out before the product and added to the rows that see them at the end.
@@ -37,7 +37,7 @@ namespace l2 {
 namespace {
 
 constexpr int KT_TILE = 128, KT_SUB = 64, KT_ROWS = 256, KT_THREADS = 512;
-constexpr int KT_MMA_WARP = 0, KT_COPY_WARP = 1, KT_ROW_WARP = 4, KT_HELP_WARP = 12;
+constexpr int KT_MMA_WARP = 0, KT_COPY_WARP = 1, KT_PLAN_WARP = 3, KT_ROW_WARP = 4, KT_HELP_WARP = 12;
 constexpr int KT_SCALE_SLOTS = 4;
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
@@ -199,8 +199,8 @@ struct KtWalk {
         w = per * blockIdx.x;
         w1 = min(spot.total, w + per);
         b = spot.b; index = -1; head = block = skip = 0;
-        if (w >= w1) return;
         k = kt_blocks(P, lim, b);
+        if (w >= w1) return;
         const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = w - spot.start;
         head = (int)kv_quotient(in, tiles);
         int64_t before;
@@ -226,21 +226,30 @@ struct KtWalk {
         w += t1 - t0;
         return true;
     }
+};
+
+// One piece as the roles read it (shared memory): tiles t0 .. t1 - 1 of positions of a block of rows.
+struct KtPiece {
+    int on;                             // 0: no more pieces
+    int t0, t1, tiles, sink_tiles, first;
+    int lo_pos, hi_pos, lo[2], hi[2];   // positions of the block's rows, and of those of each tile of rows (hi -1: it has none, and sees nothing)
+    int rows, head, b, index;           // index: pieces before this one
+    int64_t row0;                       // of the row arrays
+    __device__ __forceinline__ KvView<KT_TILE> view(int lo, int hi) const {
+        KvView<KT_TILE> v;
+        v.lo_pos = lo; v.hi_pos = hi; v.sink_tiles = sink_tiles; v.first = first; v.tiles = tiles;
+        return v;
+    }
+    __device__ __forceinline__ KvView<KT_TILE> part(int i) const { return view(lo[i], hi[i]); }
+    __device__ __forceinline__ int base(int t) const { return (t < sink_tiles ? t : first + t - sink_tiles) * KT_TILE; }
     // A bit for each of the tiles t .. t + 31 of positions (of this piece) of which f(first position) holds; by the whole warp.  What is decided once for 32
     // tiles, and by a vote, is in uniform registers, and so is all that follows from it.
     template <class F> __device__ __forceinline__ uint32_t bits(int t, F f) const {
         const int mine = t + (threadIdx.x & 31);
-        return __ballot_sync(0xffffffffu, mine >= t0 && mine < t1 && f(view.base(mine)));
-    }
-    // what tile i of the block's rows sees (its rows: 128 i and on); without rows it sees nothing
-    __device__ __forceinline__ KvView<KT_TILE> part(const KvAttendParams& P, int i) const {
-        KvView<KT_TILE> v = view;
-        const int lo = 128 * i, hi = min(rows, lo + 128) - 1;
-        v.lo_pos = view.lo_pos + kt_token(P, lo);
-        v.hi_pos = hi < lo ? -1 : view.lo_pos + kt_token(P, hi);
-        return v;
+        return __ballot_sync(0xffffffffu, mine >= t0 && mine < t1 && f(base(mine)));
     }
 };
+constexpr int KT_PIECES = 4;
 
 template <int CT, bool QB, int HD>
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
@@ -255,6 +264,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[I8 ? S::RAWS : 1], raw_empty[I8 ? S::RAWS : 1],
         sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
     __shared__ int64_t scratch[KT_THREADS / 32 + 2];
+    __shared__ __align__(8) uint64_t piece_full[KT_PIECES], piece_empty[KT_PIECES], row_meet[2];
+    __shared__ KtPiece pieces[KT_PIECES];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
     __shared__ volatile int odd[8];  // by piece: values that are not finite have been taken out of a V tile
@@ -269,9 +280,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         for (int i = 0; i < (I8 ? S::RAWS : 1); i++) { kv_bar_init(&raw_full[i], 1); kv_bar_init(&raw_empty[i], 4); }
         for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 32); kv_bar_init(&sc_empty[i], 8); }
         for (int i = 0; i < 2; i++) {
-            kv_bar_init(&q_full[i], 128); kv_bar_init(&drained[i], 1);
+            kv_bar_init(&q_full[i], 128); kv_bar_init(&drained[i], 1); kv_bar_init(&row_meet[i], 4);
             for (int h = 0; h < 2; h++) { kv_bar_init(&s_full[i][h], 1); kv_bar_init(&p_full[i][h], 4); kv_bar_init(&pv_done[i][h], 1); }
         }
+        for (int i = 0; i < KT_PIECES; i++) { kv_bar_init(&piece_full[i], 1); kv_bar_init(&piece_empty[i], 15); }
         for (int i = 0; i < 8; i++) odd[i] = 0;
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -282,14 +294,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const KvSpot spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch,
-                                              [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
+    KvSpot spot{0, 0, -1, 0};
+    if (P.step.n_seqs > 32 || warp == KT_PLAN_WARP)  // (up to 32 sequences a warp finds its way alone)
+        spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_s;
-    KtWalk walk(P, lim, spot);
     const KvWait wait{&failed};
+    // Pieces are planned by one warp and read by the others from a ring: the walk's state would cost each role thirty registers.
+    auto piece_at = [&](uint32_t n) -> const KtPiece& { wait(&piece_full[n % KT_PIECES], (n / KT_PIECES) & 1u); return pieces[n % KT_PIECES]; };
+    auto is_one = [&](const KtPiece& piece) { return __any_sync(0xffffffffu, piece.on) && !wait.over(); };
+    auto give_back = [&](uint32_t n) { __syncwarp(); if (lane == 0) kv_bar_arrive(&piece_empty[n % KT_PIECES]); };
 
     if (warp >= KT_ROW_WARP && warp < KT_HELP_WARP) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
@@ -297,31 +313,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         const int i = (warp - KT_ROW_WARP) >> 2, row = 128 * i + (tid & 127);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_row = tmem + lanes + S_COL + 128 * i, o_at = tmem + lanes + O_COL + 128 * i;
         uint32_t s_ph = 0, sc = 0, sc_ph = 0;
-        while (walk.next(P, lim)) {
-            const KvView<KT_TILE> mine = walk.part(P, i);
+        // Q of a piece is requested while the result of the piece in front is still on its way out.  HD / 8 threads have a row.
+        constexpr int Q_ROWS = 128 / LANES, Q_N = 128 / Q_ROWS;  // rows at once, and of a thread
+        uint4 qx[Q_N];
+        auto request_q = [&](const KtPiece& piece) {
+            const char* const from = P.q.data + 2 * (piece.row0 * P.q.row_stride + (int64_t)piece.head * P.group * P.q.head_stride + 8 * (tid % LANES));
+            const int rows = piece.rows;
+#pragma unroll
+            for (int n = 0; n < Q_N; n++) {  // (rows that there are not: zeros)
+                const int f = 128 * i + (tid & 127) / LANES + n * Q_ROWS, k = kt_token(P, f);
+                qx[n] = make_uint4(0, 0, 0, 0);
+                if (f < rows) qx[n] = *reinterpret_cast<const uint4*>(from + 2 * (k * P.q.row_stride + (int64_t)(f - k * P.group) * P.q.head_stride));
+            }
+        };
+        uint32_t meet_ph = 0;
+        auto meet = [&]() {  // of the four warps
+            __syncwarp();
+            if (lane == 0) kv_bar_arrive(&row_meet[i]);
+            wait(&row_meet[i], meet_ph);
+            meet_ph ^= 1u;
+            __syncwarp();
+        };
+        bool more = is_one(piece_at(0));
+        if (more) request_q(pieces[0]);
+        for (uint32_t n = 0; more; n++) {
+            const KtPiece& walk = pieces[n % KT_PIECES];
+            const KvView<KT_TILE> mine = walk.part(i);
+            const int t0 = walk.t0, t1 = walk.t1;
             const int tok = kt_token(P, min(row, walk.rows - 1));
-            const int pos = walk.view.lo_pos + tok;
+            const int pos = walk.lo_pos + tok;
             auto any = [&](int base) { return mine.any(base, KT_TILE, P.window, P.sinks); };
-            uint32_t some = 0;
-            for (int t = walk.t0; t < walk.t1 && !some; t += 32) some = walk.bits(t, any);
-            if (some) {  // Q, swizzled as the products want it, HD / 8 threads a row; rows that there are not: zeros
-                uint8_t* to = sq + i * S::SLOT;
-                const int c = tid % LANES;
-                const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
-                constexpr int AT_ONCE = 8, ROWS_ONCE = 128 / LANES;
-#pragma unroll 1
-                for (int r0 = (tid & 127) / LANES; r0 < 128; r0 += AT_ONCE * ROWS_ONCE) {
-                    uint4 x[AT_ONCE];  // (requested together: the compiler keeps a load behind the store in front of it)
+            uint32_t some = 0;  // this tile of rows sees something in the piece
+            for (int t = t0; t < t1 && !some; t += 32) some = walk.bits(t, any);
+            if (some) {  // Q, swizzled as the products want it
 #pragma unroll
-                    for (int n = 0; n < AT_ONCE; n++) {
-                        const int f = 128 * i + r0 + n * ROWS_ONCE, k = kt_token(P, f);
-                        x[n] = make_uint4(0, 0, 0, 0);
-                        if (f < walk.rows)
-                            x[n] = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((block_at + k) * P.q.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.q.head_stride + 8 * c));
-                    }
-#pragma unroll
-                    for (int n = 0; n < AT_ONCE; n++) *reinterpret_cast<uint4*>(to + kt_offset(r0 + n * ROWS_ONCE, c)) = x[n];
-                }
+                for (int n = 0; n < Q_N; n++) *reinterpret_cast<uint4*>(sq + i * S::SLOT + kt_offset((tid & 127) / LANES + n * Q_ROWS, tid % LANES)) = qx[n];
                 fence_async();
                 kv_bar_arrive(&q_full[i]);
             }
@@ -329,8 +355,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             int seen = 0;      // halves of tiles seen
             uint32_t on = 0, all = 0;  // by tile of positions: seen by some row; by every row
 #pragma unroll 1
-            for (int t = walk.t0; t < walk.t1; t++, on >>= 1, all >>= 1) {
-                if ((t - walk.t0) % 32 == 0) {
+            for (int t = t0; t < t1; t++, on >>= 1, all >>= 1) {
+                if ((t - t0) % 32 == 0) {
                     on = walk.bits(t, any);
                     all = walk.bits(t, [&](int base) { return mine.whole(base, P.window, P.sinks); });
                 }
@@ -367,7 +393,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         }
                     }
                     if (!whole) {
-                        const int base = walk.view.base(t) + KT_SUB * h;
+                        const int base = walk.base(t) + KT_SUB * h;
                         const int hi = pos - base, lo = P.window ? pos - P.window - base : -1, sinks = P.sinks - base;  // seen: j <= hi and (j > lo or j < sinks)
 #pragma unroll
                         for (int j = 0; j < KT_SUB; j++)
@@ -404,13 +430,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
                     unsigned long long sum[2] = {0ull, 0ull};
                     uint32_t p16[KT_SUB / 2];
+                    float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int j = 0; j < KT_SUB; j += 2) {
                         const float2 e = unpair(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, r2));
                         float2 p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
                         sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(p.x, p.y));
                         if constexpr (I8) {
-                            const float2 v = *reinterpret_cast<const float2*>(ks + KT_TILE + j);
+                            if (j % 4 == 0) v4 = *reinterpret_cast<const float4*>(ks + KT_TILE + j);
+                            const float2 v = j % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
                             if (whole) p = make_float2(p.x * v.x, p.y * v.y);
                             else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
                         }
@@ -431,14 +459,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 }
             }
             // ---- the result of the piece
-            const bool done = walk.t0 == 0 && walk.t1 == walk.view.tiles;
-            const bool started = seen > 0;
+            more = is_one(piece_at(n + 1));
+            if (more) request_q(pieces[(n + 1) % KT_PIECES]);
+            const bool done = t0 == 0 && t1 == walk.tiles, started = seen > 0;
             if (started) {
                 wait(&pv_done[i][1], s_ph ^ 1u);
                 __syncwarp();
                 fence_after();
             }
-            if (128 * i >= walk.rows) continue;  // (whole warps: this tile has no rows)
+            if (128 * i >= walk.rows) { give_back(n); continue; }  // (this tile has no rows)
             const bool fix = !I8 && started && odd[walk.index & 7];
             float* part = kv_part(P.work, gridDim.x, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
             const float inv = done && pos >= 0 ? 1.0f / l : 1.0f;
@@ -448,16 +477,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) o[j] = 0u;
                 if (started) { tmem_ld32(o, o_at + c); wait_ld(); }
+                else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] = 0u;
+                }
                 if constexpr (!I8) {
                     if (fix) {  // rare: the values that were taken out, one by one, to the rows that see them
 #pragma unroll 1
                         for (int t = walk.t0; t < walk.t1; t++) {
-                            const int base = walk.view.base(t);
+                            const int base = walk.base(t);
                             if (!mine.any(base, KT_TILE, P.window, P.sinks) || mine.whole(base, P.window, P.sinks)) {
-                                const KvView<KT_TILE> other = walk.part(P, i ^ 1);  // (taken out for the other tile's rows)
+                                const KvView<KT_TILE> other = walk.part(i ^ 1);  // (taken out for the other tile's rows)
                                 if (!mine.any(base, KT_TILE, P.window, P.sinks) || !other.any(base, KT_TILE, P.window, P.sinks) || other.whole(base, P.window, P.sinks)) continue;
                             }
 #pragma unroll 1
@@ -481,35 +512,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * KT_ROWS + row) * 4) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     continue;
                 }
-                float y[32];
+                const float f = pos < 0 ? 0.0f : inv;
+                if (pos < 0) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) y[j] = pos < 0 ? 0.0f : __uint_as_float(o[j]) * inv;
-                const int in = c % cols;
+                    for (int j = 0; j < 32; j++) o[j] = 0u;
+                }
+                const int in = c % cols, r = tid & 127;
+                auto y = [&](int j) { return __uint_as_float(o[j]) * f; };
                 if (wide == 4) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(stage + kt_offset(tid & 127, (in + j) / 4)) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(stage + kt_offset(r, (in + j) / 4)) = make_float4(y(j), y(j + 1), y(j + 2), y(j + 3));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 w = QB ? make_uint4(pack16<true>(y[j], y[j + 1]), pack16<true>(y[j + 2], y[j + 3]), pack16<true>(y[j + 4], y[j + 5]), pack16<true>(y[j + 6], y[j + 7]))
-                                     : make_uint4(pack16<false>(y[j], y[j + 1]), pack16<false>(y[j + 2], y[j + 3]), pack16<false>(y[j + 4], y[j + 5]), pack16<false>(y[j + 6], y[j + 7]));
-                        *reinterpret_cast<uint4*>(stage + kt_offset(tid & 127, (in + j) / 8)) = w;
-                    }
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4*>(stage + kt_offset(r, (in + j) / 8)) = make_uint4(pack16<QB>(y(j), y(j + 1)), pack16<QB>(y(j + 2), y(j + 3)), pack16<QB>(y(j + 4), y(j + 5)), pack16<QB>(y(j + 6), y(j + 7)));
                 }
                 if (in + 32 < cols) continue;
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                const int64_t block_at = walk.k.s.row0 + walk.block * walk.k.tokens;
+                meet();
                 const int ch = tid % LANES;
-                for (int r = (tid & 127) / LANES; r < 128; r += 128 / LANES) {
-                    const int f = 128 * i + r, k = kt_token(P, f);
-                    if (f >= walk.rows) break;
-                    const int64_t e = (block_at + k) * P.out.row_stride + (int64_t)(walk.head * P.group + f - k * P.group) * P.out.head_stride + (c + 32 - cols);
-                    *reinterpret_cast<uint4*>(P.out.data + e * wide + 16 * ch) = *reinterpret_cast<const uint4*>(stage + kt_offset(r, ch));
+                char* const out = P.out.data + ((walk.row0) * P.out.row_stride + (int64_t)walk.head * P.group * P.out.head_stride + (c + 32 - cols)) * wide + 16 * ch;
+#pragma unroll
+                for (int n0 = 0; n0 < Q_N; n0 += 4) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int n = 0; n < 4; n++) w[n] = *reinterpret_cast<const uint4*>(stage + kt_offset((tid & 127) / LANES + (n0 + n) * Q_ROWS, ch));
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const int fl = 128 * i + (tid & 127) / LANES + (n0 + n) * Q_ROWS, k = kt_token(P, fl);
+                        if (fl < walk.rows) *reinterpret_cast<uint4*>(out + (k * P.out.row_stride + (int64_t)(fl - k * P.group) * P.out.head_stride) * wide) = w[n];
+                    }
                 }
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                meet();
             }
             if (!done) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
             fence_before();
+            give_back(n);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -525,8 +562,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                            v_lo = desc_lo(kv_smem(ring), KT_TILE * 128 / 16);
             uint32_t slot = 0, ph = 0, ready_ph = 0, q_ph = 0, p_ph = 0;  // ready_ph: a bit for each slot
             auto step = [&]() { if (++slot == S::SLOTS) { slot = 0; ph ^= 1u; } };
-            while (__any_sync(0xffffffffu, walk.next(P, lim))) {
-                const KvView<KT_TILE> mine = walk.part(P, i), other = walk.part(P, i ^ 1);
+            for (uint32_t n = 0;; n++) {
+                const KtPiece& walk = piece_at(n);
+                if (!is_one(walk)) break;
+                const KvView<KT_TILE> mine = walk.part(i), other = walk.part(i ^ 1);
                 auto any = [&](int base) { return mine.any(base, KT_TILE, P.window, P.sinks); };
                 const int t0 = __reduce_max_sync(0xffffffffu, walk.t0), t1 = __reduce_max_sync(0xffffffffu, walk.t1);
                 uint32_t begun = 0;  // S has been computed (1), O has been written (2)
@@ -558,9 +597,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         return (any(base) && !mine.whole(base, P.window, P.sinks)) || (other.any(base, KT_TILE, P.window, P.sinks) && !other.whole(base, P.window, P.sinks)); });
                     on = walk.bits(tc, any);
                     const uint32_t next = walk.bits(tc + 1, any);
-                    const int n = min(32, t1 - tc);
+                    const int tiles = min(32, t1 - tc);
 #pragma unroll 1
-                    for (int b = 0; b < n; b++) {
+                    for (int b = 0; b < tiles; b++) {
                         const uint32_t v_slot = slot, v_ph = ph;
                         step();
                         const bool more = tc + b + 1 < t1;
@@ -595,6 +634,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         if (more) step();
                     }
                 }
+                give_back(n);
             }
             if (failed) {  // products still under way read shared memory: a bounded time to end
                 if (leader) commit(&drained[i]);
@@ -607,24 +647,28 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             constexpr int RB = HD * (I8 ? 1 : 2), W = RB < 128 ? RB : 128;  // bytes of a row, of a copy's row
             uint32_t slot = 0, ph = 1, sc = 0, sc_ph = 1;
             bool over = false;
-            while (!over && walk.next(P, lim)) {
+            for (uint32_t n = 0; !over; n++) {
+                const KtPiece& walk = piece_at(n);
+                if (!is_one(walk)) break;
+                const KvView<KT_TILE> view = walk.view(walk.lo_pos, walk.hi_pos);
+                const int t0 = walk.t0, t1 = walk.t1, head = walk.head, b = walk.b;
                 auto page_of = [&](int t) {  // the page of this lane's run of tile t, n_pages (zeros) where no row sees it or there is none
-                    const int j = walk.view.base(t) + lane * R;
-                    if (lane >= runs || !walk.view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
-                    const int x = kv_page(P.step, P.pool, walk.b, j);
+                    const int j = view.base(t) + lane * R;
+                    if (lane >= runs || !view.any(j, R, P.window, P.sinks)) return P.pool.n_pages;
+                    const int x = kv_page(P.step, P.pool, b, j);
                     return x >= 0 ? x : P.pool.n_pages;
                 };
-                int page = page_of(walk.t0);
-                for (int t = walk.t0; t < walk.t1; t++) {
-                    const int j = walk.view.base(t) + lane * R, at = j & ((1 << P.pool.page_shift) - 1);
-                    const int ahead = t + 1 < walk.t1 ? page_of(t + 1) : P.pool.n_pages;
+                int page = page_of(t0);
+                for (int t = t0; t < t1; t++) {
+                    const int j = view.base(t) + lane * R, at = j & ((1 << P.pool.page_shift) - 1);
+                    const int ahead = t + 1 < t1 ? page_of(t + 1) : P.pool.n_pages;
                     if constexpr (I8) {
                         wait(&sc_empty[sc], sc_ph);
                         if ((over = wait.over())) break;
                         // four positions a lane, of K and of V
                         const int x = 4 * lane, of = __shfl_sync(0xffffffffu, page, x / R);
                         const bool there = of < P.pool.n_pages;
-                        const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((walk.view.base(t) + x) & ((1 << P.pool.page_shift) - 1));
+                        const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + head << P.pool.page_shift) + ((view.base(t) + x) & ((1 << P.pool.page_shift) - 1));
                         const uint32_t to = kv_smem(scales + sc * 2 * KT_TILE + x);
                         kv_copy16(to, P.pool.ks + e, there);
                         kv_copy16(to + 4 * KT_TILE, P.pool.vs + e, there);
@@ -641,30 +685,56 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         if (lane < runs) {
                             const uint32_t to = kv_smem(I8 ? raw + slot * S::RAW : ring + slot * S::SLOT) + lane * R * W;
 #pragma unroll
-                            for (int h = 0; h < RB / W; h++) kv_tma4(to + h * (KT_TILE * 128), kv ? &map_v : &map_k, h * 64, at, walk.head, page, f);
+                            for (int h = 0; h < RB / W; h++) kv_tma4(to + h * (KT_TILE * 128), kv ? &map_v : &map_k, h * 64, at, head, page, f);
                         }
                         if (++slot == (I8 ? S::RAWS : S::SLOTS)) { slot = 0; ph ^= 1u; }
                     }
                     if (over) break;
                     page = ahead;
                 }
+                give_back(n);
             }
-        } else if (warp == KT_COPY_WARP + 2) {
-            // ================= what the next kernel has to know ======================================================================
+        } else if (warp == KT_PLAN_WARP) {
+            // ================= pieces, and what the next kernel has to know of them ===================================================
+            KtWalk walk(P, lim, spot);
             KvCut cut{0, 0, 0, 0, 0, 0, 0};
-            while (walk.next(P, lim))
-                if (walk.t0 == 0 && walk.t1 < walk.view.tiles)
-                    cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + walk.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.index ? 1 : 0, walk.rows, walk.head,
-                                (int64_t)walk.k.s.row0 + walk.block * walk.k.tokens, walk.view.lo_pos, 0};
+            bool more = true;
+            for (uint32_t n = 0; more; n++) {
+                more = walk.next(P, lim);
+                const int64_t row0 = (int64_t)walk.k.s.row0 + walk.block * walk.k.tokens;
+                if (more && walk.t0 == 0 && walk.t1 < walk.view.tiles)
+                    cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + walk.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.index ? 1 : 0, walk.rows, walk.head, row0, walk.view.lo_pos, 0};
+                wait(&piece_empty[n % KT_PIECES], (n / KT_PIECES & 1u) ^ 1u);
+                if (wait.over()) break;
+                if (lane == 0) {
+                    KtPiece& p = pieces[n % KT_PIECES];
+                    p.on = more;
+                    if (more) {
+                        p.t0 = walk.t0; p.t1 = walk.t1; p.tiles = walk.view.tiles; p.sink_tiles = walk.view.sink_tiles; p.first = walk.view.first;
+                        p.lo_pos = walk.view.lo_pos; p.hi_pos = walk.view.hi_pos;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const int lo = 128 * i, hi = min(walk.rows, lo + 128) - 1;
+                            p.lo[i] = walk.view.lo_pos + kt_token(P, lo);
+                            p.hi[i] = hi < lo ? -1 : walk.view.lo_pos + kt_token(P, hi);
+                        }
+                        p.rows = walk.rows; p.head = walk.head; p.b = walk.b; p.index = walk.index; p.row0 = row0;
+                    }
+                    kv_bar_arrive(&piece_full[n % KT_PIECES]);
+                }
+                __syncwarp();
+            }
             if (lane == 0) kv_cuts(P.work)[blockIdx.x] = cut;
         } else if (warp >= KT_HELP_WARP) {
             const int r = tid & 127;
             if constexpr (I8) {
                 // ================= bytes to 16-bit numbers: a position a thread ==================================================
                 uint32_t rs = 0, rph = 0, slot = 0, ph = 1;
-                while (walk.next(P, lim)) {
+                for (uint32_t n = 0;; n++) {
+                    const KtPiece& walk = piece_at(n);
+                    if (!is_one(walk)) break;
 #pragma unroll 1
-                    for (int n = 2 * (walk.t1 - walk.t0), kv = 0; n > 0; n--, kv ^= 1) {
+                    for (int left = 2 * (walk.t1 - walk.t0), kv = 0; left > 0; left--, kv ^= 1) {
                         wait(&raw_full[rs], rph);
                         wait(&empty[slot], ph);
                         __syncwarp();
@@ -687,6 +757,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         if (++rs == (uint32_t)S::RAWS) { rs = 0; rph ^= 1u; }
                         if (++slot == (uint32_t)S::SLOTS) { slot = 0; ph ^= 1u; }
                     }
+                    give_back(n);
                 }
             } else {
                 // ================= V tiles that some row sees in part: only finite values stay ===================================
@@ -697,12 +768,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     if (lane == 0) kv_bar_arrive(&empty[slot]);
                     if (++slot == S::SLOTS) { slot = 0; ph ^= 1u; }
                 };
-                while (walk.next(P, lim)) {
-                    const KvView<KT_TILE> see[2] = {walk.part(P, 0), walk.part(P, 1)};
+                for (uint32_t n = 0;; n++) {
+                    const KtPiece& walk = piece_at(n);
+                    if (!is_one(walk)) break;
+                    const KvView<KT_TILE> see[2] = {walk.part(0), walk.part(1)};
+                    const int t0 = walk.t0, t1 = walk.t1;
                     if (tid == KT_HELP_WARP * 32) odd[(walk.index + 4) & 7] = 0;  // (a piece to come)
 #pragma unroll 1
-                    for (int t = walk.t0; t < walk.t1; t++) {
-                        const int base = walk.view.base(t);
+                    for (int t = t0; t < t1; t++) {
+                        const int base = walk.base(t);
                         wait(&full[slot], ph);
                         step();
                         bool part = false;
@@ -728,6 +802,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         }
                         step();
                     }
+                    give_back(n);
                 }
             }
         }
@@ -743,38 +818,43 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     if (warp == KT_MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-constexpr int KT_COMBINE_SPLIT = 8;  // CTAs that share the rows of a block
-
-// Adds the pieces of the block of rows that begins in CTA x of the launch in front and goes on in the next.
+// Adds the pieces of the block of rows that begins in CTA x of the launch in front and goes on in the next.  A thread has a row and eight columns; the lanes of a
+// warp have rows side by side, as the pieces lie.
 template <int HD>
 __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constant__ KvAttendParams P, const int ctas) {
-    constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const KvCut cut = kv_cuts(P.work)[blockIdx.x];
-    const int d = 4 * (threadIdx.x % LANES);
+    const int r = blockIdx.y * 32 + (threadIdx.x & 31);
+    if (!cut.pieces || r >= cut.rows) return;
     auto piece = [&](int i) { return kv_part(P.work, ctas, KT_ROWS, HD, blockIdx.x + i, i == 0 ? cut.slot : 0); };
-    if (!cut.pieces) return;
-    for (int r = blockIdx.y * SLOTS + threadIdx.x / LANES; r < cut.rows; r += KT_COMBINE_SPLIT * SLOTS) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll 4
+    for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+    for (int i = 0; i < cut.pieces; i++) {
+        const float2 ml = *reinterpret_cast<const float2*>(piece(i) + KT_ROWS * HD + 2 * r);
+        sum += KvScale(ml.x - ref)(ml.y);
+    }
+    const int tok = kt_token(P, r), pos = cut.lo_pos + tok;
+    const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride;
+    const float inv = 1.0f / sum;
+    for (int d = 8 * (threadIdx.x >> 5); d < HD; d += 64) {
+        float y[8] = {};
+#pragma unroll 2
         for (int i = 0; i < cut.pieces; i++) {
             const float* p = piece(i);
-            const float2 ml = *reinterpret_cast<const float2*>(p + KT_ROWS * HD + 2 * r);
-            const KvScale f(ml.x - ref);
-            const float4 x = *reinterpret_cast<const float4*>(p + (d / 4 * KT_ROWS + r) * 4);
-            sum += f(ml.y);
-            acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
+            const KvScale f(p[KT_ROWS * HD + 2 * r] - ref);
+            const float4 a = *reinterpret_cast<const float4*>(p + (d / 4 * KT_ROWS + r) * 4), b = *reinterpret_cast<const float4*>(p + ((d / 4 + 1) * KT_ROWS + r) * 4);
+            y[0] += f(a.x); y[1] += f(a.y); y[2] += f(a.z); y[3] += f(a.w);
+            y[4] += f(b.x); y[5] += f(b.y); y[6] += f(b.z); y[7] += f(b.w);
         }
-        const int tok = r / P.group, pos = cut.lo_pos + tok;
-        const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride + d;
-        const float inv = 1.0f / sum;
-        const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
-        for (int i = 0; i < 4; i++) kv_store1(P.out, e + i, pos < 0 ? 0.0f : y[i]);
+        for (int x = 0; x < 8; x++) y[x] = pos < 0 ? 0.0f : y[x] * inv;
+        if (P.out.type == L2_F32) kv_store8(reinterpret_cast<float*>(P.out.data) + e + d, y);
+        else if (P.out.type == L2_F16) kv_store8(reinterpret_cast<__half*>(P.out.data) + e + d, y);
+        else kv_store8(reinterpret_cast<__nv_bfloat16*>(P.out.data) + e + d, y);
     }
 }
 
@@ -814,7 +894,7 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
     if (e != cudaSuccess || grid < 2) return e;
     auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;
-    return kv_launch(combine, dim3(grid - 1, KT_COMBINE_SPLIT), 256, 0, st, p, grid);
+    return kv_launch(combine, dim3(grid - 1, KT_ROWS / 32), 256, 0, st, p, grid);
 }
 
 }  // namespace l2
