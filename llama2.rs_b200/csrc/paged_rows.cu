@@ -209,19 +209,28 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
         // ================= matrix work ========================================================================================
         const int c = lane & 3, g8 = lane >> 2;
         uint32_t st = 0, ph = 0;
-        while (walk.next(P, lim)) {
-            const KrSeq<TILE>& seq = walk.q;
-            const int rows = seq.rows, G = P.group;
-            // Q into shared memory: rows beyond the last are zeros
+        // Q of a piece is requested while the results of the piece in front meet.
+        constexpr int Q_N = S::ROWS * (HD / 8) / (KR_WARPS * 32) + (S::ROWS * (HD / 8) % (KR_WARPS * 32) != 0);
+        uint4 qx[Q_N];
+        auto request_q = [&]() {  // (rows beyond the last are zeros)
+#pragma unroll
+            for (int n = 0; n < Q_N; n++) {
+                const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8), tok = r / P.group;
+                qx[n] = make_uint4(0, 0, 0, 0);
+                if (r < walk.q.rows)
+                    qx[n] = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((walk.q.s.row0 + tok) * P.q.row_stride + (int64_t)(walk.head * P.group + r - tok * P.group) * P.q.head_stride + ch * 8));
+            }
+        };
+        bool more = walk.next(P, lim);
+        if (more) request_q();
+        while (more) {
+            const KvView<TILE> view = walk.q.view;
+            const int rows = walk.q.rows, G = P.group, t0 = walk.t0, t1 = walk.t1;
             asm volatile("bar.sync 1, 128;" ::: "memory");  // (everybody has read the piece before's)
-            for (int i = tid; i < S::ROWS * (HD / 8); i += KR_WARPS * 32) {
-                const int r = i / (HD / 8), ch = i % (HD / 8);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < rows) {
-                    const int tok = r / G;
-                    x = *reinterpret_cast<const uint4*>(P.q.data + 2 * ((seq.s.row0 + tok) * P.q.row_stride + (int64_t)(walk.head * G + r - tok * G) * P.q.head_stride + ch * 8));
-                }
-                *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = x;
+#pragma unroll
+            for (int n = 0; n < Q_N; n++) {
+                const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8);
+                if (r < S::ROWS) *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = qx[n];
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             auto q_frag = [&](int nt, int ks, uint32_t& b0, uint32_t& b1) {  // columns 8 nt .., elements 16 ks .. of Q^T
@@ -238,7 +247,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) pos[nt][e] = seq.view.lo_pos + (8 * nt + 2 * c + e) / G;
+                for (int e = 0; e < 2; e++) pos[nt][e] = view.lo_pos + (8 * nt + 2 * c + e) / G;
 
             float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -249,9 +258,9 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 for (int mt = 0; mt < MT; mt++) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.0f;
             }
 #pragma unroll 1
-            for (int t = walk.t0; t < walk.t1; t++) {
-                const int base = seq.view.base(t);
-                const bool whole = seq.view.whole(base, P.window, P.sinks);
+            for (int t = t0; t < t1; t++) {
+                const int base = view.base(t);
+                const bool whole = view.whole(base, P.window, P.sinks);
                 wait(&full[st], ph);
                 __syncwarp();
                 const uint8_t* stage = ring + st * S::STAGE;
@@ -404,12 +413,23 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         }
                     }
                 }
-                if (t + 1 < walk.t1) {  // (the last tile's slot is kept for the meeting)
+                if (t + 1 < t1) {  // (the last tile's slot is kept for the meeting)
                     __syncwarp();
                     if (lane == 0) kv_bar_arrive(&empty[st]);
                     if (++st == S::STAGES) { st = 0; ph ^= 1u; }
                 }
             }
+            const int head = walk.head;
+            const int64_t row0 = walk.q.s.row0;
+            const bool done = walk.whole();
+            float* part = kv_part(P.work, gridDim.x, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
+            if (tid == 0 && walk.w >= walk.w1) {  // what the kernel behind this one has to know
+                KvCut cut{0, 0, 0, 0, 0, 0, 0};
+                if (t0 == 0 && !done) cut = KvCut{(int)kv_quotient(walk.w - t1 + view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, rows, head, row0, view.lo_pos, 0};
+                kv_cuts(P.work)[blockIdx.x] = cut;
+            }
+            more = walk.next(P, lim);
+            if (more) request_q();
             // ---- the four warps' results meet: a common maximum, then each warp adds a quarter of the elements, in the order of the warps
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -447,8 +467,6 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 for (int nt = 0; nt < NT; nt++) meet[(warp * MT * NT + mt * NT + nt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
             asm volatile("bar.sync 1, 128;" ::: "memory");
             constexpr int SHARE = MT / KR_WARPS;  // products of a warp
-            const bool done = walk.whole();
-            float* part = kv_part(P.work, gridDim.x, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
 #pragma unroll
             for (int x = 0; x < SHARE; x++)
 #pragma unroll
@@ -465,7 +483,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         const int r = 8 * nt + 2 * c + e;
                         if (r >= rows) continue;
                         const int tok = r / G;
-                        const int64_t at = (seq.s.row0 + tok) * P.out.row_stride + (int64_t)(walk.head * G + r - tok * G) * P.out.head_stride;
+                        const int64_t at = (row0 + tok) * P.out.row_stride + (int64_t)(head * G + r - tok * G) * P.out.head_stride;
                         const float inv = 1.0f / lsum[nt][e];
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
@@ -476,12 +494,6 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         if (!done && warp == 0 && x == 0 && g8 == 0) *reinterpret_cast<float2*>(part + S::ROWS * HD + 2 * r) = make_float2(m[nt][e], lsum[nt][e]);
                     }
                 }
-            if (warp == 0 && lane == 0 && walk.w >= walk.w1) {  // what the kernel behind this one has to know
-                KvCut cut{0, 0, 0, 0, 0, 0, 0};
-                if (walk.t0 == 0 && !done)
-                    cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + seq.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, rows, walk.head, seq.s.row0, seq.view.lo_pos, 0};
-                kv_cuts(P.work)[blockIdx.x] = cut;
-            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the slot goes back to the copies)
             __syncwarp();
             if (lane == 0) kv_bar_arrive(&empty[st]);
