@@ -424,6 +424,8 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (int rc = check_rows(who, "out", out, batch, pages->head_size, q->heads, &P.out)) return rc;
     if (q->type == L2_F32 || (pages->type != L2_I8 && q->type != pages->type)) return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 cache)", who);
     if (out->type != L2_F32 && out->type != q->type) return fail(L2_EINVAL, "%s: out must be of q's type or f32", who);
+    if ((int64_t)((int64_t)batch->max_rows * (q->heads / pages->n_kv_heads) / 64 + 1) * ((((int64_t)batch->table_width << P.pool.page_shift) + 127) / 128 + 1) >> 31)
+        return fail(L2_ERANGE, "%s: %d rows of a sequence over %lld positions (more than 2^31 tiles)", who, batch->max_rows, (long long)batch->table_width << P.pool.page_shift);
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);
     int sms;
     if (int rc = kv_device(&sms)) return rc;

@@ -107,24 +107,31 @@ __device__ __forceinline__ int64_t kv_scan(int64_t v) {  // inclusive sum over t
     return v;
 }
 
+// By a warp, for up to 32 sequences: v the tiles of the lane's sequence; src the sequence found (0 where there is none).
+__device__ __forceinline__ KvSpot kv_locate_few(int64_t v, int cta, int ctas, int* src) {
+    KvSpot spot{0, 0, -1, 32};
+    const int64_t inc = kv_scan(v);
+    spot.total = __shfl_sync(0xffffffffu, inc, 31);
+    spot.per = kv_quotient(spot.total + ctas - 1, ctas);
+    const int64_t at = spot.per * cta;
+    *src = 0;
+    if (at >= spot.total) return spot;
+    spot.b = *src = __ffs(__ballot_sync(0xffffffffu, inc > at)) - 1;
+    spot.start = __shfl_sync(0xffffffffu, inc - v, *src);
+    return spot;
+}
+
 // By all threads of a CTA of THREADS.  len(b): tiles of sequence b, called by whole warps, 0 for b >= n.  Scratch: THREADS / 32 + 2 words of shared memory.
 // Up to 32 sequences: every warp by itself (with barriers between, the search took 3100 clocks of a kernel that takes 13000 for one token of one sequence).
 template <int THREADS, class Len>
 __device__ __forceinline__ KvSpot kv_locate(int n, int cta, int ctas, int64_t* scratch, Len len) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    KvSpot spot{0, 0, -1, n};
     if (n <= 32) {
-        const int64_t v = len(lane), inc = kv_scan(v);
-        spot.total = __shfl_sync(0xffffffffu, inc, 31);
-        spot.per = kv_quotient(spot.total + ctas - 1, ctas);
-        const int64_t at = spot.per * cta;
-        if (at >= spot.total) return spot;
-        const int src = __ffs(__ballot_sync(0xffffffffu, inc > at)) - 1;
-        spot.b = src;
-        spot.start = __shfl_sync(0xffffffffu, inc - v, src);
-        return spot;
+        int src;
+        return kv_locate_few(len(lane), cta, ctas, &src);
     }
+    KvSpot spot{0, 0, -1, n};
     const int64_t mine = len(tid);
     int64_t sum = mine;
     for (int b0 = THREADS; b0 < n; b0 += THREADS) sum += len(b0 + tid);

@@ -139,13 +139,16 @@ __device__ __forceinline__ KvView<KT_TILE> kt_view(const KvAttendParams& P, cons
     const int t0 = block * k.tokens, t1 = min(k.s.n, t0 + k.tokens), p = k.s.kv - k.s.n;
     return KvView<KT_TILE>(p + t0, p + t1 - 1, P.window, P.sinks);
 }
-// Tiles of one kv head of the lane's sequence, by the whole warp (each lane its own sequence).
-__device__ __forceinline__ int64_t kt_tiles(const KvAttendParams& P, KtBlocks k) {
+// Tiles of one kv head of the lane's sequence, by the whole warp (each lane its own sequence).  (The host refuses steps where they could pass 31 bits.)
+__device__ __forceinline__ int kt_tiles(const KvAttendParams& P, KtBlocks k) {
     const int lane = threadIdx.x & 31;
-    int64_t sum = 0;
-    if (k.n <= 4)
+    int sum = 0;
+    if (k.n <= 4) {
+#pragma unroll 1
         for (int i = 0; i < k.n; i++) sum += kt_view(P, k, i).tiles;
+    }
     unsigned many = __ballot_sync(0xffffffffu, k.n > 4);
+#pragma unroll 1
     while (many) {  // the warp's lanes share the blocks of a long one
         const int src = __ffs(many) - 1;
         many &= many - 1;
@@ -153,30 +156,31 @@ __device__ __forceinline__ int64_t kt_tiles(const KvAttendParams& P, KtBlocks k)
         q.s.n = __shfl_sync(0xffffffffu, k.s.n, src);
         q.s.kv = __shfl_sync(0xffffffffu, k.s.kv, src);
         q.n = __shfl_sync(0xffffffffu, k.n, src);
-        int64_t x = 0;
+        int x = 0;
+#pragma unroll 1
         for (int i = lane; i < q.n; i += 32) x += kt_view(P, q, i).tiles;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        x = __reduce_add_sync(0xffffffffu, x);
         if (lane == src) sum = x;
     }
     return sum;
 }
 // The block that tile `at` of a head of the sequence is in, and the tiles in front of it; by the whole warp, all lanes with the same arguments.
-__device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBlocks& k, int64_t at, int64_t* before) {
+__device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBlocks& k, int at, int* before) {
     const int lane = threadIdx.x & 31;
-    int64_t base = 0;
+    int base = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < k.n; i0 += 32) {
-        int64_t v = i0 + lane < k.n ? kt_view(P, k, i0 + lane).tiles : 0;
+        const int mine = i0 + lane < k.n ? kt_view(P, k, i0 + lane).tiles : 0;
+        int v = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         const unsigned past = __ballot_sync(0xffffffffu, base + v > at);
         if (past) {
             const int l = __ffs(past) - 1;
-            const int64_t upto = __shfl_sync(0xffffffffu, v, max(l - 1, 0));
-            *before = l ? base + upto : base;
+            *before = base + __shfl_sync(0xffffffffu, v - mine, l);
             return i0 + l;
         }
         base += __shfl_sync(0xffffffffu, v, 31);
@@ -194,18 +198,19 @@ struct KtWalk {
     KtBlocks k;
     KvView<KT_TILE> view;
     int t0, t1, rows, index;   // rows of the block; pieces before this one
-    __device__ __forceinline__ KtWalk(const KvAttendParams& P, int lim, const KvSpot& spot) {
+    // k and tiles: the blocks of the spot's sequence, and the tiles of one of its kv heads
+    __device__ __forceinline__ KtWalk(const KvAttendParams& P, const KvSpot& spot, const KtBlocks& blocks, int tiles) : k(blocks) {
         per = spot.per;
         w = per * blockIdx.x;
         w1 = min(spot.total, w + per);
         b = spot.b; index = -1; head = block = skip = 0;
-        k = kt_blocks(P, lim, b);
         if (w >= w1) return;
-        const int64_t tiles = __shfl_sync(0xffffffffu, kt_tiles(P, k), 0), in = w - spot.start;
+        const int64_t in = w - spot.start;
         head = (int)kv_quotient(in, tiles);
-        int64_t before;
-        block = kt_find_block(P, k, in - head * tiles, &before);
-        skip = (int)(in - head * tiles - before);
+        const int at = (int)(in - (int64_t)head * tiles);
+        int before = 0;
+        if (k.n > 1) block = kt_find_block(P, k, at, &before);
+        skip = at - before;
         block--;  // (next() goes on to it)
     }
     __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
@@ -275,19 +280,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     float* scales = reinterpret_cast<float*>(raw + S::RAWS * S::RAW);  // [slot][k, v][position]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    if (tid == 0) {
-        for (int i = 0; i < S::SLOTS; i++) { kv_bar_init(&full[i], I8 ? 4 : 1); kv_bar_init(&empty[i], I8 ? 2 : 6); kv_bar_init(&ready[i], 4); }
-        for (int i = 0; i < (I8 ? S::RAWS : 1); i++) { kv_bar_init(&raw_full[i], 1); kv_bar_init(&raw_empty[i], 4); }
-        for (int i = 0; i < KT_SCALE_SLOTS; i++) { kv_bar_init(&sc_full[i], 32); kv_bar_init(&sc_empty[i], 8); }
-        for (int i = 0; i < 2; i++) {
-            kv_bar_init(&q_full[i], 128); kv_bar_init(&drained[i], 1); kv_bar_init(&row_meet[i], 4);
-            for (int h = 0; h < 2; h++) { kv_bar_init(&s_full[i][h], 1); kv_bar_init(&p_full[i][h], 4); kv_bar_init(&pv_done[i][h], 1); }
-        }
-        for (int i = 0; i < KT_PIECES; i++) { kv_bar_init(&piece_full[i], 1); kv_bar_init(&piece_empty[i], 15); }
-        for (int i = 0; i < 8; i++) odd[i] = 0;
-        failed = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    // (Code that runs once comes from far away, 100 clocks and more for eight instructions: every warp prepares a little.)
+    if (warp == 4 && lane < S::SLOTS) { kv_bar_init(&full[lane], I8 ? 4 : 1); kv_bar_init(&empty[lane], I8 ? 2 : 6); kv_bar_init(&ready[lane], 4); }
+    if (I8 && warp == 5 && lane < S::RAWS) { kv_bar_init(&raw_full[lane], 1); kv_bar_init(&raw_empty[lane], 4); }
+    if (I8 && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], 8); }
+    if (warp == 7 && lane < KT_PIECES) { kv_bar_init(&piece_full[lane], 1); kv_bar_init(&piece_empty[lane], 15); }
+    if (warp == 8 && lane < 2) { kv_bar_init(&q_full[lane], 128); kv_bar_init(&drained[lane], 1); kv_bar_init(&row_meet[lane], 4); }
+    if (warp == 9 && lane < 4) { kv_bar_init(&s_full[0][0] + lane, 1); kv_bar_init(&p_full[0][0] + lane, 4); kv_bar_init(&pv_done[0][0] + lane, 1); }
+    if (warp == 10 && lane < 8) odd[lane] = 0;
+    if (tid == 0) failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == KT_MMA_WARP) {  // all 512 columns of tensor memory
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -295,8 +297,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvSpot spot{0, 0, -1, 0};
-    if (P.step.n_seqs > 32 || warp == KT_PLAN_WARP)  // (up to 32 sequences a warp finds its way alone)
-        spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
+    if (P.step.n_seqs > 32) spot = kv_locate<KT_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) { return (int64_t)kt_tiles(P, kt_blocks(P, lim, b)) * P.pool.n_kv_heads; });
     fence_before();
     __syncthreads();
     fence_after();
@@ -696,7 +697,20 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             }
         } else if (warp == KT_PLAN_WARP) {
             // ================= pieces, and what the next kernel has to know of them ===================================================
-            KtWalk walk(P, lim, spot);
+            // (up to 32 sequences: a lane has one)
+            const bool few = P.step.n_seqs <= 32;
+            KtBlocks k = kt_blocks(P, lim, few ? lane : spot.b);
+            int tiles = kt_tiles(P, k);
+            if (few) {
+                int src;
+                spot = kv_locate_few((int64_t)tiles * P.pool.n_kv_heads, blockIdx.x, gridDim.x, &src);
+                k.s.row0 = __shfl_sync(0xffffffffu, k.s.row0, src);
+                k.s.n = __shfl_sync(0xffffffffu, k.s.n, src);
+                k.s.kv = __shfl_sync(0xffffffffu, k.s.kv, src);
+                k.n = __shfl_sync(0xffffffffu, k.n, src);
+                tiles = __shfl_sync(0xffffffffu, tiles, src);
+            }
+            KtWalk walk(P, spot, k, tiles);
             KvCut cut{0, 0, 0, 0, 0, 0, 0};
             bool more = true;
             for (uint32_t n = 0; more; n++) {
