@@ -29,6 +29,7 @@ namespace l2 {
 namespace {
 
 constexpr int KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
+constexpr int KR_SETUP = 2;  // what a pair costs besides its tiles, in tiles
 constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
@@ -94,7 +95,7 @@ template <int TILE>
 __device__ __forceinline__ int64_t kr_length(const KvAttendParams& P, int lim, int b) {
     if (b >= P.step.n_seqs) return 0;
     const KrSeq<TILE> q(P, lim, b);
-    return q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0;
+    return q.rows ? (int64_t)(q.view.tiles + KR_SETUP) * P.pool.n_kv_heads : 0;
 }
 
 // A CTA's piece of the line, one (sequence, kv head) at a time.
@@ -116,17 +117,25 @@ struct KrWalk {
     }
     __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
         if (t0 >= 0) first = false;
-        if (w >= w1) return false;
-        while (w >= start + (q.rows ? (int64_t)q.view.tiles * P.pool.n_kv_heads : 0)) {
-            if (q.rows) start += (int64_t)q.view.tiles * P.pool.n_kv_heads;
-            q = KrSeq<TILE>(P, lim, ++b);
+#pragma unroll 1
+        while (w < w1) {
+            int64_t length = q.rows ? (int64_t)(q.view.tiles + KR_SETUP) * P.pool.n_kv_heads : 0;
+            while (w >= start + length) {
+                start += length;
+                q = KrSeq<TILE>(P, lim, ++b);
+                length = q.rows ? (int64_t)(q.view.tiles + KR_SETUP) * P.pool.n_kv_heads : 0;
+            }
+            const int64_t in = w - start;
+            const int place = q.view.tiles + KR_SETUP;  // of a pair on the line, whose first KR_SETUP are no tiles
+            head = (int)kv_quotient(in, place);
+            const int at = (int)(in - (int64_t)head * place), end = (int)min((int64_t)place, at + (w1 - w));
+            w += end - at;
+            if (end <= KR_SETUP) continue;  // (the pair's tiles begin in the next CTA)
+            t0 = max(0, at - KR_SETUP);
+            t1 = end - KR_SETUP;
+            return true;
         }
-        const int64_t in = w - start;
-        head = (int)kv_quotient(in, q.view.tiles);
-        t0 = (int)(in - (int64_t)head * q.view.tiles);
-        t1 = (int)min((int64_t)q.view.tiles, t0 + (w1 - w));
-        w += t1 - t0;
-        return true;
+        return false;
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == q.view.tiles; }
 };
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
             const int64_t row0 = walk.q.s.row0;
             const bool done = walk.whole();
             float* part = kv_part(P.work, gridDim.x, S::ROWS, HD, blockIdx.x, walk.first ? 0 : 1);
-            if (tid == 0 && walk.w >= walk.w1) {  // what the kernel behind this one has to know
+            if (tid == 0) {  // what the kernel behind this one has to know of the CTA's last piece
                 KvCut cut{0, 0, 0, 0, 0, 0, 0};
                 if (t0 == 0 && !done) cut = KvCut{(int)kv_quotient(walk.w - t1 + view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, rows, head, row0, view.lo_pos, 0};
                 kv_cuts(P.work)[blockIdx.x] = cut;
@@ -577,7 +586,7 @@ int kr_nt(int lim) { return lim <= 8 ? 1 : 2; }
 int kr_tile(int type, int head_size) { return head_size * (type == L2_I8 ? 1 : 2) == 256 ? 64 : 128; }
 // CTAs of a launch: two an SM, no more than there can be tiles
 int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
-    const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + tile - 1) / tile + 1);
+    const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + tile - 1) / tile + 1 + KR_SETUP);
     return (int)std::min<int64_t>(2 * sms, tiles);
 }
 

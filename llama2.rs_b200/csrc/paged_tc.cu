@@ -8,8 +8,8 @@
 // The products take 4 x 256 clocks a tile of positions (two tiles of rows, 128 x 128 x 128 each); the exponentials 2 x 1024 if the special function
 // unit (16 a clock) did them all.
 //
-// Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs; a block that a cut goes
-// through leaves a partial (m, l, O) in each piece, which kv_tc_combine_kernel adds in order.  Causal blocks of different lengths, windows
+// Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs, with room in front of every block for what it costs
+// besides its tiles (without it the SM with most blocks of a prompt of 8191 took 1.13 times the mean); a block that a cut goes through leaves a partial (m, l, O) in each piece, which kv_tc_combine_kernel adds in order.  Causal blocks of different lengths, windows
 // and ragged sequences need no other balance.
 //
 // Roles (they meet only through mbarriers):
@@ -39,6 +39,7 @@ namespace {
 constexpr int KT_TILE = 128, KT_SUB = 64, KT_ROWS = 256, KT_THREADS = 512;
 constexpr int KT_MMA_WARP = 0, KT_COPY_WARP = 1, KT_PLAN_WARP = 3, KT_ROW_WARP = 4, KT_HELP_WARP = 12;
 constexpr int KT_SCALE_SLOTS = 4;
+constexpr int KT_SETUP = 4;  // what a block costs besides its tiles, in tiles
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
 template <int CT, int HD>
@@ -145,7 +146,7 @@ __device__ __forceinline__ int kt_tiles(const KvAttendParams& P, KtBlocks k) {
     int sum = 0;
     if (k.n <= 4) {
 #pragma unroll 1
-        for (int i = 0; i < k.n; i++) sum += kt_view(P, k, i).tiles;
+        for (int i = 0; i < k.n; i++) sum += KT_SETUP + kt_view(P, k, i).tiles;
     }
     unsigned many = __ballot_sync(0xffffffffu, k.n > 4);
 #pragma unroll 1
@@ -158,7 +159,7 @@ __device__ __forceinline__ int kt_tiles(const KvAttendParams& P, KtBlocks k) {
         q.n = __shfl_sync(0xffffffffu, k.n, src);
         int x = 0;
 #pragma unroll 1
-        for (int i = lane; i < q.n; i += 32) x += kt_view(P, q, i).tiles;
+        for (int i = lane; i < q.n; i += 32) x += KT_SETUP + kt_view(P, q, i).tiles;
         x = __reduce_add_sync(0xffffffffu, x);
         if (lane == src) sum = x;
     }
@@ -170,7 +171,7 @@ __device__ __forceinline__ int kt_find_block(const KvAttendParams& P, const KtBl
     int base = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < k.n; i0 += 32) {
-        const int mine = i0 + lane < k.n ? kt_view(P, k, i0 + lane).tiles : 0;
+        const int mine = i0 + lane < k.n ? KT_SETUP + kt_view(P, k, i0 + lane).tiles : 0;
         int v = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -214,22 +215,27 @@ struct KtWalk {
         block--;  // (next() goes on to it)
     }
     __device__ __forceinline__ bool next(const KvAttendParams& P, int lim) {
-        if (w >= w1) return false;
-        index++;
-        if (++block >= k.n) {
-            block = 0;
-            if (++head == P.pool.n_kv_heads) {
-                head = 0;
-                do k = kt_blocks(P, lim, ++b); while (!k.n && b < P.step.n_seqs);
+#pragma unroll 1
+        while (w < w1) {
+            if (++block >= k.n) {
+                block = 0;
+                if (++head == P.pool.n_kv_heads) {
+                    head = 0;
+                    do k = kt_blocks(P, lim, ++b); while (!k.n && b < P.step.n_seqs);
+                }
             }
+            view = kt_view(P, k, block);
+            const int at = skip, end = (int)min((int64_t)view.tiles + KT_SETUP, at + (w1 - w));  // of the block's place on the line, whose first KT_SETUP are no tiles
+            skip = 0;
+            w += end - at;
+            t0 = max(0, at - KT_SETUP);
+            t1 = end - KT_SETUP;
+            if (t1 <= t0) continue;  // (the block's tiles begin in the next CTA)
+            rows = min(k.tokens, k.s.n - block * k.tokens) * P.group;
+            index++;
+            return true;
         }
-        view = kt_view(P, k, block);
-        rows = min(k.tokens, k.s.n - block * k.tokens) * P.group;
-        t0 = skip;
-        skip = 0;
-        t1 = (int)min((int64_t)view.tiles, t0 + (w1 - w));
-        w += t1 - t0;
-        return true;
+        return false;
     }
 };
 
@@ -875,7 +881,7 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
 // CTAs of a launch: one an SM, no more than there can be tiles
 int kt_grid(const KvStep& s, const KvPool& p, int group, int sms) {
     const int64_t blocks = s.n_rows / (KT_ROWS / group) + s.n_seqs;
-    return (int)std::min<int64_t>(sms, blocks * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KT_TILE - 1) / KT_TILE + 1));
+    return (int)std::min<int64_t>(sms, blocks * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KT_TILE - 1) / KT_TILE + 1 + KT_SETUP));
 }
 
 bool kt_needed(const KvStep& s, int group) { return (int64_t)s.max_rows * group > kv_rows_limit(s, group); }
