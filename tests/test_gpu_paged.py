@@ -448,3 +448,20 @@ def test_refusals_of_the_python_objects(l2):
     pages.attend(batch, none, none)
     pages.append(batch, none, none)
     pages.read(batch, none, none)
+
+
+# the workspace may hold anything, whatever the cuts of the work are: few and many sequences, pieces of one sequence, singles among chunks
+@pytest.mark.parametrize("cache,io", [CACHES[1], CACHES[2]])
+@pytest.mark.parametrize("rows,kv,group", [([1], [5000], 1), ([1] * 24, list(range(30, 2500, 103)), 1), ([1] * 40, [7] * 39 + [9000], 4), ([5] * 12, list(range(300, 3000, 225)), 8),
+                                           ([300, 1, 290, 1, 1], [2000, 1500, 300, 40, 3000], 2), ([700], [700], 1)])
+def test_workspace_contents_do_not_matter(l2, cache, io, rows, kv, group):
+    c = Case(rows, kv, kv_heads=8, group=group, cache=cache)
+    q, want = run_attend(l2, c, io)
+    pages, batch = c.handles(l2)
+    work = torch.empty(pages.workspace_bytes(batch, c.heads), dtype=torch.uint8, device="cuda")
+    for fill in (0, 1, 127, 255):
+        work.fill_(fill)
+        out = torch.full_like(q, 7.0)
+        pages.attend(batch, q, out, workspace=work)
+        assert torch.equal(out, want), fill
+    assert int(c.status) == 0
