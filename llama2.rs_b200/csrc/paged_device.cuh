@@ -39,6 +39,7 @@ struct KvWait {
     }
     __device__ __forceinline__ bool over() const { return __any_sync(0xffffffffu, *failed); }  // (by whole warps)
 };
+__device__ __forceinline__ void kv_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void kv_tma4(uint32_t dst, const CUtensorMap* map, int x, int pos, int head, int page, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(pos), "r"(head), "r"(page), "r"(kv_smem(bar)) : "memory");

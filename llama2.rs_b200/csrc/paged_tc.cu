@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (warp == KT_COPY_WARP && lane < 2) kv_prefetch_map(lane ? &map_v : &map_k);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvSpot spot{0, 0, -1, 0};

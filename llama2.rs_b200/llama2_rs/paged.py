@@ -21,6 +21,7 @@ BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
 _TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.int32": I32}
 _types = {}  # the same by dtype object, filled as they are seen
 _ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
+_append, _read, _attend = lib.l2_kv_append, lib.l2_kv_read, lib.l2_kv_attend
 assert _ROWS2.size == 2 * C.sizeof(KvRowsArgs) and _ROWS4.size == 4 * C.sizeof(KvRowsArgs)
 
 
@@ -31,18 +32,27 @@ def _type(t):
     return _types[d]
 
 
-def _stream(stream, device):
-    if stream is not None:
-        return stream
+_cuda = None  # torch's functions for the current device and its current stream, found at the first call without a stream
+
+
+def _find_cuda():
+    global _cuda
     torch = sys.modules["torch"]
-    if torch.cuda.current_device() != device:
+    # (the raw stream without making a Stream object, which takes longer than the launch)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    _cuda = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device, raw)
+
+
+def _stream(device):
+    if _cuda is None:
+        _find_cuda()
+    if _cuda[0]() != device:
         raise ValueError("the tensors are on device %d, which is not the current one" % device)
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (without making a Stream object, which takes longer than the launch)
-    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
+    return _cuda[1](device)
 
 
 def _packed(t, what, device, shape, dtype):
-    if t.get_device() != device or tuple(t.shape) != shape or _type(t) != dtype or not t.is_contiguous():  # (-1: not on a CUDA device)
+    if t.shape != shape or _type(t) != dtype or not t.is_contiguous() or t.get_device() != device:  # (-1: not on a CUDA device)
         raise ValueError("%s: contiguous %s of type code %d on device %d expected, got %s of %s" % (what, shape, dtype, device, tuple(t.shape), t.dtype))
     return t.data_ptr()
 
@@ -102,12 +112,12 @@ class KvPages:
         try:
             m, h, size = t.shape
             row, head, one = t.stride()
+            kind = _types[t.dtype]
         except ValueError:
             m = h = size = one = -1
-        kind = _types.get(t.dtype)
-        if kind is None:
+        except KeyError:
             kind = _type(t)
-        if m != n or size != self.head_size or one != 1 or (heads and h != heads) or t.get_device() != self.device:
+        if m != n or size != self.head_size or one != 1 or t.get_device() != self.device or (heads and h != heads):
             raise ValueError("%s: [%d, %s, %d] on device %d with its last dimension contiguous expected, got %s" % (what, n, heads or "heads", self.head_size, self.device, tuple(t.shape)))
         return t.data_ptr(), row, head, kind, h
 
@@ -131,13 +141,17 @@ class KvPages:
             positions = cos.shape[0]
             shape = (positions, self.head_size // 2)
             cos, sin = _packed(cos, "rope", self.device, shape, F32), _packed(sin, "rope", self.device, shape, F32)
-        check(lib.l2_kv_append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(stream, self.device)))
+        rc = _append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(self.device) if stream is None else stream)
+        if rc:
+            check(rc)
 
     def read(self, batch, k, v, stream=None):
         """The cached positions of the step's rows into k and v ([rows, kv_heads, head_size], f32, f16 or bf16)."""
         n, heads = batch.n_rows, self.n_kv_heads
         _ROWS2.pack_into(self._rows, 0, *self._row(k, "k", n, heads), *self._row(v, "v", n, heads))
-        check(lib.l2_kv_read(self._ref, batch._ref, self._at[0], self._at[1], _stream(stream, self.device)))
+        rc = _read(self._ref, batch._ref, self._at[0], self._at[1], _stream(self.device) if stream is None else stream)
+        if rc:
+            check(rc)
 
     def workspace_bytes(self, batch, n_heads):
         return int(lib.l2_kv_attend_workspace_bytes(self._ref, batch._ref, n_heads))
@@ -154,6 +168,8 @@ class KvPages:
             workspace = q.new_empty(self.workspace_bytes(batch, row[4]), dtype=sys.modules["torch"].uint8)
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("workspace: a contiguous tensor on the cache's device expected")
-        check(lib.l2_kv_attend(self._ref, batch._ref, self._at[0], self._at[1], self.head_size ** -0.5 if scale is None else scale, window, sinks,
-                               workspace.data_ptr(), workspace.nbytes, _stream(stream, self.device)))
+        rc = _attend(self._ref, batch._ref, self._at[0], self._at[1], self.head_size ** -0.5 if scale is None else scale, window, sinks,
+                     workspace.data_ptr(), workspace.nbytes, _stream(self.device) if stream is None else stream)
+        if rc:
+            check(rc)
         return out
