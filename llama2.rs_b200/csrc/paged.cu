@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_c
                         // two's complement is the low byte: a conversion instruction takes four times as long.  What is not finite gives any byte: the scale is NaN.)
                         uint32_t b[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) b[i] = __float_as_uint(__fmaf_rn(x[i], inv, 12582912.0f));
+                        for (int i = 0; i < 16; i++) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f));
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) b[i / 4] = __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
                         if (!store) continue;
