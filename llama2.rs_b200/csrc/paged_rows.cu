@@ -2,15 +2,18 @@
 //
 // For one kv head of one sequence, with the rows' queries Q (8 NT rows at most), keys K and values V:
 //   S^T = K Q^T,  P^T = 2^(scale S^T - m),  O^T += V^T P^T,  l += sum P,   out = O / l
-// m is the running maximum of a row; when it moves, O and l are scaled.  The products are taken transposed: positions (S^T) and head
-// elements (O^T) are the 16 rows of an mma.sync.m16n8k16, the few query rows its 8 columns, so that one row wastes 7 of 8, not 15 of 16.
-// The kernel is bound by reading the cache: it is read once, by TMA, while the matrix work of a tile hides behind the copies of the next.
+// m is a row's maximum of some earlier tile, raised (O and l scaled) only when a score exceeds it by more than 2^8.  The products are taken transposed: positions (S^T)
+// and head elements (O^T) are the 16 rows of an mma.sync, the few query rows its 8 columns, so that one row wastes 7 of 8, not 15 of 16.
 //
-// Work.  The tiles of 64 positions of all (sequence, kv head) pairs form one line, cut evenly over the CTAs whatever the lengths are; a pair
-// that a cut goes through leaves a partial (m, l, O) in each piece, which kv_combine_kernel adds in order.  The cuts are found on the device: the host
-// does not know the lengths.
+// What bounds it: reading the cache, once, by TMA, while the matrix work of a tile hides behind the copies of the next.  bf16, 8 sequences of 40 heads, 4096 positions each
+// (672 MB): 115 us, 5.9 TB/s.  int8, 64 sequences of 8 kv heads with 8 query heads (565 MB): 112 to 118 us, 4.8 to 5.0 TB/s, for most of the time bound by the instructions that
+// widen V (173 us while a compiler made two instructions of each of their logic operations, 194 with tiles of 64 positions).
 //
-// Roles: warps 0-3 take 16 positions of a tile each, with a softmax of their own, and meet at the end of a piece; warp 4 fills a ring of
+// Work.  The tiles of all (sequence, kv head) pairs form one line, cut evenly over the CTAs whatever the lengths are, with room in front of every pair for what it costs
+// besides its tiles (134 -> 119 us for that int8 step); a pair that a cut goes through leaves a partial (m, l, O) in each piece, which kv_rows_combine_kernel adds in
+// order.  The cuts are found on the device: the host does not know the lengths.
+//
+// Roles: warps 0-3 take 16 or 32 positions of a tile each, with a softmax of their own, and meet at the end of a piece; warp 4 fills a ring of
 // tiles with TMA copies, one a page run (and the scales of an int8 cache, 16 bytes a lane).
 //
 // An int8 cache is multiplied as it is stored: K as q's type and V as bf16, both exact; the scale of a position is applied to its score and to
@@ -35,8 +38,8 @@ constexpr int KR_SETUP = 2;  // what a pair costs besides its tiles, in tiles
 constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
-// A variant: 16 KB of K and as much of V in a tile, 64 or 128 positions, of which a warp has 16 or 32 (an int8 cache with tiles of 64 positions was bound by the
-// chain of a warp's step, 2000 clocks whatever the bytes: 194 us where the same step over bf16, twice the bytes, takes 197).
+// A variant: 16 KB of K and as much of V in a tile, 64 or 128 positions, of which a warp has 16 or 32 (an int8 cache in tiles of 64 was bound by the
+// chain of a warp's step, 2000 clocks whatever the bytes).
 // Shared memory: Q and the ring; the warps' results meet in the slot of a piece's last tile.
 template <int CT, int HD, int NT>
 struct KrShape {

@@ -5,17 +5,22 @@
 // m is a row's maximum of some earlier tile: it is raised, and O and l scaled, only when a score exceeds it by more than 2^8 (the sums
 // are f32: a common factor costs nothing).
 //
-// The products take 4 x 256 clocks a tile of positions (two tiles of rows, 128 x 128 x 128 each); the exponentials 2 x 1024 if the special function
-// unit (16 a clock) did them all.
+// What bounds it.  A tile of positions is four products of 128 x 128 x 128, 2048 clocks of the tensor cores at their peak; 32768 exponentials, 2048 clocks of the
+// special function units; and, because S is taken 64 positions at a time, 320 KB through shared memory at 128 bytes a clock, 2500.  A whole prompt (8191 tokens, 32
+// heads of 128, bf16) takes about 3500 clocks a tile: 540 us on one input (1021 TFLOP/s of 1621 measured), 640 to 660 between others, as the chip's power allows.
+// Measured on the way (the same prompt): one warp issuing for both tiles of rows 1017 us (an issue takes 75 to 85 clocks, whatever its size, and a wait some hundred); two
+// 918; S in halves 803; Q requested eight lines at once 656; pieces planned by one warp, so that nothing spills, 598; room on the line for a block's other costs 539.
+// Not kept: exponentials on the FMA units (1, 2 or 4 of 16: 559 to 565 against 556), the two groups of softmax taking turns (608 against 598), a predicate in place of
+// the branch around the issue (569 against 556).  An int8 cache costs about 1700 clocks a tile more (scales of 64 positions a thread, and their products).
 //
-// Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs, with room in front of every block for what it costs
-// besides its tiles (without it the SM with most blocks of a prompt of 8191 took 1.13 times the mean); a block that a cut goes through leaves a partial (m, l, O) in each piece, which kv_tc_combine_kernel adds in order.  Causal blocks of different lengths, windows
-// and ragged sequences need no other balance.
+// Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs, with room in front of every
+// block for what it costs besides its tiles (without it the SM with most blocks of that prompt took 1.13 times the mean); a block that a cut
+// goes through leaves a partial (m, l, O) in each piece, which kv_tc_combine_kernel adds in order.  Causal blocks of different lengths,
+// windows and ragged sequences need no other balance.
 //
 // Roles (they meet only through mbarriers):
 //   warps 0, 2      one thread each issues the products of Q0 and of Q1, for 64 positions at a time, S in two halves of its room in turn: O += P V of one half,
-//                   S = Q K of the same half of the next tile, and so on; the softmax finds the next scores ready.  (One warp for both was the bound: the issue of a product
-//                   takes 80 clocks, and every wait adds a few hundred.)
+//                   S = Q K of the same half of the next tile, and so on; the softmax finds the next scores ready
 //   warp 1          K and V tiles by TMA into one ring, a copy a page run
 //   warp 3          plans the pieces of the CTA, a few ahead, and leaves the kernel behind this one a record of the block that the CTA's end cuts
 //   warps 4-7, 8-11 softmax of Q0 and Q1, a row a thread; they bring Q, and the result out

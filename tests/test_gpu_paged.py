@@ -185,6 +185,42 @@ def test_pool_with_strides(l2):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("cache,io", CACHES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pool_with_gaps(l2, cache, io, hd):
+    """Strides that are no multiples of one another: a gap of 16 bytes behind every head, another behind every position, another behind every page."""
+    gap = 16 if cache == I8 else 8
+    for rows, kv in (([1, 1], [100, 37]), ([70, 200], [150, 260])):
+        a = Case(rows, kv, cache=cache, group=2, hd=hd, seed=11)
+        q, want = run_attend(l2, a, io)
+        head, pos = hd + gap, 2 * (hd + gap) + 3 * gap
+        page = a.page * pos + 5 * gap
+        pools = []
+        for t in (a.k, a.v):
+            flat = torch.zeros(a.n_pages * page + hd, dtype=cache, device="cuda")
+            view = flat.as_strided((a.n_pages, a.page, 2, hd), (page, pos, head, 1))
+            view.copy_(t)
+            pools.append(view)
+        a.k, a.v = pools
+        _, out = run_attend(l2, a, io, q=q)
+        assert torch.equal(out, want)
+        new = torch.randn((a.n, 2, hd), device="cuda").to(io)
+        back = [torch.zeros_like(new) for _ in "kv"]
+        pages, batch = a.handles(l2)
+        pages.append(batch, new, new)
+        pages.read(batch, *back)
+        assert torch.equal(back[0], back[1]) and (cache == I8 or torch.equal(back[0], new))
+
+
+@pytest.mark.parametrize("cache,io", CACHES)
+def test_more_rows_than_positions(l2, cache, io):
+    """Rows of negative positions see nothing: 0, whole blocks of them too."""
+    for rows, kv in (([600, 1, 3], [5, 0, 0]), ([300], [0]), ([9, 1], [4, 2])):
+        c = Case(rows, kv, cache=cache, group=2, seed=2)
+        compare(l2, c, io)
+        compare(l2, c, io, window=3, sinks=1)
+
+
 @pytest.mark.parametrize("cache,io", [CACHES[1], CACHES[2]])
 def test_offsets_beyond_32_bits(l2, cache, io):
     """Pages whose elements, and bytes, start beyond 2^32."""
