@@ -25,9 +25,10 @@ cudaError_t kv_map(CUtensorMap* map, const KvPool& p, const void* base, int type
     const cuuint64_t dims[4] = {(cuuint64_t)head_size, (cuuint64_t)page, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)p.pos_stride * size, (cuuint64_t)p.head_stride * size, (cuuint64_t)p.page_stride * size};
     const cuuint32_t box[4] = {(cuuint32_t)std::min(head_size, 128 / size), (cuuint32_t)std::min(page, tile), 1, 1}, step[4] = {1, 1, 1, 1};
+    // (A row of 256 bytes comes in two copies: the first brings both halves to the L2, 115 -> 112 us for 672 MB of them; rows of 128 take 112 us as they are, 125 in pairs.)
     const CUresult r = encode(map, type == L2_I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == L2_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                               const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              head_size * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              head_size * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, head_size * size == 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
