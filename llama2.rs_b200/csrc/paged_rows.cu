@@ -35,6 +35,7 @@ namespace {
 
 constexpr int KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
 constexpr int KR_SETUP = 2;  // what a pair costs besides its tiles, in tiles
+constexpr int KR_JOIN = 2;  // CTAs that add the pieces of a pair (with 4 or 8, a step of 64 sequences takes 2 or 5 us longer: CTAs without work)
 constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
@@ -585,7 +586,8 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
 }
 
 // Adds the pieces of the pair that begins in CTA x of the launch in front and goes on in the next.
-// HD / 4 threads for a row; with fewer than eight rows the others take pieces of the same row, and meet in order.
+// HD / 4 threads for a row; with few rows the others take pieces of the same row, and meet in order.  The rows go over KR_JOIN CTAs.
+// One sequence of 60,000 positions and 8 kv heads (int8, 37 pieces a pair): attention 37 us; 46 with one CTA a pair and each thread walking all maxima and sums.
 template <int HD>
 __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_constant__ KvAttendParams P, const int ctas, const int part_rows) {
     constexpr int LANES = HD / 4, SLOTS = 256 / LANES;
@@ -596,23 +598,28 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
     if (!cut.pieces) return;
     auto piece = [&](int i) { return kv_part(P.work, ctas, part_rows, HD, blockIdx.x + i, i == 0 ? cut.slot : 0); };
     int width = 1;  // rows side by side
-    while (width < cut.rows && width < SLOTS) width <<= 1;
+    while (width * (int)gridDim.y < cut.rows && width < SLOTS) width <<= 1;
     const int share = SLOTS / width, slot = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES), mine = slot / width;
-    for (int r0 = 0; r0 < cut.rows; r0 += width) {
+    for (int r0 = blockIdx.y * width; r0 < cut.rows; r0 += gridDim.y * width) {
         const int r = r0 + slot % width;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.0f;
-        if (r < cut.rows) {
-            float top = -INFINITY;
-#pragma unroll 4
-            for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[part_rows * HD + 2 * r]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-            for (int i = 0; i < cut.pieces; i++) sum += KvScale(piece(i)[part_rows * HD + 2 * r] - ref)(piece(i)[part_rows * HD + 2 * r + 1]);
-#pragma unroll 4
+        const bool on = r < cut.rows;
+        // the common maximum and the sum: piece i by thread i % LANES of the row
+        const int ml = part_rows * HD + 2 * r;
+        float top = -INFINITY;
+        for (int i = threadIdx.x % LANES; i < cut.pieces; i += LANES) if (on) top = fmaxf(top, piece(i)[ml]);
+#pragma unroll
+        for (int x = 1; x < LANES; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int i = threadIdx.x % LANES; i < cut.pieces; i += LANES) if (on) sum += KvScale(piece(i)[ml] - ref)(piece(i)[ml + 1]);
+#pragma unroll
+        for (int x = 1; x < LANES; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (on) {
+#pragma unroll 8
             for (int i = mine; i < cut.pieces; i += share) {
                 const float* p = piece(i);
-                const KvScale f(p[part_rows * HD + 2 * r] - ref);
+                const KvScale f(p[ml] - ref);
                 const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
                 acc.x += f(x.x); acc.y += f(x.y); acc.z += f(x.z); acc.w += f(x.w);
             }
@@ -626,7 +633,7 @@ __global__ void __launch_bounds__(256) kv_rows_combine_kernel(const __grid_const
             }
             __syncthreads();
         }
-        if (r < cut.rows && mine == 0) {
+        if (on && mine == 0) {
             const int tok = r / P.group, pos = cut.lo_pos + tok;
             const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride + d;
             const float inv = 1.0f / sum;
@@ -688,7 +695,7 @@ cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int
     });
     if (e != cudaSuccess || grid < 2) return e;
     auto combine = head_size == 128 ? kv_rows_combine_kernel<128> : kv_rows_combine_kernel<64>;
-    return kv_launch(combine, dim3(grid - 1), 256, 0, st, p, grid, 8 * nt);
+    return kv_launch(combine, dim3(grid - 1, KR_JOIN), 256, 0, st, p, grid, 8 * nt);
 }
 
 }  // namespace l2

@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 }
 
 // Adds the pieces of the block of rows that begins in CTA x of the launch in front and goes on in the next.  A thread has a row and eight columns; the lanes of a
-// warp have rows side by side, as the pieces lie.
+// warp have rows side by side, as the pieces lie; blockIdx.z has 64 columns (one sequence of 5 x 8 rows, 18 pieces a kv head: 24.2 -> 22.5 us).
 template <int HD>
 __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constant__ KvAttendParams P, const int ctas) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -855,10 +855,10 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
     if (!cut.pieces || r >= cut.rows) return;
     auto piece = [&](int i) { return kv_part(P.work, ctas, KT_ROWS, HD, blockIdx.x + i, i == 0 ? cut.slot : 0); };
     float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < cut.pieces; i++) top = fmaxf(top, piece(i)[KT_ROWS * HD + 2 * r]);
     const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < cut.pieces; i++) {
         const float2 ml = *reinterpret_cast<const float2*>(piece(i) + KT_ROWS * HD + 2 * r);
         sum += KvScale(ml.x - ref)(ml.y);
@@ -866,22 +866,21 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
     const int tok = kt_token(P, r), pos = cut.lo_pos + tok;
     const int64_t e = (cut.row0 + tok) * P.out.row_stride + (int64_t)(cut.head * P.group + r - tok * P.group) * P.out.head_stride;
     const float inv = 1.0f / sum;
-    for (int d = 8 * (threadIdx.x >> 5); d < HD; d += 64) {
-        float y[8] = {};
-#pragma unroll 2
-        for (int i = 0; i < cut.pieces; i++) {
-            const float* p = piece(i);
-            const KvScale f(p[KT_ROWS * HD + 2 * r] - ref);
-            const float4 a = *reinterpret_cast<const float4*>(p + (d / 4 * KT_ROWS + r) * 4), b = *reinterpret_cast<const float4*>(p + ((d / 4 + 1) * KT_ROWS + r) * 4);
-            y[0] += f(a.x); y[1] += f(a.y); y[2] += f(a.z); y[3] += f(a.w);
-            y[4] += f(b.x); y[5] += f(b.y); y[6] += f(b.z); y[7] += f(b.w);
-        }
-#pragma unroll
-        for (int x = 0; x < 8; x++) y[x] = pos < 0 ? 0.0f : y[x] * inv;
-        if (P.out.type == L2_F32) kv_store8(reinterpret_cast<float*>(P.out.data) + e + d, y);
-        else if (P.out.type == L2_F16) kv_store8(reinterpret_cast<__half*>(P.out.data) + e + d, y);
-        else kv_store8(reinterpret_cast<__nv_bfloat16*>(P.out.data) + e + d, y);
+    const int d = 8 * (threadIdx.x >> 5) + 64 * blockIdx.z;
+    float y[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < cut.pieces; i++) {
+        const float* p = piece(i);
+        const KvScale f(p[KT_ROWS * HD + 2 * r] - ref);
+        const float4 a = *reinterpret_cast<const float4*>(p + (d / 4 * KT_ROWS + r) * 4), b = *reinterpret_cast<const float4*>(p + ((d / 4 + 1) * KT_ROWS + r) * 4);
+        y[0] += f(a.x); y[1] += f(a.y); y[2] += f(a.z); y[3] += f(a.w);
+        y[4] += f(b.x); y[5] += f(b.y); y[6] += f(b.z); y[7] += f(b.w);
     }
+#pragma unroll
+    for (int x = 0; x < 8; x++) y[x] = pos < 0 ? 0.0f : y[x] * inv;
+    if (P.out.type == L2_F32) kv_store8(reinterpret_cast<float*>(P.out.data) + e + d, y);
+    else if (P.out.type == L2_F16) kv_store8(reinterpret_cast<__half*>(P.out.data) + e + d, y);
+    else kv_store8(reinterpret_cast<__nv_bfloat16*>(P.out.data) + e + d, y);
 }
 
 // CTAs of a launch: one an SM, no more than there can be tiles
@@ -920,7 +919,7 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
     if (e != cudaSuccess || grid < 2) return e;
     auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;
-    return kv_launch(combine, dim3(grid - 1, KT_ROWS / 32), 256, 0, st, p, grid);
+    return kv_launch(combine, dim3(grid - 1, KT_ROWS / 32, head_size / 64), 256, 0, st, p, grid);
 }
 
 }  // namespace l2
