@@ -254,6 +254,14 @@ def test_many_sequences_and_splits(l2):
     compare(l2, Case([40, 3], [20000, 3], group=8, kv_heads=1, cache=BF16), BF16)
 
 
+# one pair cut into more pieces than a warp has threads: few rows (1, 3, 9, 16) and a block of 2 x 20
+@pytest.mark.parametrize("tokens,group", [(1, 1), (1, 3), (3, 3), (2, 8), (2, 20)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cache,io", [CACHES[1], CACHES[3]])
+def test_many_pieces(l2, cache, io, hd, tokens, group):
+    compare(l2, Case([tokens], [25001], hd=hd, group=group, cache=cache, kv_heads=1, page=64), io)
+
+
 def test_same_bits_every_time(l2):
     for rows, kv in (([1] * 9, [700, 3, 5000, 64, 1, 90, 1200, 333, 2]), ([300, 200], [3000, 200])):
         c = Case(rows, kv, cache=BF16, group=4)
