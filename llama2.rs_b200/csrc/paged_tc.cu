@@ -11,7 +11,9 @@
 // Measured on the way (the same prompt): one warp issuing for both tiles of rows 1017 us (an issue takes 75 to 85 clocks, whatever its size, and a wait some hundred); two
 // 918; S in halves 803; Q requested eight lines at once 656; pieces planned by one warp, so that nothing spills, 598; room on the line for a block's other costs 539.
 // Not kept: exponentials on the FMA units (1, 2 or 4 of 16: 559 to 565 against 556), the two groups of softmax taking turns (608 against 598), a predicate in place of
-// the branch around the issue (569 against 556).  An int8 cache costs about 1700 clocks a tile more (scales of 64 positions a thread, and their products).
+// the branch around the issue (569 against 556).  An int8 cache costs about 1500 clocks a tile more (scales of 64 positions
+// a thread and their products, and bytes to widen: 512 tokens of 64 heads behind 14,488 positions take 360 us, 252 without either and 350 without one of them; four rows
+// a quad of threads, so that each thread reads a quarter of the scales, took 349, but 40 rows a kv head 58 instead of 52).
 //
 // Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs, with room in front of every
 // block for what it costs besides its tiles (without it the SM with most blocks of that prompt took 1.13 times the mean); a block that a cut
@@ -120,6 +122,11 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     unsigned long long d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
     unsigned long long d;
@@ -399,10 +406,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 #pragma unroll
                         for (int j = 0; j < KT_SUB; j += 4) {
                             const float4 k = *reinterpret_cast<const float4*>(ks + j);
-                            x[j] = __float_as_uint(__uint_as_float(x[j]) * k.x);
-                            x[j + 1] = __float_as_uint(__uint_as_float(x[j + 1]) * k.y);
-                            x[j + 2] = __float_as_uint(__uint_as_float(x[j + 2]) * k.z);
-                            x[j + 3] = __float_as_uint(__uint_as_float(x[j + 3]) * k.w);
+                            const float2 a = unpair(mul2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), pair(k.x, k.y)));
+                            const float2 b = unpair(mul2(pair(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), pair(k.z, k.w)));
+                            x[j] = __float_as_uint(a.x); x[j + 1] = __float_as_uint(a.y); x[j + 2] = __float_as_uint(b.x); x[j + 3] = __float_as_uint(b.y);
                         }
                     }
                     if (!whole) {
@@ -442,22 +448,26 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     const float ref = m == -INFINITY ? 0.0f : m;
                     const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
                     unsigned long long sum[2] = {0ull, 0ull};
-                    uint32_t p16[KT_SUB / 2];
-                    float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
+                    auto probabilities = [&](auto is_whole) {  // (an int8 cache with the choice at every element: 378 us instead of 362)
+                        uint32_t p16[KT_SUB / 2];
+                        float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int j = 0; j < KT_SUB; j += 2) {
-                        const float2 e = unpair(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, r2));
-                        float2 p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
-                        sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(p.x, p.y));
-                        if constexpr (I8) {
-                            if (j % 4 == 0) v4 = *reinterpret_cast<const float4*>(ks + KT_TILE + j);
-                            const float2 v = j % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
-                            if (whole) p = make_float2(p.x * v.x, p.y * v.y);
-                            else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
+                        for (int j = 0; j < KT_SUB; j += 2) {
+                            const float2 e = unpair(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, r2));
+                            float2 p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
+                            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(p.x, p.y));
+                            if constexpr (I8) {
+                                if (j % 4 == 0) v4 = *reinterpret_cast<const float4*>(ks + KT_TILE + j);
+                                const float2 v = j % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                                if constexpr (decltype(is_whole)::value) p = unpair(mul2(pair(p.x, p.y), pair(v.x, v.y)));
+                                else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
+                            }
+                            p16[j / 2] = pack16<PB>(p.x, p.y);
                         }
-                        p16[j / 2] = pack16<PB>(p.x, p.y);
-                    }
-                    tmem_st32(s_at, p16);
+                        tmem_st32(s_at, p16);
+                    };
+                    if (!I8 || whole) probabilities(std::true_type());
+                    else probabilities(std::false_type());
                     const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
                     l += (s0.x + s0.y) + (s1.x + s1.y);
                     wait_st();
