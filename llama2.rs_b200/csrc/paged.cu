@@ -345,6 +345,16 @@ int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_
     return L2_OK;
 }
 
+// What attention asks of the heads and sizes, before anything divides by them: query heads per kv head, and tiles that are counted in 31 bits.
+int check_heads(const char* who, const l2_kv_pages* p, const l2_kv_batch* b, int n_heads) {
+    if (n_heads < 1 || n_heads % p->n_kv_heads || n_heads / p->n_kv_heads > 64)
+        return fail(L2_EINVAL, "%s: %d query heads, %d kv heads (1 to 64 times as many)", who, n_heads, p->n_kv_heads);
+    const int64_t positions = (int64_t)b->table_width * p->page_size;
+    if (((int64_t)b->max_rows * (n_heads / p->n_kv_heads) / 64 + 1) * ((positions + 127) / 128 + 1) >> 31)
+        return fail(L2_ERANGE, "%s: %d rows of a sequence over %lld positions (more than 2^31 tiles)", who, b->max_rows, (long long)positions);
+    return L2_OK;
+}
+
 template <class F>
 cudaError_t by_type(int type, int head_size, F f) {
     if (head_size == 128) {
@@ -428,8 +438,7 @@ extern "C" size_t l2_kv_attend_workspace_bytes(const l2_kv_pages* pages, const l
     KvPool pool;
     KvStep step;
     int sms;
-    if (check_pages(who, pages, &pool) || check_batch(who, batch, pages->page_size, &step) || kv_device(&sms)) return 0;
-    if (n_heads < 1 || n_heads % pool.n_kv_heads) { fail(L2_EINVAL, "%s: %d heads, %d kv heads", who, n_heads, pool.n_kv_heads); return 0; }
+    if (check_pages(who, pages, &pool) || check_batch(who, batch, pages->page_size, &step) || check_heads(who, pages, batch, n_heads) || kv_device(&sms)) return 0;
     return kv_attend_work(step, pool, n_heads, pages->type, pages->head_size, sms);
 }
 
@@ -440,14 +449,12 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     KvAttendParams P{};
     if (int rc = check_pages(who, pages, &P.pool)) return rc;
     if (int rc = check_batch(who, batch, pages->page_size, &P.step)) return rc;
-    if (!q || q->heads < 1 || q->heads % pages->n_kv_heads || q->heads / pages->n_kv_heads > 64)
-        return fail(L2_EINVAL, "%s: the heads of q must be 1 to 64 times the kv heads", who);
+    if (!q) return fail(L2_EINVAL, "%s: no q", who);
+    if (int rc = check_heads(who, pages, batch, q->heads)) return rc;
     if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, &P.q)) return rc;
     if (int rc = check_rows(who, "out", out, batch, pages->head_size, q->heads, &P.out)) return rc;
     if (q->type == L2_F32 || (pages->type != L2_I8 && q->type != pages->type)) return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 cache)", who);
     if (out->type != L2_F32 && out->type != q->type) return fail(L2_EINVAL, "%s: out must be of q's type or f32", who);
-    if ((int64_t)((int64_t)batch->max_rows * (q->heads / pages->n_kv_heads) / 64 + 1) * ((((int64_t)batch->table_width << P.pool.page_shift) + 127) / 128 + 1) >> 31)
-        return fail(L2_ERANGE, "%s: %d rows of a sequence over %lld positions (more than 2^31 tiles)", who, batch->max_rows, (long long)batch->table_width << P.pool.page_shift);
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);
     int sms;
     if (int rc = kv_device(&sms)) return rc;

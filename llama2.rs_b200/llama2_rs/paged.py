@@ -21,7 +21,7 @@ BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
 _TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.int32": I32}
 _types = {}  # the same by dtype object, filled as they are seen
 _ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
-_append, _read, _attend = lib.l2_kv_append, lib.l2_kv_read, lib.l2_kv_attend
+_append, _read, _attend, _workspace_bytes = lib.l2_kv_append, lib.l2_kv_read, lib.l2_kv_attend, lib.l2_kv_attend_workspace_bytes
 assert _ROWS2.size == 2 * C.sizeof(KvRowsArgs) and _ROWS4.size == 4 * C.sizeof(KvRowsArgs)
 
 
@@ -154,7 +154,10 @@ class KvPages:
             check(rc)
 
     def workspace_bytes(self, batch, n_heads):
-        return int(lib.l2_kv_attend_workspace_bytes(self._ref, batch._ref, n_heads))
+        n = _workspace_bytes(self._ref, batch._ref, n_heads)
+        if not n:  # (never of a batch that is right)
+            check(-1)
+        return n
 
     def attend(self, batch, q, out, scale=None, window=0, sinks=0, workspace=None, stream=None):
         """Attention of the step's rows q [rows, heads, head_size] over the cache into out; scale defaults to head_size ** -0.5.
@@ -165,7 +168,8 @@ class KvPages:
         if workspace is None:
             if stream is not None:
                 raise ValueError("a stream of your own needs a workspace of your own: one made here is handed out again in the order of torch's stream")
-            workspace = q.new_empty(self.workspace_bytes(batch, row[4]), dtype=sys.modules["torch"].uint8)
+            # (0 bytes of what is refused: the call says why)
+            workspace = q.new_empty(_workspace_bytes(self._ref, batch._ref, row[4]), dtype=sys.modules["torch"].uint8)
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("workspace: a contiguous tensor on the cache's device expected")
         rc = _attend(self._ref, batch._ref, self._at[0], self._at[1], self.head_size ** -0.5 if scale is None else scale, window, sinks,

@@ -1,0 +1,26 @@
+"""What the paged cache's entry points and objects refuse at the edges of their ranges (no GPU needed)."""
+import pytest
+
+from test_paged_arguments import A, attend, batch, pages, ref, rows
+
+
+# the size of a workspace is asked for before attention itself checks anything: heads that no kernel takes must not reach its divisions
+@pytest.mark.parametrize("heads,kv_heads", [(65, 1), (130, 2), (256, 1), (257, 1), (1 << 20, 1), (3, 2), (0, 1), (-2, 2)])
+def test_workspace_of_heads_out_of_range(l2, heads, kv_heads):
+    p, b = pages(l2, n_kv_heads=kv_heads), batch(l2)
+    assert l2.lib.l2_kv_attend_workspace_bytes(ref(p), ref(b), heads) == 0
+    assert b"query heads" in l2.lib.l2_last_error()
+    r = rows(l2, heads=heads)
+    assert attend(l2, p, b, r, r, work=A, size=1 << 30) == -1 and b"query heads" in l2.lib.l2_last_error()
+
+
+def test_workspace_of_too_many_tiles(l2):
+    p, b = pages(l2), batch(l2, table_width=1 << 26, max_rows=1 << 29)
+    assert l2.lib.l2_kv_attend_workspace_bytes(ref(p), ref(b), 2) == 0 and b"2^31 tiles" in l2.lib.l2_last_error()
+
+
+def test_workspace_in_python(l2):
+    stand_in = pytest.importorskip("stand_in")
+    for heads in (3, 130, 514):
+        with pytest.raises(l2.L2Error, match="query heads"):
+            stand_in.pages(l2).workspace_bytes(stand_in.batch(l2), heads)
