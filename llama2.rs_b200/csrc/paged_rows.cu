@@ -18,8 +18,10 @@
 //
 // An int8 cache is multiplied as it is stored: K as q's type and V as bf16, both exact; the scale of a position is applied to its score and to
 // its probability.  (The probabilities times scales are rounded to bf16 even where q is f16: they can leave f16's range.)
-// Up to eight rows: K goes into integer products (s8) as it is, and a row of Q as three signed digits of 8 bits, 2^22 for the power of two above its largest
-// element: q is kept to 2^-23 of that, less than what the f32 sum of the products would lose.  (Widening K took 256 of 870 instructions of a warp's step.)
+// Up to eight rows: K goes into integer products (s8) as it is, and a row of Q as four signed digits of 8 bits, 2^30 for the power of two above its largest
+// element.  Only where they hold every element of all rows exactly (f16: always below 64): beside a large element that K has no part in, what a small one
+// loses would decide.  Else K is widened for these rows as for more of them.  (64 sequences, 8 kv heads: 115 us; 122 with K always widened; 116 with three
+// digits, which fail to hold one piece in six of normally distributed bf16, 112 with three and the loss.)
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -37,6 +39,7 @@ constexpr int KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12
 constexpr int KR_SETUP = 2;  // what a pair costs besides its tiles, in tiles
 constexpr int KR_JOIN = 2;  // CTAs that add the pieces of a pair (with 4 or 8, a step of 64 sequences takes 2 or 5 us longer: CTAs without work)
 constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
+constexpr int KR_DIGITS = 4;  // of Q against int8 K
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
 // A variant: 16 KB of K and as much of V in a tile, 64 or 128 positions, of which a warp has 16 or 32 (an int8 cache in tiles of 64 was bound by the
@@ -47,12 +50,12 @@ struct KrShape {
     static constexpr bool I8 = CT == L2_I8;
     static constexpr int ROWS = 8 * NT, ROW_BYTES = HD * (I8 ? 1 : 2);
     static constexpr int TILE = ROW_BYTES == 256 ? 64 : 128, PER_WARP = TILE / KR_WARPS, MB = PER_WARP / 16;
-    static constexpr bool DIGITS = I8 && NT == 1;                               // Q in digits
-    static constexpr int Q_PITCH = HD * (DIGITS ? 1 : 2) + 16, Q_PLANE = ROWS * Q_PITCH;  // bytes between rows of Q (no bank conflicts), of a digit's plane
+    static constexpr int DIGITS = I8 && NT == 1 ? KR_DIGITS : 0;                // of Q, where it can be in digits
+    static constexpr int Q_PITCH = 2 * HD + 16, D_PITCH = HD + 16, D_PLANE = ROWS * D_PITCH;  // bytes between rows of Q, of a digit (no bank conflicts); of a digit's plane
     static constexpr int KV_BYTES = TILE * ROW_BYTES;                           // K or V of a tile
     static constexpr int SCALE_BYTES = I8 ? TILE * 4 : 0;
     static constexpr int STAGE = (2 * (KV_BYTES + SCALE_BYTES) + 1023) / 1024 * 1024;
-    static constexpr int FIXED = 1024 + Q_PLANE * (DIGITS ? 3 : 1);
+    static constexpr int FIXED = 1024 + ROWS * Q_PITCH + DIGITS * D_PLANE;
     static constexpr int STAGES = (KR_SMEM - FIXED) / STAGE < KR_MAX_STAGES ? (KR_SMEM - FIXED) / STAGE : KR_MAX_STAGES;
     static constexpr int SMEM = FIXED + STAGES * STAGE;
     static_assert(STAGES >= 2 && KR_WARPS * ROWS * HD * 4 <= STAGE, "ring");
@@ -164,10 +167,11 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES];
     __shared__ int64_t scratch[KR_THREADS / 32 + 2];
     __shared__ float meet_ml[KR_WARPS][S::ROWS][2];
-    __shared__ float q_factor[S::DIGITS ? S::ROWS : 1];  // of a row's digits
+    __shared__ float q_factor[S::ROWS];  // of a row's digits
     __shared__ volatile int failed;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kr_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t* sq = ring + S::STAGES * S::STAGE;
+    uint8_t* sd = sq + S::ROWS * S::Q_PITCH;  // the digits
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -250,59 +254,74 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
             const KvView<TILE> view = walk.q.view;
             const int rows = walk.q.rows, G = P.group, t0 = walk.t0, t1 = walk.t1;
             asm volatile("bar.sync 1, 128;" ::: "memory");  // (everybody has read the piece before's)
-            if constexpr (S::DIGITS) {
+#pragma unroll
+            for (int n = 0; n < Q_N; n++) {
+                const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8);
+                if (r < S::ROWS) *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = qx[n];
+            }
+            bool digits = false;  // Q is in digits: they hold every element of all rows
+            if constexpr (S::DIGITS > 0) {
                 const int r = tid / (HD / 8), ch = tid % (HD / 8);
                 float x[8], most = 0.0f;
                 const uint32_t w[4] = {qx[0].x, qx[0].y, qx[0].z, qx[0].w};
-                bool finite = true;
+                bool held = true;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     x[k] = QB ? __uint_as_float(k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16) : __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k % 2)))));
-                    const bool ok = fabsf(x[k]) < INFINITY;
-                    finite &= ok;
-                    if (!ok) x[k] = 0.0f;
+                    held &= fabsf(x[k]) < INFINITY;
                     most = fmaxf(most, fabsf(x[k]));
                 }
 #pragma unroll
-                for (int o = 1; o < HD / 8; o <<= 1) {
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    finite &= (bool)__shfl_xor_sync(0xffffffffu, (int)finite, o);
-                }
-                const int e = max((int)(__float_as_uint(most) >> 23) - 126, -100);  // most < 2^e
-                const float up = __uint_as_float((uint32_t)(22 - e + 127) << 23);
-                uint32_t plane[3][2] = {};
+                for (int o = 1; o < HD / 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                constexpr int BITS = 8 * S::DIGITS - 2;
+                const int e = max((int)(__float_as_uint(most) >> 23) - 126, BITS - 122);  // most < 2^e; 2^(BITS - e) and its inverse are normal numbers
+                const float up = __uint_as_float((uint32_t)(BITS - e + 127) << 23);
+                uint32_t plane[S::DIGITS][2] = {};
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const uint32_t v = (uint32_t)(__float2int_rn(x[k] * up) + 0x808080) ^ 0x808080u;  // three balanced digits
+                    const float y = x[k] * up;
+                    const int whole = __float2int_rn(y);
+                    held &= (float)whole == y;
+                    constexpr uint32_t HALF = 0x80808080u >> (32 - 8 * S::DIGITS);
+                    const uint32_t v = ((uint32_t)whole + HALF) ^ HALF;  // balanced digits
 #pragma unroll
-                    for (int p = 0; p < 3; p++) plane[p][k / 4] |= (v >> (8 * p) & 255u) << (8 * (k % 4));
+                    for (int p = 0; p < S::DIGITS; p++) plane[p][k / 4] |= (v >> (8 * p) & 255u) << (8 * (k % 4));
                 }
                 if (r < S::ROWS) {
 #pragma unroll
-                    for (int p = 0; p < 3; p++) *reinterpret_cast<uint2*>(sq + p * S::Q_PLANE + r * S::Q_PITCH + 8 * ch) = make_uint2(plane[p][0], plane[p][1]);
-                    if (ch == 0) q_factor[r] = finite ? __uint_as_float((uint32_t)(e - 22 + 127) << 23) : __int_as_float(0x7fc00000);
+                    for (int p = 0; p < S::DIGITS; p++) *reinterpret_cast<uint2*>(sd + p * S::D_PLANE + r * S::D_PITCH + 8 * ch) = make_uint2(plane[p][0], plane[p][1]);
+                    if (ch == 0) q_factor[r] = __uint_as_float((uint32_t)(e - BITS + 127) << 23);
                 }
+                uint32_t all;
+                asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((uint32_t)held) : "memory");
+                digits = __all_sync(0xffffffffu, all);  // (a vote's result is uniform)
+            } else {
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            // Q^T as the second factor: columns 8 nt .., two words for each 16 elements (digits: for each 32, of each digit)
+            constexpr int Q_WORDS = S::DIGITS * HD / 32 > NT * KS ? S::DIGITS * HD / 32 : NT * KS;
+            uint32_t qr[Q_WORDS][2];
+            float by_row[2] = {1.0f, 1.0f};
+            if (digits) {
+#pragma unroll
+                for (int a = 0; a < S::DIGITS; a++)
+#pragma unroll
+                    for (int c2 = 0; c2 < HD / 32; c2++) {
+                        const uint8_t* p = sd + a * S::D_PLANE + g8 * S::D_PITCH + c2 * 32 + 4 * c;
+                        qr[a * (HD / 32) + c2][0] = *reinterpret_cast<const uint32_t*>(p);
+                        qr[a * (HD / 32) + c2][1] = *reinterpret_cast<const uint32_t*>(p + 16);
+                    }
+                by_row[0] = q_factor[2 * c]; by_row[1] = q_factor[2 * c + 1];
             } else {
 #pragma unroll
-                for (int n = 0; n < Q_N; n++) {
-                    const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8);
-                    if (r < S::ROWS) *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = qx[n];
-                }
+                for (int a = 0; a < NT; a++)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        const uint8_t* p = sq + (8 * a + g8) * S::Q_PITCH + ks * 32;
+                        if constexpr (I8) { const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * c); qr[a * KS + ks][0] = x.x; qr[a * KS + ks][1] = x.y; }
+                        else { qr[a * KS + ks][0] = *reinterpret_cast<const uint32_t*>(p + 4 * c); qr[a * KS + ks][1] = *reinterpret_cast<const uint32_t*>(p + 16 + 4 * c); }
+                    }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            // Q^T as the second factor: columns 8 nt .., two words for each 16 elements (digits: for each 32, of each digit)
-            constexpr int QA = S::DIGITS ? 3 : NT, QS = S::DIGITS ? HD / 32 : KS;
-            uint32_t qr[QA][QS][2];
-            float by_row[2] = {1.0f, 1.0f};
-#pragma unroll
-            for (int a = 0; a < QA; a++)
-#pragma unroll
-                for (int ks = 0; ks < QS; ks++) {
-                    const uint8_t* p = sq + (S::DIGITS ? a * S::Q_PLANE + g8 * S::Q_PITCH : (8 * a + g8) * S::Q_PITCH) + ks * 32;
-                    if constexpr (I8 && !S::DIGITS) { const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * c); qr[a][ks][0] = x.x; qr[a][ks][1] = x.y; }
-                    else { qr[a][ks][0] = *reinterpret_cast<const uint32_t*>(p + 4 * c); qr[a][ks][1] = *reinterpret_cast<const uint32_t*>(p + 16 + 4 * c); }
-                }
-            if constexpr (S::DIGITS) { by_row[0] = q_factor[2 * c]; by_row[1] = q_factor[2 * c + 1]; }
             int pos[NT][2];  // positions of this thread's two rows of each eight
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -334,10 +353,11 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 const int kr = S::PER_WARP * warp + (lane & 15);
                 auto by_k = [&](int mb, int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[mb][nt], a0, a1, a2, a3, qr[nt][ks][0], qr[nt][ks][1]);
+                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[mb][nt], a0, a1, a2, a3, qr[nt * KS + ks][0], qr[nt * KS + ks][1]);
                 };
-                if constexpr (S::DIGITS) {
-                    int d[MB][3][4] = {};
+                if (digits) {
+                    constexpr int N = S::DIGITS ? S::DIGITS : 1;
+                    int d[MB][N][4] = {};
 #pragma unroll
                     for (int c2 = 0; c2 < HD / 32; c2++)
 #pragma unroll
@@ -345,13 +365,17 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                             uint32_t a[4];
                             ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
 #pragma unroll
-                            for (int p = 0; p < 3; p++) mma_s8(d[mb][p], a, qr[p][c2][0], qr[p][c2][1]);
+                            for (int p = 0; p < N; p++) mma_s8(d[mb][p], a, qr[p * (HD / 32) + c2][0], qr[p * (HD / 32) + c2][1]);
                         }
 #pragma unroll
                     for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            s[mb][0][i] = by_row[i & 1] * fmaf(from_int(d[mb][2][i]), 65536.0f, fmaf(from_int(d[mb][1][i]), 256.0f, from_int(d[mb][0][i])));
+                        for (int i = 0; i < 4; i++) {
+                            float x = from_int(d[mb][0][i]);
+#pragma unroll
+                            for (int p = 1; p < N; p++) x = fmaf(from_int(d[mb][p][i]), (float)(1 << (8 * p)), x);
+                            s[mb][0][i] = by_row[i & 1] * x;
+                        }
                 } else if constexpr (I8) {
 #pragma unroll
                     for (int c2 = 0; c2 < KS / 2; c2++)  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
