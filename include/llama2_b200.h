@@ -263,7 +263,8 @@ typedef struct l2_kv_batch {
 } l2_kv_batch;
 
 #define L2_KV_BAD_PAGE 1   /* a page that is needed is outside 0 .. n_pages - 1: taken as zeros, not written */
-#define L2_KV_BAD_LENGTH 2 /* kv_len outside 0 .. table_width * page_size: taken as the nearest of them */
+#define L2_KV_BAD_LENGTH 2 /* kv_len outside 0 .. table_width * page_size: l2_kv_append and l2_kv_read leave the sequence's rows out;
+                              l2_kv_attend takes it as the nearest of them (its rows then see what the table holds) */
 #define L2_KV_BAD_ROWS 4   /* row_start not ascending, outside 0 .. n_rows or more than max_rows apart: that sequence brings no rows */
 #define L2_KV_BAD_ROPE 8   /* a position beyond the rope table: its rows are left out */
 #define L2_KV_TIMEOUT 16   /* a bounded wait inside a kernel gave up: the call's results are not valid */

@@ -38,6 +38,7 @@ __device__ __forceinline__ KvPlace kv_place(const KvCopyParams& P, int r) {
     if (r >= P.step.n_rows) return w;
     const int b = kv_find_seq(P.step, r);
     const KvSeq s = kv_seq(P.step, P.pool.page_shift, b);
+    if (P.step.kv_len[b] != s.kv) return w;  // (a length beyond the table: what lies at its end belongs to other rows)
     const int pos = s.kv - s.n + (r - s.row0);
     if (r < s.row0 || r >= s.row0 + s.n || pos < 0) return w;
     if (P.cos && pos >= P.rope_len) { kv_report(P.step.status, L2_KV_BAD_ROPE); return w; }

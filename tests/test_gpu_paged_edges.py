@@ -5,7 +5,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 from paged_reference import Case  # noqa: E402
-from test_gpu_paged import BF16, F16, I8, compare  # noqa: E402
+from test_gpu_paged import BF16, CACHES, F16, I8, compare  # noqa: E402
 
 
 # a large element of q where K has nothing stored: the others count as much as without it (up to 8 rows, up to 16, a block of rows)
@@ -19,3 +19,36 @@ def test_elements_of_q_that_are_far_apart(l2, cache, io, large, hd, tokens, grou
     q = torch.randn((c.n, c.heads, hd), generator=g, device="cuda")
     q[..., 5] = large
     compare(l2, c, io, q=q.to(io), what="large %g" % large)
+
+
+# a table that is too short for the length a step states: nothing is written over what the table does hold, nothing is read from the wrong place
+@pytest.mark.parametrize("length", [65, 66, 1 << 29, (1 << 31) - 1, -1, -(1 << 31)])
+@pytest.mark.parametrize("cache,io", CACHES)
+def test_append_and_read_leave_out_a_length_beyond_the_table(l2, cache, io, length):
+    from llama2_rs import paged
+    c = Case([1, 3, 2], [40, 64, 60], cache=cache, page=16)
+    c.table = c.table[:, :4].contiguous()
+    c.device_arrays()
+    c.d_kv[1] = length
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn((c.n, 2, 128), generator=g, device="cuda").to(io) for _ in "kv")
+    q_out = torch.full((c.n, 2, 128), 7.0, dtype=io, device="cuda")
+    back = [torch.full((c.n, 2, 128), 7.0, device="cuda") for _ in "kv"]
+    before = [None if t is None else t.clone() for t in (c.k, c.v, *c.scales)]
+    pages, batch = c.handles(l2)
+    pages.append(batch, k, v, q=k, q_out=q_out)
+    assert int(c.status) == paged.BAD_LENGTH
+    mine = [c.slot(1, j) for j in range(64)]
+    for new, old in zip((c.k, c.v, *c.scales), before):
+        if new is not None:
+            for page, off in mine:
+                assert torch.equal(c.at(new, page, off), c.at(old, page, off)), (page, off)
+    assert (q_out[1:4] == 7.0).all() and torch.equal(q_out[:1], k[:1]) and torch.equal(q_out[4:], k[4:])
+    c.status.zero_()
+    pages.read(batch, *back)
+    assert int(c.status) == paged.BAD_LENGTH
+    for t, new in zip(back, (k, v)):
+        assert (t[1:4] == 7.0).all()
+        for r in (0, 4, 5):  # the others are there
+            step = new[r].float().abs().amax(-1, keepdim=True) / 127 if cache == I8 else 0.0
+            assert ((t[r] - new[r].float()).abs() <= 0.51 * step).all()
