@@ -411,12 +411,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                             x[j] = __float_as_uint(a.x); x[j + 1] = __float_as_uint(a.y); x[j + 2] = __float_as_uint(b.x); x[j + 3] = __float_as_uint(b.y);
                         }
                     }
-                    if (!whole) {
+                    auto visible = [&]() {  // a bit for each of the 64 positions: j <= hi and (j > lo or j < sinks)
                         const int base = walk.base(t) + KT_SUB * h;
-                        const int hi = pos - base, lo = P.window ? pos - P.window - base : -1, sinks = P.sinks - base;  // seen: j <= hi and (j > lo or j < sinks)
+                        auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+                        return below(pos - base + 1) & (P.window ? ~below(pos - P.window - base + 1) | below(P.sinks - base) : ~0ull);
+                    };
+                    if (!whole) {
+                        const unsigned long long bits = visible();
 #pragma unroll
                         for (int j = 0; j < KT_SUB; j++)
-                            if (!(j <= hi && (j > lo || j < sinks))) x[j] = 0xff800000u;
+                            if (!(bits >> j & 1ull)) x[j] = 0xff800000u;
                     }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -451,6 +455,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     auto probabilities = [&](auto is_whole) {  // (an int8 cache with the choice at every element: 378 us instead of 362)
                         uint32_t p16[KT_SUB / 2];
                         float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const unsigned long long bits = decltype(is_whole)::value ? 0ull : visible();
 #pragma unroll
                         for (int j = 0; j < KT_SUB; j += 2) {
                             const float2 e = unpair(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, r2));
@@ -460,7 +465,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                                 if (j % 4 == 0) v4 = *reinterpret_cast<const float4*>(ks + KT_TILE + j);
                                 const float2 v = j % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
                                 if constexpr (decltype(is_whole)::value) p = unpair(mul2(pair(p.x, p.y), pair(v.x, v.y)));
-                                else p = make_float2(p.x == 0.0f ? 0.0f : p.x * v.x, p.y == 0.0f ? 0.0f : p.y * v.y);  // (what is not seen may have any scale)
+                                else p = make_float2(bits >> j & 1ull ? p.x * v.x : 0.0f, bits >> j & 2ull ? p.y * v.y : 0.0f);  // (what is not seen may have any scale)
                             }
                             p16[j / 2] = pack16<PB>(p.x, p.y);
                         }

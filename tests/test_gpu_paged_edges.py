@@ -1,11 +1,13 @@
 """The paged cache and its attention at the edges of what they are given."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 from paged_reference import Case  # noqa: E402
-from test_gpu_paged import BF16, CACHES, F16, I8, compare  # noqa: E402
+from test_gpu_paged import BF16, CACHES, F16, I8, compare, run_attend  # noqa: E402
 
 
 # a large element of q where K has nothing stored: the others count as much as without it (up to 8 rows, up to 16, a block of rows)
@@ -52,3 +54,23 @@ def test_append_and_read_leave_out_a_length_beyond_the_table(l2, cache, io, leng
         for r in (0, 4, 5):  # the others are there
             step = new[r].float().abs().amax(-1, keepdim=True) / 127 if cache == I8 else 0.0
             assert ((t[r] - new[r].float()).abs() <= 0.51 * step).all()
+
+
+# a position that a row sees, whose probability is too small for any number, holds a NaN or an infinity: 0 x NaN is NaN wherever the row lies in a tile
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("tokens,group,window", [(1, 2, 0), (100, 2, 0), (100, 2, 90), (8, 16, 70), (60, 1, 0)])
+@pytest.mark.parametrize("io", [F16, BF16])
+def test_a_scale_that_is_not_finite_behind_a_probability_of_zero(l2, io, tokens, group, window, value):
+    c = Case([tokens], [200], cache=I8, group=group, seed=8)
+    c.k.clamp_(1, 2)  # (with queries of ones no score is far below the others)
+    j = 160 if tokens > 40 else 199 - tokens // 2
+    page, off = c.slot(0, j)
+    c.k[page, off] = -127
+    c.scales[0][page, :, off] = 1.0
+    q = torch.ones((c.n, c.heads, 128), dtype=io, device="cuda")
+    _, clean = run_attend(l2, c, io, q=q, window=window)
+    c.scales[1][page, :, off] = value
+    _, out = run_attend(l2, c, io, q=q, window=window)
+    first = j - (200 - tokens)  # the position's own row
+    assert clean.isfinite().all() and (not window or tokens - first <= window)  # (all rows from there on see it)
+    assert torch.equal(out[:first], clean[:first]) and out[first:].isnan().all()
