@@ -463,7 +463,9 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (workspace_bytes < need || (need && (!workspace || !aligned16(workspace)))) return fail(L2_EINVAL, "%s: a workspace of %zu bytes on a 16-byte boundary needed", who, need);
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
     P.scale_log2 = scale * 1.4426950408889634f;
-    P.window = window; P.sinks = window ? sinks : 0;
+    // (a window as wide as the table leaves nothing out; below that, positions and windows of up to 2^30 can be added and subtracted in 32 bits)
+    P.window = window < (int64_t)batch->table_width << P.pool.page_shift ? window : 0;
+    P.sinks = P.window ? sinks : 0;
     P.group = q->heads / pages->n_kv_heads;
     P.group_inv = (65536 + P.group - 1) / P.group;
     P.work = workspace;

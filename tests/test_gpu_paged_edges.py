@@ -74,3 +74,19 @@ def test_a_scale_that_is_not_finite_behind_a_probability_of_zero(l2, io, tokens,
     first = j - (200 - tokens)  # the position's own row
     assert clean.isfinite().all() and (not window or tokens - first <= window)  # (all rows from there on see it)
     assert torch.equal(out[:first], clean[:first]) and out[first:].isnan().all()
+
+
+# a window that leaves nothing out, up to the largest number ("no limit"): the bits of no window, for rows of negative positions beside others too
+@pytest.mark.parametrize("rows,kv,group", [([600, 1, 3], [5, 0, 0], 2), ([300, 70], [40, 69], 1), ([9, 1], [4, 2], 1), ([1, 1, 4], [300, 17, 90], 4), ([200, 140], [333, 140], 2)])
+@pytest.mark.parametrize("cache,io", CACHES)
+def test_windows_as_wide_as_the_table(l2, cache, io, rows, kv, group):
+    c = Case(rows, kv, cache=cache, group=group, seed=12)
+    room = c.table.shape[1] * c.page
+    q, want = run_attend(l2, c, io)
+    compare(l2, c, io, q=q)
+    for window in (room, room + 1, 1 << 30, (1 << 31) - 1):
+        for sinks in (0, 4, (1 << 31) - 1):
+            assert torch.equal(run_attend(l2, c, io, q=q, window=window, sinks=sinks)[1], want), (window, sinks)
+    for window, sinks in ((room - 1, 0), (max(kv), 3), (max(kv) - 1, (1 << 31) - 1)):
+        compare(l2, c, io, q=q, window=window, sinks=sinks, what="window %d" % window)
+    assert int(c.status) == 0
