@@ -57,6 +57,12 @@ def _packed(t, what, device, shape, dtype):
     return t.data_ptr()
 
 
+def _int32(**numbers):  # (ctypes would cut what is wider without a word)
+    for what, n in numbers.items():
+        if not -1 << 31 <= n < 1 << 31:
+            raise ValueError("%s: %d is beyond 32 bits" % (what, n))
+
+
 class KvBatch:
     """One step of a batch: page_table [n_seqs, width], kv_len [n_seqs] and row_start [n_seqs + 1] int32 on the device; n_rows rows in all,
     at most max_rows of one sequence.  `status` (one int32 on the device, optional) gets the BAD_* bits of what only the device can see."""
@@ -66,6 +72,7 @@ class KvBatch:
             raise ValueError("page_table: [n_seqs, width] on a CUDA device expected")
         self.device = page_table.get_device()
         n_seqs, width = page_table.shape
+        _int32(n_seqs=n_seqs, table_width=width, n_rows=n_rows, max_rows=max_rows)
         self._args = KvBatchArgs(_packed(page_table, "page_table", self.device, (n_seqs, width), I32),
                                  _packed(kv_len, "kv_len", self.device, (n_seqs,), I32),
                                  _packed(row_start, "row_start", self.device, (n_seqs + 1,), I32),
@@ -90,6 +97,7 @@ class KvPages:
             raise ValueError("k and v: the same shape, type and strides, the last dimension contiguous")
         at, head = (1, 2) if layout == "NHD" else (2, 1)
         self.n_pages, self.page_size, self.n_kv_heads, self.head_size = k.shape[0], k.shape[at], k.shape[head], k.shape[3]
+        _int32(n_pages=self.n_pages, page_size=self.page_size, n_kv_heads=self.n_kv_heads)
         kind = _type(k)
         scales = [None, None]
         if kind == I8:
@@ -154,6 +162,7 @@ class KvPages:
             check(rc)
 
     def workspace_bytes(self, batch, n_heads):
+        _int32(n_heads=n_heads)
         n = _workspace_bytes(self._ref, batch._ref, n_heads)
         if not n:  # (never of a batch that is right)
             check(-1)
@@ -163,6 +172,8 @@ class KvPages:
         """Attention of the step's rows q [rows, heads, head_size] over the cache into out; scale defaults to head_size ** -0.5.
         `workspace`: a uint8 tensor of workspace_bytes(); one is made where none is given."""
         n = batch.n_rows
+        if window >> 31 or sinks >> 31:
+            _int32(window=window, sinks=sinks)
         row = self._row(q, "q", n, 0)
         _ROWS2.pack_into(self._rows, 0, *row, *self._row(out, "out", n, row[4]))
         if workspace is None:

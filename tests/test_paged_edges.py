@@ -24,3 +24,24 @@ def test_workspace_in_python(l2):
     for heads in (3, 130, 514):
         with pytest.raises(l2.L2Error, match="query heads"):
             stand_in.pages(l2).workspace_bytes(stand_in.batch(l2), heads)
+
+
+# ctypes cuts numbers to 32 bits: a window of 2^32 + 5 would be a window of 5
+@pytest.mark.parametrize("wide", [1 << 31, (1 << 32) + 5, -(1 << 31) - 1, 1 << 70])
+def test_numbers_beyond_32_bits(l2, wide):
+    stand_in = pytest.importorskip("stand_in")
+    torch = stand_in.torch
+    pages, batch = stand_in.pages(l2), stand_in.batch(l2)
+    q = stand_in.tensor((5, 2, 128), torch.float16)
+    work = stand_in.tensor((1 << 20,), torch.uint8)
+    for bad in (lambda: pages.attend(batch, q, q, window=wide, workspace=work, stream=0), lambda: pages.attend(batch, q, q, window=9, sinks=wide, workspace=work, stream=0),
+                lambda: stand_in.batch(l2, rows=wide), lambda: stand_in.batch(l2, most=wide), lambda: pages.workspace_bytes(batch, wide)):
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            bad()
+
+
+def test_sizes_beyond_32_bits(l2):
+    stand_in = pytest.importorskip("stand_in")
+    for bad in (lambda: stand_in.pages(l2, n_pages=1 << 32), lambda: stand_in.pages(l2, heads=(1 << 32) + 2), lambda: stand_in.batch(l2, width=(1 << 32) + 3)):
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            bad()
