@@ -43,12 +43,15 @@ def _find_cuda():
     _cuda = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device, raw)
 
 
-def _stream(device):
+def _stream(device, batch, stream):
+    """The stream of a call, after a look at whether pages, batch and launch are all on one device."""
+    if batch.device != device:
+        raise ValueError("the batch is on device %d, the pages on device %d" % (batch.device, device))
     if _cuda is None:
         _find_cuda()
     if _cuda[0]() != device:
         raise ValueError("the tensors are on device %d, which is not the current one" % device)
-    return _cuda[1](device)
+    return _cuda[1](device) if stream is None else stream
 
 
 def _packed(t, what, device, shape, dtype):
@@ -149,7 +152,7 @@ class KvPages:
             positions = cos.shape[0]
             shape = (positions, self.head_size // 2)
             cos, sin = _packed(cos, "rope", self.device, shape, F32), _packed(sin, "rope", self.device, shape, F32)
-        rc = _append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(self.device) if stream is None else stream)
+        rc = _append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(self.device, batch, stream))
         if rc:
             check(rc)
 
@@ -157,7 +160,7 @@ class KvPages:
         """The cached positions of the step's rows into k and v ([rows, kv_heads, head_size], f32, f16 or bf16)."""
         n, heads = batch.n_rows, self.n_kv_heads
         _ROWS2.pack_into(self._rows, 0, *self._row(k, "k", n, heads), *self._row(v, "v", n, heads))
-        rc = _read(self._ref, batch._ref, self._at[0], self._at[1], _stream(self.device) if stream is None else stream)
+        rc = _read(self._ref, batch._ref, self._at[0], self._at[1], _stream(self.device, batch, stream))
         if rc:
             check(rc)
 
@@ -184,7 +187,7 @@ class KvPages:
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("workspace: a contiguous tensor on the cache's device expected")
         rc = _attend(self._ref, batch._ref, self._at[0], self._at[1], self.head_size ** -0.5 if scale is None else scale, window, sinks,
-                     workspace.data_ptr(), workspace.nbytes, _stream(self.device) if stream is None else stream)
+                     workspace.data_ptr(), workspace.nbytes, _stream(self.device, batch, stream))
         if rc:
             check(rc)
         return out

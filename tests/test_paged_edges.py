@@ -45,3 +45,28 @@ def test_sizes_beyond_32_bits(l2):
     for bad in (lambda: stand_in.pages(l2, n_pages=1 << 32), lambda: stand_in.pages(l2, heads=(1 << 32) + 2), lambda: stand_in.batch(l2, width=(1 << 32) + 3)):
         with pytest.raises(ValueError, match="beyond 32 bits"):
             bad()
+
+
+# pages, batch and launch belong to one device: the table and lengths of another would be read (and its status word written) there
+@pytest.mark.parametrize("pages_on,batch_on,current", [(0, 1, 0), (1, 0, 1), (1, 1, 0), (0, 0, 1)])
+@pytest.mark.parametrize("stream", [None, 1234])
+def test_one_device(l2, monkeypatch, stream, pages_on, batch_on, current):
+    stand_in = pytest.importorskip("stand_in")
+    torch = stand_in.torch
+    from llama2_rs import paged
+
+    def launched(*args):
+        raise AssertionError("a launch")
+
+    monkeypatch.setattr(paged, "_cuda", (lambda: current, lambda device: 0))
+    for call in ("_append", "_read", "_attend"):
+        monkeypatch.setattr(paged, call, launched)
+    pages, batch = stand_in.pages(l2, pages_on), stand_in.batch(l2, batch_on)
+    x, work = stand_in.tensor((5, 2, 128), torch.float16, pages_on), stand_in.tensor((1 << 20,), torch.uint8, pages_on)
+    for bad in (lambda: pages.append(batch, x, x, stream=stream), lambda: pages.read(batch, x, x, stream=stream),
+                lambda: pages.attend(batch, x, x, workspace=work, stream=stream)):
+        with pytest.raises(ValueError, match="device"):
+            bad()
+    monkeypatch.setattr(paged, "_cuda", (lambda: pages_on, lambda device: 0))
+    with pytest.raises(AssertionError, match="a launch"):  # (all on one device)
+        pages.append(stand_in.batch(l2, pages_on), x, x, stream=stream)
