@@ -17,7 +17,7 @@
 
 namespace l2 {
 
-unsigned long long g_launches = 0;
+LaunchCount g_launches;
 
 // ---- small device helpers --------------------------------------------------------------
 

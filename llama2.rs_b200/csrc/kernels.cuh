@@ -2,6 +2,8 @@
 #pragma once
 
 #include <cuda_runtime.h>
+
+#include <atomic>
 #include <cstdint>
 
 namespace l2 {
@@ -298,6 +300,12 @@ void launch_select(const SelectParams& p, cudaStream_t st, bool pdl);
 void launch_scatter(const float* src, int n, float* const* dst, const int* const* idx, int ndst, cudaStream_t st, bool pdl);
 cudaError_t kernels_init();  // opt-in shared memory sizes; call once per device
 
-extern unsigned long long g_launches;
+// Kernels launched by this process, and by the calling thread.  Threads with handles of their own may be inside the library side by side.
+struct LaunchCount {
+    std::atomic<unsigned long long> all{0};
+    inline static thread_local unsigned long long mine = 0;
+    void operator++(int) { mine++; all.fetch_add(1, std::memory_order_relaxed); }
+};
+extern LaunchCount g_launches;
 
 }  // namespace l2

@@ -799,12 +799,12 @@ static int run_forward(l2_state* s, int kind) {
     if (!s->graphs[kind]) {
         cudaStream_t cap;
         L2_CUDA(cudaStreamCreateWithFlags(&cap, cudaStreamNonBlocking));
-        const unsigned long long before = g_launches;
+        const unsigned long long before = LaunchCount::mine;
         L2_CUDA(cudaStreamBeginCapture(cap, cudaStreamCaptureModeThreadLocal));
         int rc = enqueue_forward(s, kind, cap);
         cudaGraph_t graph = nullptr;
         cudaError_t e = cudaStreamEndCapture(cap, &graph);
-        g_launches = before;  // captured launches have not run
+        g_launches.all -= LaunchCount::mine - before;  // captured launches have not run
         if (rc != L2_OK) { if (graph) cudaGraphDestroy(graph); cudaStreamDestroy(cap); return rc; }
         if (e != cudaSuccess) { cudaStreamDestroy(cap); return fail(L2_ECUDA, "graph capture failed: %s", cudaGetErrorString(e)); }
         e = cudaGraphInstantiate(&s->graphs[kind], graph, 0);
@@ -814,7 +814,7 @@ static int run_forward(l2_state* s, int kind) {
         s->graph_nodes[kind] = nodes_per_forward(s, kind);
     }
     L2_CUDA(cudaGraphLaunch(s->graphs[kind], m->stream));
-    g_launches += s->graph_nodes[kind];
+    g_launches.all += s->graph_nodes[kind];
     return L2_OK;
 }
 
@@ -846,7 +846,7 @@ static int upload_prompt(l2_state* s, const int32_t* prompt, int n_prompt) {
 
 // ---- C ABI: model -------------------------------------------------------------------------------
 
-extern "C" uint64_t l2_launch_count(void) { return g_launches; }
+extern "C" uint64_t l2_launch_count(void) { return g_launches.all; }
 
 static int resolve_shape(const l2_options* opt, const int32_t* header, Shape* out) {
     // Config::load + check_static (src/constants.rs:94-119); n_kv_heads in the file is ignored.

@@ -90,3 +90,33 @@ def test_windows_as_wide_as_the_table(l2, cache, io, rows, kv, group):
     for window, sinks in ((room - 1, 0), (max(kv), 3), (max(kv) - 1, (1 << 31) - 1)):
         compare(l2, c, io, q=q, window=window, sinks=sinks, what="window %d" % window)
     assert int(c.status) == 0
+
+
+def test_launches_of_several_threads_are_counted(l2):
+    """Threads with pages and streams of their own, side by side inside the library (a foreign call gives up the interpreter's lock)."""
+    import threading
+    calls, n_threads = 5000, 8
+    own = []
+    for i in range(n_threads):
+        c = Case([1], [9], seed=i)
+        pages, batch = c.handles(l2)
+        rows = [torch.zeros((1, 2, 128), dtype=F16, device="cuda") for _ in "kv"]
+        pages.read(batch, *rows)  # (fills the row records)
+        own.append((pages, batch, rows, c, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(n_threads), []
+
+    def work(pages, batch, stream):
+        start.wait()
+        for _ in range(calls):
+            if l2.lib.l2_kv_read(pages._ref, batch._ref, pages._at[0], pages._at[1], stream):
+                failed.append(1)
+
+    before = l2.lib.l2_launch_count()
+    threads = [threading.Thread(target=work, args=(p, b, s.cuda_stream)) for p, b, _, _, s in own]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed and l2.lib.l2_launch_count() - before == calls * n_threads
