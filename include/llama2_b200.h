@@ -277,10 +277,17 @@ typedef struct l2_kv_rows {
     int32_t heads;
 } l2_kv_rows;
 
-/* K and V of the batch's rows into their pages.  With rope tables ([rope_len][head_size / 2] each, f32, see l2_rope_table) k is rotated at its
- * position first (element d with d + head_size / 2, as src/models.rs:100-135 does), and so is q into q_out where q is not NULL; without them
- * q is rounded to q_out's type only.  int8: a row and head is scaled by 127 / its largest magnitude and rounded to nearest even.  One that holds a
- * NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros. */
+/* How RoPE turns (a, b), elements d and d + head_size / 2 of a head, by an angle of cosine c and sine s: */
+#define L2_ROPE_PAIRS 0 /* a' = a c - b s, b' = b c + a s: the pair turned as a vector */
+#define L2_ROPE_MODEL 1 /* a' = a c - b s, b' = b c + a' s: in place, the second from the turned first, as src/models.rs:100-129 does it and with it
+                           all models of this library and l2_attention_decode_dev, whose keys these are.  The two differ by O(1). */
+/* K and V of the batch's rows into their pages.  With rope tables ([rope_len][head_size / 2] each, f32) k is turned at its position first, and so is
+ * q into q_out where q is not NULL; without them q is rounded to q_out's type only.  Programs that share caches or checkpoints with the rest of
+ * this library take the tables of l2_rope_table and L2_ROPE_MODEL.  int8: a row and head is scaled by 127 / its largest magnitude and rounded to
+ * nearest even.  One that holds a NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros. */
+int l2_kv_append_rope(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
+                      const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, int rotation, void* cuda_stream);
+/* The same with L2_ROPE_PAIRS. */
 int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
                  const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, void* cuda_stream);
 /* The other way: the cached positions of the batch's rows as rows of f32, f16 or bf16 (all of a sequence where it brings kv_len[b] rows). */

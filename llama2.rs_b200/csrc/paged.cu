@@ -2,7 +2,8 @@
 //
 //   16 bits:  cache = round(x)
 //   8 bits:   a = max |x| over a row and head, scale = a / 127, cache = rint(x * (127 / a)), and back: value = cache * scale
-//   RoPE:     (x[d], x[d + hd/2]) turned by the angle of the row's position, first
+//   RoPE:     (a, b) = (x[d], x[d + hd/2]) turned by the angle of the row's position, first: a' = a c - b s, b' = b c + a s, or, as the
+//             token loop of this library does it in place, b' = b c + a' s
 //
 // Both are copies: what they cannot do without is each row read once and written once, and nothing is used twice.
 #include <cuda_runtime.h>
@@ -26,7 +27,7 @@ struct KvCopyParams {
     KvStep step;
     KvRows k, v, q, q_out;
     const float* cos; const float* sin;
-    int rope_len;
+    int rope_len, rope_in_place;
     int rows;  // of a CTA
     uint32_t by_heads, by_q_heads;  // reciprocals of the kv heads (kv_read_kernel: twice as many) and of q's
 };
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_c
                         for (int i = 0; i < 8; i++) {
                             const float y = x[i], z = x[i + 8];
                             x[i] = __fsub_rn(__fmul_rn(y, c[i]), __fmul_rn(z, s[i]));
-                            x[i + 8] = __fadd_rn(__fmul_rn(y, s[i]), __fmul_rn(z, c[i]));
+                            x[i + 8] = __fadd_rn(__fmul_rn(P.rope_in_place ? x[i] : y, s[i]), __fmul_rn(z, c[i]));
                         }
                     }
                     if (what == 2) {
@@ -386,6 +387,11 @@ using namespace l2;
 
 extern "C" int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
                             const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, void* cuda_stream) {
+    return l2_kv_append_rope(pages, batch, k, v, q, q_out, rope_cos, rope_sin, rope_len, L2_ROPE_PAIRS, cuda_stream);
+}
+
+extern "C" int l2_kv_append_rope(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
+                                 const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, int rotation, void* cuda_stream) {
     clear_error();
     const char* who = "l2_kv_append";
     KvCopyParams P{};
@@ -401,7 +407,8 @@ extern "C" int l2_kv_append(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     }
     if (!rope_cos != !rope_sin || (rope_cos && (rope_len < 1 || !aligned16(rope_cos) || !aligned16(rope_sin))))
         return fail(L2_EINVAL, "%s: both rope tables, on a 16-byte boundary, of at least one position", who);
-    P.cos = rope_cos; P.sin = rope_sin; P.rope_len = rope_len;
+    if (rotation != L2_ROPE_PAIRS && rotation != L2_ROPE_MODEL) return fail(L2_EINVAL, "%s: rotation %d (L2_ROPE_PAIRS or L2_ROPE_MODEL)", who, rotation);
+    P.cos = rope_cos; P.sin = rope_sin; P.rope_len = rope_len; P.rope_in_place = rotation == L2_ROPE_MODEL;
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;

@@ -17,14 +17,14 @@ import numpy as np
 
 from . import _lib
 from ._lib import Config, L2Error, Options, check, lib
-from .paged import KvBatch, KvPages
+from .paged import KvBatch, KvPages, KvRope
 
 START = 1  # python/llama2_rs/__init__.py:4
 RET = 13   # python/llama2_rs/__init__.py:5
 
 __all__ = ["LlamaModel", "Tokenizer", "Random", "Config", "generate", "generate_ids", "RunState", "QLinear",
            "START", "RET", "preset_config", "checkpoint_bytes", "synth_fill", "synth_write_file", "L2Error",
-           "KvPages", "KvBatch"]
+           "KvPages", "KvBatch", "KvRope"]
 
 
 def tp_unique_id():

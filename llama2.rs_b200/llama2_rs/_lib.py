@@ -102,6 +102,7 @@ SIGNATURES = {
     "l2_attention_decode_dev": (C.c_int, [C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "l2_attention_decode_noalloc": (C.c_int, [C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "l2_kv_append": (C.c_int, [_vp] * 8 + [C.c_int, _vp]),
+    "l2_kv_append_rope": (C.c_int, [_vp] * 8 + [C.c_int, C.c_int, _vp]),
     "l2_kv_read": (C.c_int, [_vp] * 5),
     "l2_kv_attend": (C.c_int, [_vp] * 4 + [C.c_float, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
     "l2_kv_attend_workspace_bytes": (C.c_size_t, [_vp, _vp, C.c_int]),

@@ -3,7 +3,7 @@
     pages = KvPages(k, v)                                   # [n_pages, page_size, kv_heads, head_size], f16 or bf16
     pages = KvPages(k, v, k_scale, v_scale)                 # int8, scales [n_pages, kv_heads, page_size] f32
     batch = KvBatch(page_table, kv_len, row_start, n_rows, max_rows)   # one step, for all layers
-    pages.append(batch, k_rows, v_rows, rope=(cos, sin), q=q_rows, q_out=q16)
+    pages.append(batch, k_rows, v_rows, rope=KvRope(4096), q=q_rows, q_out=q16)
     pages.attend(batch, q16, out, window=4096, sinks=4)
     pages.read(batch, k_back, v_back)
 
@@ -14,14 +14,15 @@ import ctypes as C
 import struct
 import sys
 
-from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, check, lib
+from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, as_f32p, check, lib
 
 F32, F16, BF16, I8, I32 = 0, 1, 2, 3, 4
 BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
 _TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.int32": I32}
 _types = {}  # the same by dtype object, filled as they are seen
 _ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
-_append, _read, _attend, _workspace_bytes = lib.l2_kv_append, lib.l2_kv_read, lib.l2_kv_attend, lib.l2_kv_attend_workspace_bytes
+_ROTATIONS = {"pairs": 0, "model": 1}  # L2_ROPE_*
+_append, _read, _attend, _workspace_bytes = lib.l2_kv_append_rope, lib.l2_kv_read, lib.l2_kv_attend, lib.l2_kv_attend_workspace_bytes
 assert _ROWS2.size == 2 * C.sizeof(KvRowsArgs) and _ROWS4.size == 4 * C.sizeof(KvRowsArgs)
 
 
@@ -86,6 +87,19 @@ class KvBatch:
         self.n_rows = n_rows
 
 
+class KvRope(tuple):
+    """The tables of this package's models (l2_rope_table; heads of 128) for `positions` positions as two tensors on a device: (cos, sin).
+    `append` turns with them as the models do, rotation "model"."""
+
+    rotation = "model"
+
+    def __new__(cls, positions, device="cuda"):
+        import torch
+        host = torch.empty((2, positions, 64))
+        check(lib.l2_rope_table(positions, as_f32p(host[0].numpy()), as_f32p(host[1].numpy())))
+        return super().__new__(cls, host.to(device))
+
+
 class KvPages:
     """The pages of one layer's cache: k and v of one shape and one set of strides, [n_pages, page_size, kv_heads, head_size] (layout "NHD") or
     [n_pages, kv_heads, page_size, head_size] ("HND"), f16, bf16 or int8 (with scales)."""
@@ -132,8 +146,10 @@ class KvPages:
             raise ValueError("%s: [%d, %s, %d] on device %d with its last dimension contiguous expected, got %s" % (what, n, heads or "heads", self.head_size, self.device, tuple(t.shape)))
         return t.data_ptr(), row, head, kind, h
 
-    def append(self, batch, k, v, rope=None, q=None, q_out=None, stream=None):
-        """K and V rows of the step into their pages; rope = (cos, sin), [positions, head_size / 2] f32, rotates k and, into q_out, q."""
+    def append(self, batch, k, v, rope=None, q=None, q_out=None, stream=None, rotation=None):
+        """K and V rows of the step into their pages; rope = (cos, sin), [positions, head_size / 2] f32, rotates k and, into q_out, q.
+        rotation: "pairs" turns (x[d], x[d + head_size / 2]) as a vector; "model" does it in place, the second half from the turned first, as this
+        package's models and l2_attention_decode_dev do (a cache of theirs, or their checkpoints).  Default: "model" for a KvRope, else "pairs"."""
         n, heads = batch.n_rows, self.n_kv_heads
         a = self._at
         if q is None and q_out is None:
@@ -146,13 +162,16 @@ class KvPages:
                              *self._row(q, "q", n, 0), *self._row(q_out, "q_out", n, q.shape[1]))
             q_at, q_out_at = a[2], a[3]
         cos = sin = None
-        positions = 0
+        positions = turn = 0
         if rope is not None:
             cos, sin = rope
+            turn = _ROTATIONS.get(rotation or getattr(rope, "rotation", "pairs"))
+            if turn is None:
+                raise ValueError("rotation: pairs or model")
             positions = cos.shape[0]
             shape = (positions, self.head_size // 2)
             cos, sin = _packed(cos, "rope", self.device, shape, F32), _packed(sin, "rope", self.device, shape, F32)
-        rc = _append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, _stream(self.device, batch, stream))
+        rc = _append(self._ref, batch._ref, a[0], a[1], q_at, q_out_at, cos, sin, positions, turn, _stream(self.device, batch, stream))
         if rc:
             check(rc)
 

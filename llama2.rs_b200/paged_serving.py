@@ -5,7 +5,8 @@
 
 A step takes up to --budget rows: one of every sequence that is past its prompt, the rest of the room for prompts, in order.  Pages are handed out as
 sequences grow and, with a window, given back when no row can see them any more.  There is no model behind the layer: a prompt is random rows, and the
-next row of a sequence is the layer's own (normalised) output for the row before.  Weights are random in the checkpoint's layout.
+next row of a sequence is the layer's own (normalised) output for the row before.  Weights are random in the checkpoint's layout; RoPE is that of the
+package's models (--rotation pairs: of plain pairs, for weights that want it).
 """
 import argparse
 import os
@@ -19,7 +20,7 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 class PagedLayer:
     """wq / wk / wv -> RoPE, append -> attend -> wo on device tensors; the cache's pages and who has them."""
 
-    def __init__(self, dim, heads, kv_heads, *, cache="i8", n_pages=512, page_size=32, positions=4096, window=0, sinks=0, group_size=64, seed=0, weights=None):
+    def __init__(self, dim, heads, kv_heads, *, cache="i8", n_pages=512, page_size=32, positions=4096, window=0, sinks=0, group_size=64, seed=0, weights=None, rotation="pairs"):
         import torch
         import llama2_rs as l2
         from qlinear_bench import random_qlinear
@@ -35,9 +36,7 @@ class PagedLayer:
         scales = [torch.zeros((n_pages, kv_heads, page_size), device="cuda") for _ in "kv"] if cache == "i8" else []
         self.pages = l2.KvPages(k, v, *scales)
         self.q_type = torch.float16 if cache == "f16" else torch.bfloat16
-        cos, sin = (np.empty((positions, 64), np.float32) for _ in "cs")
-        l2.check(l2.lib.l2_rope_table(positions, l2._lib.as_f32p(cos), l2._lib.as_f32p(sin)))
-        self.rope = tuple(torch.from_numpy(t).cuda() for t in (cos, sin))
+        self.rope, self.rotation = l2.KvRope(positions), rotation
         self.free = list(range(n_pages))[::-1]
         self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
 
@@ -60,7 +59,7 @@ class PagedLayer:
         batch = self.l2.KvBatch(table, kv_len, start, n, max(rows), status=self.status)
         q, k, v = (self._project(name, x) for name in "qkv")
         q16 = torch.empty((n, self.heads, 128), dtype=self.q_type, device="cuda")
-        self.pages.append(batch, k.view(n, -1, 128), v.view(n, -1, 128), rope=self.rope, q=q.view(n, -1, 128), q_out=q16)
+        self.pages.append(batch, k.view(n, -1, 128), v.view(n, -1, 128), rope=self.rope, rotation=self.rotation, q=q.view(n, -1, 128), q_out=q16)
         out = self.pages.attend(batch, q16, torch.empty((n, self.heads, 128), device="cuda"), window=self.window, sinks=self.sinks)
         if self.window:  # pages that no later row sees
             for s in sequences:
@@ -107,11 +106,12 @@ def main():
     ap.add_argument("--sequences", type=int, default=16)
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--budget", type=int, default=512)
+    ap.add_argument("--rotation", choices=["model", "pairs"], default="model", help="RoPE as the package's models do it, or of plain pairs")
     args = ap.parse_args()
     import torch
     if not torch.cuda.is_available():
         raise SystemExit("paged_serving needs a GPU: there is no CPU path")
-    layer = PagedLayer(args.heads * 128, args.heads, args.kv_heads, cache=args.cache, window=args.window, sinks=args.sinks, n_pages=2048)
+    layer = PagedLayer(args.heads * 128, args.heads, args.kv_heads, cache=args.cache, window=args.window, sinks=args.sinks, n_pages=2048, rotation=args.rotation)
     rng = np.random.default_rng(1)
     prompts = [torch.randn(int(n), layer.dim, device="cuda") for n in rng.integers(5, 900, args.sequences)]
     serve(layer, prompts, 2, args.budget)  # the layers' buffers, the kernels' first launches

@@ -70,3 +70,9 @@ def test_one_device(l2, monkeypatch, stream, pages_on, batch_on, current):
     monkeypatch.setattr(paged, "_cuda", (lambda: pages_on, lambda device: 0))
     with pytest.raises(AssertionError, match="a launch"):  # (all on one device)
         pages.append(stand_in.batch(l2, pages_on), x, x, stream=stream)
+
+
+def test_rotation_out_of_range(l2):
+    p, b, r = pages(l2), batch(l2), rows(l2)
+    for rotation in (-1, 2):
+        assert l2.lib.l2_kv_append_rope(ref(p), ref(b), ref(r), ref(r), None, None, A, A, 9, rotation, None) == -1 and b"rotation" in l2.lib.l2_last_error()
