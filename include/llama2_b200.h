@@ -241,7 +241,7 @@ typedef struct l2_kv_pages {
     void* v;
     float* k_scale;         /* L2_I8: [n_pages][n_kv_heads][page_size], value = stored * scale; else NULL */
     float* v_scale;
-    int64_t page_stride, position_stride, head_stride;  /* in elements; multiples of 16 bytes, the same for k and v */
+    int64_t page_stride, position_stride, head_stride;  /* in elements; multiples of 16 bytes, the same for k and v, nothing on one another */
     int32_t type;           /* L2_F16, L2_BF16 or L2_I8 */
     int32_t n_pages;
     int32_t page_size;      /* 8, 16, 32, 64, 128 or 256 */
@@ -269,7 +269,8 @@ typedef struct l2_kv_batch {
 #define L2_KV_BAD_ROPE 8   /* a position beyond the rope table: its rows are left out */
 #define L2_KV_TIMEOUT 16   /* a bounded wait inside a kernel gave up: the call's results are not valid */
 
-/* An array [row][head][head_size]: element d of (row, head) at row * row_stride + head * head_stride + d; strides multiples of 16 bytes. */
+/* An array [row][head][head_size]: element d of (row, head) at row * row_stride + head * head_stride + d; strides multiples of 16 bytes.  Rows that a
+ * call reads may lie on one another (a stride of 0), rows that it writes may not. */
 typedef struct l2_kv_rows {
     void* data;
     int64_t row_stride, head_stride;  /* in elements */

@@ -8,6 +8,7 @@
 // Both are copies: what they cannot do without is each row read once and written once, and nothing is used twice.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "host_common.h"
@@ -298,6 +299,20 @@ int kv_device(int* sms) {
 int elem_bytes(int type) { return type == L2_F32 ? 4 : type == L2_I8 ? 1 : 2; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Whether runs of head_size elements lie apart, each dimension's steps beyond all that is inside it (as every array that is a part of a larger one has it).
+struct KvDim { int64_t stride, extent; };
+template <size_t N>
+bool apart(KvDim (&d)[N], int head_size) {
+    std::sort(d, d + N, [](const KvDim& a, const KvDim& b) { return a.stride < b.stride; });
+    __int128 span = head_size;
+    for (const KvDim& x : d) {
+        if (x.extent <= 1) continue;
+        if (x.stride < span) return false;
+        span += (__int128)x.stride * (x.extent - 1);
+    }
+    return true;
+}
+
 int check_pages(const char* who, const l2_kv_pages* p, KvPool* out) {
     if (!p) return fail(L2_EINVAL, "%s: no pages", who);
     if (p->type != L2_F16 && p->type != L2_BF16 && p->type != L2_I8) return fail(L2_EINVAL, "%s: a cache is f16, bf16 or int8 (type %d)", who, p->type);
@@ -311,8 +326,8 @@ int check_pages(const char* who, const l2_kv_pages* p, KvPool* out) {
     const int least = 16 / elem_bytes(p->type);
     for (int64_t x : s)
         if (x < least || x % least || x > ((int64_t)1 << 36)) return fail(L2_EINVAL, "%s: a stride of %lld elements (multiples of 16 bytes)", who, (long long)x);
-    if ((p->position_stride < p->head_size && p->page_size > 1) || (p->head_stride < p->head_size && p->n_kv_heads > 1))
-        return fail(L2_EINVAL, "%s: positions or heads overlap", who);
+    KvDim dims[3] = {{p->page_stride, p->n_pages}, {p->position_stride, p->page_size}, {p->head_stride, p->n_kv_heads}};
+    if (!apart(dims, p->head_size)) return fail(L2_EINVAL, "%s: pages, positions or heads overlap", who);
     if (p->type == L2_I8 && (!p->k_scale || !p->v_scale || !aligned16(p->k_scale) || !aligned16(p->v_scale)))
         return fail(L2_EINVAL, "%s: an int8 cache needs scales that start on a 16-byte boundary", who);
     out->k = static_cast<char*>(p->k); out->v = static_cast<char*>(p->v);
@@ -333,7 +348,8 @@ int check_batch(const char* who, const l2_kv_batch* b, int page_size, KvStep* ou
     return L2_OK;
 }
 
-int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_kv_batch* b, int head_size, int heads, KvRows* out) {
+// (rows that are read may lie on one another: one row for all, by a stride of 0)
+int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_kv_batch* b, int head_size, int heads, bool written, KvRows* out) {
     if (!r) return fail(L2_EINVAL, "%s: no %s", who, what);
     if (r->type != L2_F32 && r->type != L2_F16 && r->type != L2_BF16) return fail(L2_EINVAL, "%s: %s is f32, f16 or bf16 (type %d)", who, what, r->type);
     if (r->heads != heads) return fail(L2_EINVAL, "%s: %s has %d heads, not %d", who, what, r->heads, heads);
@@ -343,7 +359,8 @@ int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_
         return fail(L2_EINVAL, "%s: %s has strides of %lld and %lld elements (multiples of 16 bytes)", who, what, (long long)r->row_stride, (long long)r->head_stride);
     out->data = static_cast<char*>(r->data); out->row_stride = r->row_stride; out->head_stride = r->head_stride;
     out->type = r->type; out->heads = heads;
-    (void)head_size;
+    KvDim dims[2] = {{r->row_stride, b->n_rows}, {r->head_stride, heads}};
+    if (written && !apart(dims, head_size)) return fail(L2_EINVAL, "%s: rows or heads of %s overlap", who, what);
     return L2_OK;
 }
 
@@ -397,13 +414,13 @@ extern "C" int l2_kv_append_rope(const l2_kv_pages* pages, const l2_kv_batch* ba
     KvCopyParams P{};
     if (int rc = check_pages(who, pages, &P.pool)) return rc;
     if (int rc = check_batch(who, batch, pages->page_size, &P.step)) return rc;
-    if (int rc = check_rows(who, "k", k, batch, pages->head_size, pages->n_kv_heads, &P.k)) return rc;
-    if (int rc = check_rows(who, "v", v, batch, pages->head_size, pages->n_kv_heads, &P.v)) return rc;
+    if (int rc = check_rows(who, "k", k, batch, pages->head_size, pages->n_kv_heads, false, &P.k)) return rc;
+    if (int rc = check_rows(who, "v", v, batch, pages->head_size, pages->n_kv_heads, false, &P.v)) return rc;
     if (!q != !q_out) return fail(L2_EINVAL, "%s: q and q_out go together", who);
     if (q) {
         if (q->heads < 1 || q->heads > 4096) return fail(L2_EINVAL, "%s: q has %d heads", who, q->heads);
-        if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, &P.q)) return rc;
-        if (int rc = check_rows(who, "q_out", q_out, batch, pages->head_size, q->heads, &P.q_out)) return rc;
+        if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, false, &P.q)) return rc;
+        if (int rc = check_rows(who, "q_out", q_out, batch, pages->head_size, q->heads, true, &P.q_out)) return rc;
     }
     if (!rope_cos != !rope_sin || (rope_cos && (rope_len < 1 || !aligned16(rope_cos) || !aligned16(rope_sin))))
         return fail(L2_EINVAL, "%s: both rope tables, on a 16-byte boundary, of at least one position", who);
@@ -427,8 +444,8 @@ extern "C" int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, co
     KvCopyParams P{};
     if (int rc = check_pages(who, pages, &P.pool)) return rc;
     if (int rc = check_batch(who, batch, pages->page_size, &P.step)) return rc;
-    if (int rc = check_rows(who, "k", k, batch, pages->head_size, pages->n_kv_heads, &P.k)) return rc;
-    if (int rc = check_rows(who, "v", v, batch, pages->head_size, pages->n_kv_heads, &P.v)) return rc;
+    if (int rc = check_rows(who, "k", k, batch, pages->head_size, pages->n_kv_heads, true, &P.k)) return rc;
+    if (int rc = check_rows(who, "v", v, batch, pages->head_size, pages->n_kv_heads, true, &P.v)) return rc;
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
@@ -459,8 +476,8 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (int rc = check_batch(who, batch, pages->page_size, &P.step)) return rc;
     if (!q) return fail(L2_EINVAL, "%s: no q", who);
     if (int rc = check_heads(who, pages, batch, q->heads)) return rc;
-    if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, &P.q)) return rc;
-    if (int rc = check_rows(who, "out", out, batch, pages->head_size, q->heads, &P.out)) return rc;
+    if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, false, &P.q)) return rc;
+    if (int rc = check_rows(who, "out", out, batch, pages->head_size, q->heads, true, &P.out)) return rc;
     if (q->type == L2_F32 || (pages->type != L2_I8 && q->type != pages->type)) return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 cache)", who);
     if (out->type != L2_F32 && out->type != q->type) return fail(L2_EINVAL, "%s: out must be of q's type or f32", who);
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);

@@ -1,7 +1,7 @@
 """What the paged cache's entry points and objects refuse at the edges of their ranges (no GPU needed)."""
 import pytest
 
-from test_paged_arguments import A, attend, batch, pages, ref, rows
+from test_paged_arguments import A, append, attend, batch, pages, ref, rows
 
 
 # the size of a workspace is asked for before attention itself checks anything: heads that no kernel takes must not reach its divisions
@@ -76,3 +76,28 @@ def test_rotation_out_of_range(l2):
     p, b, r = pages(l2), batch(l2), rows(l2)
     for rotation in (-1, 2):
         assert l2.lib.l2_kv_append_rope(ref(p), ref(b), ref(r), ref(r), None, None, A, A, 9, rotation, None) == -1 and b"rotation" in l2.lib.l2_last_error()
+
+
+# a pool of 4 pages of 16 positions and 2 heads of 128: what would lie on one another is refused, whatever dimension it is
+@pytest.mark.parametrize("strides", [(4096, 128, 128), (4096, 256, 144), (4000, 256, 128), (128, 1024, 256), (256, 256, 128), (4096, 256, 256), (128, 2048, 128), (2048, 128, 2048)])
+def test_pools_that_overlap(l2, strides):
+    p, b, r = pages(l2, **dict(zip(("page_stride", "position_stride", "head_stride"), strides))), batch(l2), rows(l2)
+    assert append(l2, p, b, r, r) == -1 and b"overlap" in l2.lib.l2_last_error()
+
+
+# page by page, head by head, position by position, with gaps: all of these are pools
+@pytest.mark.parametrize("strides", [(4096, 256, 128), (4096, 128, 2048), (128, 512, 8192), (128, 1024, 512), (4160, 256, 128), (4352, 272, 136), (256, 1024, 128)])
+def test_pools_that_do_not(l2, strides):
+    p, b = pages(l2, **dict(zip(("page_stride", "position_stride", "head_stride"), strides))), batch(l2)
+    r = rows(l2, heads=3)  # (refused for its heads, after the pool has been looked at)
+    assert append(l2, p, b, r, r) == -1 and b"3 heads" in l2.lib.l2_last_error()
+
+
+# several rows written to one place: refused; read from one place: not
+@pytest.mark.parametrize("bad", [dict(row_stride=0), dict(row_stride=128), dict(head_stride=64), dict(head_stride=0), dict(row_stride=64, head_stride=320), dict(row_stride=128, head_stride=512)])
+def test_written_rows_that_overlap(l2, bad):
+    p, b, r, x = pages(l2), batch(l2), rows(l2), rows(l2, **bad)
+    for call in (lambda: l2.lib.l2_kv_read(ref(p), ref(b), ref(x), ref(r), None), lambda: l2.lib.l2_kv_read(ref(p), ref(b), ref(r), ref(x), None),
+                 lambda: append(l2, p, b, r, r, q=r, q_out=x), lambda: attend(l2, p, b, r, x, work=A, size=1 << 30)):
+        assert call() == -1 and b"overlap" in l2.lib.l2_last_error()
+    assert append(l2, p, b, x, x, q=x, q_out=rows(l2, row_stride=100)) == -1 and b"q_out has strides" in l2.lib.l2_last_error()  # (k, v and q went through)
