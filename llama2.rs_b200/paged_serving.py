@@ -4,7 +4,7 @@
     python llama2.rs_b200/paged_serving.py --heads 64 --kv-heads 8 --cache f16 --window 1024 --sinks 4
 
 A step takes up to --budget rows: one of every sequence that is past its prompt, the rest of the room for prompts, in order.  Pages are handed out as
-sequences grow and, with a window, given back when no row can see them any more.  There is no model behind the layer: a prompt is random rows, and the
+sequences grow and given back when these end and, with a window, when no row can see them any more.  There is no model behind the layer: a prompt is random rows, and the
 next row of a sequence is the layer's own (normalised) output for the row before.  Weights are random in the checkpoint's layout; RoPE is that of the
 package's models (--rotation pairs: of plain pairs, for weights that want it).
 """
@@ -45,13 +45,24 @@ class PagedLayer:
         self.linear[name].matvec_dev(x.data_ptr(), out.data_ptr(), x.shape[0], self.torch.cuda.current_stream().cuda_stream)
         return out
 
+    def pages_for(self, sequence, rows):
+        """Pages that a sequence needs besides its own for so many more rows."""
+        return max(0, -(-(sequence["length"] + rows) // self.page_size) - len(sequence["table"]))
+
+    def release(self, sequence):
+        """Gives back the pages of a sequence that has ended.  (Work enqueued before is in front of what their next owner enqueues.)"""
+        self.free += [page for page in sequence["table"] if page >= 0]
+        sequence["table"], sequence["length"] = [], 0
+
     def step(self, x, sequences, rows):
         """x [rows in all, dim] f32, rows[i] new rows of sequences[i] (dicts with `length` and `table`): the layer's output, f32."""
         torch, n = self.torch, x.shape[0]
-        for s, r in zip(sequences, rows):
+        new = [self.pages_for(s, r) for s, r in zip(sequences, rows)]
+        if sum(new) > len(self.free):
+            raise RuntimeError("%d pages needed, %d left" % (sum(new), len(self.free)))
+        for s, r, pages in zip(sequences, rows, new):
             s["length"] += r
-            while len(s["table"]) * self.page_size < s["length"]:
-                s["table"].append(self.free.pop())
+            s["table"] += [self.free.pop() for _ in range(pages)]
         width = max(len(s["table"]) for s in sequences)
         table = torch.tensor([s["table"] + [-1] * (width - len(s["table"])) for s in sequences], dtype=torch.int32).cuda()
         kv_len = torch.tensor([s["length"] for s in sequences], dtype=torch.int32).cuda()
@@ -92,6 +103,8 @@ def serve(layer, prompts, tokens, budget):
         y = layer.step(torch.cat(xs), picked, rows)
         for s, part in zip(picked, y.split(rows)):
             s["out"].append(part)
+            if not len(s["todo"]) and s["left"] <= 0:
+                layer.release(s)
         steps, total = steps + 1, total + sum(rows)
     return [torch.cat(s["out"]) for s in seqs], steps, total
 
