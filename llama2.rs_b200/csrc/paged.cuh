@@ -80,37 +80,7 @@ __device__ __forceinline__ int kv_find_seq(const KvStep& s, int r) {
     return lo;
 }
 
-// Type codes as template arguments: how 8 elements are loaded as f32 and stored.
-template <int T> struct KvElem;
-template <> struct KvElem<L2_F32> { using type = float; };
-template <> struct KvElem<L2_F16> { using type = __half; };
-template <> struct KvElem<L2_BF16> { using type = __nv_bfloat16; };
-
-__device__ __forceinline__ void kv_load8(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void kv_load8(const __half* p, float (&x)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x; x[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ void kv_load8(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void kv_load8(const int8_t* p, float (&x)[8]) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    const uint32_t w[2] = {a.x, a.y};
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
-}
+// 8 f32 stored as a type
 __device__ __forceinline__ void kv_store8(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -126,19 +96,6 @@ __device__ __forceinline__ void kv_store8(__nv_bfloat16* p, const float (&x)[8])
 #pragma unroll
     for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
-}
-// by a type known at run time (row arrays)
-__device__ __forceinline__ void kv_load8(const KvRows& r, int64_t row, int head, int d, float (&x)[8]) {
-    const int64_t e = row * r.row_stride + head * r.head_stride + d;
-    if (r.type == L2_F32) kv_load8(reinterpret_cast<const float*>(r.data) + e, x);
-    else if (r.type == L2_F16) kv_load8(reinterpret_cast<const __half*>(r.data) + e, x);
-    else kv_load8(reinterpret_cast<const __nv_bfloat16*>(r.data) + e, x);
-}
-__device__ __forceinline__ void kv_store8(const KvRows& r, int64_t row, int head, int d, const float (&x)[8]) {
-    const int64_t e = row * r.row_stride + head * r.head_stride + d;
-    if (r.type == L2_F32) kv_store8(reinterpret_cast<float*>(r.data) + e, x);
-    else if (r.type == L2_F16) kv_store8(reinterpret_cast<__half*>(r.data) + e, x);
-    else kv_store8(reinterpret_cast<__nv_bfloat16*>(r.data) + e, x);
 }
 #endif
 

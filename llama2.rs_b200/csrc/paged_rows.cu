@@ -681,7 +681,7 @@ cudaError_t kr_by_variant(int type, bool qb, int hd, int nt, F f) {
 
 int kr_nt(int lim) { return lim <= 8 ? 1 : 2; }
 int kr_tile(int type, int head_size) { return head_size * (type == L2_I8 ? 1 : 2) == 256 ? 64 : 128; }
-// CTAs of a launch: two an SM, no more than there can be tiles
+// CTAs of a launch: two an SM, no more than the line can be long (which is KR_SETUP + 1 or more)
 int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
     const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + tile - 1) / tile + 1 + KR_SETUP);
     return (int)std::min<int64_t>(2 * sms, tiles);
@@ -717,7 +717,7 @@ cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int
         if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KrShape<T, HD, NT>::SMEM)) return x;
         return kv_launch(kernel, dim3(grid), KR_THREADS, KrShape<T, HD, NT>::SMEM, st, p, lim, mk, mv);
     });
-    if (e != cudaSuccess || grid < 2) return e;
+    if (e != cudaSuccess) return e;
     auto combine = head_size == 128 ? kv_rows_combine_kernel<128> : kv_rows_combine_kernel<64>;
     return kv_launch(combine, dim3(grid - 1, KR_JOIN), 256, 0, st, p, grid, 8 * nt);
 }

@@ -898,7 +898,7 @@ __global__ void __launch_bounds__(256) kv_tc_combine_kernel(const __grid_constan
     else kv_store8(reinterpret_cast<__nv_bfloat16*>(P.out.data) + e + d, y);
 }
 
-// CTAs of a launch: one an SM, no more than there can be tiles
+// CTAs of a launch: one an SM, no more than the line can be long (which is KT_SETUP + 1 or more)
 int kt_grid(const KvStep& s, const KvPool& p, int group, int sms) {
     const int64_t blocks = s.n_rows / (KT_ROWS / group) + s.n_seqs;
     return (int)std::min<int64_t>(sms, blocks * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + KT_TILE - 1) / KT_TILE + 1 + KT_SETUP));
@@ -932,7 +932,7 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
     const cudaError_t e = type == L2_F16 ? by_hd(std::integral_constant<int, L2_F16>(), std::false_type())
                         : type == L2_BF16 ? by_hd(std::integral_constant<int, L2_BF16>(), std::true_type())
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
-    if (e != cudaSuccess || grid < 2) return e;
+    if (e != cudaSuccess) return e;
     auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;
     return kv_launch(combine, dim3(grid - 1, KT_ROWS / 32, head_size / 64), 256, 0, st, p, grid);
 }
