@@ -691,7 +691,7 @@ int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
 
 int kv_rows_limit(const KvStep& s, int group) {
     const int64_t most = (int64_t)s.max_rows * group;
-    if (most <= 16) return (int)most;
+    if (most <= 16) return std::max(1, (int)most);  // (0, a step said to bring no rows: somebody has to look whether that is so)
     return group <= 16 && (int64_t)s.n_seqs * s.max_rows > s.n_rows ? group : 0;
 }
 

@@ -120,3 +120,19 @@ def test_launches_of_several_threads_are_counted(l2):
         t.join()
     torch.cuda.synchronize()
     assert not failed and l2.lib.l2_launch_count() - before == calls * n_threads
+
+
+# a step said to have no rows that does bring some: left out and reported, as any that brings more than it says
+@pytest.mark.parametrize("cache,io", CACHES)
+def test_rows_of_a_step_that_says_it_has_none(l2, cache, io):
+    from llama2_rs import paged
+    c = Case([2, 1], [30, 40], cache=cache)
+    pages, batch = c.handles(l2, max_rows=0)
+    q = torch.ones((3, 2, 128), dtype=io, device="cuda")
+    out = torch.full_like(q, 7.0)
+    pages.attend(batch, q, out)
+    assert (out == 7.0).all() and int(c.status) == paged.BAD_ROWS
+    c = Case([0, 0], [30, 40], cache=cache, spare_rows=3)
+    pages, batch = c.handles(l2)
+    pages.attend(batch, q, out)
+    assert (out == 7.0).all() and int(c.status) == 0
