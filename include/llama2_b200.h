@@ -297,7 +297,8 @@ int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_r
  * where window > 0, p - j < window or j < sinks.  out = softmax(scale * q k) v over what it sees; 0 where it sees nothing.  What a row does not see
  * does not reach its result, NaN and infinities included.  heads of q a multiple of n_kv_heads (at most 64 times).  q: f16 or bf16, the
  * cache's type or either with an int8 cache; out: q's type or f32.  Products of q and k are exact and all sums are f32; the probabilities
- * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16).
+ * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16), whatever out's type.  Sums are of probabilities
+ * times up to 2^32, divided at the end: values of V up to 2^64 cannot overflow them, however many positions there are.
  * Pages that no row of the call sees are not read: with a window they can be given back. */
 int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* q, const l2_kv_rows* out, float scale, int window, int sinks,
                  void* workspace, size_t workspace_bytes, void* cuda_stream);

@@ -6,7 +6,7 @@
 // and head elements (O^T) are the 16 rows of an mma.sync, the few query rows its 8 columns, so that one row wastes 7 of 8, not 15 of 16.
 //
 // What bounds it: reading the cache, once, by TMA, while the matrix work of a tile hides behind the copies of the next.  bf16, 8 sequences of 40 heads, 4096 positions each
-// (672 MB): 115 us, 5.9 TB/s.  int8, 64 sequences of 8 kv heads with 8 query heads (565 MB): 112 to 118 us, 4.8 to 5.0 TB/s, for most of the time bound by the instructions that
+// (672 MB): 114 us, 5.9 TB/s.  int8, 64 sequences of 8 kv heads with 8 query heads (565 MB): 115 to 123 us, 4.6 to 4.9 TB/s, for most of the time bound by the instructions that
 // widen V (173 us while a compiler made two instructions of each of their logic operations, 194 with tiles of 64 positions).
 //
 // Work.  The tiles of all (sequence, kv head) pairs form one line, cut evenly over the CTAs whatever the lengths are, with room in front of every pair for what it costs
@@ -36,7 +36,9 @@ namespace l2 {
 namespace {
 
 constexpr int KR_WARPS = 4, KR_THREADS = (KR_WARPS + 1) * 32, KR_MAX_STAGES = 12;
-constexpr int KR_SETUP = 2;  // what a pair costs besides its tiles, in tiles
+// What a pair costs besides its tiles, in tiles.  1 or 4 instead, steps of 40 to 64 sequences: int8, 8 rows a kv head 1.5 % slower and up to 1.5 % slower (heads of 64: 3 %, none);
+// 16 rows a kv head, int8 5 % slower and 7 % faster, bf16 5 % slower and 1 % faster; bf16 with heads of 64 no difference.
+constexpr int KR_SETUP = 2;
 constexpr int KR_JOIN = 2;  // CTAs that add the pieces of a pair (with 4 or 8, a step of 64 sequences takes 2 or 5 us longer: CTAs without work)
 constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr int KR_DIGITS = 4;  // of Q against int8 K
@@ -156,6 +158,7 @@ struct KrWalk {
 };
 
 // CT: cache type; QB: q is bf16, else f16
+// (Eight rows: no spills.  Sixteen: int8 with heads of 128 spills 236 bytes, 16 bits 24.)
 template <int CT, bool QB, int HD, int NT>
 __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
                                                                const __grid_constant__ CUtensorMap map_v) {

@@ -8,11 +8,13 @@
 // What bounds it.  A tile of positions is four products of 128 x 128 x 128, 2048 clocks of the tensor cores at their peak; 32768 exponentials, 2048 clocks of the
 // special function units; and, because S is taken 64 positions at a time, 320 KB through shared memory at 128 bytes a clock, 2500.  A whole prompt (8191 tokens, 32
 // heads of 128, bf16) takes about 3500 clocks a tile: 540 us on one input (1021 TFLOP/s of 1621 measured), 640 to 660 between others, as the chip's power allows.
+// Counters of that prompt: tensor pipe 52 %, special functions 52 %, shared memory 53 % (48 for the products, 5 for the rest): none is full, the chain
+// scores, softmax, product of the two row tiles is what is left.
 // Measured on the way (the same prompt): one warp issuing for both tiles of rows 1017 us (an issue takes 75 to 85 clocks, whatever its size, and a wait some hundred); two
-// 918; S in halves 803; Q requested eight lines at once 656; pieces planned by one warp, so that nothing spills, 598; room on the line for a block's other costs 539.
+// 918; S in halves 803; Q requested eight lines at once 656; pieces planned by one warp, so that next to nothing spills (12 bytes; int8 196, 64 wide 132), 598; room on the line for a block's other costs 539.
 // Not kept: exponentials on the FMA units (1, 2 or 4 of 16: 559 to 565 against 556), the two groups of softmax taking turns (608 against 598), a predicate in place of
 // the branch around the issue (569 against 556).  An int8 cache costs about 1500 clocks a tile more (scales of 64 positions
-// a thread and their products, and bytes to widen: 512 tokens of 64 heads behind 14,488 positions take 360 us, 252 without either and 350 without one of them; four rows
+// a thread and their products, and bytes to widen: 512 tokens of 64 heads behind 14,488 positions take 360 us on one input, 252 without either and 350 without one of them; four rows
 // a quad of threads, so that each thread reads a quarter of the scales, took 349, but 40 rows a kv head 58 instead of 52).
 //
 // Work.  The tiles of positions of all (sequence, kv head, block) triples form one line, cut evenly over the SMs, with room in front of every
@@ -46,7 +48,9 @@ namespace {
 constexpr int KT_TILE = 128, KT_SUB = 64, KT_ROWS = 256, KT_THREADS = 512;
 constexpr int KT_MMA_WARP = 0, KT_COPY_WARP = 1, KT_PLAN_WARP = 3, KT_ROW_WARP = 4, KT_HELP_WARP = 12;
 constexpr int KT_SCALE_SLOTS = 4;
-constexpr int KT_SETUP = 4;  // what a block costs besides its tiles, in tiles
+// What a block costs besides its tiles, in tiles.  2 or 8 instead: 12 sequences with 5 tokens 9 % slower (int8 3 and 9 %); a prompt of 4095 tokens with heads of 64 4 %
+// faster and 6 % slower; chunks of 512 over long caches within 1 % (int8 with heads of 64: 1 % faster, 4 % slower).
+constexpr int KT_SETUP = 4;
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
 template <int CT, int HD>
