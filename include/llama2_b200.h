@@ -228,7 +228,8 @@ int l2_attention_decode_noalloc(int n_heads, int n_kv_heads, int pos, const floa
  * and kv head.  Position j of sequence b is in page page_table[b][j / page_size], at j % page_size.  All arrays belong to the caller
  * and are device memory of the current device; every call is enqueued on cuda_stream (NULL: the default stream) and does not wait.
  *
- * The lengths are read on the device, so a step's record serves all layers and may be captured in a graph.  What only the device can
+ * The lengths are read on the device, so a step's record serves all layers and may be captured in a graph.  They and the tables must stay as
+ * they are while a call that reads them runs (each CTA looks for its share of the work by itself).  What only the device can
  * see to be wrong it reports in the batch's status word (L2_KV_*); the entry concerned is left out, nothing is read or written
  * outside the caller's arrays. */
 #define L2_F32 0

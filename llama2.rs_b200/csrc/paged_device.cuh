@@ -10,7 +10,7 @@ namespace l2 {
 
 // ---- mbarriers and copies ---------------------------------------------------------------------------------------------
 
-constexpr uint32_t KV_WAIT_LIMIT = 1u << 22;
+constexpr uint32_t KV_WAIT_LIMIT = 1u << 22;  // polls, each parked for up to 4 us
 
 __device__ __forceinline__ uint32_t kv_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void kv_bar_init(uint64_t* bar, uint32_t count) {

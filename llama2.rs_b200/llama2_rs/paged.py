@@ -8,7 +8,8 @@
     pages.read(batch, k_back, v_back)
 
 The objects keep the tensors they are made of.  Work is enqueued on the current torch stream unless `stream` (a cudaStream_t) is given; a call
-does not wait for it.  One host thread at a time uses a KvPages.
+does not wait for it.  With another stream than a tensor's own the caller orders the two and keeps rows and workspace until the work has run, as
+with any torch kernel.  One host thread at a time uses a KvPages.
 """
 import ctypes as C
 import struct
