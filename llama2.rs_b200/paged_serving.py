@@ -18,7 +18,8 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 
 class PagedLayer:
-    """wq / wk / wv -> RoPE, append -> attend -> wo on device tensors; the cache's pages and who has them."""
+    """wq / wk / wv -> RoPE, append -> attend -> wo on device tensors; the cache's pages and who has them.  rotation: "pairs", or "model" as the package's
+    models do it, for their weights."""
 
     def __init__(self, dim, heads, kv_heads, *, cache="i8", n_pages=512, page_size=32, positions=4096, window=0, sinks=0, group_size=64, seed=0, weights=None, rotation="pairs"):
         import torch
