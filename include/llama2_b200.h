@@ -224,8 +224,8 @@ int l2_attention_decode_noalloc(int n_heads, int n_kv_heads, int pos, const floa
 
 /* ---- paged KV cache and its attention on device buffers (no counterpart in the reference, whose cache is one sequence's, in f32) ----
  *
- * One layer's cache of many sequences, in pages of page_size positions: K and V in f16, bf16, or int8 with one f32 scale per position
- * and kv head.  Position j of sequence b is in page page_table[b][j / page_size], at j % page_size.  All arrays belong to the caller
+ * One layer's cache of many sequences, in pages of page_size positions: K and V in f16, bf16, int8 with one f32 scale per position
+ * and kv head, or 4 bits with a scale and a zero in bf16 per position and kv head.  Position j of sequence b is in page page_table[b][j / page_size], at j % page_size.  All arrays belong to the caller
  * and are device memory of the current device; every call is enqueued on cuda_stream (NULL: the default stream) and does not wait.
  *
  * The lengths are read on the device, so a step's record serves all layers and may be captured in a graph.  They and the tables must stay as
@@ -236,14 +236,16 @@ int l2_attention_decode_noalloc(int n_heads, int n_kv_heads, int pos, const floa
 #define L2_F16 1
 #define L2_BF16 2
 #define L2_I8 3
+#define L2_U4 4  /* numbers u of 0 .. 15, two a byte, the element of even index in the low half; value = zero + u * scale */
 
 typedef struct l2_kv_pages {
     void* k;                /* element d of (page, position, kv head): page * page_stride + position * position_stride + head * head_stride + d */
     void* v;
-    float* k_scale;         /* L2_I8: [n_pages][n_kv_heads][page_size], value = stored * scale; else NULL */
+    float* k_scale;         /* L2_I8: [n_pages][n_kv_heads][page_size], value = stored * scale.  L2_U4: as many words of 32 bits, each a pair of bf16, the
+                               scale in its low half, the zero in its high one.  Else NULL */
     float* v_scale;
-    int64_t page_stride, position_stride, head_stride;  /* in elements; multiples of 16 bytes, the same for k and v, nothing on one another */
-    int32_t type;           /* L2_F16, L2_BF16 or L2_I8 */
+    int64_t page_stride, position_stride, head_stride;  /* in elements; multiples of 16 bytes (L2_U4: of 32 elements), the same for k and v, nothing on one another */
+    int32_t type;           /* L2_F16, L2_BF16, L2_I8 or L2_U4 */
     int32_t n_pages;
     int32_t page_size;      /* 8, 16, 32, 64, 128 or 256 */
     int32_t n_kv_heads;
@@ -286,7 +288,10 @@ typedef struct l2_kv_rows {
 /* K and V of the batch's rows into their pages.  With rope tables ([rope_len][head_size / 2] each, f32) k is turned at its position first, and so is
  * q into q_out where q is not NULL; without them q is rounded to q_out's type only.  Programs that share caches or checkpoints with the rest of
  * this library take the tables of l2_rope_table and L2_ROPE_MODEL.  int8: a row and head is scaled by 127 / its largest magnitude and rounded to
- * nearest even.  One that holds a NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros. */
+ * nearest even.  One that holds a NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros.
+ * 4 bits: of a row and head, zero = the bf16 number at or below its least element, span = its largest less zero, scale = the least bf16 number s with
+ * 15 s >= span, u = (x - zero) * (1 / scale), differences and reciprocal rounded to 32 bits, their product rounded once, to a whole number (nearest
+ * even).  A span below 2^-100: scale and u 0.  A NaN, an infinity or a span beyond f32: scale and zero NaN. */
 int l2_kv_append_rope(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
                       const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, int rotation, void* cuda_stream);
 /* The same with L2_ROPE_PAIRS. */

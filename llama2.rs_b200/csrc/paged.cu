@@ -2,6 +2,9 @@
 //
 //   16 bits:  cache = round(x)
 //   8 bits:   a = max |x| over a row and head, scale = a / 127, cache = rint(x * (127 / a)), and back: value = cache * scale
+//   4 bits:   zero = bf16 at or below min x, scale = least bf16 with 15 scale >= max x - zero, cache = rint((x - zero) / scale), value = zero + scale * cache.  Both are
+//             rounded outwards, so that cache stays in 0 .. 15 and no element lies more than half a step off; bf16 because it has f32's range in half the bytes (a pair beside
+//             the 64 bytes of a head of 128)
 //   RoPE:     (a, b) = (x[d], x[d + hd/2]) turned by the angle of the row's position, first: a' = a c - b s, b' = b c + a s, or, as the
 //             token loop of this library does it in place, b' = b c + a' s
 //
@@ -109,6 +112,16 @@ __device__ __forceinline__ void stream8(char* base, int64_t e, const float* x) {
         __stcs(reinterpret_cast<uint4*>(base + 2 * e), make_uint4(kv_pack<T>(x[0], x[1]), kv_pack<T>(x[2], x[3]), kv_pack<T>(x[4], x[5]), kv_pack<T>(x[6], x[7])));
     }
 }
+__device__ __forceinline__ float min_nan(float a, float x) {  // NaN if one of them is
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(x));
+    return y;
+}
 __device__ __forceinline__ float max_abs(float a, float x) {  // NaN if one of them is
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(fabsf(x)));
@@ -121,7 +134,7 @@ __device__ __forceinline__ float max_abs(float a, float x) {  // NaN if one of t
 // whose look-ups nothing hid, took 76; so did 16 elements of one run a thread with conversion instructions and 110 registers (18 instructions an element).
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_constant__ KvCopyParams P) {
-    constexpr bool I8 = T == L2_I8;
+    constexpr bool I8 = T == L2_I8, U4 = T == L2_U4;
     constexpr int LANES = HD / 16, GROUPS = KV_THREADS / LANES, HALF = HD / 2;
     __shared__ KvPlace place[KV_MAX_ROWS];
     const int sub = threadIdx.x % LANES, grp = threadIdx.x / LANES, d = 8 * sub;
@@ -206,6 +219,32 @@ __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_c
                         *reinterpret_cast<uint2*>(to + e + HALF) = make_uint2(b[2], b[3]);
                         if (sub == 0) scales[place[at_row].scale + ((int64_t)head[a] << P.pool.page_shift)] =
                             !finite ? __int_as_float(0x7fc00000) : zero ? 0.0f : __fmul_rn(m, 1.0f / 127.0f);
+                    } else if constexpr (U4) {
+                        float lo = x[0], hi = x[0];
+#pragma unroll
+                        for (int i = 1; i < 16; i++) { lo = min_nan(lo, x[i]); hi = max_nan(hi, x[i]); }
+#pragma unroll
+                        for (int o = LANES / 2; o; o >>= 1) { lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
+                        const uint32_t low = __float_as_uint(lo);
+                        const float zero = __uint_as_float((low + (lo < 0.0f ? 0xffffu : 0u)) & 0xffff0000u), span = __fsub_rn(hi, zero);
+                        uint32_t step = __float_as_uint(__fmul_rn(span, 1.0f / 15.0f)) & 0xffff0000u;  // (15 times a bf16 number is exact)
+                        if (__fmul_rn(__uint_as_float(step), 15.0f) < span) step += 0x10000u;
+                        const bool finite = span < INFINITY, flat = span < 0x1p-100f;
+                        const float inv = flat ? 0.0f : __frcp_rn(__uint_as_float(step));
+                        // ((x - zero) inv is at most 15 and a few units in the last place.  One rounding to a whole number, as above, of the exact product: rows of 16 bits often
+                        // lie next to the middle of a step.  What the number 1.5 x 2^23 adds to all eight is taken off the word.)
+                        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+                        for (int i = 7; i >= 0; i--) {
+                            w[0] = (w[0] << 4) + __float_as_uint(__fmaf_rn(__fsub_rn(x[i], zero), inv, 12582912.0f));
+                            w[1] = (w[1] << 4) + __float_as_uint(__fmaf_rn(__fsub_rn(x[8 + i], zero), inv, 12582912.0f));
+                        }
+                        if (!store) continue;
+                        constexpr uint32_t ADDED = 0x4b400000u * 0x11111111u;
+                        *reinterpret_cast<uint32_t*>(to + e / 2) = w[0] - ADDED;
+                        *reinterpret_cast<uint32_t*>(to + (e + HALF) / 2) = w[1] - ADDED;
+                        if (sub == 0) reinterpret_cast<uint32_t*>(scales)[place[at_row].scale + ((int64_t)head[a] << P.pool.page_shift)] =
+                            !finite ? 0x7fc07fc0u : __float_as_uint(zero) | (flat ? 0u : step >> 16);
                     } else if (store) {
                         store8<T>(to, e, x);
                         store8<T>(to, e + HALF, x + 8);
@@ -224,8 +263,8 @@ __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_c
 // registers, although the int8 forms then spill 13 words: with four and ordinary stores it took 218 us, with six 233.
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const __grid_constant__ KvCopyParams P) {
-    constexpr bool I8 = T == L2_I8;
-    constexpr int N = I8 ? 16 : 8, LANES = HD / N, GROUPS = KV_THREADS / LANES;
+    constexpr bool I8 = T == L2_I8, U4 = T == L2_U4;
+    constexpr int N = I8 || U4 ? 16 : 8, LANES = HD / N, GROUPS = KV_THREADS / LANES;
     __shared__ KvPlace place[KV_MAX_ROWS];
     const int d = N * (threadIdx.x % LANES), grp = threadIdx.x / LANES, heads = P.pool.n_kv_heads, units = 2 * P.rows * heads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -243,8 +282,13 @@ __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const __grid_con
                 f[a] = 0.0f;
                 if (u < units && place[r].at >= 0) {
                     const char* from = h < heads ? P.pool.k : P.pool.v;
-                    x[a] = __ldcs(reinterpret_cast<const uint4*>(from + (place[r].at + head * P.pool.head_stride + d) * (I8 ? 1 : 2)));
-                    if constexpr (I8) f[a] = (h < heads ? P.pool.ks : P.pool.vs)[place[r].scale + ((int64_t)head << P.pool.page_shift)];
+                    if constexpr (U4) {
+                        const uint2 w = __ldcs(reinterpret_cast<const uint2*>(from + (place[r].at + head * P.pool.head_stride + d) / 2));
+                        x[a].x = w.x; x[a].y = w.y;
+                    } else {
+                        x[a] = __ldcs(reinterpret_cast<const uint4*>(from + (place[r].at + head * P.pool.head_stride + d) * (I8 ? 1 : 2)));
+                    }
+                    if constexpr (I8 || U4) f[a] = (h < heads ? P.pool.ks : P.pool.vs)[place[r].scale + ((int64_t)head << P.pool.page_shift)];
                 }
             }
 #pragma unroll
@@ -253,11 +297,12 @@ __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const __grid_con
                 if (u >= units || place[r].pos < 0) continue;
                 const KvRows& to = h < heads ? P.k : P.v;
                 float y[N];
-                const uint32_t w[4] = {x[a].x, x[a].y, x[a].z, x[a].w};
+                const uint32_t w[4] = {x[a].x, x[a].y, x[a].z, x[a].w}, pair = __float_as_uint(f[a]);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     // 2^23 + 128 + byte, less 2^23 + 128: exact, and no conversion instruction
                     if constexpr (I8) y[i] = (__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (i % 4))) - 8388736.0f) * f[a];
+                    else if constexpr (U4) y[i] = __fmaf_rn(__uint_as_float((w[i / 8] >> (4 * (i % 8)) & 15u) | 0x4b000000u) - 8388608.0f, kv_pair_scale(pair), kv_pair_zero(pair));
                     else if constexpr (T == L2_F16) y[i] = __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i % 2)))));
                     else y[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
                 }
@@ -296,7 +341,7 @@ int kv_device(int* sms) {
     return L2_OK;
 }
 
-int elem_bytes(int type) { return type == L2_F32 ? 4 : type == L2_I8 ? 1 : 2; }
+int elem_bits(int type) { return type == L2_F32 ? 32 : type == L2_I8 ? 8 : type == L2_U4 ? 4 : 16; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Whether runs of head_size elements lie apart, each dimension's steps beyond all that is inside it (as every array that is a part of a larger one has it).
@@ -315,7 +360,7 @@ bool apart(KvDim (&d)[N], int head_size) {
 
 int check_pages(const char* who, const l2_kv_pages* p, KvPool* out) {
     if (!p) return fail(L2_EINVAL, "%s: no pages", who);
-    if (p->type != L2_F16 && p->type != L2_BF16 && p->type != L2_I8) return fail(L2_EINVAL, "%s: a cache is f16, bf16 or int8 (type %d)", who, p->type);
+    if (p->type != L2_F16 && p->type != L2_BF16 && p->type != L2_I8 && p->type != L2_U4) return fail(L2_EINVAL, "%s: a cache is f16, bf16, int8 or u4 (type %d)", who, p->type);
     if (p->head_size != 64 && p->head_size != 128) return fail(L2_EINVAL, "%s: head size %d (64 or 128)", who, p->head_size);
     int shift = 3;
     while (shift < 8 && (1 << shift) < p->page_size) shift++;
@@ -323,13 +368,13 @@ int check_pages(const char* who, const l2_kv_pages* p, KvPool* out) {
     if (p->n_pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 1024) return fail(L2_EINVAL, "%s: %d pages, %d kv heads", who, p->n_pages, p->n_kv_heads);
     if (!p->k || !p->v || !aligned16(p->k) || !aligned16(p->v)) return fail(L2_EINVAL, "%s: k and v must start on a 16-byte boundary", who);
     const int64_t s[3] = {p->page_stride, p->position_stride, p->head_stride};
-    const int least = 16 / elem_bytes(p->type);
+    const int least = 128 / elem_bits(p->type);
     for (int64_t x : s)
         if (x < least || x % least || x > ((int64_t)1 << 36)) return fail(L2_EINVAL, "%s: a stride of %lld elements (multiples of 16 bytes)", who, (long long)x);
     KvDim dims[3] = {{p->page_stride, p->n_pages}, {p->position_stride, p->page_size}, {p->head_stride, p->n_kv_heads}};
     if (!apart(dims, p->head_size)) return fail(L2_EINVAL, "%s: pages, positions or heads overlap", who);
-    if (p->type == L2_I8 && (!p->k_scale || !p->v_scale || !aligned16(p->k_scale) || !aligned16(p->v_scale)))
-        return fail(L2_EINVAL, "%s: an int8 cache needs scales that start on a 16-byte boundary", who);
+    if ((p->type == L2_I8 || p->type == L2_U4) && (!p->k_scale || !p->v_scale || !aligned16(p->k_scale) || !aligned16(p->v_scale)))
+        return fail(L2_EINVAL, "%s: an int8 or u4 cache needs scales that start on a 16-byte boundary", who);
     out->k = static_cast<char*>(p->k); out->v = static_cast<char*>(p->v);
     out->ks = p->k_scale; out->vs = p->v_scale;
     out->page_stride = p->page_stride; out->pos_stride = p->position_stride; out->head_stride = p->head_stride;
@@ -354,7 +399,7 @@ int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_
     if (r->type != L2_F32 && r->type != L2_F16 && r->type != L2_BF16) return fail(L2_EINVAL, "%s: %s is f32, f16 or bf16 (type %d)", who, what, r->type);
     if (r->heads != heads) return fail(L2_EINVAL, "%s: %s has %d heads, not %d", who, what, r->heads, heads);
     if (b->n_rows && (!r->data || !aligned16(r->data))) return fail(L2_EINVAL, "%s: %s must start on a 16-byte boundary", who, what);
-    const int least = 16 / elem_bytes(r->type);
+    const int least = 128 / elem_bits(r->type);
     if ((b->n_rows > 1 && (r->row_stride % least || r->row_stride < 0)) || (heads > 1 && (r->head_stride % least || r->head_stride < 0)))
         return fail(L2_EINVAL, "%s: %s has strides of %lld and %lld elements (multiples of 16 bytes)", who, what, (long long)r->row_stride, (long long)r->head_stride);
     out->data = static_cast<char*>(r->data); out->row_stride = r->row_stride; out->head_stride = r->head_stride;
@@ -379,10 +424,12 @@ cudaError_t by_type(int type, int head_size, F f) {
     if (head_size == 128) {
         if (type == L2_F16) return f(std::integral_constant<int, L2_F16>(), std::integral_constant<int, 128>());
         if (type == L2_BF16) return f(std::integral_constant<int, L2_BF16>(), std::integral_constant<int, 128>());
+        if (type == L2_U4) return f(std::integral_constant<int, L2_U4>(), std::integral_constant<int, 128>());
         return f(std::integral_constant<int, L2_I8>(), std::integral_constant<int, 128>());
     }
     if (type == L2_F16) return f(std::integral_constant<int, L2_F16>(), std::integral_constant<int, 64>());
     if (type == L2_BF16) return f(std::integral_constant<int, L2_BF16>(), std::integral_constant<int, 64>());
+    if (type == L2_U4) return f(std::integral_constant<int, L2_U4>(), std::integral_constant<int, 64>());
     return f(std::integral_constant<int, L2_I8>(), std::integral_constant<int, 64>());
 }
 
@@ -449,7 +496,7 @@ extern "C" int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, co
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!batch->n_rows || !batch->n_seqs) return L2_OK;
-    const dim3 grid = copy_grid(P, 2 * pages->n_kv_heads, 1, KV_THREADS / (pages->head_size / (pages->type == L2_I8 ? 16 : 8)), 8, sms);
+    const dim3 grid = copy_grid(P, 2 * pages->n_kv_heads, 1, KV_THREADS / (pages->head_size / (pages->type == L2_I8 || pages->type == L2_U4 ? 16 : 8)), 8, sms);
     P.by_heads = reciprocal(2 * pages->n_kv_heads);
     L2_CUDA(by_type(pages->type, pages->head_size, [&](auto t, auto hd) {
         return kv_launch(kv_read_kernel<decltype(t)::value, decltype(hd)::value>, grid, KV_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), P);
@@ -478,7 +525,8 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (int rc = check_heads(who, pages, batch, q->heads)) return rc;
     if (int rc = check_rows(who, "q", q, batch, pages->head_size, q->heads, false, &P.q)) return rc;
     if (int rc = check_rows(who, "out", out, batch, pages->head_size, q->heads, true, &P.out)) return rc;
-    if (q->type == L2_F32 || (pages->type != L2_I8 && q->type != pages->type)) return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 cache)", who);
+    if (q->type == L2_F32 || (pages->type != L2_I8 && pages->type != L2_U4 && q->type != pages->type))
+        return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 or u4 cache)", who);
     if (out->type != L2_F32 && out->type != q->type) return fail(L2_EINVAL, "%s: out must be of q's type or f32", who);
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);
     int sms;

@@ -13,7 +13,7 @@ namespace l2 {
 
 struct KvPool {  // l2_kv_pages as the kernels take it
     char* k; char* v;
-    float* ks; float* vs;
+    float* ks; float* vs;  // L2_U4: words of 32 bits, see kv_pair_scale
     int64_t page_stride, pos_stride, head_stride;  // elements
     int n_pages, page_shift, n_kv_heads;
 };
@@ -45,6 +45,11 @@ struct KvSeq { int row0, n, kv; };
 #ifdef __CUDACC__
 // (The kernels are launched programmatically: lengths and tables may be written by the kernel in front, for whose end they wait, so nothing here is read through
 // the read-only path.)
+// L2_U4: a position's pair of bf16, the scale in the low half of the word, the zero in the high one
+__device__ __forceinline__ float kv_pair_scale(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float kv_pair_zero(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ bool kv_pair_not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+
 __device__ __forceinline__ void kv_report(int* status, int bit) { if (status) atomicOr(status, bit); }
 
 __device__ __forceinline__ KvSeq kv_seq(const KvStep& s, int page_shift, int b) {

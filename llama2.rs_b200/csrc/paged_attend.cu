@@ -21,14 +21,16 @@ cudaError_t kv_map(CUtensorMap* map, const KvPool& p, const void* base, int type
         encode = reinterpret_cast<Encode>(f);
         known.store(encode, std::memory_order_release);
     }
-    const int size = type == L2_I8 ? 1 : 2, page = 1 << p.page_shift;
-    const cuuint64_t dims[4] = {(cuuint64_t)head_size, (cuuint64_t)page, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)p.pos_stride * size, (cuuint64_t)p.head_stride * size, (cuuint64_t)p.page_stride * size};
-    const cuuint32_t box[4] = {(cuuint32_t)std::min(head_size, 128 / size), (cuuint32_t)std::min(page, tile), 1, 1}, step[4] = {1, 1, 1, 1};
+    const bool bytes = type == L2_I8 || type == L2_U4;  // elements of the tensor, two of the cache in one of L2_U4
+    const int size = bytes ? 1 : 2, per = type == L2_U4 ? 2 : 1, page = 1 << p.page_shift, row = head_size / per * size;
+    const cuuint64_t dims[4] = {(cuuint64_t)(head_size / per), (cuuint64_t)page, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(p.pos_stride / per) * size, (cuuint64_t)(p.head_stride / per) * size, (cuuint64_t)(p.page_stride / per) * size};
+    const cuuint32_t box[4] = {(cuuint32_t)(std::min(row, 128) / size), (cuuint32_t)std::min(page, tile), 1, 1}, step[4] = {1, 1, 1, 1};
     // (A row of 256 bytes comes in two copies: the first brings both halves to the L2, 115 -> 112 us for 672 MB of them; rows of 128 take 112 us as they are, 125 in pairs.)
-    const CUresult r = encode(map, type == L2_I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == L2_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+    const CUresult r = encode(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == L2_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                               const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              head_size * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, head_size * size == 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              row == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              row == 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 

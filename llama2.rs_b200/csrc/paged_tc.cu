@@ -40,6 +40,7 @@
 #include "kernels.cuh"
 #include "paged_attend.h"
 #include "paged_device.cuh"
+#include "paged_rows4.cuh"
 
 namespace l2 {
 
@@ -53,13 +54,14 @@ constexpr int KT_SCALE_SLOTS = 4;
 constexpr int KT_SETUP = 4;
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
+// WIDE, of a cache in 4 bits: see kt_held
 template <int CT, int HD>
 struct KtShape {
-    static constexpr bool I8 = CT == L2_I8;
+    static constexpr bool I8 = CT == L2_I8, U4 = CT == L2_U4, WIDEN = I8 || U4;  // WIDEN: tiles come as bytes, and helpers make numbers of 16 bits of them
     static constexpr int SLOT = KT_TILE * HD * 2;                     // K or V of a tile in 16 bits
-    static constexpr int RAW = I8 ? KT_TILE * HD : 0;                 // ... in 8
-    static constexpr int SLOTS = HD == 64 ? 6 : I8 ? 3 : 5, RAWS = I8 ? (HD == 64 ? 4 : 3) : 0;
-    static constexpr int SCALES = I8 ? KT_SCALE_SLOTS * 2 * KT_TILE * 4 : 0;
+    static constexpr int RAW = WIDEN ? KT_TILE * HD / (U4 ? 2 : 1) : 0;  // ... in 8 or 4
+    static constexpr int SLOTS = HD == 64 ? 6 : I8 ? 3 : U4 ? 4 : 5, RAWS = WIDEN ? (HD == 64 ? 4 : 3) : 0;
+    static constexpr int SCALES = WIDEN ? KT_SCALE_SLOTS * 2 * KT_TILE * 4 : 0;
     static constexpr int Q_BYTES = 2 * SLOT;
     // (always more than half of an SM's shared memory: one CTA, one owner of the tensor memory, per SM)
     static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + SCALES > 120 * 1024 ? 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + SCALES : 120 * 1024;
@@ -140,6 +142,57 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
 // byte offset of 16-byte chunk c of row r in a tile of 128 rows: halves of 128 bytes one after the other, 128-byte swizzle (rows of 64 bytes: 64-byte swizzle)
 __device__ __forceinline__ uint32_t kt_offset(int r, int c) { return (c >> 3) * (KT_TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 __device__ __forceinline__ uint32_t kt_offset64(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
+__device__ __forceinline__ uint32_t kt_offset32(int r, int c) { return r * 32 + ((c ^ ((r >> 2) & 1)) << 4); }
+
+// ---- numbers of 4 bits as values of 16 ------------------------------------------------------------------------------------------
+// zero + scale u, rounded once, to f16: K, V, Q (a row of bf16 times a power of two) and the probabilities all go through the products in it.  Where some row sees
+// a pair that f16 does not hold, the CTA says so, and the launch behind this one, which else returns at once, does the call again in bf16 (WIDE): three bits less, and
+// f32's range.  (All of them in bf16 in the first place: errors of 0.0046 relative to the result where f16 has 0.0018.)
+// A word's eight elements come out as (0, 4), (1, 5), (2, 6), (3, 7): Q is brought in that order, and O is read in it.
+__device__ __forceinline__ uint4 kt_order(uint4 w) {
+    return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
+}
+__device__ constexpr int kt_place(int d) { return (d & ~7) | (d & 3) << 1 | (d >> 2 & 1); }  // where element d is
+template <bool BF>
+__device__ __forceinline__ uint32_t fma16(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    if constexpr (BF) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ uint4 kt_values(uint32_t w, uint32_t scale, uint32_t zero) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t u = (w >> (4 * i)) & 0x000f000fu;  // 0x4300 | u is 128 + u in bf16, 0x6400 | u 1024 + u in f16
+        if constexpr (BF) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(u | 0x43004300u), "r"(0x43004300u));
+        else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(u) : "r"(u | 0x64006400u), "r"(0x64006400u));
+        r[i] = fma16<BF>(u, scale, zero);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// Whether f16 holds the values of a pair to 2^-12 of the larger ones of a head, or as well as its steps of 2^-24 do where those are small beside the pair's own (2^-16 or more).
+__device__ __forceinline__ bool kt_held(float scale, float zero) {
+    const float s = fabsf(scale), z = fabsf(zero);
+    return z + 15.0f * s <= 65504.0f && (s >= 0x1p-16f || (s == 0.0f && (z == 0.0f || z >= 0x1p-14f)));
+}
+// Eight elements of Q in f16 (BF: a row of bf16, times `up`) or, WIDE, in bf16.
+template <bool BF, bool WIDE>
+__device__ __forceinline__ uint4 kt_query(uint4 x, float up) {
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (BF && !WIDE) w[i] = pack16<false>(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
+        if constexpr (!BF && WIDE) w[i] = pack16<true>(__half2float(__ushort_as_half((unsigned short)w[i])), __half2float(__ushort_as_half((unsigned short)(w[i] >> 16))));
+    }
+    return kt_order(make_uint4(w[0], w[1], w[2], w[3]));
+}
+// Whether some value of a pair of V is not finite in bf16: the position is then taken as NaN.
+__device__ __forceinline__ bool kt_bad_pair(uint32_t pair) {
+    const uint32_t zero = pair >> 16, last = fma16<true>(0x4170u, pair & 0xffffu, zero);  // (0x4170 is 15)
+    return not_finite<true>(zero | last << 16) != 0;
+}
 
 // ---- the line: sequence by sequence, kv head by kv head, block by block, tile by tile ---------------------------------------
 struct KtBlocks { KvSeq s; int tokens, n; };  // blocks of a sequence, of `tokens` tokens; n = 0: not this kernel's
@@ -278,23 +331,27 @@ struct KtPiece {
 };
 constexpr int KT_PIECES = 4;
 
-template <int CT, bool QB, int HD>
+// QB: q is bf16, else f16.  gate: of a WIDE launch, what the CTAs of the launch in front say (see kt_held); else where they say it
+template <int CT, bool QB, int HD, bool WIDE>
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
-                                                              const __grid_constant__ CUtensorMap map_v) {
+                                                              const __grid_constant__ CUtensorMap map_v, int* const gate) {
     using S = KtShape<CT, HD>;
-    constexpr bool I8 = S::I8, PB = I8 || QB;
+    constexpr bool I8 = S::I8, U4 = S::U4, WIDEN = S::WIDEN;
+    constexpr bool KB = U4 ? WIDE : QB, PB = U4 ? WIDE : I8 || QB;  // K and Q, V and the probabilities go through the products in bf16
     constexpr int LANES = HD / 8;
     constexpr uint32_t S_COL = 0, O_COL = 256;                   // tensor memory: S0 S1 O0 O1, 128 columns each; P over S
     // Probabilities carry a factor of 2^BIAS, so that small ones are normal numbers: f16 at most 2^(7 + KT_RAISE); f32 and bf16 have room (2^95 for a V).
     constexpr float BIAS = PB ? 24.0f : 7.0f;
     extern __shared__ __align__(1024) uint8_t kt_smem[];
-    __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[I8 ? S::RAWS : 1], raw_empty[I8 ? S::RAWS : 1],
+    __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[WIDEN ? S::RAWS : 1], raw_empty[WIDEN ? S::RAWS : 1],
         sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
     __shared__ int64_t scratch[KT_THREADS / 32 + 2];
     __shared__ __align__(8) uint64_t piece_full[KT_PIECES], piece_empty[KT_PIECES], row_meet[2];
     __shared__ KtPiece pieces[KT_PIECES];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
+    __shared__ volatile int not_held;  // 4 bits: some row sees a pair that f16 does not hold
+    __shared__ float q_by[U4 ? KT_ROWS : 1];  // 4 bits: of a row of Q, the inverse of its power of two
     __shared__ volatile int odd[8];  // by piece: values that are not finite have been taken out of a V tile
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem) + 1023) & ~(uintptr_t)1023);  // Q0, Q1
     uint8_t* ring = sq + S::Q_BYTES;
@@ -302,15 +359,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     float* scales = reinterpret_cast<float*>(raw + S::RAWS * S::RAW);  // [slot][k, v][position]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if constexpr (U4 && WIDE) {  // (nearly always there is nothing to do)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!__syncthreads_or(tid < gridDim.x && gate[tid] != 0)) return;
+    }
     // (Code that runs once comes from far away, 100 clocks and more for eight instructions: every warp prepares a little.)
-    if (warp == 4 && lane < S::SLOTS) { kv_bar_init(&full[lane], I8 ? 4 : 1); kv_bar_init(&empty[lane], I8 ? 2 : 6); kv_bar_init(&ready[lane], 4); }
-    if (I8 && warp == 5 && lane < S::RAWS) { kv_bar_init(&raw_full[lane], 1); kv_bar_init(&raw_empty[lane], 4); }
-    if (I8 && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], 8); }
+    if (warp == 4 && lane < S::SLOTS) { kv_bar_init(&full[lane], WIDEN ? 4 : 1); kv_bar_init(&empty[lane], WIDEN ? 2 : 6); kv_bar_init(&ready[lane], 4); }
+    if (WIDEN && warp == 5 && lane < S::RAWS) { kv_bar_init(&raw_full[lane], 1); kv_bar_init(&raw_empty[lane], 4); }
+    if (WIDEN && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], I8 ? 8 : 4); }  // (read by the softmax; by the helpers)
     if (warp == 7 && lane < KT_PIECES) { kv_bar_init(&piece_full[lane], 1); kv_bar_init(&piece_empty[lane], 15); }
     if (warp == 8 && lane < 2) { kv_bar_init(&q_full[lane], 128); kv_bar_init(&drained[lane], 1); kv_bar_init(&row_meet[lane], 4); }
     if (warp == 9 && lane < 4) { kv_bar_init(&s_full[0][0] + lane, 1); kv_bar_init(&p_full[0][0] + lane, 4); kv_bar_init(&pv_done[0][0] + lane, 1); }
     if (warp == 10 && lane < 8) odd[lane] = 0;
-    if (tid == 0) failed = 0;
+    if (tid == 0) { failed = 0; not_held = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == KT_MMA_WARP) {  // all 512 columns of tensor memory
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_smem(&tmem_s)) : "memory");
@@ -371,9 +432,32 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             for (int t = t0; t < t1 && !some; t += 32) some = walk.bits(t, any);
             if (some) {  // Q, swizzled as the products want it
 #pragma unroll
-                for (int n = 0; n < Q_N; n++) *reinterpret_cast<uint4*>(sq + i * S::SLOT + kt_offset((tid & 127) / LANES + n * Q_ROWS, tid % LANES)) = qx[n];
+                for (int n = 0; n < Q_N; n++) {
+                    if constexpr (U4) {
+                        float up = 1.0f, by = 1.0f;
+                        if constexpr (QB && !WIDE) {
+                            const uint32_t w[4] = {qx[n].x, qx[n].y, qx[n].z, qx[n].w};
+                            float top = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+#pragma unroll
+                            for (int x = 1; x < LANES; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                            kr4_q_factors(top, &up, &by);
+                        }
+                        if (tid % LANES == 0) q_by[128 * i + (tid & 127) / LANES + n * Q_ROWS] = by;
+                        qx[n] = kt_query<QB, WIDE>(qx[n], up);
+                    }
+                    *reinterpret_cast<uint4*>(sq + i * S::SLOT + kt_offset((tid & 127) / LANES + n * Q_ROWS, tid % LANES)) = qx[n];
+                }
                 fence_async();
                 kv_bar_arrive(&q_full[i]);
+            }
+            float by_row = P.scale_log2;
+            if constexpr (U4 && QB && !WIDE) {
+                if (some) {
+                    meet();
+                    by_row *= q_by[row];
+                }
             }
             float m = -INFINITY, l = 0.0f;
             int seen = 0;      // halves of tiles seen
@@ -431,7 +515,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     for (int j = 0; j < KT_SUB; j += 8)
 #pragma unroll
                         for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c])));
-                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale_log2 - BIAS;
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by_row - BIAS;
                     const bool raise = most > m + KT_RAISE;
                     if (__any_sync(0xffffffffu, raise)) {
                         const float m1 = raise ? most : m;  // (a row's result does not depend on the others of its warp)
@@ -454,7 +538,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         }
                     }
                     const float ref = m == -INFINITY ? 0.0f : m;
-                    const unsigned long long f2 = pair(P.scale_log2, P.scale_log2), r2 = pair(-ref, -ref);
+                    const unsigned long long f2 = pair(by_row, by_row), r2 = pair(-ref, -ref);
                     unsigned long long sum[2] = {0ull, 0ull};
                     auto probabilities = [&](auto is_whole) {  // (an int8 cache with the choice at every element: 378 us instead of 362)
                         uint32_t p16[KT_SUB / 2];
@@ -501,6 +585,21 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             }
             if (128 * i >= walk.rows) { give_back(n); continue; }  // (this tile has no rows)
             const bool fix = !I8 && started && odd[walk.index & 7];
+            bool none = false;  // 4 bits: the row sees a position of V that is taken as NaN
+            if (U4 && fix) {
+#pragma unroll 1
+                for (int t = walk.t0; t < walk.t1; t++) {
+                    const int base = walk.base(t);
+                    if (!mine.any(base, KT_TILE, P.window, P.sinks)) continue;
+#pragma unroll 1
+                    for (int j = base; j < base + KT_TILE; j++) {
+                        if (!kv_sees(pos, j, P.window, P.sinks)) continue;
+                        const int page = kv_page(P.step, P.pool, walk.b, j);
+                        if (page < 0) continue;
+                        none |= kt_bad_pair(reinterpret_cast<const uint32_t*>(P.pool.vs)[((int64_t)page * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + (j & ((1 << P.pool.page_shift) - 1))]);
+                    }
+                }
+            }
             float* part = kv_part(P.work, gridDim.x, KT_ROWS, HD, blockIdx.x, walk.index ? 1 : 0);
             const float inv = done && pos >= 0 ? 1.0f / l : 1.0f;
             // A whole block's result goes through this tile's room of Q (its products are done), so that rows leave in whole lines.
@@ -514,7 +613,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 #pragma unroll
                     for (int j = 0; j < 32; j++) o[j] = 0u;
                 }
-                if constexpr (!I8) {
+                if constexpr (U4) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] = none ? 0x7fc00000u : o[kt_place(j)];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] = x[j];
+                }
+                if constexpr (!WIDEN) {
                     if (fix) {  // rare: the values that were taken out, one by one, to the rows that see them
 #pragma unroll 1
                         for (int t = walk.t0; t < walk.t1; t++) {
@@ -587,7 +693,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             // (All of the tensor memory is this CTA's: it starts at 0.  The operands are uniform registers: the whole warp walks, one elected lane issues.)
             const int i = warp == KT_MMA_WARP ? 0 : 1;
             const bool leader = elect();
-            constexpr uint32_t fmt = QB ? 1u : 0u, fmt_p = PB ? 1u : 0u;
+            constexpr uint32_t fmt = KB ? 1u : 0u, fmt_p = PB ? 1u : 0u;
             constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (((uint32_t)KT_SUB >> 3) << 17) | ((128u >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | (fmt_p << 7) | (fmt_p << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);  // V: elements contiguous
             const uint32_t s_col = S_COL + 128 * i, o_col = O_COL + 128 * i, q_lo = desc_lo(kv_smem(sq + i * S::SLOT), 1), k_lo = desc_lo(kv_smem(ring), 1),
@@ -625,7 +731,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 step();
 #pragma unroll 1
                 for (int tc = t0; tc < t1; tc += 32) {
-                    const uint32_t part = I8 ? 0u : walk.bits(tc, [&](int base) {
+                    const uint32_t part = WIDEN ? 0u : walk.bits(tc, [&](int base) {
                         return (any(base) && !mine.whole(base, P.window, P.sinks)) || (other.any(base, KT_TILE, P.window, P.sinks) && !other.whole(base, P.window, P.sinks)); });
                     on = walk.bits(tc, any);
                     const uint32_t next = walk.bits(tc + 1, any);
@@ -676,7 +782,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
         } else if (warp == KT_COPY_WARP) {
             // ================= copies: lane l brings run l of a tile ==============================================================
             const int R = min(KT_TILE, 1 << P.pool.page_shift), runs = KT_TILE / R;
-            constexpr int RB = HD * (I8 ? 1 : 2), W = RB < 128 ? RB : 128;  // bytes of a row, of a copy's row
+            constexpr int RB = U4 ? HD / 2 : HD * (I8 ? 1 : 2), W = RB < 128 ? RB : 128;  // bytes of a row, of a copy's row
             uint32_t slot = 0, ph = 1, sc = 0, sc_ph = 1;
             bool over = false;
             for (uint32_t n = 0; !over; n++) {
@@ -694,7 +800,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 for (int t = t0; t < t1; t++) {
                     const int j = view.base(t) + lane * R, at = j & ((1 << P.pool.page_shift) - 1);
                     const int ahead = t + 1 < t1 ? page_of(t + 1) : P.pool.n_pages;
-                    if constexpr (I8) {
+                    if constexpr (WIDEN) {
                         wait(&sc_empty[sc], sc_ph);
                         if ((over = wait.over())) break;
                         // four positions a lane, of K and of V
@@ -709,17 +815,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     }
 #pragma unroll
                     for (int kv = 0; kv < 2; kv++) {
-                        uint64_t *f = I8 ? &raw_full[slot] : &full[slot], *e = I8 ? &raw_empty[slot] : &empty[slot];
+                        uint64_t *f = WIDEN ? &raw_full[slot] : &full[slot], *e = WIDEN ? &raw_empty[slot] : &empty[slot];
                         wait(e, ph);
                         if ((over = wait.over())) break;
                         if (lane == 0) kv_bar_expect(f, KT_TILE * RB);
                         __syncwarp();
                         if (lane < runs) {
-                            const uint32_t to = kv_smem(I8 ? raw + slot * S::RAW : ring + slot * S::SLOT) + lane * R * W;
+                            const uint32_t to = kv_smem(WIDEN ? raw + slot * S::RAW : ring + slot * S::SLOT) + lane * R * W;
 #pragma unroll
                             for (int h = 0; h < RB / W; h++) kv_tma4(to + h * (KT_TILE * 128), kv ? &map_v : &map_k, h * 64, at, head, page, f);
                         }
-                        if (++slot == (I8 ? S::RAWS : S::SLOTS)) { slot = 0; ph ^= 1u; }
+                        if (++slot == (WIDEN ? S::RAWS : S::SLOTS)) { slot = 0; ph ^= 1u; }
                     }
                     if (over) break;
                     page = ahead;
@@ -804,6 +910,66 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     }
                     give_back(n);
                 }
+            } else if constexpr (U4) {
+                // ================= numbers of 4 bits to values of 16: a position a thread =======================================
+                uint32_t rs = 0, rph = 0, slot = 0, ph = 1, sc = 0, sc_ph = 0;
+                for (uint32_t n = 0;; n++) {
+                    const KtPiece& walk = piece_at(n);
+                    if (!is_one(walk)) break;
+                    if (tid == KT_HELP_WARP * 32) odd[(walk.index + 4) & 7] = 0;  // (a piece to come)
+                    uint32_t pair = 0;
+                    int t = walk.t0;
+                    bool seen = false;  // some row of the block sees the position.  (The rest of a page may hold anything.)
+#pragma unroll 1
+                    for (int left = 2 * (walk.t1 - walk.t0), kv = 0; left > 0; left--, kv ^= 1) {
+                        if (!kv) {
+                            wait(&sc_full[sc], sc_ph);
+                            seen = walk.view(walk.lo_pos, walk.hi_pos).any(walk.base(t++) + r, 1, P.window, P.sinks);
+                        }
+                        wait(&raw_full[rs], rph);
+                        wait(&empty[slot], ph);
+                        __syncwarp();
+                        pair = reinterpret_cast<const uint32_t*>(scales)[(2 * sc + kv) * KT_TILE + r];
+                        if (kv) {
+                            __syncwarp();
+                            if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
+                            if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
+                        }
+                        const uint8_t* from = raw + rs * S::RAW;
+                        uint8_t* to = ring + slot * S::SLOT;
+                        auto turn = [&](auto values) {
+#pragma unroll
+                            for (int c = 0; c < HD / 32; c++) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(from + (HD == 64 ? kt_offset32(r, c) : kt_offset64(r, c)));
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 4 * c)) = values(w.x);
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 4 * c + 1)) = values(w.y);
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 4 * c + 2)) = values(w.z);
+                                *reinterpret_cast<uint4*>(to + kt_offset(r, 4 * c + 3)) = values(w.w);
+                            }
+                        };
+                        if (!seen) pair = 0;
+                        if (kv && kt_bad_pair(pair)) {  // rare: 0 x NaN is NaN, and a row must not be reached by what it does not see; rows that see it are mended at the end
+                            pair = 0;
+                            odd[walk.index & 7] = 1;
+                            __threadfence_block();
+                        }
+                        if constexpr (WIDE) {
+                            const uint32_t scale = __byte_perm(pair, 0, 0x1010), zero = __byte_perm(pair, 0, 0x3232);
+                            turn([&](uint32_t w) { return kt_values<true>(w, scale, zero); });
+                        } else {
+                            const float s = kv_pair_scale(pair), z = kv_pair_zero(pair);
+                            if (!kt_held(s, z) && !(kv_pair_not_finite(pair))) not_held = 1;
+                            const uint32_t scale = pack16<false>(s, s), zero = pack16<false>(z, z);
+                            turn([&](uint32_t w) { return kt_values<false>(w, scale, zero); });
+                        }
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) { kv_bar_arrive(&raw_empty[rs]); kv_bar_arrive(&full[slot]); }
+                        if (++rs == (uint32_t)S::RAWS) { rs = 0; rph ^= 1u; }
+                        if (++slot == (uint32_t)S::SLOTS) { slot = 0; ph ^= 1u; }
+                    }
+                    give_back(n);
+                }
             } else {
                 // ================= V tiles that some row sees in part: only finite values stay ===================================
                 // (they see every slot of the ring and give it back with the products: neither can be a round ahead of the other)
@@ -854,8 +1020,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     }
     fence_before();
     __syncthreads();
+    if constexpr (U4 && !WIDE) {
+        if (tid == 0) gate[blockIdx.x] = not_held;
+    }
     if (failed) {  // copies may still be on their way into this CTA's shared memory: a bounded time to land
-        uint64_t* bar = tid < S::SLOTS ? &full[tid] : tid < S::SLOTS + S::RAWS ? &raw_full[tid - S::SLOTS] : tid < S::SLOTS + S::RAWS + KT_SCALE_SLOTS && I8 ? &sc_full[tid - S::SLOTS - S::RAWS] : nullptr;
+        uint64_t* bar = tid < S::SLOTS ? &full[tid] : tid < S::SLOTS + S::RAWS ? &raw_full[tid - S::SLOTS] : tid < S::SLOTS + S::RAWS + KT_SCALE_SLOTS && WIDEN ? &sc_full[tid - S::SLOTS - S::RAWS] : nullptr;
         if (bar)
             for (int i = 0; i < 64; i++) { kv_bar_try(bar, 0); kv_bar_try(bar, 1); }
         if (tid == 0) kv_report(P.step.status, L2_KV_TIMEOUT);
@@ -912,10 +1081,13 @@ bool kt_needed(const KvStep& s, int group) { return (int64_t)s.max_rows * group 
 
 }  // namespace
 
+// behind the cuts and the pieces: a word a CTA, see kt_held
+static size_t kt_gate_offset(int grid, int head_size) { return kv_cut_bytes(grid) + (size_t)grid * 2 * KT_ROWS * (head_size + 2) * sizeof(float); }
+
 size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
     if (!kt_needed(s, group)) return 0;
     const int grid = kt_grid(s, p, group, sms);
-    return kv_cut_bytes(grid) + (size_t)grid * 2 * KT_ROWS * (head_size + 2) * sizeof(float);
+    return kt_gate_offset(grid, head_size) + (size_t)grid * sizeof(int);
 }
 
 cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
@@ -924,17 +1096,26 @@ cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int s
     CUtensorMap mk, mv;
     if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, KT_TILE)) return e;
     if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, KT_TILE)) return e;
-    auto go = [&](auto t, auto b, auto h) {
+    int* const gate = reinterpret_cast<int*>(static_cast<char*>(p.work) + kt_gate_offset(grid, head_size));
+    auto launch = [&](auto t, auto b, auto h, auto wide) {
         constexpr int T = decltype(t)::value, HD = decltype(h)::value;
-        auto kernel = kv_tc_kernel<T, decltype(b)::value, HD>;
+        auto kernel = kv_tc_kernel<T, decltype(b)::value, HD, decltype(wide)::value>;
         static KvOnce once;
         if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), KtShape<T, HD>::SMEM)) return x;
-        return kv_launch(kernel, dim3(grid), KT_THREADS, KtShape<T, HD>::SMEM, st, p, lim, mk, mv);
+        return kv_launch(kernel, dim3(grid), KT_THREADS, KtShape<T, HD>::SMEM, st, p, lim, mk, mv, gate);
+    };
+    auto go = [&](auto t, auto b, auto h) {
+        cudaError_t x = launch(t, b, h, std::false_type());
+        if constexpr (decltype(t)::value == L2_U4) {
+            if (x == cudaSuccess) x = launch(t, b, h, std::true_type());
+        }
+        return x;
     };
     auto by_hd = [&](auto t, auto b) { return head_size == 128 ? go(t, b, std::integral_constant<int, 128>()) : go(t, b, std::integral_constant<int, 64>()); };
     const bool qb = p.q.type == L2_BF16;
     const cudaError_t e = type == L2_F16 ? by_hd(std::integral_constant<int, L2_F16>(), std::false_type())
                         : type == L2_BF16 ? by_hd(std::integral_constant<int, L2_BF16>(), std::true_type())
+                        : type == L2_U4 ? qb ? by_hd(std::integral_constant<int, L2_U4>(), std::true_type()) : by_hd(std::integral_constant<int, L2_U4>(), std::false_type())
                         : qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
     if (e != cudaSuccess) return e;
     auto combine = head_size == 128 ? kv_tc_combine_kernel<128> : kv_tc_combine_kernel<64>;

@@ -2,6 +2,7 @@
 
     pages = KvPages(k, v)                                   # [n_pages, page_size, kv_heads, head_size], f16 or bf16
     pages = KvPages(k, v, k_scale, v_scale)                 # int8, scales [n_pages, kv_heads, page_size] f32
+    pages = KvPages(k, v, k_scale, v_scale)                 # 4 bits: uint8 [.., head_size / 2], scales [n_pages, kv_heads, page_size, 2] bf16
     batch = KvBatch(page_table, kv_len, row_start, n_rows, max_rows)   # one step, for all layers
     pages.append(batch, k_rows, v_rows, rope=KvRope(4096), q=q_rows, q_out=q16)
     pages.attend(batch, q16, out, window=4096, sinks=4)
@@ -17,9 +18,9 @@ import sys
 
 from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, as_f32p, check, lib
 
-F32, F16, BF16, I8, I32 = 0, 1, 2, 3, 4
+F32, F16, BF16, I8, U4, I32 = 0, 1, 2, 3, 4, 5
 BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
-_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.int32": I32}
+_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.uint8": U4, "torch.int32": I32}
 _types = {}  # the same by dtype object, filled as they are seen
 _ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
 _ROTATIONS = {"pairs": 0, "model": 1}  # L2_ROPE_*
@@ -103,7 +104,8 @@ class KvRope(tuple):
 
 class KvPages:
     """The pages of one layer's cache: k and v of one shape and one set of strides, [n_pages, page_size, kv_heads, head_size] (layout "NHD") or
-    [n_pages, kv_heads, page_size, head_size] ("HND"), f16, bf16 or int8 (with scales)."""
+    [n_pages, kv_heads, page_size, head_size] ("HND"), f16, bf16 or int8 (with scales); or uint8 with head_size / 2 for its last dimension: 4 bits, the
+    element of even index in the low half of a byte, and scales [n_pages, kv_heads, page_size, 2] in bf16, (scale, zero): value = zero + scale * stored."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None, layout="NHD"):
         if layout not in ("NHD", "HND"):
@@ -115,17 +117,19 @@ class KvPages:
             raise ValueError("k and v: the same shape, type and strides, the last dimension contiguous")
         at, head = (1, 2) if layout == "NHD" else (2, 1)
         self.n_pages, self.page_size, self.n_kv_heads, self.head_size = k.shape[0], k.shape[at], k.shape[head], k.shape[3]
+        kind, per = _type(k), 1
+        if kind == U4:  # two elements a byte: sizes and strides are in elements
+            per, self.head_size = 2, 2 * self.head_size
         _int32(n_pages=self.n_pages, page_size=self.page_size, n_kv_heads=self.n_kv_heads)
-        kind = _type(k)
         scales = [None, None]
-        if kind == I8:
+        if kind in (I8, U4):
             if k_scale is None or v_scale is None:
-                raise ValueError("an int8 cache needs k_scale and v_scale")
-            shape = (self.n_pages, self.n_kv_heads, self.page_size)
-            scales = [_packed(s, "scales", self.device, shape, F32) for s in (k_scale, v_scale)]
+                raise ValueError("an int8 or 4-bit cache needs k_scale and v_scale")
+            shape = (self.n_pages, self.n_kv_heads, self.page_size) + (2,) * (kind == U4)
+            scales = [_packed(s, "scales", self.device, shape, F32 if kind == I8 else BF16) for s in (k_scale, v_scale)]
         elif k_scale is not None or v_scale is not None:
-            raise ValueError("scales belong to an int8 cache")
-        self._args = KvPagesArgs(k.data_ptr(), v.data_ptr(), scales[0], scales[1], k.stride(0), k.stride(at), k.stride(head), kind,
+            raise ValueError("scales belong to an int8 or 4-bit cache")
+        self._args = KvPagesArgs(k.data_ptr(), v.data_ptr(), scales[0], scales[1], per * k.stride(0), per * k.stride(at), per * k.stride(head), kind,
                                  self.n_pages, self.page_size, self.n_kv_heads, self.head_size)
         self._ref = C.byref(self._args)
         self._keep = (k, v, k_scale, v_scale)
