@@ -270,6 +270,7 @@ typedef struct l2_kv_batch {
                               l2_kv_attend takes it as the nearest of them (its rows then see what the table holds) */
 #define L2_KV_BAD_ROWS 4   /* row_start not ascending, outside 0 .. n_rows or more than max_rows apart: that sequence brings no rows */
 #define L2_KV_BAD_ROPE 8   /* a position beyond the rope table: its rows are left out */
+#define L2_KV_NO_ROOM 32   /* l2_kv_plan: more rows than n_rows or more pages than are free; nothing changes, no sequence brings rows */
 #define L2_KV_TIMEOUT 16   /* a bounded wait inside a kernel gave up: the call's results are not valid */
 
 /* An array [row][head][head_size]: element d of (row, head) at row * row_stride + head * head_stride + d; strides multiples of 16 bytes.  Rows that a
@@ -311,6 +312,56 @@ int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv
 /* Bytes of device scratch that l2_kv_attend needs for such a batch (contents need not be kept between calls; calls that may overlap
  * need one each), 0 where the arguments are not valid. */
 size_t l2_kv_attend_workspace_bytes(const l2_kv_pages* pages, const l2_kv_batch* batch, int n_heads);
+
+/* ---- tables of a step on the device (no counterpart in the reference) ------------------------------------------------------------
+ *
+ * Who has which pages: a table of every sequence, its length, and a list of free pages, all in device memory of the caller's, so that steps can be planned
+ * without the host and captured in a graph.  A page is in one table or in the list.  Calls on the same arrays are ordered by the caller, as by one stream.
+ * What cannot be is reported in the status word, as by the calls above: L2_KV_BAD_LENGTH, a length (or length to keep) outside 0 .. table_width * page_size, before or after the
+ * step: the sequence brings no rows and stays as it is; L2_KV_BAD_ROWS, new rows outside 0 .. max_rows: it brings none; L2_KV_BAD_PAGE, an entry that is no page (and not -1) where one
+ * is needed, taken as none (-1), *free_count outside 0 .. n_pages, taken as the nearest, or more pages given back than there are, of which the rest is dropped. */
+typedef struct l2_kv_tables {
+    int32_t* page_table;  /* [n_seqs][table_width] */
+    int32_t* kv_len;      /* [n_seqs]: positions held */
+    int32_t* free_pages;  /* [n_pages]: the first *free_count are free; taken from the end */
+    int32_t* free_count;  /* one */
+    int32_t* status;      /* as in l2_kv_batch, or NULL */
+    int32_t n_seqs, table_width;
+    int32_t n_pages;
+    int32_t page_size;    /* as in l2_kv_pages */
+} l2_kv_tables;
+
+/* A step in which sequence b brings new_rows[b] more rows (0: none), at most max_rows each and n_rows in all: row_start [n_seqs + 1] as in l2_kv_batch, kv_len grown, page_table
+ * with pages from the list for what is new, in the order of the sequences.  For each of n_rows rows, where wanted (NULL: not): slots, page * page_size + position % page_size,
+ * and positions, its position in the sequence; both -1 behind the last row.  All or nothing: see L2_KV_NO_ROOM. */
+int l2_kv_plan(const l2_kv_tables* tables, const int32_t* new_rows, int32_t* row_start, int64_t* slots, int32_t* positions, int n_rows, int max_rows, void* cuda_stream);
+/* Sequence b keeps its first keep[b] positions (0: it has ended; as many as it has or more: all; keep NULL: all of all), and where window > 0 only pages that rows
+ * from there on can see, with that window and so many sinks.  The others' entries become -1 and the pages go to the list, the last one taken first: a release of what a plan has added
+ * leaves everything as it was.  (A sequence that is cut back into pages which a window has given back does not get them again: rows that go there find none, L2_KV_BAD_PAGE.) */
+int l2_kv_release(const l2_kv_tables* tables, const int32_t* keep, int window, int sinks, void* cuda_stream);
+
+/* ---- norms before and after a block (src/model.rs:22-31 on device rows, with what stands around it) --------------------------------------------
+ *
+ * For each of `rows` rows of `dim` elements, with norm(x) = x / sqrt(mean(x^2) + eps):
+ *   t = norm(block) * post_weight       (post_weight NULL: t = block)
+ *   r = residual + scale * gate * t     (residual NULL: 0; gate NULL: 1; block NULL: r = residual)
+ *   residual_out = r,  out = norm(r) * pre_weight     (pre_weight NULL: 1)
+ * in f32, each result rounded once to its array's type; out goes by r before it is rounded.  residual_out may be residual itself and out may be block itself (same data, strides
+ * and type); results otherwise overlap nothing.  A row stride of 0 in block, residual or gate: one row for all.  One of residual_out and out may be absent. */
+typedef struct l2_rows {
+    void* data;          /* element e of row i at i * row_stride + e; NULL: absent */
+    int64_t row_stride;  /* in elements */
+    int32_t type;        /* L2_F32, L2_F16 or L2_BF16 */
+} l2_rows;
+typedef struct l2_block_norm_args {
+    l2_rows block, residual, gate, residual_out, out;
+    const float* post_weight;  /* [dim] */
+    const float* pre_weight;   /* [dim] */
+    float scale, eps;
+    int32_t rows;
+    int32_t dim;               /* 1 to 32768 */
+} l2_block_norm_args;
+int l2_block_norm(const l2_block_norm_args* args, void* cuda_stream);
 
 /* ---- measurement hooks (no counterpart in the reference, which times whole runs only,
  *      src/main.rs:61-65) --------------------------------------------------------------- */

@@ -21,6 +21,25 @@
 
 namespace l2 {
 
+int kv_device(int* sms) {
+    static std::atomic<int> known[64];  // SM counts of devices looked at before (zero: none yet)
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fail(L2_ECUDA, "no usable CUDA device (%s); this library has no CPU fallback", cudaGetErrorString(e));
+    if (dev < 0 || dev >= 64) return fail(L2_EINVAL, "device ordinal %d unsupported", dev);
+    int n = known[dev].load(std::memory_order_acquire);
+    if (!n) {
+        int major = 0;
+        const cudaError_t a = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+        if (a != cudaSuccess) return fail(L2_ECUDA, "no usable CUDA device (%s); this library has no CPU fallback", cudaGetErrorString(a));
+        if (major < 10) return fail(L2_ECUDA, "device %d: this library is built for sm_100a only", dev);
+        L2_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        known[dev].store(n, std::memory_order_release);
+    }
+    *sms = n;
+    return L2_OK;
+}
+
 namespace {
 
 constexpr int KV_THREADS = 256, KV_WARPS = KV_THREADS / 32, KV_MAX_ROWS = 16;
@@ -319,26 +338,6 @@ __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const __grid_con
         }
         __syncthreads();
     }
-}
-
-// SM count of the current device; L2_ECUDA where there is none that this library runs on.
-int kv_device(int* sms) {
-    static std::atomic<int> known[64];  // SM counts of devices looked at before (zero: none yet)
-    int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return fail(L2_ECUDA, "no usable CUDA device (%s); this library has no CPU fallback", cudaGetErrorString(e));
-    if (dev < 0 || dev >= 64) return fail(L2_EINVAL, "device ordinal %d unsupported", dev);
-    int n = known[dev].load(std::memory_order_acquire);
-    if (!n) {
-        int major = 0;
-        const cudaError_t a = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-        if (a != cudaSuccess) return fail(L2_ECUDA, "no usable CUDA device (%s); this library has no CPU fallback", cudaGetErrorString(a));
-        if (major < 10) return fail(L2_ECUDA, "device %d: this library is built for sm_100a only", dev);
-        L2_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        known[dev].store(n, std::memory_order_release);
-    }
-    *sms = n;
-    return L2_OK;
 }
 
 int elem_bits(int type) { return type == L2_F32 ? 32 : type == L2_I8 ? 8 : type == L2_U4 ? 4 : 16; }

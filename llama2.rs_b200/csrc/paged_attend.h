@@ -11,6 +11,9 @@
 
 namespace l2 {
 
+// SM count of the current device; L2_ECUDA where there is none that this library runs on (paged.cu).
+int kv_device(int* sms);
+
 // Sets a kernel's opt-in shared memory once per device (a static of the launch).
 struct KvOnce {
     std::atomic<uint64_t> done{0};

@@ -50,6 +50,23 @@ class KvRowsArgs(C.Structure):
     _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("type", C.c_int32), ("heads", C.c_int32)]
 
 
+class KvTablesArgs(C.Structure):
+    """l2_kv_tables."""
+    _fields_ = [("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("free_pages", C.c_void_p), ("free_count", C.c_void_p), ("status", C.c_void_p),
+                ("n_seqs", C.c_int32), ("table_width", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32)]
+
+
+class RowsArgs(C.Structure):
+    """l2_rows."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("type", C.c_int32)]
+
+
+class BlockNormArgs(C.Structure):
+    """l2_block_norm_args."""
+    _fields_ = [("block", RowsArgs), ("residual", RowsArgs), ("gate", RowsArgs), ("residual_out", RowsArgs), ("out", RowsArgs),
+                ("post_weight", C.c_void_p), ("pre_weight", C.c_void_p), ("scale", C.c_float), ("eps", C.c_float), ("rows", C.c_int32), ("dim", C.c_int32)]
+
+
 FLAG_NO_GRAPH = 1
 FLAG_NO_PDL = 2
 
@@ -106,6 +123,9 @@ SIGNATURES = {
     "l2_kv_read": (C.c_int, [_vp] * 5),
     "l2_kv_attend": (C.c_int, [_vp] * 4 + [C.c_float, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
     "l2_kv_attend_workspace_bytes": (C.c_size_t, [_vp, _vp, C.c_int]),
+    "l2_kv_plan": (C.c_int, [_vp] * 5 + [C.c_int, C.c_int, _vp]),
+    "l2_kv_release": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp]),
+    "l2_block_norm": (C.c_int, [_vp, _vp]),
     "l2_bench_projection": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int]),
     "l2_projection_bytes": (C.c_uint64, [_vp, C.c_int]),
     "l2_debug_trace": (C.c_int, [C.c_int, _p(C.c_uint64), C.c_int]),

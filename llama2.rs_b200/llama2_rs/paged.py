@@ -8,6 +8,10 @@
     pages.attend(batch, q16, out, window=4096, sinks=4)
     pages.read(batch, k_back, v_back)
 
+    tables = KvTables(page_table, kv_len, free_pages, free_count, page_size)           # who has which pages, on the device
+    tables.plan(new_rows, row_start, n_rows, max_rows, slots=slots)                    # the batch's lengths, tables and rows for a step
+    tables.release(keep)                                                               # and pages that are no longer needed
+
 The objects keep the tensors they are made of.  Work is enqueued on the current torch stream unless `stream` (a cudaStream_t) is given; a call
 does not wait for it.  With another stream than a tensor's own the caller orders the two and keeps rows and workspace until the work has run, as
 with any torch kernel.  One host thread at a time uses a KvPages.
@@ -16,14 +20,15 @@ import ctypes as C
 import struct
 import sys
 
-from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, as_f32p, check, lib
+from ._lib import KvBatchArgs, KvPagesArgs, KvRowsArgs, KvTablesArgs, as_f32p, check, lib
 
-F32, F16, BF16, I8, U4, I32 = 0, 1, 2, 3, 4, 5
-BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT = 1, 2, 4, 8, 16
-_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.uint8": U4, "torch.int32": I32}
+F32, F16, BF16, I8, U4, I32, I64 = 0, 1, 2, 3, 4, 5, 6
+BAD_PAGE, BAD_LENGTH, BAD_ROWS, BAD_ROPE, TIMEOUT, NO_ROOM = 1, 2, 4, 8, 16, 32
+_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": I8, "torch.uint8": U4, "torch.int32": I32, "torch.int64": I64}
 _types = {}  # the same by dtype object, filled as they are seen
 _ROWS2, _ROWS4 = struct.Struct("@" + "Pqqii" * 2), struct.Struct("@" + "Pqqii" * 4)  # l2_kv_rows, two and four in a row
 _ROTATIONS = {"pairs": 0, "model": 1}  # L2_ROPE_*
+_plan, _release = lib.l2_kv_plan, lib.l2_kv_release
 _append, _read, _attend, _workspace_bytes = lib.l2_kv_append_rope, lib.l2_kv_read, lib.l2_kv_attend, lib.l2_kv_attend_workspace_bytes
 assert _ROWS2.size == 2 * C.sizeof(KvRowsArgs) and _ROWS4.size == 4 * C.sizeof(KvRowsArgs)
 
@@ -50,6 +55,10 @@ def _stream(device, batch, stream):
     """The stream of a call, after a look at whether pages, batch and launch are all on one device."""
     if batch.device != device:
         raise ValueError("the batch is on device %d, the pages on device %d" % (batch.device, device))
+    return _stream_on(device, stream)
+
+
+def _stream_on(device, stream):
     if _cuda is None:
         _find_cuda()
     if _cuda[0]() != device:
@@ -87,6 +96,47 @@ class KvBatch:
         self._ref = C.byref(self._args)
         self._keep = (page_table, kv_len, row_start, status)
         self.n_rows = n_rows
+
+
+class KvTables:
+    """The tables of a batch on the device and the pages that are free: page_table [n_seqs, width], kv_len [n_seqs], free_pages [n_pages] and free_count [1], all
+    int32; a page is in one table or among the first free_count of free_pages.  page_table and kv_len may be those of a KvBatch, which then is the planned
+    step.  `status` as there."""
+
+    def __init__(self, page_table, kv_len, free_pages, free_count, page_size, status=None):
+        if page_table.dim() != 2 or not page_table.is_cuda or free_pages.dim() != 1:
+            raise ValueError("page_table: [n_seqs, width] on a CUDA device, free_pages: [n_pages] expected")
+        self.device = device = page_table.get_device()
+        n_seqs, width = page_table.shape
+        n_pages = free_pages.shape[0]
+        _int32(n_seqs=n_seqs, table_width=width, n_pages=n_pages, page_size=page_size)
+        self._args = KvTablesArgs(_packed(page_table, "page_table", device, (n_seqs, width), I32), _packed(kv_len, "kv_len", device, (n_seqs,), I32),
+                                  _packed(free_pages, "free_pages", device, (n_pages,), I32), _packed(free_count, "free_count", device, (1,), I32),
+                                  _packed(status, "status", device, (1,), I32) if status is not None else None, n_seqs, width, n_pages, page_size)
+        self._ref = C.byref(self._args)
+        self._keep = (page_table, kv_len, free_pages, free_count, status)
+        self._shape, self._starts = (n_seqs,), (n_seqs + 1,)
+
+    def plan(self, new_rows, row_start, n_rows, max_rows, slots=None, positions=None, stream=None):
+        """A step in which each sequence brings new_rows [n_seqs] int32 more rows, at most max_rows each and n_rows in all: row_start [n_seqs + 1] int32 is written, lengths and
+        tables grow.  slots [n_rows] int64 gets page * page_size + offset of each row, positions [n_rows] int32 its position; -1 behind the last row.  Without room (BAD_* bits
+        and NO_ROOM in status) nothing changes and no sequence brings rows."""
+        if n_rows >> 31 or max_rows >> 31:
+            _int32(n_rows=n_rows, max_rows=max_rows)
+        device = self.device
+        rc = _plan(self._ref, _packed(new_rows, "new_rows", device, self._shape, I32), _packed(row_start, "row_start", device, self._starts, I32),
+                   _packed(slots, "slots", device, (n_rows,), I64) if slots is not None else None,
+                   _packed(positions, "positions", device, (n_rows,), I32) if positions is not None else None, n_rows, max_rows, _stream_on(device, stream))
+        if rc:
+            check(rc)
+
+    def release(self, keep=None, window=0, sinks=0, stream=None):
+        """Each sequence keeps its first keep [n_seqs] int32 positions (0: it has ended; None: all), and with a window only the pages that later rows can see."""
+        if window >> 31 or sinks >> 31:
+            _int32(window=window, sinks=sinks)
+        rc = _release(self._ref, _packed(keep, "keep", self.device, self._shape, I32) if keep is not None else None, window, sinks, _stream_on(self.device, stream))
+        if rc:
+            check(rc)
 
 
 class KvRope(tuple):
