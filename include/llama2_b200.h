@@ -326,7 +326,7 @@ typedef struct l2_kv_tables {
     int32_t* free_pages;  /* [n_pages]: the first *free_count are free; taken from the end */
     int32_t* free_count;  /* one */
     int32_t* status;      /* as in l2_kv_batch, or NULL */
-    int32_t n_seqs, table_width;
+    int32_t n_seqs, table_width;  /* at most 16384 sequences, 2^30 entries */
     int32_t n_pages;
     int32_t page_size;    /* as in l2_kv_pages */
 } l2_kv_tables;

@@ -13,7 +13,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 HOST_CXX = "/usr/bin/g++"
 
 CU_SOURCES = ["decode_kernels.cu", "gemv_kernels.cu", "token_kernel.cu", "gemm_tc.cu", "prefill_kernels.cu", "prefill.cu", "model.cu", "host_stage.cu", "attention_noalloc.cu",
-              "paged.cu", "paged_attend.cu", "paged_rows.cu", "paged_tc.cu", "paged_tables.cu", "block_norm.cu"]
+              "paged.cu", "paged_attend.cu", "paged_rows.cu", "paged_rows4.cu", "paged_tc.cu", "paged_tables.cu", "block_norm.cu"]
 CPP_SOURCES = ["layout.cpp", "synth.cpp", "repack.cpp", "tokenizer.cpp", "tp.cpp"]
 
 NVCC_FLAGS = [

@@ -54,6 +54,10 @@ int kv_rows_limit(const KvStep& s, int group);
 size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms);
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);
 
+// Of a cache in 4 bits: sequences with at most `lim` rows, which is not 0.
+size_t kv_rows4_work(const KvStep& s, const KvPool& p, int lim, int head_size, int sms);
+cudaError_t launch_kv_rows4(const KvAttendParams& p, int lim, int head_size, int sms, cudaStream_t st);
+
 // The others: tcgen05.
 size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms);
 cudaError_t launch_kv_tc(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st);

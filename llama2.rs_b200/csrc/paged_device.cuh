@@ -189,6 +189,19 @@ __device__ __forceinline__ void kv_store1(const KvRows& o, int64_t e, float x) {
     else reinterpret_cast<__nv_bfloat16*>(o.data)[e] = __float2bfloat16_rn(x);
 }
 
+// ---- fragments of warp-wide products --------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // ---- bytes as 16-bit numbers -------------------------------------------------------------------------------------------------
 // The 16-bit numbers of bytes SEL & 3 and SEL >> 4 & 3 of w (two's complement), exact.
 template <bool BF, uint32_t SEL>
@@ -223,6 +236,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// ---- caches in 4 bits --------------------------------------------------------------------------------------------------------
+// For a row of bf16 whose largest element is `most`: a power of two that brings it to 2^15 .. 2^16 (f16 holds 65504, bf16 goes up to 65280 there), and its inverse, both normal
+// numbers.  (Elements of 2^118 and more are beyond f16 then, and the row gives NaN.)
+__device__ __forceinline__ void kv_q_factors(float most, float* up, float* by) {
+    const int e = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23), 16), 244) : 142;
+    *up = __uint_as_float((uint32_t)(127 + 127 + 15 - e) << 23);
+    *by = __uint_as_float((uint32_t)(e - 15) << 23);
 }
 
 }  // namespace l2

@@ -30,7 +30,6 @@
 #include "kernels.cuh"
 #include "paged_device.cuh"
 #include "paged_attend.h"
-#include "paged_rows4.cuh"
 
 namespace l2 {
 
@@ -45,21 +44,18 @@ constexpr int KR_RAISE = 8;  // powers of two that a score may exceed the runnin
 constexpr int KR_DIGITS = 4;  // of Q against int8 K
 constexpr int KR_SMEM = 111 * 1024;  // of a CTA: two on an SM, with what is static and reserved
 
-// (cache in 4 bits: 64 or 128 positions a warp in steps of 32)
-constexpr int kr_tile(int type, int head_size, int nt) { return type == L2_U4 ? nt == 1 ? 128 : 256 : head_size * (type == L2_I8 ? 1 : 2) == 256 ? 64 : 128; }
-
 // A variant: 16 KB of K and as much of V in a tile, 64 or 128 positions, of which a warp has 16 or 32 (an int8 cache in tiles of 64 was bound by the
 // chain of a warp's step, 2000 clocks whatever the bytes).
 // Shared memory: Q and the ring; the warps' results meet in the slot of a piece's last tile.
 template <int CT, int HD, int NT>
 struct KrShape {
-    static constexpr bool I8 = CT == L2_I8, U4 = CT == L2_U4, SCALED = I8 || U4;
-    static constexpr int ROWS = 8 * NT, ROW_BYTES = U4 ? HD / 2 : HD * (I8 ? 1 : 2);
-    static constexpr int TILE = kr_tile(CT, HD, NT), PER_WARP = TILE / KR_WARPS, MB = PER_WARP / 16;
+    static constexpr bool I8 = CT == L2_I8;
+    static constexpr int ROWS = 8 * NT, ROW_BYTES = HD * (I8 ? 1 : 2);
+    static constexpr int TILE = ROW_BYTES == 256 ? 64 : 128, PER_WARP = TILE / KR_WARPS, MB = PER_WARP / 16;
     static constexpr int DIGITS = I8 && NT == 1 ? KR_DIGITS : 0;                // of Q, where it can be in digits
     static constexpr int Q_PITCH = 2 * HD + 16, D_PITCH = HD + 16, D_PLANE = ROWS * D_PITCH;  // bytes between rows of Q, of a digit (no bank conflicts); of a digit's plane
     static constexpr int KV_BYTES = TILE * ROW_BYTES;                           // K or V of a tile
-    static constexpr int SCALE_BYTES = SCALED ? TILE * 4 : 0;
+    static constexpr int SCALE_BYTES = I8 ? TILE * 4 : 0;
     static constexpr int STAGE = (2 * (KV_BYTES + SCALE_BYTES) + 1023) / 1024 * 1024;
     static constexpr int FIXED = 1024 + ROWS * Q_PITCH + DIGITS * D_PLANE;
     static constexpr int STAGES = (KR_SMEM - FIXED) / STAGE < KR_MAX_STAGES ? (KR_SMEM - FIXED) / STAGE : KR_MAX_STAGES;
@@ -70,26 +66,14 @@ struct KrShape {
 // Where 16-byte chunk c16 of row r of a tile is: rows of 128 bytes (two halves of a tile one after the other) or 64, as the TMA swizzles them.
 template <int ROW_BYTES, int TILE>
 __device__ __forceinline__ uint32_t kr_offset(int r, int c16) {
-    if constexpr (ROW_BYTES == 32) return r * 32 + ((c16 ^ ((r >> 2) & 1)) << 4);
-    else if constexpr (ROW_BYTES == 64) return r * 64 + ((c16 ^ ((r >> 1) & 3)) << 4);
+    if constexpr (ROW_BYTES == 64) return r * 64 + ((c16 ^ ((r >> 1) & 3)) << 4);
     else return (c16 >> 3) * (TILE * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
-}
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float from_int(int x) { return __int_as_float(x + 0x4b400000) - 12582912.0f; }  // |x| < 2^22, exact
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
 template <bool BF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (BF)
@@ -168,14 +152,14 @@ template <int CT, bool QB, int HD, int NT>
 __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
                                                                const __grid_constant__ CUtensorMap map_v) {
     using S = KrShape<CT, HD, NT>;
-    constexpr bool I8 = S::I8, U4 = S::U4, PB = I8 || QB;       // probabilities and V in bf16
+    constexpr bool I8 = S::I8, PB = I8 || QB;       // probabilities and V in bf16
     constexpr int KS = HD / 16, MT = HD / 16, RB = S::ROW_BYTES, TILE = S::TILE, MB = S::MB;
-    constexpr float BIAS = PB || U4 ? 24.0f : 7.0f;  // probabilities carry a factor of 2^BIAS, so that small ones are normal numbers; f16 at most 2^(7 + KR_RAISE)
+    constexpr float BIAS = PB ? 24.0f : 7.0f;       // probabilities carry a factor of 2^BIAS, so that small ones are normal numbers; f16 at most 2^(7 + KR_RAISE)
     extern __shared__ __align__(1024) uint8_t kr_smem[];
     __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES];
     __shared__ int64_t scratch[KR_THREADS / 32 + 2];
     __shared__ float meet_ml[KR_WARPS][S::ROWS][2];
-    __shared__ float q_factor[S::ROWS], q_sum[U4 ? S::ROWS : 1];  // of a row's digits (4 bits: of its elements in f16), the sum of these
+    __shared__ float q_factor[S::ROWS];  // of a row's digits
     __shared__ volatile int failed;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kr_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t* sq = ring + S::STAGES * S::STAGE;
@@ -183,7 +167,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < S::STAGES; i++) { kv_bar_init(&full[i], S::SCALED ? 33 : 1); kv_bar_init(&empty[i], KR_WARPS); }
+        for (int i = 0; i < S::STAGES; i++) { kv_bar_init(&full[i], I8 ? 33 : 1); kv_bar_init(&empty[i], KR_WARPS); }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -228,16 +212,13 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         kv_tma4(v_to + to, &map_v, h * 64, at, walk.head, page, &full[st]);
                     }
                 }
-                if constexpr (S::SCALED) {  // the scales (pairs): four positions a lane, of K and of V
-#pragma unroll
-                    for (int p0 = 0; p0 < TILE; p0 += 128) {
-                        const int pos = p0 + 4 * lane, of = __shfl_sync(0xffffffffu, pages, k * runs + pos / R);
-                        const bool there = of < P.pool.n_pages;
-                        const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((j + pos) & ((1 << P.pool.page_shift) - 1));
-                        const uint32_t to = kv_smem(stage + 2 * S::KV_BYTES) + 4 * pos;
-                        kv_copy16(to, P.pool.ks + e, there);
-                        kv_copy16(to + S::SCALE_BYTES, P.pool.vs + e, there);
-                    }
+                if constexpr (I8) {  // the scales: four positions a lane, of K and of V
+                    const int pos = 4 * lane, of = __shfl_sync(0xffffffffu, pages, k * runs + pos / R);
+                    const bool there = of < P.pool.n_pages;
+                    const int64_t e = ((int64_t)(there ? of : 0) * P.pool.n_kv_heads + walk.head << P.pool.page_shift) + ((j + pos) & ((1 << P.pool.page_shift) - 1));
+                    const uint32_t to = kv_smem(stage + 2 * S::KV_BYTES) + 16 * lane;
+                    kv_copy16(to, P.pool.ks + e, there);
+                    kv_copy16(to + S::SCALE_BYTES, P.pool.vs + e, there);
                     kv_copy16_arrive(&full[st]);
                 }
                 if (++st == S::STAGES) { st = 0; ph ^= 1u; }
@@ -265,6 +246,74 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
             const KvView<TILE> view = walk.q.view;
             const int rows = walk.q.rows, G = P.group, t0 = walk.t0, t1 = walk.t1;
             asm volatile("bar.sync 1, 128;" ::: "memory");  // (everybody has read the piece before's)
+#pragma unroll
+            for (int n = 0; n < Q_N; n++) {
+                const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8);
+                if (r < S::ROWS) *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = qx[n];
+            }
+            bool digits = false;  // Q is in digits: they hold every element of all rows
+            if constexpr (S::DIGITS > 0) {
+                const int r = tid / (HD / 8), ch = tid % (HD / 8);
+                float x[8], most = 0.0f;
+                const uint32_t w[4] = {qx[0].x, qx[0].y, qx[0].z, qx[0].w};
+                bool held = true;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    x[k] = QB ? __uint_as_float(k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16) : __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k % 2)))));
+                    held &= fabsf(x[k]) < INFINITY;
+                    most = fmaxf(most, fabsf(x[k]));
+                }
+#pragma unroll
+                for (int o = 1; o < HD / 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                constexpr int BITS = 8 * S::DIGITS - 2;
+                const int e = max((int)(__float_as_uint(most) >> 23) - 126, BITS - 122);  // most < 2^e; 2^(BITS - e) and its inverse are normal numbers
+                const float up = __uint_as_float((uint32_t)(BITS - e + 127) << 23);
+                uint32_t plane[S::DIGITS][2] = {};
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float y = x[k] * up;
+                    const int whole = __float2int_rn(y);
+                    held &= (float)whole == y;
+                    constexpr uint32_t HALF = 0x80808080u >> (32 - 8 * S::DIGITS);
+                    const uint32_t v = ((uint32_t)whole + HALF) ^ HALF;  // balanced digits
+#pragma unroll
+                    for (int p = 0; p < S::DIGITS; p++) plane[p][k / 4] |= (v >> (8 * p) & 255u) << (8 * (k % 4));
+                }
+                if (r < S::ROWS) {
+#pragma unroll
+                    for (int p = 0; p < S::DIGITS; p++) *reinterpret_cast<uint2*>(sd + p * S::D_PLANE + r * S::D_PITCH + 8 * ch) = make_uint2(plane[p][0], plane[p][1]);
+                    if (ch == 0) q_factor[r] = __uint_as_float((uint32_t)(e - BITS + 127) << 23);
+                }
+                uint32_t all;
+                asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((uint32_t)held) : "memory");
+                digits = __all_sync(0xffffffffu, all);  // (a vote's result is uniform)
+            } else {
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            // Q^T as the second factor: columns 8 nt .., two words for each 16 elements (digits: for each 32, of each digit)
+            constexpr int Q_WORDS = S::DIGITS * HD / 32 > NT * KS ? S::DIGITS * HD / 32 : NT * KS;
+            uint32_t qr[Q_WORDS][2];
+            float by_row[2] = {1.0f, 1.0f};
+            if (digits) {
+#pragma unroll
+                for (int a = 0; a < S::DIGITS; a++)
+#pragma unroll
+                    for (int c2 = 0; c2 < HD / 32; c2++) {
+                        const uint8_t* p = sd + a * S::D_PLANE + g8 * S::D_PITCH + c2 * 32 + 4 * c;
+                        qr[a * (HD / 32) + c2][0] = *reinterpret_cast<const uint32_t*>(p);
+                        qr[a * (HD / 32) + c2][1] = *reinterpret_cast<const uint32_t*>(p + 16);
+                    }
+                by_row[0] = q_factor[2 * c]; by_row[1] = q_factor[2 * c + 1];
+            } else {
+#pragma unroll
+                for (int a = 0; a < NT; a++)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        const uint8_t* p = sq + (8 * a + g8) * S::Q_PITCH + ks * 32;
+                        if constexpr (I8) { const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * c); qr[a * KS + ks][0] = x.x; qr[a * KS + ks][1] = x.y; }
+                        else { qr[a * KS + ks][0] = *reinterpret_cast<const uint32_t*>(p + 4 * c); qr[a * KS + ks][1] = *reinterpret_cast<const uint32_t*>(p + 16 + 4 * c); }
+                    }
+            }
             int pos[NT][2];  // positions of this thread's two rows of each eight
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -272,352 +321,194 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                 for (int e = 0; e < 2; e++) pos[nt][e] = view.lo_pos + (8 * nt + 2 * c + e) / G;
 
             float o[MT][NT][4], m[NT][2], l[NT][2];
-            if constexpr (U4) {
-                // Q in f16, of eight elements the words (0, 4), (2, 6), (1, 5), (3, 7), as the numbers of a word of K come out
-                Kr4Rows<HD, NT> r;
 #pragma unroll
-                for (int n = 0; n < Q_N; n++) {
-                    const int u = tid + n * KR_WARPS * 32, row = u / (HD / 8), ch = u % (HD / 8);
-                    const uint32_t w[4] = {qx[n].x, qx[n].y, qx[n].z, qx[n].w};
-                    float x[8], sum = 0.0f, up = 1.0f, by = 1.0f;
+            for (int nt = 0; nt < NT; nt++) {
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        x[k] = QB ? __uint_as_float(k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16) : __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k % 2)))));
-                    if constexpr (QB) {
-                        float most = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) most = fmaxf(most, fabsf(x[k]));
-#pragma unroll
-                        for (int o = 1; o < HD / 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        kr4_q_factors(most, &up, &by);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] *= up;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) sum += x[k];
-#pragma unroll
-                    for (int o = 1; o < HD / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (row < S::ROWS) {
-                        *reinterpret_cast<uint4*>(sq + row * S::Q_PITCH + ch * 16) =
-                            make_uint4(pack16<false>(x[0], x[4]), pack16<false>(x[2], x[6]), pack16<false>(x[1], x[5]), pack16<false>(x[3], x[7]));
-                        if (ch == 0) { q_factor[row] = by; q_sum[row] = sum; }
-                    }
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int ch = 0; ch < HD / 32; ch++) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(sq + (8 * nt + g8) * S::Q_PITCH + 64 * ch + 16 * c);
-                        r.q[ch][nt][0] = x.x; r.q[ch][nt][1] = x.y; r.q[ch][nt][2] = x.z; r.q[ch][nt][3] = x.w;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {  // (the products are of numbers times 2^-24)
-                        r.by[nt][e] = q_factor[8 * nt + 2 * c + e] * (P.scale_log2 * 0x1p24f);
-                        r.sum[nt][e] = q_sum[8 * nt + 2 * c + e] * 0x1p-24f;
-                        r.pos[nt][e] = pos[nt][e];
-                        r.m[nt][e] = -INFINITY;
-                        r.l[nt][e] = r.y[nt][e] = 0.0f;
-                        r.h[nt][e] = 1.0f;
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) r.o[mt][nt][0] = r.o[mt][nt][1] = r.o[mt][nt][2] = r.o[mt][nt][3] = 0.0f;
-                }
+                for (int mt = 0; mt < MT; mt++) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.0f;
+            }
 #pragma unroll 1
-                for (int t = t0; t < t1; t++) {
-                    const int base = view.base(t);
-                    const bool whole = view.whole(base, P.window, P.sinks);
-                    wait(&full[st], ph);
-                    __syncwarp();
-                    const uint8_t* stage = ring + st * S::STAGE;
-                    const uint32_t k_at = kv_smem(stage);
-                    const uint32_t* pairs = reinterpret_cast<const uint32_t*>(stage + 2 * S::KV_BYTES);
-#pragma unroll 1
-                    for (int row = S::PER_WARP * warp; row < S::PER_WARP * (warp + 1); row += 32)
-                        kr4_step<HD, NT>(P, r, k_at, k_at + S::KV_BYTES, row, pairs + row + g8, pairs + TILE + row + g8, base + row + g8, whole, BIAS, KR_RAISE,
-                                         kr_offset<RB, TILE>, ldsm4, ldsm4_t, transpose8);
-                    if (t + 1 < t1) {  // (the last tile's slot is kept for the meeting)
-                        __syncwarp();
-                        if (lane == 0) kv_bar_arrive(&empty[st]);
-                        if (++st == S::STAGES) { st = 0; ph ^= 1u; }
-                    }
-                }
-                // the sums in units of 2^-m, with what the zeros give every element
+            for (int t = t0; t < t1; t++) {
+                const int base = view.base(t);
+                const bool whole = view.whole(base, P.window, P.sinks);
+                wait(&full[st], ph);
+                __syncwarp();
+                const uint8_t* stage = ring + st * S::STAGE;
+                const uint32_t k_at = kv_smem(stage), v_at = k_at + S::KV_BYTES;
+                // ---- scores of this warp's positions, 16 at a time: rows g8 and g8 + 8, columns 2 c and 2 c + 1
+                float s[MB][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float y = r.y[nt][e];
-                        y += __shfl_xor_sync(0xffffffffu, y, 4);
-                        y += __shfl_xor_sync(0xffffffffu, y, 8);
-                        y += __shfl_xor_sync(0xffffffffu, y, 16);
-                        const float by = 0x1p20f / r.h[nt][e];  // (a power of two between 2^-44 and 2^120)
-                        m[nt][e] = r.m[nt][e];
-                        l[nt][e] = r.l[nt][e];
+                    for (int nt = 0; nt < NT; nt++) s[mb][nt][0] = s[mb][nt][1] = s[mb][nt][2] = s[mb][nt][3] = 0.0f;
+                const int kr = S::PER_WARP * warp + (lane & 15);
+                auto by_k = [&](int mb, int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            o[mt][nt][e] = fmaf(r.o[mt][nt][e], 16.0f * by, y);
-                            o[mt][nt][e + 2] = fmaf(r.o[mt][nt][e + 2], by, y);
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int n = 0; n < Q_N; n++) {
-                    const int u = tid + n * KR_WARPS * 32, r = u / (HD / 8), ch = u % (HD / 8);
-                    if (r < S::ROWS) *reinterpret_cast<uint4*>(sq + r * S::Q_PITCH + ch * 16) = qx[n];
-                }
-                bool digits = false;  // Q is in digits: they hold every element of all rows
-                if constexpr (S::DIGITS > 0) {
-                    const int r = tid / (HD / 8), ch = tid % (HD / 8);
-                    float x[8], most = 0.0f;
-                    const uint32_t w[4] = {qx[0].x, qx[0].y, qx[0].z, qx[0].w};
-                    bool held = true;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        x[k] = QB ? __uint_as_float(k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16) : __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k % 2)))));
-                        held &= fabsf(x[k]) < INFINITY;
-                        most = fmaxf(most, fabsf(x[k]));
-                    }
-#pragma unroll
-                    for (int o = 1; o < HD / 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    constexpr int BITS = 8 * S::DIGITS - 2;
-                    const int e = max((int)(__float_as_uint(most) >> 23) - 126, BITS - 122);  // most < 2^e; 2^(BITS - e) and its inverse are normal numbers
-                    const float up = __uint_as_float((uint32_t)(BITS - e + 127) << 23);
-                    uint32_t plane[S::DIGITS][2] = {};
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float y = x[k] * up;
-                        const int whole = __float2int_rn(y);
-                        held &= (float)whole == y;
-                        constexpr uint32_t HALF = 0x80808080u >> (32 - 8 * S::DIGITS);
-                        const uint32_t v = ((uint32_t)whole + HALF) ^ HALF;  // balanced digits
-#pragma unroll
-                        for (int p = 0; p < S::DIGITS; p++) plane[p][k / 4] |= (v >> (8 * p) & 255u) << (8 * (k % 4));
-                    }
-                    if (r < S::ROWS) {
-#pragma unroll
-                        for (int p = 0; p < S::DIGITS; p++) *reinterpret_cast<uint2*>(sd + p * S::D_PLANE + r * S::D_PITCH + 8 * ch) = make_uint2(plane[p][0], plane[p][1]);
-                        if (ch == 0) q_factor[r] = __uint_as_float((uint32_t)(e - BITS + 127) << 23);
-                    }
-                    uint32_t all;
-                    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((uint32_t)held) : "memory");
-                    digits = __all_sync(0xffffffffu, all);  // (a vote's result is uniform)
-                } else {
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                }
-                // Q^T as the second factor: columns 8 nt .., two words for each 16 elements (digits: for each 32, of each digit)
-                constexpr int Q_WORDS = S::DIGITS * HD / 32 > NT * KS ? S::DIGITS * HD / 32 : NT * KS;
-                uint32_t qr[Q_WORDS][2];
-                float by_row[2] = {1.0f, 1.0f};
+                    for (int nt = 0; nt < NT; nt++) mma<QB>(s[mb][nt], a0, a1, a2, a3, qr[nt * KS + ks][0], qr[nt * KS + ks][1]);
+                };
                 if (digits) {
+                    constexpr int N = S::DIGITS ? S::DIGITS : 1;
+                    int d[MB][N][4] = {};
 #pragma unroll
-                    for (int a = 0; a < S::DIGITS; a++)
+                    for (int c2 = 0; c2 < HD / 32; c2++)
 #pragma unroll
-                        for (int c2 = 0; c2 < HD / 32; c2++) {
-                            const uint8_t* p = sd + a * S::D_PLANE + g8 * S::D_PITCH + c2 * 32 + 4 * c;
-                            qr[a * (HD / 32) + c2][0] = *reinterpret_cast<const uint32_t*>(p);
-                            qr[a * (HD / 32) + c2][1] = *reinterpret_cast<const uint32_t*>(p + 16);
+                        for (int mb = 0; mb < MB; mb++) {
+                            uint32_t a[4];
+                            ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
+#pragma unroll
+                            for (int p = 0; p < N; p++) mma_s8(d[mb][p], a, qr[p * (HD / 32) + c2][0], qr[p * (HD / 32) + c2][1]);
                         }
-                    by_row[0] = q_factor[2 * c]; by_row[1] = q_factor[2 * c + 1];
-                } else {
-#pragma unroll
-                    for (int a = 0; a < NT; a++)
-#pragma unroll
-                        for (int ks = 0; ks < KS; ks++) {
-                            const uint8_t* p = sq + (8 * a + g8) * S::Q_PITCH + ks * 32;
-                            if constexpr (I8) { const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * c); qr[a * KS + ks][0] = x.x; qr[a * KS + ks][1] = x.y; }
-                            else { qr[a * KS + ks][0] = *reinterpret_cast<const uint32_t*>(p + 4 * c); qr[a * KS + ks][1] = *reinterpret_cast<const uint32_t*>(p + 16 + 4 * c); }
-                        }
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    m[nt][0] = m[nt][1] = -INFINITY;
-                    l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.0f;
-                }
-#pragma unroll 1
-                for (int t = t0; t < t1; t++) {
-                    const int base = view.base(t);
-                    const bool whole = view.whole(base, P.window, P.sinks);
-                    wait(&full[st], ph);
-                    __syncwarp();
-                    const uint8_t* stage = ring + st * S::STAGE;
-                    const uint32_t k_at = kv_smem(stage), v_at = k_at + S::KV_BYTES;
-                    // ---- scores of this warp's positions, 16 at a time: rows g8 and g8 + 8, columns 2 c and 2 c + 1
-                    float s[MB][NT][4];
 #pragma unroll
                     for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) s[mb][nt][0] = s[mb][nt][1] = s[mb][nt][2] = s[mb][nt][3] = 0.0f;
-                    const int kr = S::PER_WARP * warp + (lane & 15);
-                    auto by_k = [&](int mb, int ks, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                        for (int i = 0; i < 4; i++) {
+                            float x = from_int(d[mb][0][i]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma<QB>(s[mb][nt], a0, a1, a2, a3, qr[nt * KS + ks][0], qr[nt * KS + ks][1]);
-                    };
-                    if (digits) {
-                        constexpr int N = S::DIGITS ? S::DIGITS : 1;
-                        int d[MB][N][4] = {};
-#pragma unroll
-                        for (int c2 = 0; c2 < HD / 32; c2++)
-#pragma unroll
-                            for (int mb = 0; mb < MB; mb++) {
-                                uint32_t a[4];
-                                ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
-#pragma unroll
-                                for (int p = 0; p < N; p++) mma_s8(d[mb][p], a, qr[p * (HD / 32) + c2][0], qr[p * (HD / 32) + c2][1]);
-                            }
-#pragma unroll
-                        for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                float x = from_int(d[mb][0][i]);
-#pragma unroll
-                                for (int p = 1; p < N; p++) x = fmaf(from_int(d[mb][p][i]), (float)(1 << (8 * p)), x);
-                                s[mb][0][i] = by_row[i & 1] * x;
-                            }
-                    } else if constexpr (I8) {
-#pragma unroll
-                        for (int c2 = 0; c2 < KS / 2; c2++)  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
-#pragma unroll
-                            for (int mb = 0; mb < MB; mb++) {
-                                uint32_t a[4];
-                                ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
-                                by_k(mb, 2 * c2, widen<QB, 0x10>(a[0]), widen<QB, 0x10>(a[1]), widen<QB, 0x32>(a[0]), widen<QB, 0x32>(a[1]));
-                                by_k(mb, 2 * c2 + 1, widen<QB, 0x10>(a[2]), widen<QB, 0x10>(a[3]), widen<QB, 0x32>(a[2]), widen<QB, 0x32>(a[3]));
-                            }
-                    } else {
-#pragma unroll
-                        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                            for (int mb = 0; mb < MB; mb++) {
-                                uint32_t a[4];
-                                ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * ks + (lane >> 4)));
-                                by_k(mb, ks, a[0], a[1], a[2], a[3]);
-                            }
-                    }
-                    // ---- softmax
-                    const int j0 = base + S::PER_WARP * warp + g8;  // this thread's positions: j0 + 16 mb, and 8 more
-                    auto sees = [&](int nt, int mb, int i) { return kv_sees(pos[nt][i & 1], j0 + 16 * mb + 8 * (i >> 1), P.window, P.sinks); };
-                    float v_scale[MB][2], most[NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) most[nt][0] = most[nt][1] = -INFINITY;
-#pragma unroll
-                    for (int mb = 0; mb < MB; mb++) {
-                        float f0 = P.scale_log2, f1 = P.scale_log2;
-                        if constexpr (I8) {
-                            const float* sc = reinterpret_cast<const float*>(stage + 2 * S::KV_BYTES) + S::PER_WARP * warp + 16 * mb + g8;
-                            f0 *= sc[0]; f1 *= sc[8];
-                            v_scale[mb][0] = sc[TILE]; v_scale[mb][1] = sc[TILE + 8];
+                            for (int p = 1; p < N; p++) x = fmaf(from_int(d[mb][p][i]), (float)(1 << (8 * p)), x);
+                            s[mb][0][i] = by_row[i & 1] * x;
                         }
+                } else if constexpr (I8) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            s[mb][nt][0] *= f0; s[mb][nt][1] *= f0; s[mb][nt][2] *= f1; s[mb][nt][3] *= f1;
-                            if (!whole) {
-#pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    if (!sees(nt, mb, i)) s[mb][nt][i] = -INFINITY;
-                            }
-                            most[nt][0] = fmaxf(most[nt][0], fmaxf(s[mb][nt][0], s[mb][nt][2]));
-                            most[nt][1] = fmaxf(most[nt][1], fmaxf(s[mb][nt][1], s[mb][nt][3]));
-                        }
-                    }
-                    bool raise = false;
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) raise |= most[nt][0] - BIAS > m[nt][0] + KR_RAISE || most[nt][1] - BIAS > m[nt][1] + KR_RAISE;
-                    if (__any_sync(0xffffffffu, raise)) {  // seldom: only then do the lanes of a row need their common maximum
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                float x = most[nt][e] - BIAS;
-                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                                const float m1 = x > m[nt][e] + KR_RAISE ? x : m[nt][e];  // (a row's result does not depend on the others)
-                                const KvScale f(m1 == -INFINITY ? 0.0f : m[nt][e] - m1);
-                                m[nt][e] = m1;
-                                l[nt][e] = f(l[nt][e]);
-#pragma unroll
-                                for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
-                            }
-                    }
-                    uint32_t pb[MB][NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const float ref[2] = {m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m[nt][1] == -INFINITY ? 0.0f : m[nt][1]};
+                    for (int c2 = 0; c2 < KS / 2; c2++)  // 32 elements; of each 16, element 4 c + i is k index 2 c + i (i < 2) or 8 + 2 c + i - 2
 #pragma unroll
                         for (int mb = 0; mb < MB; mb++) {
-                            float p[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                p[i] = kv_exp2(s[mb][nt][i] - ref[i & 1]);
-                                l[nt][i & 1] += p[i];
-                                if constexpr (I8) p[i] = !whole && !sees(nt, mb, i) ? 0.0f : p[i] * v_scale[mb][i >> 1];
-                            }
-                            pb[mb][nt][0] = transpose8(pack16<PB>(p[0], p[1]));
-                            pb[mb][nt][1] = transpose8(pack16<PB>(p[2], p[3]));
+                            uint32_t a[4];
+                            ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * c2 + (lane >> 4)));
+                            by_k(mb, 2 * c2, widen<QB, 0x10>(a[0]), widen<QB, 0x10>(a[1]), widen<QB, 0x32>(a[0]), widen<QB, 0x32>(a[1]));
+                            by_k(mb, 2 * c2 + 1, widen<QB, 0x10>(a[2]), widen<QB, 0x10>(a[3]), widen<QB, 0x32>(a[2]), widen<QB, 0x32>(a[3]));
                         }
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int mb = 0; mb < MB; mb++) {
+                            uint32_t a[4];
+                            ldsm4(a, k_at + kr_offset<RB, TILE>(kr + 16 * mb, 2 * ks + (lane >> 4)));
+                            by_k(mb, ks, a[0], a[1], a[2], a[3]);
+                        }
+                }
+                // ---- softmax
+                const int j0 = base + S::PER_WARP * warp + g8;  // this thread's positions: j0 + 16 mb, and 8 more
+                auto sees = [&](int nt, int mb, int i) { return kv_sees(pos[nt][i & 1], j0 + 16 * mb + 8 * (i >> 1), P.window, P.sinks); };
+                float v_scale[MB][2], most[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) most[nt][0] = most[nt][1] = -INFINITY;
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) {
+                    float f0 = P.scale_log2, f1 = P.scale_log2;
+                    if constexpr (I8) {
+                        const float* sc = reinterpret_cast<const float*>(stage + 2 * S::KV_BYTES) + S::PER_WARP * warp + 16 * mb + g8;
+                        f0 *= sc[0]; f1 *= sc[8];
+                        v_scale[mb][0] = sc[TILE]; v_scale[mb][1] = sc[TILE + 8];
                     }
-                    // ---- O^T += V^T P^T
-                    const int vr = S::PER_WARP * warp + (lane & 7) + 8 * (lane >> 4);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        s[mb][nt][0] *= f0; s[mb][nt][1] *= f0; s[mb][nt][2] *= f1; s[mb][nt][3] *= f1;
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (!sees(nt, mb, i)) s[mb][nt][i] = -INFINITY;
+                        }
+                        most[nt][0] = fmaxf(most[nt][0], fmaxf(s[mb][nt][0], s[mb][nt][2]));
+                        most[nt][1] = fmaxf(most[nt][1], fmaxf(s[mb][nt][1], s[mb][nt][3]));
+                    }
+                }
+                bool raise = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) raise |= most[nt][0] - BIAS > m[nt][0] + KR_RAISE || most[nt][1] - BIAS > m[nt][1] + KR_RAISE;
+                if (__any_sync(0xffffffffu, raise)) {  // seldom: only then do the lanes of a row need their common maximum
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float x = most[nt][e] - BIAS;
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            const float m1 = x > m[nt][e] + KR_RAISE ? x : m[nt][e];  // (a row's result does not depend on the others)
+                            const KvScale f(m1 == -INFINITY ? 0.0f : m[nt][e] - m1);
+                            m[nt][e] = m1;
+                            l[nt][e] = f(l[nt][e]);
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) { o[mt][nt][e] = f(o[mt][nt][e]); o[mt][nt][e + 2] = f(o[mt][nt][e + 2]); }
+                        }
+                }
+                uint32_t pb[MB][NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float ref[2] = {m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m[nt][1] == -INFINITY ? 0.0f : m[nt][1]};
 #pragma unroll
                     for (int mb = 0; mb < MB; mb++) {
-                        if constexpr (I8) {
+                        float p[4];
 #pragma unroll
-                            for (int m2 = 0; m2 < (MT + 1) / 2; m2++) {  // 32 elements; row i of a product is element 2 i, row 8 + i element 2 i + 1
-                                uint32_t a[4];
-                                ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * m2 + ((lane >> 3) & 1)));
+                        for (int i = 0; i < 4; i++) {
+                            p[i] = kv_exp2(s[mb][nt][i] - ref[i & 1]);
+                            l[nt][i & 1] += p[i];
+                            if constexpr (I8) p[i] = !whole && !sees(nt, mb, i) ? 0.0f : p[i] * v_scale[mb][i >> 1];
+                        }
+                        pb[mb][nt][0] = transpose8(pack16<PB>(p[0], p[1]));
+                        pb[mb][nt][1] = transpose8(pack16<PB>(p[2], p[3]));
+                    }
+                }
+                // ---- O^T += V^T P^T
+                const int vr = S::PER_WARP * warp + (lane & 7) + 8 * (lane >> 4);
 #pragma unroll
-                                for (int h = 0; h < 2; h++) {
-                                    const uint32_t x0 = widen<true, 0x20>(a[h]), x1 = widen<true, 0x31>(a[h]), x2 = widen<true, 0x20>(a[h + 2]), x3 = widen<true, 0x31>(a[h + 2]);
+                for (int mb = 0; mb < MB; mb++) {
+                    if constexpr (I8) {
 #pragma unroll
-                                    for (int nt = 0; nt < NT; nt++) mma<true>(o[2 * m2 + h][nt], x0, x1, x2, x3, pb[mb][nt][0], pb[mb][nt][1]);
+                        for (int m2 = 0; m2 < (MT + 1) / 2; m2++) {  // 32 elements; row i of a product is element 2 i, row 8 + i element 2 i + 1
+                            uint32_t a[4];
+                            ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * m2 + ((lane >> 3) & 1)));
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t x0 = widen<true, 0x20>(a[h]), x1 = widen<true, 0x31>(a[h]), x2 = widen<true, 0x20>(a[h + 2]), x3 = widen<true, 0x31>(a[h + 2]);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) mma<true>(o[2 * m2 + h][nt], x0, x1, x2, x3, pb[mb][nt][0], pb[mb][nt][1]);
+                            }
+                        }
+                    } else {
+                        bool odd = false;
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            uint32_t a[4];
+                            ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * mt + ((lane >> 3) & 1)));
+                            if (!whole) {  // 0 x NaN is NaN: a value that some row does not see may only be multiplied where it is finite
+                                if (__any_sync(0xffffffffu, not_finite<PB>(a[0]) | not_finite<PB>(a[1]) | not_finite<PB>(a[2]) | not_finite<PB>(a[3]))) {
+                                    odd = true;
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) a[i] = only_finite<PB>(a[i]);
                                 }
                             }
-                        } else {
-                            bool odd = false;
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++) {
-                                uint32_t a[4];
-                                ldsm4_t(a, v_at + kr_offset<RB, TILE>(vr + 16 * mb, 2 * mt + ((lane >> 3) & 1)));
-                                if (!whole) {  // 0 x NaN is NaN: a value that some row does not see may only be multiplied where it is finite
-                                    if (__any_sync(0xffffffffu, not_finite<PB>(a[0]) | not_finite<PB>(a[1]) | not_finite<PB>(a[2]) | not_finite<PB>(a[3]))) {
-                                        odd = true;
-#pragma unroll
-                                        for (int i = 0; i < 4; i++) a[i] = only_finite<PB>(a[i]);
-                                    }
-                                }
-#pragma unroll
-                                for (int nt = 0; nt < NT; nt++) mma<PB>(o[mt][nt], a[0], a[1], a[2], a[3], pb[mb][nt][0], pb[mb][nt][1]);
-                            }
-                            if (odd) {  // rare: the values that are not finite, one by one, to the rows that see them
+                            for (int nt = 0; nt < NT; nt++) mma<PB>(o[mt][nt], a[0], a[1], a[2], a[3], pb[mb][nt][0], pb[mb][nt][1]);
+                        }
+                        if (odd) {  // rare: the values that are not finite, one by one, to the rows that see them
 #pragma unroll 1
-                                for (int i = 0; i < 16; i++) {
-                                    const int r = S::PER_WARP * warp + 16 * mb + i;
+                            for (int i = 0; i < 16; i++) {
+                                const int r = S::PER_WARP * warp + 16 * mb + i;
 #pragma unroll
-                                    for (int mt = 0; mt < MT; mt++)
+                                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                                        for (int h = 0; h < 2; h++) {
-                                            const uint16_t bits = *reinterpret_cast<const uint16_t*>(stage + S::KV_BYTES + kr_offset<RB, TILE>(r, 2 * mt + h) + 2 * g8);
-                                            if (not_finite<PB>(bits)) {
-                                                const float x = PB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+                                    for (int h = 0; h < 2; h++) {
+                                        const uint16_t bits = *reinterpret_cast<const uint16_t*>(stage + S::KV_BYTES + kr_offset<RB, TILE>(r, 2 * mt + h) + 2 * g8);
+                                        if (not_finite<PB>(bits)) {
+                                            const float x = PB ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
 #pragma unroll
-                                                for (int nt = 0; nt < NT; nt++)
+                                            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                                    for (int e = 0; e < 2; e++)
-                                                        if (kv_sees(pos[nt][e], base + r, P.window, P.sinks)) o[mt][nt][2 * h + e] += x;
-                                            }
+                                                for (int e = 0; e < 2; e++)
+                                                    if (kv_sees(pos[nt][e], base + r, P.window, P.sinks)) o[mt][nt][2 * h + e] += x;
                                         }
-                                }
+                                    }
                             }
                         }
                     }
-                    if (t + 1 < t1) {  // (the last tile's slot is kept for the meeting)
-                        __syncwarp();
-                        if (lane == 0) kv_bar_arrive(&empty[st]);
-                        if (++st == S::STAGES) { st = 0; ph ^= 1u; }
-                    }
+                }
+                if (t + 1 < t1) {  // (the last tile's slot is kept for the meeting)
+                    __syncwarp();
+                    if (lane == 0) kv_bar_arrive(&empty[st]);
+                    if (++st == S::STAGES) { st = 0; ph ^= 1u; }
                 }
             }
             const int head = walk.head;
@@ -688,7 +579,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) kv_rows_kernel(const __grid_con
                         const float inv = 1.0f / lsum[nt][e];
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int d = U4 ? 32 * (mt >> 1) + 4 * g8 + 2 * (mt & 1) + h : I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
+                            const int d = I8 ? 16 * mt + 2 * g8 + h : 16 * mt + 8 * h + g8;
                             if (done) kv_store1(P.out, at + d, pos[nt][e] < 0 ? 0.0f : y[2 * h + e] * inv);
                             else part[r * HD + d] = y[2 * h + e];
                         }
@@ -777,11 +668,11 @@ cudaError_t kr_by_variant(int type, bool qb, int hd, int nt, F f) {
     auto by_hd = [&](auto t, auto b) { return hd == 128 ? by_nt(t, b, std::integral_constant<int, 128>()) : by_nt(t, b, std::integral_constant<int, 64>()); };
     if (type == L2_F16) return by_hd(std::integral_constant<int, L2_F16>(), std::false_type());
     if (type == L2_BF16) return by_hd(std::integral_constant<int, L2_BF16>(), std::true_type());
-    if (type == L2_U4) return qb ? by_hd(std::integral_constant<int, L2_U4>(), std::true_type()) : by_hd(std::integral_constant<int, L2_U4>(), std::false_type());
     return qb ? by_hd(std::integral_constant<int, L2_I8>(), std::true_type()) : by_hd(std::integral_constant<int, L2_I8>(), std::false_type());
 }
 
 int kr_nt(int lim) { return lim <= 8 ? 1 : 2; }
+int kr_tile(int type, int head_size) { return head_size * (type == L2_I8 ? 1 : 2) == 256 ? 64 : 128; }
 // CTAs of a launch: two an SM, no more than the line can be long (which is KR_SETUP + 1 or more)
 int kr_grid(const KvStep& s, const KvPool& p, int tile, int sms) {
     const int64_t tiles = (int64_t)s.n_seqs * p.n_kv_heads * ((((int64_t)s.width << p.page_shift) + tile - 1) / tile + 1 + KR_SETUP);
@@ -799,18 +690,20 @@ int kv_rows_limit(const KvStep& s, int group) {
 size_t kv_rows_work(const KvStep& s, const KvPool& p, int group, int type, int head_size, int sms) {
     const int lim = kv_rows_limit(s, group);
     if (!lim) return 0;
-    const int grid = kr_grid(s, p, kr_tile(type, head_size, kr_nt(lim)), sms);
+    if (type == L2_U4) return kv_rows4_work(s, p, lim, head_size, sms);
+    const int grid = kr_grid(s, p, kr_tile(type, head_size), sms);
     return kv_cut_bytes(grid) + (size_t)grid * 2 * 8 * kr_nt(lim) * (head_size + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_rows(const KvAttendParams& p, int type, int head_size, int sms, cudaStream_t st) {
     const int lim = kv_rows_limit(p.step, p.group);
     if (!lim) return cudaSuccess;
-    const int nt = kr_nt(lim), tile = kr_tile(type, head_size, nt);
+    if (type == L2_U4) return launch_kv_rows4(p, lim, head_size, sms, st);
+    const int tile = kr_tile(type, head_size);
     CUtensorMap mk, mv;
     if (cudaError_t e = kv_map(&mk, p.pool, p.pool.k, type, head_size, tile)) return e;
     if (cudaError_t e = kv_map(&mv, p.pool, p.pool.v, type, head_size, tile)) return e;
-    const int grid = kr_grid(p.step, p.pool, tile, sms);
+    const int nt = kr_nt(lim), grid = kr_grid(p.step, p.pool, tile, sms);
     cudaError_t e = kr_by_variant(type, p.q.type == L2_BF16, head_size, nt, [&](auto t, auto b, auto h, auto n) {
         constexpr int T = decltype(t)::value, HD = decltype(h)::value, NT = decltype(n)::value;
         auto kernel = kv_rows_kernel<T, decltype(b)::value, HD, NT>;

@@ -5,8 +5,9 @@
 //   release: positions from keep_b on, and those that a window has left behind, go: page i of all of them to free[count + total - 1 - i],
 //            so that a release of what a plan has added leaves lists and tables as they were
 //
-// A few kilobytes and a chain of dependent loads: nothing but latency.  So one launch of one cluster: a CTA has a run of sequences, a thread a sequence (pages of one that has many: the
-// lanes of its warp), and the sums in front of a CTA's run come from the others' shared memory.  Nothing goes through atomics, and the order of pages does not depend on who was first.
+// A few kilobytes and a chain of dependent loads: nothing but latency.  So one launch of one cluster, and work shared out by rows and by entries, not by sequences (long prompts
+// often stand side by side: with a warp for a sequence's pages, 24 of them among 500 took 79 us).  Every CTA sums up all sequences by itself, in shared memory, which costs less than
+// asking the others; they meet once, before the first writes what another may still read.  Nothing goes through atomics, and the order of pages does not depend on who was first.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -21,8 +22,7 @@ namespace l2 {
 namespace {
 
 constexpr int TB_THREADS = 512, TB_WARPS = TB_THREADS / 32, TB_CLUSTER = 8;
-constexpr int TB_STARTS = 8192;  // first rows that a CTA keeps in shared memory
-constexpr int TB_ALONE = 4;      // pages that a lane takes by itself
+constexpr int TB_SEQS = 16384;  // whose sums a CTA's shared memory holds
 
 struct TbParams {
     int* table; int* kv_len; int* free_pages; int* free_count; int* status;
@@ -31,10 +31,9 @@ struct TbParams {
     int* row_start; long long* slots; int* positions;
     int n_rows, max_rows;
     int window, sinks;
-    int per;            // sequences of a CTA
 };
 
-__device__ __forceinline__ void tb_sync(int ctas) {  // of the cluster, what was written to memory included
+__device__ __forceinline__ void tb_sync(int ctas) {  // of the cluster
     if (ctas == 1) { __syncthreads(); return; }
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
@@ -76,20 +75,6 @@ __device__ __forceinline__ void tb_sums(const long long (&v)[N], long long (&bef
     }
 }
 
-// What the CTAs in front of this one have, and all of them: mine is this CTA's totals, in shared memory.
-template <int N>
-__device__ __forceinline__ void tb_cluster(const long long (*mine)[N], int cta, int ctas, long long (&before)[N], long long (&total)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int lane = threadIdx.x & 31;
-        long long s = 0;
-        if (lane < ctas) s = ctas == 1 ? (*mine)[i] : tb_remote(&(*mine)[i], lane);
-        const long long inc = tb_scan(s);
-        total[i] = __shfl_sync(0xffffffffu, inc, ctas - 1);
-        before[i] = __shfl_sync(0xffffffffu, inc - s, cta);
-    }
-}
-
 // The number of free pages, put right (and reported) where it cannot be one.
 __device__ __forceinline__ int tb_free(const TbParams& P, bool report) {
     const int n = *P.free_count;
@@ -98,122 +83,105 @@ __device__ __forceinline__ int tb_free(const TbParams& P, bool report) {
     return n < 0 ? 0 : P.n_pages;
 }
 __device__ __forceinline__ int tb_pages(const TbParams& P, long long positions) { return (int)((positions + (1 << P.page_shift) - 1) >> P.page_shift); }
-
-struct TbPlan { int len, n, have, need; };  // positions, new rows; pages before and after
-__device__ __forceinline__ TbPlan tb_plan(const TbParams& P, int b, bool report) {
-    TbPlan s{P.kv_len[b], P.counts[b], 0, 0};
-    const long long most = (long long)P.width << P.page_shift;
-    int wrong = 0;
-    if (s.n < 0 || s.n > P.max_rows) { wrong = L2_KV_BAD_ROWS; s.n = 0; }
-    if (s.len < 0 || (long long)s.len + s.n > most) { wrong |= L2_KV_BAD_LENGTH; s.n = 0; }
-    if (wrong && report) kv_report(P.status, wrong);
-    if (s.n) { s.have = tb_pages(P, s.len); s.need = tb_pages(P, (long long)s.len + s.n); }
-    return s;
+__device__ __forceinline__ bool tb_is_page(const TbParams& P, int e) { return (unsigned)e < (unsigned)P.n_pages; }
+// The last of n ascending numbers that is not above x (the first is not).
+__device__ __forceinline__ int tb_find(const int* a, int n, int x) {
+    int lo = 0;
+    for (int hi = n; hi - lo > 1;) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
 }
 
 __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_constant__ TbParams P) {
-    __shared__ long long scratch[TB_WARPS][2], mine[1][2];
-    __shared__ int starts[TB_STARTS + 1];
-    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
-    const int b0 = min((long long)P.n_seqs, (long long)cta * P.per), b1 = min((long long)P.n_seqs, (long long)b0 + P.per);
+    extern __shared__ int tb_smem[];
+    int* const starts = tb_smem;                      // [n_seqs + 1] first rows
+    int* const taken = tb_smem + P.n_seqs + 1;        // [n_seqs + 1] pages taken in front of a sequence
+    int* const lengths = tb_smem + 2 * P.n_seqs + 2;  // [n_seqs] before the step
+    __shared__ long long scratch[TB_WARPS][2];
+    const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int count = tb_free(P, cta == 0 && tid == 0);
-    // ---- rows and pages of this CTA's sequences; the first of a thread stays in registers
-    TbPlan first{0, 0, 0, 0};
-    long long sum[2] = {0, 0}, before[2], total[2];
-    for (int b = b0 + tid; b < b1; b += TB_THREADS) {
-        const TbPlan s = tb_plan(P, b, true);
-        if (b == b0 + tid) first = s;
-        sum[0] += s.n;
-        sum[1] += s.need - s.have;
+    // ---- rows and pages of all sequences.  (Sums that pass 31 bits are of steps without room, whose sums nobody uses.)
+    long long all[2] = {0, 0};
+    for (int b0 = 0; b0 < P.n_seqs; b0 += TB_THREADS) {
+        const int b = b0 + tid;
+        long long v[2] = {0, 0}, before[2], total[2];
+        if (b < P.n_seqs) {
+            const int len = P.kv_len[b];
+            int n = P.counts[b], wrong = 0;
+            if (n < 0 || n > P.max_rows) { wrong = L2_KV_BAD_ROWS; n = 0; }
+            if (len < 0 || (long long)len + n > (long long)P.width << P.page_shift) { wrong |= L2_KV_BAD_LENGTH; n = 0; }
+            if (wrong && cta == 0) kv_report(P.status, wrong);
+            v[0] = n;
+            if (n) v[1] = tb_pages(P, (long long)len + n) - tb_pages(P, len);
+            lengths[b] = len;
+        }
+        tb_sums<2>(v, before, total, scratch);
+        if (b < P.n_seqs) { starts[b] = (int)(all[0] + before[0]); taken[b] = (int)(all[1] + before[1]); }
+        all[0] += total[0];
+        all[1] += total[1];
     }
-    tb_sums<2>(sum, before, total, scratch);
-    if (tid == 0) { mine[0][0] = total[0]; mine[0][1] = total[1]; }
-    tb_sync(ctas);
-    long long front[2], all[2];
-    tb_cluster<2>(mine, cta, ctas, front, all);
     const bool room = all[0] <= P.n_rows && all[1] <= count;
-    if (!room) {  // nothing changes, and no sequence brings rows
-        if (cta == 0 && tid == 0) kv_report(P.status, L2_KV_NO_ROOM);
-        for (int b = b0 + tid; b < b1; b += TB_THREADS) P.row_start[b] = 0;
-        if (cta == 0 && tid == 0) P.row_start[P.n_seqs] = 0;
-        all[0] = 0;
-    } else {
-        if (cta == 0 && tid == 0) { *P.free_count = count - (int)all[1]; P.row_start[P.n_seqs] = (int)all[0]; }
-        const bool once = b1 - b0 <= TB_THREADS;
-        for (int c0 = b0; c0 < b1; c0 += TB_THREADS) {
-            const int b = c0 + tid;
-            TbPlan s = first;
-            if (c0 != b0) s = b < b1 ? tb_plan(P, b, false) : TbPlan{0, 0, 0, 0};
-            long long at[2] = {before[0], before[1]};
-            if (!once) {
-                const long long v[2] = {s.n, s.need - s.have};
-                long long t[2];
-                tb_sums<2>(v, at, t, scratch);
-                at[0] += front[0]; at[1] += front[1];
-                front[0] += t[0]; front[1] += t[1];
-            } else {
-                at[0] += front[0]; at[1] += front[1];
-            }
-            if (b < b1) {
-                P.row_start[b] = (int)at[0];
-                if (s.n) P.kv_len[b] = s.len + s.n;
-            }
-            // pages: of the free list from its end
-            auto take = [&](int seq, int have, int from, int i) {
-                int page = P.free_pages[count - 1 - (from + i)];
-                if ((unsigned)page >= (unsigned)P.n_pages) { kv_report(P.status, L2_KV_BAD_PAGE); page = -1; }
-                P.table[(size_t)seq * P.width + have + i] = page;
-            };
-            const int n = s.need - s.have, from = (int)at[1];
-            if (n <= TB_ALONE)
-                for (int i = 0; i < n; i++) take(b, s.have, from, i);
-            for (unsigned many = __ballot_sync(0xffffffffu, n > TB_ALONE); many; many &= many - 1) {
-                const int src = __ffs(many) - 1;
-                const int m = __shfl_sync(0xffffffffu, n, src), f = __shfl_sync(0xffffffffu, from, src), h = __shfl_sync(0xffffffffu, s.have, src);
-                for (int i = lane; i < m; i += 32) take(b - lane + src, h, f, i);
-            }
-        }
+    const int rows = room ? (int)all[0] : 0, pages = room ? (int)all[1] : 0;
+    if (tid == 0) { starts[P.n_seqs] = rows; taken[P.n_seqs] = pages; }
+    tb_sync(ctas);  // all have read the lengths and the number of free pages
+    if (cta == 0 && tid == 0) {
+        if (!room) kv_report(P.status, L2_KV_NO_ROOM);  // nothing changes, and no sequence brings rows
+        else *P.free_count = count - pages;
+        P.row_start[P.n_seqs] = rows;
     }
-    tb_sync(ctas);  // (also: nobody reads this CTA's shared memory any more)
-    if (!P.slots && !P.positions) return;
-    // ---- a slot and a position for every row, four rows a thread
-    // (What other CTAs have written is read past the L1.)
-    const bool near = P.n_seqs <= TB_STARTS;
-    if (near) {
-        for (int b = tid; b <= P.n_seqs; b += TB_THREADS) starts[b] = __ldcg(P.row_start + b);
-        __syncthreads();
+    for (int b = cta * TB_THREADS + tid; b < P.n_seqs; b += ctas * TB_THREADS) {
+        P.row_start[b] = room ? starts[b] : 0;
+        const int n = room ? starts[b + 1] - starts[b] : 0;
+        if (n) P.kv_len[b] = lengths[b] + n;
     }
-    auto start = [&](int b) { return near ? starts[b] : __ldcg(P.row_start + b); };
-    const int rows = (int)all[0], mask = (1 << P.page_shift) - 1;
-    for (int r0 = 4 * (cta * TB_THREADS + tid); r0 < P.n_rows; r0 += 4 * ctas * TB_THREADS) {
-        int b = 0, end = 0, len = 0;
-        if (r0 < rows) {  // the last sequence that begins at r0 or before
-            int hi = P.n_seqs;
-            while (hi - b > 1) {
-                const int mid = (b + hi) >> 1;
-                if (start(mid) <= r0) b = mid;
-                else hi = mid;
-            }
-            end = start(b + 1);
-            len = __ldcg(P.kv_len + b);
+    // page i of the step: of the free list, from its end
+    auto page = [&](int i) {
+        const int e = P.free_pages[count - 1 - i];
+        if (tb_is_page(P, e)) return e;
+        kv_report(P.status, L2_KV_BAD_PAGE);
+        return -1;
+    };
+    if (!P.slots && !P.positions) {
+        for (int i = cta * TB_THREADS + tid; i < pages; i += ctas * TB_THREADS) {
+            const int b = tb_find(taken, P.n_seqs, i);  // (the last sequence with so many in front: the one that takes it)
+            P.table[(size_t)b * P.width + tb_pages(P, lengths[b]) + i - taken[b]] = page(i);
         }
-        long long slot[4];
-        int pos[4];
+        return;
+    }
+    // ---- a slot and a position for every row, a few rows a thread; the first row of a new page brings it into the table
+    const int mask = (1 << P.page_shift) - 1;
+    constexpr int N = 4;
+    for (int r0 = N * (cta * TB_THREADS + tid); r0 < P.n_rows; r0 += N * ctas * TB_THREADS) {
+        long long slot[N];
+        int pos[N];
+        int b = r0 < rows ? tb_find(starts, P.n_seqs, r0) : 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < N; i++) {
             const int r = r0 + i;
             slot[i] = pos[i] = -1;
             if (r >= rows) continue;
-            while (r >= end) { b++; end = start(b + 1); if (r < end) len = __ldcg(P.kv_len + b); }
-            pos[i] = len - (end - r);
-            const int page = __ldcg(P.table + (size_t)b * P.width + (pos[i] >> P.page_shift));
-            if ((unsigned)page < (unsigned)P.n_pages) slot[i] = ((long long)page << P.page_shift) + (pos[i] & mask);
-            else kv_report(P.status, L2_KV_BAD_PAGE);
+            while (r >= starts[b + 1]) b++;
+            const int len = lengths[b], have = tb_pages(P, len);
+            pos[i] = len + r - starts[b];
+            const int at = pos[i] >> P.page_shift;
+            int* const entry = P.table + (size_t)b * P.width + at;
+            int e;
+            if (at >= have) {
+                e = page(taken[b] + at - have);
+                if ((pos[i] & mask) == 0) *entry = e;
+            } else {
+                e = *entry;
+                if (!tb_is_page(P, e)) { kv_report(P.status, L2_KV_BAD_PAGE); e = -1; }
+            }
+            if (e >= 0) slot[i] = ((long long)e << P.page_shift) + (pos[i] & mask);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < N; i++)
             if (r0 + i < P.n_rows) {
                 if (P.slots) P.slots[r0 + i] = slot[i];
                 if (P.positions) P.positions[r0 + i] = pos[i];
@@ -221,114 +189,101 @@ __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_consta
     }
 }
 
-// Pages of a sequence that go: entries lo[0] .. hi[0] - 1 (behind the window) and lo[1] .. hi[1] - 1 (from the length to keep on).
-struct TbRelease { int len, keep, lo[2], hi[2]; };
-__device__ __forceinline__ TbRelease tb_release(const TbParams& P, int b, bool report) {
-    TbRelease s{P.kv_len[b], 0, {0, 0}, {0, 0}};
-    const long long most = (long long)P.width << P.page_shift;
-    const int keep = P.counts ? P.counts[b] : s.len;
-    s.keep = min(s.len, keep);
-    if (s.len < 0 || s.len > most || keep < 0) {  // left as it is
-        if (report) kv_report(P.status, L2_KV_BAD_LENGTH);
-        s.keep = s.len;
-        return s;
-    }
-    s.lo[1] = tb_pages(P, s.keep);
-    s.hi[1] = tb_pages(P, s.len);
+// Entries of a sequence that go, behind the window and from the length to keep on: first[0] .. first[0] + n[0] - 1, then first[1] .. first[1] + n[1] - 1.
+struct TbGone { int first[2], n[2]; };
+__device__ __forceinline__ TbGone tb_gone(const TbParams& P, int len, int keep) {
+    TbGone g;
+    g.first[1] = tb_pages(P, keep);
+    g.n[1] = tb_pages(P, len) - g.first[1];
+    g.first[0] = g.n[0] = 0;
     if (P.window) {  // the next row, at position keep, sees none from keep - window on back, but for the sinks
-        s.lo[0] = (int)min((long long)s.lo[1], ((long long)P.sinks + (1 << P.page_shift) - 1) >> P.page_shift);
-        s.hi[0] = max(s.lo[0], max(0, s.keep - P.window + 1) >> P.page_shift);
+        g.first[0] = (int)min((long long)g.first[1], ((long long)P.sinks + (1 << P.page_shift) - 1) >> P.page_shift);
+        g.n[0] = max(0, (max(0, keep - P.window + 1) >> P.page_shift) - g.first[0]);
     }
-    return s;
+    return g;
 }
 
 __global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_constant__ TbParams P) {
-    __shared__ long long scratch[TB_WARPS][1], mine[1][1];
-    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
-    const int b0 = min((long long)P.n_seqs, (long long)cta * P.per), b1 = min((long long)P.n_seqs, (long long)b0 + P.per);
+    extern __shared__ int tb_smem[];
+    int* const from = tb_smem;                     // [n_seqs] entries in front of a sequence's
+    int* const lengths = tb_smem + P.n_seqs;       // [n_seqs]
+    int* const kept = tb_smem + 2 * P.n_seqs;      // [n_seqs]
+    __shared__ long long scratch[TB_WARPS][1], mine;
+    const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int count = tb_free(P, cta == 0 && tid == 0);
-    // f(entry, its place in the free list) for the pages of the lanes' sequences that go, from `place` down; how many they are
-    auto walk = [&](const TbRelease& s, int b, bool report, long long place, auto f) {
-        int pages = 0;
-        auto look = [&](int seq, int i) {
-            const int e = P.table[(size_t)seq * P.width + i];
-            const bool is = (unsigned)e < (unsigned)P.n_pages;
-            if (!is && e != -1 && report) kv_report(P.status, L2_KV_BAD_PAGE);
-            return is;
-        };
-        const int n = s.hi[0] - s.lo[0] + s.hi[1] - s.lo[1];
-        if (n <= 2 * TB_ALONE) {
-            for (int k = 0; k < n; k++) {
-                const int i = k < s.hi[0] - s.lo[0] ? s.lo[0] + k : s.lo[1] + k - (s.hi[0] - s.lo[0]);
-                if (look(b, i)) f((size_t)b * P.width + i, place - pages++);
+    long long entries = 0;
+    for (int b0 = 0; b0 < P.n_seqs; b0 += TB_THREADS) {
+        const int b = b0 + tid;
+        long long v[1] = {0}, before[1], total[1];
+        if (b < P.n_seqs) {
+            int len = P.kv_len[b], keep = P.counts ? P.counts[b] : len;
+            if (len < 0 || len > (long long)P.width << P.page_shift || keep < 0) {  // left as it is
+                if (cta == 0) kv_report(P.status, L2_KV_BAD_LENGTH);
+                lengths[b] = kept[b] = -1;
+            } else {
+                lengths[b] = len;
+                kept[b] = min(len, keep);
+                const TbGone g = tb_gone(P, len, kept[b]);
+                v[0] = g.n[0] + g.n[1];
             }
         }
-        for (unsigned many = __ballot_sync(0xffffffffu, n > 2 * TB_ALONE); many; many &= many - 1) {
-            const int src = __ffs(many) - 1;
-            int at = 0;
-            const long long top = __shfl_sync(0xffffffffu, place, src);
-#pragma unroll
-            for (int part = 0; part < 2; part++) {
-                const int lo = __shfl_sync(0xffffffffu, s.lo[part], src), hi = __shfl_sync(0xffffffffu, s.hi[part], src);
-                for (int i0 = lo; i0 < hi; i0 += 32) {
-                    const bool is = i0 + lane < hi && look(b - lane + src, i0 + lane);
-                    const unsigned votes = __ballot_sync(0xffffffffu, is);
-                    if (is) f((size_t)(b - lane + src) * P.width + i0 + lane, top - at - __popc(votes & ((1u << lane) - 1)));
-                    at += __popc(votes);
-                }
-            }
-            if (lane == src) pages = at;
-        }
-        return pages;
+        tb_sums<1>(v, before, total, scratch);
+        if (b < P.n_seqs) from[b] = (int)(entries + before[0]);
+        entries += total[0];
+    }
+    __syncthreads();
+    // ---- a run of the entries for each CTA.  The pages among them are counted, then put on the list below those of the entries in front
+    const int per = (int)((entries + ctas - 1) / ctas), e0 = (int)min(entries, (long long)cta * per), e1 = (int)min(entries, (long long)e0 + per);
+    auto find = [&](int i) {  // entry i of all, in the tables
+        const int b = tb_find(from, P.n_seqs, i);
+        const TbGone g = tb_gone(P, lengths[b], kept[b]);
+        const int k = i - from[b];
+        return P.table + (size_t)b * P.width + (k < g.n[0] ? g.first[0] + k : g.first[1] + k - g.n[0]);
     };
-    auto nothing = [](size_t, long long) {};
-    TbRelease first{0, 0, {0, 0}, {0, 0}};
-    int first_pages = 0;
-    long long sum[1] = {0}, before[1], total[1];
-    for (int c0 = b0; c0 < b1; c0 += TB_THREADS) {
-        const int b = c0 + tid;
-        TbRelease s{0, 0, {0, 0}, {0, 0}};
-        if (b < b1) s = tb_release(P, b, true);
-        const int pages = walk(s, b, true, 0, nothing);
-        if (c0 == b0) { first = s; first_pages = pages; }
-        sum[0] += pages;
-    }
-    tb_sums<1>(sum, before, total, scratch);
-    if (tid == 0) mine[0][0] = total[0];
-    tb_sync(ctas);
-    long long front[1], all[1];
-    tb_cluster<1>(mine, cta, ctas, front, all);
-    if (cta == 0 && tid == 0) {
-        if (all[0] > P.n_pages - count) kv_report(P.status, L2_KV_BAD_PAGE);  // (more pages than there are: some were in two tables)
-        *P.free_count = (int)min((long long)P.n_pages, count + all[0]);
-    }
-    const bool once = b1 - b0 <= TB_THREADS;
-    for (int c0 = b0; c0 < b1; c0 += TB_THREADS) {
-        const int b = c0 + tid;
-        TbRelease s = first;
-        long long at = before[0];
-        if (!once) {
-            int pages = first_pages;
-            if (c0 != b0) {
-                s = b < b1 ? tb_release(P, b, false) : TbRelease{0, 0, {0, 0}, {0, 0}};
-                pages = walk(s, b, false, 0, nothing);
-            }
-            const long long v[1] = {pages};
-            long long a[1], t[1];
-            tb_sums<1>(v, a, t, scratch);
-            at = a[0] + front[0];
-            front[0] += t[0];
-        } else {
-            at += front[0];
+    int* at = nullptr;
+    int e = -1;
+    long long v[1] = {0}, before[1], total[1];
+    for (int i0 = e0; i0 < e1; i0 += TB_THREADS) {
+        at = nullptr;
+        e = -1;
+        if (i0 + tid < e1) {
+            at = find(i0 + tid);
+            e = *at;
+            if (tb_is_page(P, e)) v[0]++;
+            else if (e != -1) kv_report(P.status, L2_KV_BAD_PAGE);
         }
-        walk(s, b, false, count + all[0] - 1 - at, [&](size_t entry, long long to) {
-            if (to >= 0 && to < P.n_pages) P.free_pages[to] = P.table[entry];
-            P.table[entry] = -1;
-        });
-        if (b < b1 && s.keep != s.len) P.kv_len[b] = s.keep;
     }
+    const bool once = e1 - e0 <= TB_THREADS;  // (at and e are then what they will be below)
+    tb_sums<1>(v, before, total, scratch);
+    if (tid == 0) mine = total[0];
+    tb_sync(ctas);  // (also: all have read the lengths and the number of free pages)
+    long long others = 0;
+    if ((tid & 31) < ctas) others = ctas == 1 ? mine : tb_remote(&mine, tid & 31);
+    const long long inc = tb_scan(others), all = __shfl_sync(0xffffffffu, inc, ctas - 1);
+    long long front = __shfl_sync(0xffffffffu, inc - others, cta);
+    if (cta == 0 && tid == 0) {
+        if (all > P.n_pages - count) kv_report(P.status, L2_KV_BAD_PAGE);  // (more pages than there are: some were in two tables)
+        *P.free_count = (int)min((long long)P.n_pages, count + all);
+    }
+    for (int i0 = e0; i0 < e1; i0 += TB_THREADS) {
+        if (!once) {
+            at = nullptr;
+            e = -1;
+            if (i0 + tid < e1) { at = find(i0 + tid); e = *at; }
+            v[0] = tb_is_page(P, e);
+            tb_sums<1>(v, before, total, scratch);
+        }
+        if (at && tb_is_page(P, e)) {
+            const long long to = count + all - 1 - (front + before[0]);
+            if (to >= 0 && to < P.n_pages) P.free_pages[to] = e;
+            *at = -1;
+        }
+        front += total[0];
+    }
+    for (int b = cta * TB_THREADS + tid; b < P.n_seqs; b += ctas * TB_THREADS)
+        if (kept[b] < lengths[b]) P.kv_len[b] = kept[b];
     tb_sync(ctas);  // (nobody reads this CTA's shared memory any more)
 }
 
@@ -337,8 +292,8 @@ int check_tables(const char* who, const l2_kv_tables* t, TbParams* out) {
     int shift = 3;
     while (shift < 8 && (1 << shift) < t->page_size) shift++;
     if ((1 << shift) != t->page_size) return fail(L2_EINVAL, "%s: page size %d (8, 16, 32, 64, 128 or 256)", who, t->page_size);
-    if (t->n_seqs < 0 || t->n_seqs > 65536 || t->table_width < 0 || t->n_pages < 1) return fail(L2_EINVAL, "%s: %d sequences (at most 65536), tables of %d, %d pages", who, t->n_seqs, t->table_width, t->n_pages);
-    if ((int64_t)t->table_width * t->page_size > (1 << 30)) return fail(L2_ERANGE, "%s: more than 2^30 positions", who);
+    if (t->n_seqs < 0 || t->n_seqs > TB_SEQS || t->table_width < 0 || t->n_pages < 1) return fail(L2_EINVAL, "%s: %d sequences (at most %d), tables of %d, %d pages", who, t->n_seqs, TB_SEQS, t->table_width, t->n_pages);
+    if ((int64_t)t->table_width * t->page_size > (1 << 30) || (int64_t)t->n_seqs * t->table_width > (1 << 30)) return fail(L2_ERANGE, "%s: more than 2^30 positions, or entries of tables", who);
     if (!t->free_pages || !t->free_count || (t->n_seqs && (!t->kv_len || (t->table_width && !t->page_table)))) return fail(L2_EINVAL, "%s: null device pointer", who);
     const void* words[] = {t->page_table, t->kv_len, t->free_pages, t->free_count, t->status};
     for (const void* p : words)
@@ -348,15 +303,18 @@ int check_tables(const char* who, const l2_kv_tables* t, TbParams* out) {
     return L2_OK;
 }
 
-// One cluster of `ctas`, launched programmatically.
-cudaError_t tb_launch(void (*kernel)(const TbParams), TbParams& P, int64_t ctas, cudaStream_t st) {
+// One cluster of up to `ctas`, launched programmatically.
+cudaError_t tb_launch(void (*kernel)(const TbParams), const TbParams& P, int64_t ctas, KvOnce& once, cudaStream_t st) {
+    const int smem = (3 * P.n_seqs + 2) * (int)sizeof(int);
+    if (smem > 40 * 1024)
+        if (cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kernel), (3 * TB_SEQS + 2) * (int)sizeof(int))) return e;
     int n = 1;
     while (n < TB_CLUSTER && n < ctas) n *= 2;
-    P.per = (P.n_seqs + n - 1) / n;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(n);
     cfg.blockDim = dim3(TB_THREADS);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -386,8 +344,8 @@ extern "C" int l2_kv_plan(const l2_kv_tables* tables, const int32_t* new_rows, i
     P.counts = new_rows; P.row_start = row_start; P.slots = reinterpret_cast<long long*>(slots); P.positions = positions; P.n_rows = n_rows; P.max_rows = max_rows;
     int sms;
     if (int rc = kv_device(&sms)) return rc;
-    const int64_t by_rows = slots || positions ? (n_rows + 4 * TB_THREADS - 1) / (4 * TB_THREADS) : 1;
-    L2_CUDA(tb_launch(kv_plan_kernel, P, std::max<int64_t>(by_rows, (P.n_seqs + TB_THREADS - 1) / TB_THREADS), static_cast<cudaStream_t>(cuda_stream)));
+    static KvOnce once;
+    L2_CUDA(tb_launch(kv_plan_kernel, P, (n_rows + 2 * TB_THREADS - 1) / (2 * TB_THREADS), once, static_cast<cudaStream_t>(cuda_stream)));
     return L2_OK;
 }
 
@@ -402,6 +360,7 @@ extern "C" int l2_kv_release(const l2_kv_tables* tables, const int32_t* keep, in
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!P.n_seqs) return L2_OK;
-    L2_CUDA(tb_launch(kv_release_kernel, P, (P.n_seqs + TB_THREADS - 1) / TB_THREADS, static_cast<cudaStream_t>(cuda_stream)));
+    static KvOnce once;
+    L2_CUDA(tb_launch(kv_release_kernel, P, ((int64_t)P.n_seqs * P.width + 4 * TB_THREADS - 1) / (4 * TB_THREADS), once, static_cast<cudaStream_t>(cuda_stream)));
     return L2_OK;
 }

@@ -40,7 +40,6 @@
 #include "kernels.cuh"
 #include "paged_attend.h"
 #include "paged_device.cuh"
-#include "paged_rows4.cuh"
 
 namespace l2 {
 
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                             for (int k = 0; k < 4; k++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
 #pragma unroll
                             for (int x = 1; x < LANES; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                            kr4_q_factors(top, &up, &by);
+                            kv_q_factors(top, &up, &by);
                         }
                         if (tid % LANES == 0) q_by[128 * i + (tid & 127) / LANES + n * Q_ROWS] = by;
                         qx[n] = kt_query<QB, WIDE>(qx[n], up);

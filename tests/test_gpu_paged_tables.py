@@ -93,7 +93,7 @@ def check_plan(tables, lists, new, n_rows, max_rows, **kw):
 
 # one sequence, a few, more than a CTA has threads, more than one run of threads a CTA; steps of single tokens, chunks, and none
 @pytest.mark.parametrize("page", [8, 16, 64, 256])
-@pytest.mark.parametrize("seqs", [1, 2, 31, 33, 64, 511, 513, 1500, 5000])
+@pytest.mark.parametrize("seqs", [1, 2, 31, 33, 64, 511, 513, 1500, 5000, 16384])
 def test_steps(l2, seqs, page):
     rng = np.random.default_rng(seqs + page)
     width = 12

@@ -20,7 +20,7 @@ def release(l2, t, keep=A, window=0, sinks=0):
     return l2.lib.l2_kv_release(C.byref(t) if t is not None else None, keep, window, sinks, None)
 
 
-BAD_TABLES = [dict(page_size=0), dict(page_size=24), dict(page_size=4), dict(page_size=512), dict(n_seqs=-1), dict(n_seqs=65537), dict(table_width=-1), dict(n_pages=0), dict(free_pages=None),
+BAD_TABLES = [dict(page_size=0), dict(page_size=24), dict(page_size=4), dict(page_size=512), dict(n_seqs=-1), dict(n_seqs=16385), dict(table_width=-1), dict(n_pages=0), dict(free_pages=None),
               dict(free_count=None), dict(kv_len=None), dict(page_table=None), dict(kv_len=A + 2), dict(status=A + 1), dict(free_pages=A + 3)]
 
 
@@ -36,6 +36,7 @@ def test_arguments(l2):
     for bad in (dict(window=-1), dict(sinks=-1), dict(keep=A + 2)):
         assert release(l2, t, **bad) == -1, bad
     assert plan(l2, None) == -1 and release(l2, None) == -1
+    assert plan(l2, tables(l2, table_width=1 << 20, n_seqs=1 << 11)) == -5
     assert plan(l2, tables(l2, table_width=1 << 27)) == -5 and release(l2, tables(l2, table_width=1 << 27)) == -5
 
 
