@@ -33,7 +33,7 @@ namespace l2 {
 namespace {
 
 constexpr int R4_WARPS = 4, R4_THREADS = 32 * R4_WARPS;
-constexpr int R4_SETUP = 2;  // what a piece costs besides its tiles, in tiles
+constexpr int R4_SETUP = 3;  // what a piece costs besides its tiles, in tiles
 constexpr int R4_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr float R4_BIAS = 24.0f;  // probabilities carry a factor of 2^24
 
@@ -52,7 +52,7 @@ struct R4Shape {
 struct R4Split { int heads, wph; };
 __host__ __device__ constexpr R4Split r4_split(int n_kv_heads) { return n_kv_heads % 4 == 0 ? R4Split{4, 1} : n_kv_heads % 2 == 0 ? R4Split{2, 2} : R4Split{1, 4}; }
 // The line's tiles: a step of each warp of a head (64 positions where that would be less).
-__host__ __device__ constexpr int r4_shift(int wph, int nt) { return nt == 1 ? wph == 1 ? 6 : wph == 2 ? 7 : 8 : wph == 4 ? 7 : 6; }
+constexpr int r4_least_shift(int wph, int nt) { return nt == 1 ? wph == 1 ? 6 : wph == 2 ? 7 : 8 : wph == 4 ? 7 : 6; }
 
 // Where 16-byte chunk c of row r is: no bank conflicts for eight rows side by side
 template <int ROW>
@@ -102,39 +102,79 @@ struct R4Seq {
         rows = n <= lim ? (int)n : 0;
         view = R4View(s.kv - s.n, s.kv - 1, P.window, P.sinks, shift);
     }
-    __device__ __forceinline__ int64_t length(int units) const { return rows ? (int64_t)(view.tiles + R4_SETUP) * units : 0; }  // on the line
+    __device__ __forceinline__ int length(int units) const { return rows ? (view.tiles + R4_SETUP) * units : 0; }  // on the line
 };
 
-// A CTA's part of the line, one (sequence, heads) at a time.
+// A CTA's part of the line, one (sequence, heads) at a time.  (The line is shorter than 2^31: the host takes tiles that are large enough.)
 struct R4Walk {
-    int64_t w, w1, start, per;
-    int b;
+    int w, w1, start, per, b;
     R4Seq q;
     int unit, t0, t1;
     bool first;  // the piece is the CTA's first
-    __device__ __forceinline__ R4Walk(const KvAttendParams& P, int lim, int shift, const KvSpot& spot) {
-        per = spot.per;
-        w = per * blockIdx.x;
-        w1 = min(spot.total, w + per);
-        start = spot.start; b = spot.b;
+    __device__ __forceinline__ R4Walk() {}
+    // Where the CTA's part begins, by every warp for itself; a lane has four sequences of 128.
+    __device__ __forceinline__ R4Walk(const KvAttendParams& P, int lim, int shift, int units) {
+        const int lane = threadIdx.x & 31;
+        auto lengths = [&](int b0, int (&v)[4]) {  // their sum over the lanes up to this one
+            int sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = b0 + 4 * lane + i;
+                v[i] = at < P.step.n_seqs ? R4Seq(P, lim, shift, at).length(units) : 0;
+                sum += v[i];
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            return sum;
+        };
+        int v[4], inc = lengths(0, v), total = __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll 1
+        for (int b0 = 128; b0 < P.step.n_seqs; b0 += 128) {
+            int x[4];
+            total += __shfl_sync(0xffffffffu, lengths(b0, x), 31);
+        }
+        per = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
+        w = (int)min((int64_t)total, (int64_t)per * blockIdx.x);
+        w1 = (int)min((int64_t)total, (int64_t)w + per);
         first = true;
         t0 = -1; t1 = 0;
-        if (w < w1) q = R4Seq(P, lim, shift, b);
+        start = 0; b = 0;
+        if (w >= w1) return;
+        int front = 0;
+#pragma unroll 1
+        for (int b0 = 0;; b0 += 128) {
+            if (b0) inc = lengths(b0, v);
+            const unsigned past = __ballot_sync(0xffffffffu, front + inc > w);
+            if (past) {
+                const int src = __ffs(past) - 1;
+                int at = front + inc - (v[0] + v[1] + v[2] + v[3]), i = 0;  // (of the lane found, the sequence that w is in)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    if (i == k && at + v[k] <= w) { at += v[k]; i = k + 1; }
+                start = __shfl_sync(0xffffffffu, at, src);
+                b = b0 + 4 * src + __shfl_sync(0xffffffffu, i, src);
+                break;
+            }
+            front += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        q = R4Seq(P, lim, shift, b);
     }
     __device__ __forceinline__ bool next(const KvAttendParams& P, int lim, int shift, int units) {
         if (t0 >= 0) first = false;
 #pragma unroll 1
         while (w < w1) {
-            int64_t length = q.length(units);
-            while (w >= start + length) {
+            int length = q.length(units);
+            while (w - start >= length) {
                 start += length;
                 q = R4Seq(P, lim, shift, ++b);
                 length = q.length(units);
             }
-            const int64_t in = w - start;
-            const int place = q.view.tiles + R4_SETUP;  // of a unit on the line, whose first R4_SETUP are no tiles
-            unit = (int)kv_quotient(in, place);
-            const int at = (int)(in - (int64_t)unit * place), end = (int)min((int64_t)place, at + (w1 - w));
+            const int in = w - start, place = q.view.tiles + R4_SETUP;  // of a unit on the line, whose first R4_SETUP are no tiles
+            unit = (uint32_t)in / (uint32_t)place;
+            const int at = in - unit * place, end = min(place, at + (w1 - w));
             w += end - at;
             if (end <= R4_SETUP) continue;  // (its tiles begin in the next CTA)
             t0 = max(0, at - R4_SETUP);
@@ -289,7 +329,9 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
         top &= 0x7fff7fffu;
         return most >= 0x1p100f || (top & 0xffffu) >= R4_LIMIT || (top >> 16) >= R4_LIMIT;
     };
-    if (__any_sync(0xffffffffu, whole ? probabilities(std::true_type()) : probabilities(std::false_type())) || r.unset) {
+    bool again = r.unset;
+    if (!again) again = __any_sync(0xffffffffu, whole ? probabilities(std::true_type()) : probabilities(std::false_type()));
+    if (again) {
         // seldom: a row's m is raised, or its h lowered, and what was summed is scaled.  (A row's result does not depend on the others.)
         bool none = false;
 #pragma unroll
@@ -366,27 +408,23 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
 // ---- the kernel ----------------------------------------------------------------------------------------------------------------
 // QB: q is bf16, else f16
 template <bool QB, int HD, int NT>
-__global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4_kernel(const __grid_constant__ KvAttendParams P, const int lim) {
+__global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int shift) {
     using S = R4Shape<HD, NT>;
     constexpr int CHUNKS = S::ROW / 16, PER_COPY = 32 / CHUNKS, PAIR_LANES = S::STEP / 4, COPIES = S::STEP / PER_COPY;  // 16-byte chunks of a row; positions of a copy by the warp, copies of a step
     extern __shared__ __align__(128) uint8_t r4_smem[];
-    __shared__ int64_t scratch[R4_WARPS + 2];
     __shared__ R4Piece pieces[R4_WARPS][2];
     __shared__ int2 marks[R4_WARPS][4];  // of a slot: the step's first position; bit 0: every row sees all of it, 1: some row sees something, 2: the piece's last step
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c = lane & 3;
     const R4Split split = r4_split(P.pool.n_kv_heads);
     const int units = P.pool.n_kv_heads / split.heads, of_head = warp / split.wph, share = warp % split.wph;  // this warp's head of the unit, its place among that one's warps
-    const int shift = r4_shift(split.wph, NT), steps = (1 << shift) / (S::STEP * split.wph), slots = S::slots(split.wph);
+    const int steps = (1 << shift) / (S::STEP * split.wph), slots = S::slots(split.wph);
     uint8_t* const ring = r4_smem + warp * slots * S::SLOT;
 
+    // ================= copies: the step in front =====================================================================================
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const KvSpot spot = kv_locate<R4_THREADS>(P.step.n_seqs, blockIdx.x, gridDim.x, scratch, [&](int b) {
-        return b < P.step.n_seqs ? R4Seq(P, lim, shift, b).length(units) : 0; });
+    R4Walk walk(P, lim, shift, units);
     if (tid == 0) kv_cuts(P.work)[blockIdx.x].pieces = 0;  // (no unit that begins here goes on, until one does)
-
-    // ================= copies: the step in front =====================================================================================
-    R4Walk walk(P, lim, shift, spot);
     int t = 0, k = 0, begun = 0, ended = 0, put = 0;  // tile and step in it; pieces begun by the copies, ended by the products; slot to fill
     bool over = false;
     int pages = 0, next_pages = 0, page0 = 0, next0 = -1;  // a lane has entry page0 + lane of the table
@@ -399,10 +437,10 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
     constexpr int SIDE = PER_COPY / 4, IN_BLOCK = 32 / PER_COPY;
     const uint32_t lane_row = ((lane / CHUNKS & 3) * 8 + (lane / CHUNKS >> 2)) * S::ROW, lane_chunk = 16 * (lane % CHUNKS);
     static_assert(SIDE * S::ROW == 128, "the rows of a copy behind those of the one in front");
-    auto look_up = [&](int first) {  // the entries that some row sees; -1 where there is none
-        const int i = first + lane, j = i << P.pool.page_shift;
-        if (i > walk.q.view.hi >> P.pool.page_shift || !walk.q.view.any(j, 1 << P.pool.page_shift, P.window, P.sinks)) return -1;
-        return kv_page(P.step, P.pool, walk.b, i << P.pool.page_shift);
+    auto look_up = [&](int first) {  // the entries that some row sees, as they are (nothing waits for them before they are needed); -2: none of these
+        const int i = first + lane;
+        if (i > walk.q.view.hi >> P.pool.page_shift || (P.window && !walk.q.view.any(i << P.pool.page_shift, 1 << P.pool.page_shift, P.window, P.sinks))) return -2;
+        return P.step.table[(size_t)walk.b * P.step.width + i];
     };
     auto issue = [&]() {  // whether there was a step to bring
         if (t >= walk.t1) {
@@ -414,7 +452,7 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
             const bool done = walk.t0 == 0 && walk.t1 == walk.q.view.tiles;
             if (lane == 0) pieces[warp][begun & 1] = R4Piece{walk.q.s.row0, walk.q.rows, head, walk.q.view.lo, done ? -1 : walk.first ? 0 : 1};
             if (tid == 0 && walk.t0 == 0 && !done)  // what the kernel behind this one has to know of the CTA's last piece
-                kv_cuts(P.work)[blockIdx.x] = KvCut{(int)kv_quotient(walk.w - walk.t1 + walk.q.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, walk.q.rows,
+                kv_cuts(P.work)[blockIdx.x] = KvCut{(int)((uint32_t)(walk.w - walk.t1 + walk.q.view.tiles - 1) / (uint32_t)walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, walk.q.rows,
                                                     walk.unit * split.heads, walk.q.s.row0, walk.q.view.lo, 0};
             k_lane = P.pool.k + (int64_t)head * (P.pool.head_stride / 2) + lane_chunk + (PER_COPY <= 8 || mask >= PER_COPY - 1 ? lane / CHUNKS : lane / CHUNKS & mask) * pos_bytes;
             pair_lane = reinterpret_cast<const char*>(lane < PAIR_LANES ? P.pool.ks : P.pool.vs) + (((int64_t)head << P.pool.page_shift) + (4 * (lane % PAIR_LANES) & mask)) * 4;
@@ -433,6 +471,8 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
                 else { page0 = want; pages = look_up(page0); }
                 next0 = page0 + 32;  // (steps go on by whole pages, or within one, and by a divisor of 32 of them)
                 next_pages = look_up(next0);
+                if (pages != -2 && (unsigned)pages >= (unsigned)P.pool.n_pages) kv_report(P.step.status, L2_KV_BAD_PAGE);
+                if ((unsigned)pages >= (unsigned)P.pool.n_pages) pages = -1;
                 there = __ballot_sync(0xffffffffu, pages >= 0);
             }
             // (a step begins a page or lies inside one)
@@ -702,30 +742,35 @@ __global__ void __launch_bounds__(256) kv_rows4_combine_kernel(const __grid_cons
 }
 
 int r4_nt(int lim) { return lim <= 8 ? 1 : 2; }
-// CTAs of a launch: no more than the line can be long (which is R4_SETUP + 1 or more)
-int r4_grid(const KvStep& s, const KvPool& p, int nt, int sms) {
+// Tiles that are so large that the line stays below 2^31, and the CTAs of a launch: no more than the line can be long (which is R4_SETUP + 1 or more).
+struct R4Grid { int shift, ctas; };
+R4Grid r4_grid(const KvStep& s, const KvPool& p, int nt, int sms) {
     const R4Split split = r4_split(p.n_kv_heads);
-    const int shift = r4_shift(split.wph, nt);
-    const int64_t tiles = (int64_t)s.n_seqs * (p.n_kv_heads / split.heads) * (((((int64_t)s.width << p.page_shift) + (1 << shift) - 1) >> shift) + 1 + R4_SETUP);
-    return (int)std::min<int64_t>((nt == 1 ? R4Shape<128, 1>::ctas(split.wph) : R4Shape<128, 2>::ctas(split.wph)) * sms, tiles);
+    for (int shift = r4_least_shift(split.wph, nt);; shift++) {
+        const int64_t most = (int64_t)s.n_seqs * (p.n_kv_heads / split.heads) * (((((int64_t)s.width << p.page_shift) + (1 << shift) - 1) >> shift) + 1 + R4_SETUP);
+        if (most < ((int64_t)1 << 31) - 65536 || shift == 30)
+            return {shift, (int)std::min<int64_t>((nt == 1 ? R4Shape<128, 1>::ctas(split.wph) : R4Shape<128, 2>::ctas(split.wph)) * sms, most)};
+    }
 }
 
 }  // namespace
 
 size_t kv_rows4_work(const KvStep& s, const KvPool& p, int lim, int head_size, int sms) {
-    const int nt = r4_nt(lim), grid = r4_grid(s, p, nt, sms);
+    const int nt = r4_nt(lim), grid = r4_grid(s, p, nt, sms).ctas;
     return kv_cut_bytes(grid) + (size_t)grid * 2 * r4_split(p.n_kv_heads).heads * 8 * nt * (head_size + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_rows4(const KvAttendParams& p, int lim, int head_size, int sms, cudaStream_t st) {
-    const int nt = r4_nt(lim), grid = r4_grid(p.step, p.pool, nt, sms);
+    const int nt = r4_nt(lim);
+    const R4Grid of = r4_grid(p.step, p.pool, nt, sms);
+    const int grid = of.ctas;
     const R4Split split = r4_split(p.pool.n_kv_heads);
     auto go = [&](auto b, auto h, auto n) {
         using S = R4Shape<decltype(h)::value, decltype(n)::value>;
         auto kernel = kv_rows4_kernel<decltype(b)::value, decltype(h)::value, decltype(n)::value>;
         static KvOnce once;
         if (cudaError_t x = once.shared_memory(reinterpret_cast<const void*>(kernel), std::max(S::smem(1), S::smem(4)))) return x;
-        return kv_launch(kernel, dim3(grid), R4_THREADS, S::smem(split.wph), st, p, lim);
+        return kv_launch(kernel, dim3(grid), R4_THREADS, S::smem(split.wph), st, p, lim, of.shift);
     };
     auto by_nt = [&](auto b, auto h) { return nt == 1 ? go(b, h, std::integral_constant<int, 1>()) : go(b, h, std::integral_constant<int, 2>()); };
     auto by_hd = [&](auto b) { return head_size == 128 ? by_nt(b, std::integral_constant<int, 128>()) : by_nt(b, std::integral_constant<int, 64>()); };

@@ -21,7 +21,7 @@ namespace l2 {
 
 namespace {
 
-constexpr int TB_THREADS = 512, TB_WARPS = TB_THREADS / 32, TB_CLUSTER = 8;
+constexpr int TB_CLUSTER = 8, TB_MOST = 1024, TB_WARPS = TB_MOST / 32;  // CTAs and threads at most
 constexpr int TB_SEQS = 16384;  // whose sums a CTA's shared memory holds
 
 struct TbParams {
@@ -68,8 +68,8 @@ __device__ __forceinline__ void tb_sums(const long long (&v)[N], long long (&bef
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const long long s = tb_scan(lane < TB_WARPS ? scratch[lane][i] : 0);
-        total[i] = __shfl_sync(0xffffffffu, s, TB_WARPS - 1);
+        const long long s = tb_scan(lane < (int)(blockDim.x >> 5) ? scratch[lane][i] : 0);
+        total[i] = __shfl_sync(0xffffffffu, s, 31);
         const long long w = __shfl_sync(0xffffffffu, s, warp ? warp - 1 : 0);
         if (warp) before[i] += w;
     }
@@ -95,19 +95,19 @@ __device__ __forceinline__ int tb_find(const int* a, int n, int x) {
     return lo;
 }
 
-__global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_constant__ TbParams P) {
+__global__ void __launch_bounds__(TB_MOST) kv_plan_kernel(const __grid_constant__ TbParams P) {
     extern __shared__ int tb_smem[];
     int* const starts = tb_smem;                      // [n_seqs + 1] first rows
     int* const taken = tb_smem + P.n_seqs + 1;        // [n_seqs + 1] pages taken in front of a sequence
     int* const lengths = tb_smem + 2 * P.n_seqs + 2;  // [n_seqs] before the step
     __shared__ long long scratch[TB_WARPS][2];
-    const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
+    const int tid = threadIdx.x, threads = blockDim.x, cta = blockIdx.x, ctas = gridDim.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int count = tb_free(P, cta == 0 && tid == 0);
     // ---- rows and pages of all sequences.  (Sums that pass 31 bits are of steps without room, whose sums nobody uses.)
     long long all[2] = {0, 0};
-    for (int b0 = 0; b0 < P.n_seqs; b0 += TB_THREADS) {
+    for (int b0 = 0; b0 < P.n_seqs; b0 += threads) {
         const int b = b0 + tid;
         long long v[2] = {0, 0}, before[2], total[2];
         if (b < P.n_seqs) {
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_consta
         else *P.free_count = count - pages;
         P.row_start[P.n_seqs] = rows;
     }
-    for (int b = cta * TB_THREADS + tid; b < P.n_seqs; b += ctas * TB_THREADS) {
+    for (int b = cta * threads + tid; b < P.n_seqs; b += ctas * threads) {
         P.row_start[b] = room ? starts[b] : 0;
         const int n = room ? starts[b + 1] - starts[b] : 0;
         if (n) P.kv_len[b] = lengths[b] + n;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_consta
         return -1;
     };
     if (!P.slots && !P.positions) {
-        for (int i = cta * TB_THREADS + tid; i < pages; i += ctas * TB_THREADS) {
+        for (int i = cta * threads + tid; i < pages; i += ctas * threads) {
             const int b = tb_find(taken, P.n_seqs, i);  // (the last sequence with so many in front: the one that takes it)
             P.table[(size_t)b * P.width + tb_pages(P, lengths[b]) + i - taken[b]] = page(i);
         }
@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_consta
     // ---- a slot and a position for every row, a few rows a thread; the first row of a new page brings it into the table
     const int mask = (1 << P.page_shift) - 1;
     constexpr int N = 4;
-    for (int r0 = N * (cta * TB_THREADS + tid); r0 < P.n_rows; r0 += N * ctas * TB_THREADS) {
+    const bool wide = ((reinterpret_cast<uintptr_t>(P.slots) | reinterpret_cast<uintptr_t>(P.positions)) & 15) == 0;
+    for (int r0 = N * (cta * threads + tid); r0 < P.n_rows; r0 += N * ctas * threads) {
         long long slot[N];
         int pos[N];
         int b = r0 < rows ? tb_find(starts, P.n_seqs, r0) : 0;
@@ -179,6 +180,14 @@ __global__ void __launch_bounds__(TB_THREADS) kv_plan_kernel(const __grid_consta
                 if (!tb_is_page(P, e)) { kv_report(P.status, L2_KV_BAD_PAGE); e = -1; }
             }
             if (e >= 0) slot[i] = ((long long)e << P.page_shift) + (pos[i] & mask);
+        }
+        if (wide && r0 + N <= P.n_rows) {  // (every array that there is starts on a boundary of 16 bytes)
+            if (P.slots) {
+                reinterpret_cast<longlong2*>(P.slots + r0)[0] = make_longlong2(slot[0], slot[1]);
+                reinterpret_cast<longlong2*>(P.slots + r0)[1] = make_longlong2(slot[2], slot[3]);
+            }
+            if (P.positions) *reinterpret_cast<int4*>(P.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            continue;
         }
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -203,18 +212,18 @@ __device__ __forceinline__ TbGone tb_gone(const TbParams& P, int len, int keep) 
     return g;
 }
 
-__global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_constant__ TbParams P) {
+__global__ void __launch_bounds__(TB_MOST) kv_release_kernel(const __grid_constant__ TbParams P) {
     extern __shared__ int tb_smem[];
     int* const from = tb_smem;                     // [n_seqs] entries in front of a sequence's
     int* const lengths = tb_smem + P.n_seqs;       // [n_seqs]
     int* const kept = tb_smem + 2 * P.n_seqs;      // [n_seqs]
     __shared__ long long scratch[TB_WARPS][1], mine;
-    const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
+    const int tid = threadIdx.x, threads = blockDim.x, cta = blockIdx.x, ctas = gridDim.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int count = tb_free(P, cta == 0 && tid == 0);
     long long entries = 0;
-    for (int b0 = 0; b0 < P.n_seqs; b0 += TB_THREADS) {
+    for (int b0 = 0; b0 < P.n_seqs; b0 += threads) {
         const int b = b0 + tid;
         long long v[1] = {0}, before[1], total[1];
         if (b < P.n_seqs) {
@@ -245,7 +254,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_con
     int* at = nullptr;
     int e = -1;
     long long v[1] = {0}, before[1], total[1];
-    for (int i0 = e0; i0 < e1; i0 += TB_THREADS) {
+    for (int i0 = e0; i0 < e1; i0 += threads) {
         at = nullptr;
         e = -1;
         if (i0 + tid < e1) {
@@ -255,7 +264,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_con
             else if (e != -1) kv_report(P.status, L2_KV_BAD_PAGE);
         }
     }
-    const bool once = e1 - e0 <= TB_THREADS;  // (at and e are then what they will be below)
+    const bool once = e1 - e0 <= threads;  // (at and e are then what they will be below)
     tb_sums<1>(v, before, total, scratch);
     if (tid == 0) mine = total[0];
     tb_sync(ctas);  // (also: all have read the lengths and the number of free pages)
@@ -267,7 +276,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_con
         if (all > P.n_pages - count) kv_report(P.status, L2_KV_BAD_PAGE);  // (more pages than there are: some were in two tables)
         *P.free_count = (int)min((long long)P.n_pages, count + all);
     }
-    for (int i0 = e0; i0 < e1; i0 += TB_THREADS) {
+    for (int i0 = e0; i0 < e1; i0 += threads) {
         if (!once) {
             at = nullptr;
             e = -1;
@@ -282,7 +291,7 @@ __global__ void __launch_bounds__(TB_THREADS) kv_release_kernel(const __grid_con
         }
         front += total[0];
     }
-    for (int b = cta * TB_THREADS + tid; b < P.n_seqs; b += ctas * TB_THREADS)
+    for (int b = cta * threads + tid; b < P.n_seqs; b += ctas * threads)
         if (kept[b] < lengths[b]) P.kv_len[b] = kept[b];
     tb_sync(ctas);  // (nobody reads this CTA's shared memory any more)
 }
@@ -303,8 +312,11 @@ int check_tables(const char* who, const l2_kv_tables* t, TbParams* out) {
     return L2_OK;
 }
 
-// One cluster of up to `ctas`, launched programmatically.
-cudaError_t tb_launch(void (*kernel)(const TbParams), const TbParams& P, int64_t ctas, KvOnce& once, cudaStream_t st) {
+// One cluster for so many rows or entries, launched programmatically.
+cudaError_t tb_launch(void (*kernel)(const TbParams), const TbParams& P, int64_t items, KvOnce& once, cudaStream_t st) {
+    // (few rows: fewer warps to meet; else as many as there are, two rows or so a thread)
+    const int threads = items <= 1024 && P.n_seqs <= 512 ? 256 : TB_MOST;
+    const int64_t ctas = (items + 2 * threads - 1) / (2 * threads);
     const int smem = (3 * P.n_seqs + 2) * (int)sizeof(int);
     if (smem > 40 * 1024)
         if (cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kernel), (3 * TB_SEQS + 2) * (int)sizeof(int))) return e;
@@ -313,7 +325,7 @@ cudaError_t tb_launch(void (*kernel)(const TbParams), const TbParams& P, int64_t
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(n);
-    cfg.blockDim = dim3(TB_THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -345,7 +357,7 @@ extern "C" int l2_kv_plan(const l2_kv_tables* tables, const int32_t* new_rows, i
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     static KvOnce once;
-    L2_CUDA(tb_launch(kv_plan_kernel, P, (n_rows + 2 * TB_THREADS - 1) / (2 * TB_THREADS), once, static_cast<cudaStream_t>(cuda_stream)));
+    L2_CUDA(tb_launch(kv_plan_kernel, P, n_rows, once, static_cast<cudaStream_t>(cuda_stream)));
     return L2_OK;
 }
 
@@ -361,6 +373,6 @@ extern "C" int l2_kv_release(const l2_kv_tables* tables, const int32_t* keep, in
     if (int rc = kv_device(&sms)) return rc;
     if (!P.n_seqs) return L2_OK;
     static KvOnce once;
-    L2_CUDA(tb_launch(kv_release_kernel, P, ((int64_t)P.n_seqs * P.width + 4 * TB_THREADS - 1) / (4 * TB_THREADS), once, static_cast<cudaStream_t>(cuda_stream)));
+    L2_CUDA(tb_launch(kv_release_kernel, P, std::min<int64_t>((int64_t)P.n_seqs * P.width, 16 * (int64_t)P.n_seqs), once, static_cast<cudaStream_t>(cuda_stream)));
     return L2_OK;
 }

@@ -9,16 +9,19 @@ _call = lib.l2_block_norm
 _ARGS = struct.Struct("@" + "Pqi0q" * 5 + "PPffii")  # l2_block_norm_args
 assert _ARGS.size == C.sizeof(BlockNormArgs)
 _NONE = (0, 0, 0)
+_types = paged._types
 
 
 def _rows(t, what, device, shape, one_for_all):
     """The fields of an l2_rows for t [rows, dim], or [dim] for all rows."""
-    if t.shape != shape and not (one_for_all and t.shape == shape[1:]):
-        raise ValueError("%s: [%d, %d] expected, got %s" % (what, *shape, tuple(t.shape)))
-    stride = t.stride()
-    if (stride[-1] != 1 and shape[1] > 1) or t.get_device() != device:
+    strides = t.stride()
+    if t.shape != shape:
+        if not one_for_all or t.shape != shape[1:]:
+            raise ValueError("%s: [%d, %d] expected, got %s" % (what, *shape, tuple(t.shape)))
+        strides = (0, *strides)
+    if (strides[1] != 1 and shape[1] > 1) or t.get_device() != device:
         raise ValueError("%s: on device %d with its last dimension contiguous expected" % (what, device))
-    return t.data_ptr(), stride[0] if t.dim() == 2 else 0, paged._type(t)
+    return t.data_ptr(), strides[0], _types[t.dtype] if t.dtype in _types else paged._type(t)
 
 
 def block_norm(block, residual=None, out=None, *, residual_out=None, post_weight=None, pre_weight=None, gate=None, scale=1.0, eps=1e-5, stream=None):
@@ -39,16 +42,15 @@ def block_norm(block, residual=None, out=None, *, residual_out=None, post_weight
         paged._int32(rows=rows, dim=dim)
     if device < 0:
         raise ValueError("tensors on a CUDA device expected")
-    record = C.create_string_buffer(_ARGS.size)
-    _ARGS.pack_into(record, 0,
-                    *(_rows(block, "block", device, shape, False) if block is not None else _NONE),
-                    *(_rows(residual, "residual", device, shape, False) if residual is not None else _NONE),
-                    *(_rows(gate, "gate", device, shape, True) if gate is not None else _NONE),
-                    *(_rows(residual_out, "residual_out", device, shape, False) if residual_out is not None else _NONE),
-                    *(_rows(out, "out", device, shape, False) if out is not None else _NONE),
-                    paged._packed(post_weight, "post_weight", device, (dim,), paged.F32) if post_weight is not None else 0,
-                    paged._packed(pre_weight, "pre_weight", device, (dim,), paged.F32) if pre_weight is not None else 0,
-                    scale, eps, rows, dim)
+    record = _ARGS.pack(
+        *(_rows(block, "block", device, shape, False) if block is not None else _NONE),
+        *(_rows(residual, "residual", device, shape, False) if residual is not None else _NONE),
+        *(_rows(gate, "gate", device, shape, True) if gate is not None else _NONE),
+        *(_rows(residual_out, "residual_out", device, shape, False) if residual_out is not None else _NONE),
+        *(_rows(out, "out", device, shape, False) if out is not None else _NONE),
+        paged._packed(post_weight, "post_weight", device, (dim,), paged.F32) if post_weight is not None else 0,
+        paged._packed(pre_weight, "pre_weight", device, (dim,), paged.F32) if pre_weight is not None else 0,
+        scale, eps, rows, dim)
     rc = _call(record, paged._stream_on(device, stream))
     if rc:
         check(rc)

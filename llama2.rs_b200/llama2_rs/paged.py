@@ -67,7 +67,7 @@ def _stream_on(device, stream):
 
 
 def _packed(t, what, device, shape, dtype):
-    if t.shape != shape or _type(t) != dtype or not t.is_contiguous() or t.get_device() != device:  # (-1: not on a CUDA device)
+    if t.shape != shape or (_types[t.dtype] if t.dtype in _types else _type(t)) != dtype or not t.is_contiguous() or t.get_device() != device:  # (-1: not on a CUDA device)
         raise ValueError("%s: contiguous %s of type code %d on device %d expected, got %s of %s" % (what, shape, dtype, device, tuple(t.shape), t.dtype))
     return t.data_ptr()
 
