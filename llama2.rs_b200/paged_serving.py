@@ -1,10 +1,12 @@
-"""Several sequences through one attention layer with a paged cache: quantised projections, RoPE, int8 or f16 pages, chunked prompts among single tokens.
+"""Several sequences through one attention layer with a paged cache: quantised projections, RoPE, 4-bit, int8 or f16 pages, chunked prompts among single tokens.
 
     python llama2.rs_b200/paged_serving.py                                   # 7B heads, int8 pages, 16 sequences
     python llama2.rs_b200/paged_serving.py --heads 64 --kv-heads 8 --cache f16 --window 1024 --sinks 4
+    python llama2.rs_b200/paged_serving.py --cache u4 --tables device        # pages handed out on the GPU
 
 A step takes up to --budget rows: one of every sequence that is past its prompt, the rest of the room for prompts, in order.  Pages are handed out as
-sequences grow and given back when these end and, with a window, when no row can see them any more.  There is no model behind the layer: a prompt is random rows, and the
+sequences grow and given back when these end and, with a window, when no row can see them any more: by lists of this program, whose tables are copied to the GPU in
+every step, or (--tables device) by l2_kv_plan and l2_kv_release, with tables that never leave it.  There is no model behind the layer: a prompt is random rows, and the
 next row of a sequence is the layer's own (normalised) output for the row before.  Weights are random in the checkpoint's layout; RoPE is that of the
 package's models (--rotation pairs: of plain pairs, for weights that want it).
 """
@@ -32,9 +34,13 @@ class PagedLayer:
         shapes = {"q": (dim, heads * 128), "k": (dim, kv_heads * 128), "v": (dim, kv_heads * 128), "o": (heads * 128, dim)}
         self.weights = weights or {n: random_qlinear(rng, i, o, group_size) for n, (i, o) in shapes.items()}
         self.linear = {n: l2.QLinear(*w, group_size) for n, w in self.weights.items()}
-        kind = {"i8": torch.int8, "f16": torch.float16, "bf16": torch.bfloat16}[cache]
-        k, v = (torch.zeros((n_pages, page_size, kv_heads, 128), dtype=kind, device="cuda") for _ in "kv")
-        scales = [torch.zeros((n_pages, kv_heads, page_size), device="cuda") for _ in "kv"] if cache == "i8" else []
+        kind = {"u4": torch.uint8, "i8": torch.int8, "f16": torch.float16, "bf16": torch.bfloat16}[cache]
+        k, v = (torch.zeros((n_pages, page_size, kv_heads, 64 if cache == "u4" else 128), dtype=kind, device="cuda") for _ in "kv")
+        scales = []
+        if cache == "i8":
+            scales = [torch.zeros((n_pages, kv_heads, page_size), device="cuda") for _ in "kv"]
+        if cache == "u4":
+            scales = [torch.zeros((n_pages, kv_heads, page_size, 2), dtype=torch.bfloat16, device="cuda") for _ in "kv"]
         self.pages = l2.KvPages(k, v, *scales)
         self.q_type = torch.float16 if cache == "f16" else torch.bfloat16
         self.rope, self.rotation = l2.KvRope(positions), rotation
@@ -69,17 +75,87 @@ class PagedLayer:
         kv_len = torch.tensor([s["length"] for s in sequences], dtype=torch.int32).cuda()
         start = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32).cuda()
         batch = self.l2.KvBatch(table, kv_len, start, n, max(rows), status=self.status)
-        q, k, v = (self._project(name, x) for name in "qkv")
-        q16 = torch.empty((n, self.heads, 128), dtype=self.q_type, device="cuda")
-        self.pages.append(batch, k.view(n, -1, 128), v.view(n, -1, 128), rope=self.rope, rotation=self.rotation, q=q.view(n, -1, 128), q_out=q16)
-        out = self.pages.attend(batch, q16, torch.empty((n, self.heads, 128), device="cuda"), window=self.window, sinks=self.sinks)
+        out = self._attention(batch, x)
         if self.window:  # pages that no later row sees
             for s in sequences:
                 for i in range(-(-self.sinks // self.page_size), max(0, s["length"] - self.window + 1) // self.page_size):
                     if s["table"][i] >= 0:
                         self.free.append(s["table"][i])
                         s["table"][i] = -1
-        return self._project("o", out.view(n, -1))
+        return self._project("o", out)
+
+    def _attention(self, batch, x):
+        n, torch = x.shape[0], self.torch
+        q, k, v = (self._project(name, x) for name in "qkv")
+        q16 = torch.zeros((n, self.heads, 128), dtype=self.q_type, device="cuda")
+        self.pages.append(batch, k.view(n, -1, 128), v.view(n, -1, 128), rope=self.rope, rotation=self.rotation, q=q.view(n, -1, 128), q_out=q16)
+        out = self.pages.attend(batch, q16, torch.zeros((n, self.heads, 128), device="cuda"), window=self.window, sinks=self.sinks)
+        return out.view(n, -1)
+
+    def normed(self, y):
+        """The rows' next inputs."""
+        return self.l2.block_norm(y, None, self.torch.empty_like(y))[1]
+
+
+class PlannedLayer(PagedLayer):
+    """The same with the tables, the lengths and the free pages of up to `n_seqs` sequences on the device: the host says how many rows each brings, and which have ended."""
+
+    def __init__(self, *args, n_seqs, budget, positions=4096, n_pages=512, page_size=32, **kw):
+        super().__init__(*args, positions=positions, n_pages=n_pages, page_size=page_size, **kw)
+        torch = self.torch
+        ints = lambda *shape, fill=0: torch.full(shape, fill, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.table, self.lengths, self.row_start = ints(n_seqs, -(-positions // page_size), fill=-1), ints(n_seqs), ints(n_seqs + 1)
+        self.free_pages, self.free_count = torch.arange(n_pages, dtype=torch.int32, device="cuda"), ints(1, fill=n_pages)
+        self.tables = self.l2.KvTables(self.table, self.lengths, self.free_pages, self.free_count, page_size, status=self.status)
+        self.n_seqs, self.budget = n_seqs, budget
+
+    def step_planned(self, x, rows):
+        """x [rows in all, dim] f32, rows[b] of them of sequence b, one after the other: the layer's output, f32."""
+        n, torch = x.shape[0], self.torch
+        if n > self.budget:
+            raise ValueError("%d rows, of %d" % (n, self.budget))
+        self.tables.plan(torch.tensor(rows, dtype=torch.int32).cuda(), self.row_start, n, max(rows))
+        out = self._attention(self.l2.KvBatch(self.table, self.lengths, self.row_start, n, max(rows), status=self.status), x)
+        if self.window:
+            self.tables.release(window=self.window, sinks=self.sinks)
+        return self._project("o", out)
+
+    def end(self, sequences):
+        """Gives back the pages of sequences (indices) that have ended."""
+        keep = [1 << 30] * self.n_seqs
+        for b in sequences:
+            keep[b] = 0
+        self.tables.release(self.torch.tensor(keep, dtype=self.torch.int32).cuda())
+
+
+def serve_planned(layer, prompts, tokens, budget):
+    """As serve, by a PlannedLayer."""
+    torch = layer.torch
+    seqs = [{"todo": p, "out": [], "left": tokens} for p in prompts]
+    steps = total = 0
+    while any(len(s["todo"]) or s["left"] > 0 for s in seqs):
+        room, rows, xs, ended = budget, [0] * layer.n_seqs, {}, []
+        for b in sorted((b for b, s in enumerate(seqs) if len(s["todo"]) or s["left"] > 0), key=lambda b: len(seqs[b]["todo"]) > 1):  # single rows first
+            s = seqs[b]
+            r = rows[b] = min(room, len(s["todo"]) or 1)
+            if r == 0:
+                break
+            if len(s["todo"]):
+                xs[b] = s["todo"][:r]
+            else:
+                xs[b] = layer.normed(s["out"][-1][-1:])
+                s["left"] -= 1
+            s["todo"] = s["todo"][r:]
+            room -= r
+        y = layer.step_planned(torch.cat([xs[b] for b in sorted(xs)]), rows)
+        for b, part in zip(sorted(xs), y.split([rows[b] for b in sorted(xs)])):
+            seqs[b]["out"].append(part)
+            if not len(seqs[b]["todo"]) and seqs[b]["left"] <= 0:
+                ended.append(b)
+        if ended:
+            layer.end(ended)
+        steps, total = steps + 1, total + sum(rows)
+    return [torch.cat(s["out"]) for s in seqs], steps, total
 
 
 def serve(layer, prompts, tokens, budget):
@@ -95,8 +171,7 @@ def serve(layer, prompts, tokens, budget):
                 break
             x = s["todo"][:r] if len(s["todo"]) else None
             if x is None:  # past its prompt: the row before it, normalised, goes in again
-                y = s["out"][-1][-1:]
-                x = y / (y.square().mean() + 1e-5).sqrt()
+                x = layer.normed(s["out"][-1][-1:])
                 s["left"] -= 1
             s["todo"] = s["todo"][r:]
             picked.append(s), rows.append(r), xs.append(x)
@@ -114,7 +189,8 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--heads", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=32)
-    ap.add_argument("--cache", choices=["i8", "f16", "bf16"], default="i8")
+    ap.add_argument("--cache", choices=["u4", "i8", "f16", "bf16"], default="i8")
+    ap.add_argument("--tables", choices=["host", "device"], default="host", help="who hands out pages")
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=0)
     ap.add_argument("--sequences", type=int, default=16)
@@ -125,14 +201,16 @@ def main():
     import torch
     if not torch.cuda.is_available():
         raise SystemExit("paged_serving needs a GPU: there is no CPU path")
-    layer = PagedLayer(args.heads * 128, args.heads, args.kv_heads, cache=args.cache, window=args.window, sinks=args.sinks, n_pages=2048, rotation=args.rotation)
+    more = {"n_seqs": args.sequences, "budget": args.budget} if args.tables == "device" else {}
+    layer = (PlannedLayer if more else PagedLayer)(args.heads * 128, args.heads, args.kv_heads, cache=args.cache, window=args.window, sinks=args.sinks, n_pages=2048, rotation=args.rotation, **more)
+    run = serve_planned if more else serve
     rng = np.random.default_rng(1)
     prompts = [torch.randn(int(n), layer.dim, device="cuda") for n in rng.integers(5, 900, args.sequences)]
-    serve(layer, prompts, 2, args.budget)  # the layers' buffers, the kernels' first launches
+    run(layer, prompts, 2, args.budget)  # the layers' buffers, the kernels' first launches
     torch.cuda.synchronize()
     begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     begin.record()
-    outs, steps, rows = serve(layer, prompts, args.tokens, args.budget)
+    outs, steps, rows = run(layer, prompts, args.tokens, args.budget)
     end.record()
     torch.cuda.synchronize()
     if int(layer.status):
