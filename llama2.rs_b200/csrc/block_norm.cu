@@ -45,11 +45,16 @@ __device__ __forceinline__ BnRaw<V> bn_load(const BnRows& a, int64_t row, int e)
     return r;
 }
 template <int V>
-__device__ __forceinline__ void bn_values(const BnRaw<V>& r, int type, float* x) {
+__device__ __forceinline__ void bn_values(const BnRaw<V>& r, int type, float* x) {  // (branches, all threads the same way: a choice at every element is three conversions each)
+    if (type == L2_F32) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const uint32_t half = V == 4 ? r.w[i / 2] >> (16 * (i % 2)) : r.w[0];
-        x[i] = type == L2_F32 ? __uint_as_float(r.w[i]) : type == L2_F16 ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16);
+        for (int i = 0; i < V; i++) x[i] = __uint_as_float(r.w[i]);
+    } else if (type == L2_BF16) {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = __uint_as_float(V == 4 && i % 2 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = __half2float(__ushort_as_half((unsigned short)(V == 4 ? r.w[i / 2] >> (16 * (i % 2)) : r.w[0])));
     }
 }
 template <int V>
@@ -356,7 +361,7 @@ extern "C" int l2_block_norm(const l2_block_norm_args* a, void* cuda_stream) {
     if (int rc = kv_device(&sms)) return rc;
     if (!a->rows) return L2_OK;
     // Many rows of some length: by the kernel that has the next row under way.
-    if (quads && a->rows >= 2 * sms && a->dim >= 1024 && a->dim <= 16384 && (P.block.data || P.residual.data)) {
+    if (quads && a->rows >= 8 * sms && a->dim >= 1024 && a->dim <= 16384 && (P.block.data || P.residual.data)) {
         auto bytes = [](const BnRows& r) { return r.data && r.stride ? 4 * bn_bytes(r.type) : 0; };  // (one row for all: from the caches)
         const int of[3] = {P.block.data ? 4 * bn_bytes(P.block.type) : 0, bytes(P.residual), bytes(P.gate)};
         const int elements = a->dim > 8192 ? 32 : 16, threads = (a->dim + 32 * elements - 1) / (32 * elements) * 32;
