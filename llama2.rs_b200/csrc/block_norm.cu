@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 #include "kernels.cuh"
@@ -114,6 +115,15 @@ __device__ __forceinline__ float bn_sum(float x, float* scratch) {
     return x;
 }
 
+// f with the type as a constant: loops over a thread's elements go inside, so that there is one choice an array.
+template <class F>
+__device__ __forceinline__ void bn_by_type(int type, F f) {
+    if (type == L2_F32) f(std::integral_constant<int, L2_F32>());
+    else if (type == L2_BF16) f(std::integral_constant<int, L2_BF16>());
+    else f(std::integral_constant<int, L2_F16>());
+}
+__device__ __forceinline__ BnRows bn_of(BnRows a, int type) { a.type = type; return a; }
+
 // E elements a thread, V of them side by side.  WARP: a warp has a row, else a CTA.
 template <int E, int V, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const __grid_constant__ BnParams P) {
@@ -126,16 +136,25 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const __g
     for (int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x; row < P.rows; row += step) {
         BnRaw<V> y[N], x[N];
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int e = (n * threads + t) * V;
+        for (int n = 0; n < N; n++)
 #pragma unroll
             for (int i = 0; i < V; i++) y[n].w[i] = x[n].w[i] = 0u;
-            if (e < P.dim && P.block.data) y[n] = bn_load<V>(P.block, row, e);
-            if (e < P.dim && P.residual.data) x[n] = bn_load<V>(P.residual, row, e);
-        }
-        float r[E], by = P.scale;
+        auto load = [&](const BnRows& from, BnRaw<V>* to) {
+            bn_by_type(from.type, [&](auto type) {
 #pragma unroll
-        for (int n = 0; n < N; n++) bn_values<V>(y[n], P.block.type, r + n * V);
+                for (int n = 0; n < N; n++) {
+                    const int e = (n * threads + t) * V;
+                    if (e < P.dim) to[n] = bn_load<V>(bn_of(from, decltype(type)::value), row, e);
+                }
+            });
+        };
+        if (P.block.data) load(P.block, y);
+        if (P.residual.data) load(P.residual, x);
+        float r[E];
+        bn_by_type(P.block.type, [&](auto type) {
+#pragma unroll
+            for (int n = 0; n < N; n++) bn_values<V>(y[n], decltype(type)::value, r + n * V);
+        });
         if (P.post) {
             float sum = 0.0f;
 #pragma unroll
@@ -155,26 +174,35 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const __g
             }
         }
         if (P.gate.data) {
+            bn_by_type(P.gate.type, [&](auto type) {
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                const int e = (n * threads + t) * V;
-                if (e < P.dim) {
+                for (int n = 0; n < N; n++) {
+                    const int e = (n * threads + t) * V;
+                    if (e >= P.dim) continue;
                     float g[V];
-                    bn_values<V>(bn_load<V>(P.gate, row, e), P.gate.type, g);
+                    bn_values<V>(bn_load<V>(bn_of(P.gate, decltype(type)::value), row, e), decltype(type)::value, g);
 #pragma unroll
                     for (int i = 0; i < V; i++) r[n * V + i] *= g[i];
                 }
+            });
+        }
+        bn_by_type(P.residual.type, [&](auto type) {
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                float v[V];
+                bn_values<V>(x[n], decltype(type)::value, v);
+#pragma unroll
+                for (int i = 0; i < V; i++) r[n * V + i] = fmaf(P.scale, r[n * V + i], v[i]);
             }
-        }
+        });
+        if (P.residual_out.data)
+            bn_by_type(P.residual_out.type, [&](auto type) {
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            float v[V];
-            bn_values<V>(x[n], P.residual.type, v);
-#pragma unroll
-            for (int i = 0; i < V; i++) r[n * V + i] = fmaf(by, r[n * V + i], v[i]);
-            const int e = (n * threads + t) * V;
-            if (P.residual_out.data && e < P.dim) bn_store<V>(P.residual_out, row, e, r + n * V);
-        }
+                for (int n = 0; n < N; n++) {
+                    const int e = (n * threads + t) * V;
+                    if (e < P.dim) bn_store<V>(bn_of(P.residual_out, decltype(type)::value), row, e, r + n * V);
+                }
+            });
         if (!P.out.data) {
             if (!WARP && P.post) __syncthreads();  // (the scratch of this row's sum, before the next row's)
             continue;
@@ -196,9 +224,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const __g
                 else w[0] = P.pre[e];
             }
 #pragma unroll
-            for (int i = 0; i < V; i++) w[i] = r[n * V + i] * f * w[i];
-            bn_store<V>(P.out, row, e, w);
+            for (int i = 0; i < V; i++) r[n * V + i] = r[n * V + i] * f * w[i];
         }
+        bn_by_type(P.out.type, [&](auto type) {
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const int e = (n * threads + t) * V;
+                if (e < P.dim) bn_store<V>(bn_of(P.out, decltype(type)::value), row, e, r + n * V);
+            }
+        });
         if constexpr (!WARP) {
             if (!P.post) __syncthreads();  // (the scratch of one row's second sum, before the next row's)
         }
