@@ -17,8 +17,10 @@
 // piece.  The tiles of all (sequence, heads) form one line, cut evenly over the CTAs, with room in front for what a piece costs besides its tiles; what a cut goes through leaves partial
 // (m, l, O), which kv_rows4_combine_kernel adds in order.
 //
-// Copies.  Every warp brings its own positions, 16 bytes a lane, three or four steps ahead, across the ends of pieces, and waits for nobody.  (By TMA, one warp for four others, the copies
-// alone took 84 of 97 us: it brings a row of 64 bytes every 4.5 clocks, where it could bring one of 128.)
+// Copies.  Every warp of products has a warp of copies that brings its positions, 16 bytes a lane, up to three or four steps ahead, across the ends of pieces; the two meet through
+// mbarriers only.  64 sequences of 8 kv heads and 64 query heads, up to 8192 positions (292 MB): 79 us.  By the warps of products themselves 84 (a copy waits where memory is busy, and all
+// behind it); by TMA, one warp for four, 93, of which the copies alone took 84: it brings a row of 64 bytes every 4.5 clocks, where it could bring one of 128.  What bounds it now: a start of
+// some 13 us (place on the line, table, first positions, first step), then copies (alone 66 us with the start) and steps (alone 68 us) that hide each other in part.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -32,8 +34,9 @@ namespace l2 {
 
 namespace {
 
-constexpr int R4_WARPS = 4, R4_THREADS = 32 * R4_WARPS;
-constexpr int R4_SETUP = 3;  // what a piece costs besides its tiles, in tiles
+constexpr int R4_WARPS = 4, R4_THREADS = 2 * 32 * R4_WARPS;  // warps of products, and as many of copies
+constexpr int R4_CTAS = 2;   // of an SM
+constexpr int R4_SETUP = 3;  // what a piece costs besides its tiles, in tiles (79.1 us at the size above; 2: 80.6, 5: 80.2)
 constexpr int R4_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr float R4_BIAS = 24.0f;  // probabilities carry a factor of 2^24
 
@@ -42,10 +45,9 @@ struct R4Shape {
     static constexpr int ROWS = 8 * NT, STEP = NT == 1 ? 64 : 32;          // positions of a warp's step
     static constexpr int ROW = HD / 2, KV = STEP * ROW, SLOT = 2 * KV + 2 * STEP * 4;
     static constexpr int O_BYTES = ROWS * HD * 4, MEET = 2 * (O_BYTES + ROWS * 8);  // a warp's results; of two warps
-    __host__ __device__ static constexpr int ctas(int wph) { return NT == 1 && wph == 1 ? 3 : 2; }  // of an SM
-    __host__ __device__ static constexpr int slots(int wph) { return NT == 1 ? ctas(wph) == 3 ? 2 : 3 : 4; }
-    __host__ __device__ static constexpr int smem(int wph) { return R4_WARPS * slots(wph) * SLOT + (wph > 1 ? MEET : 0); }
-    static_assert(ctas(1) * (smem(1) + 2048) <= 228 * 1024 && ctas(4) * (smem(4) + 2048) <= 228 * 1024, "shared memory");
+    static constexpr int SLOTS = NT == 1 && HD == 128 ? 3 : 4;
+    __host__ __device__ static constexpr int smem(int wph) { return R4_WARPS * SLOTS * SLOT + (wph > 1 ? MEET : 0); }
+    static_assert(R4_CTAS * (smem(4) + 2048) <= 228 * 1024, "shared memory");
 };
 
 // Heads of a CTA, and the warps of a head.
@@ -67,14 +69,6 @@ __device__ __forceinline__ int64_t r4_times(int n, int64_t bytes) {  // (n is no
 __device__ __forceinline__ void r4_copy_if(uint32_t dst, const void* src, bool there) {  // (zeros where there is nothing to bring)
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void r4_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void r4_wait(int under_way) {  // until no more than so many groups are
-    if (under_way >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (under_way == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (under_way == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
-
 // What rows at positions lo .. hi see, in tiles of 2^shift: KvView with a size that is not known before the call.
 struct R4View {
     int lo, hi, sink_tiles, first, tiles;
@@ -408,134 +402,162 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
 // ---- the kernel ----------------------------------------------------------------------------------------------------------------
 // QB: q is bf16, else f16
 template <bool QB, int HD, int NT>
-__global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int shift) {
+__global__ void __launch_bounds__(R4_THREADS, R4_CTAS) kv_rows4_kernel(const __grid_constant__ KvAttendParams P, const int lim, const int shift) {
     using S = R4Shape<HD, NT>;
     constexpr int CHUNKS = S::ROW / 16, PER_COPY = 32 / CHUNKS, PAIR_LANES = S::STEP / 4, COPIES = S::STEP / PER_COPY;  // 16-byte chunks of a row; positions of a copy by the warp, copies of a step
     extern __shared__ __align__(128) uint8_t r4_smem[];
-    __shared__ R4Piece pieces[R4_WARPS][2];
-    __shared__ int2 marks[R4_WARPS][4];  // of a slot: the step's first position; bit 0: every row sees all of it, 1: some row sees something, 2: the piece's last step
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c = lane & 3;
+    __shared__ R4Piece pieces[R4_WARPS][4];
+    __shared__ __align__(8) uint64_t full[R4_WARPS][4], empty[R4_WARPS][4], met[2];
+    __shared__ volatile int failed;
+    __shared__ int2 marks[R4_WARPS][4];  // of a slot: the step's first position; bit 0: every row sees all of it, 1: some row sees something, 2: the piece's last step, 3: there is none
+    const int tid = threadIdx.x, warp = (tid >> 5) % R4_WARPS, lane = tid & 31, g8 = lane >> 2, c = lane & 3;
     const R4Split split = r4_split(P.pool.n_kv_heads);
     const int units = P.pool.n_kv_heads / split.heads, of_head = warp / split.wph, share = warp % split.wph;  // this warp's head of the unit, its place among that one's warps
-    const int steps = (1 << shift) / (S::STEP * split.wph), slots = S::slots(split.wph);
+    const int steps = (1 << shift) / (S::STEP * split.wph), slots = S::SLOTS;
     uint8_t* const ring = r4_smem + warp * slots * S::SLOT;
+    if (tid < R4_WARPS * 4) { kv_bar_init(&full[0][0] + tid, 33); kv_bar_init(&empty[0][0] + tid, 1); }
+    if (tid < 2) kv_bar_init(&met[tid], split.wph);
+    if (tid == 0) failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    const KvWait wait{&failed};
 
-    // ================= copies: the step in front =====================================================================================
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    R4Walk walk(P, lim, shift, units);
-    if (tid == 0) kv_cuts(P.work)[blockIdx.x].pieces = 0;  // (no unit that begins here goes on, until one does)
-    int t = 0, k = 0, begun = 0, ended = 0, put = 0;  // tile and step in it; pieces begun by the copies, ended by the products; slot to fill
-    bool over = false;
-    int pages = 0, next_pages = 0, page0 = 0, next0 = -1;  // a lane has entry page0 + lane of the table
-    uint32_t there = 0;                                    // which of them are pages
-    // Of K, where the lane's 16 bytes of the head's first position are, and its row of a copy from there on; and of the pairs.  V lies as far behind K everywhere.
-    const char *k_lane = nullptr, *pair_lane = nullptr;
-    const int64_t to_v = P.pool.v - P.pool.k, page_bytes = P.pool.page_stride / 2, pos_bytes = P.pool.pos_stride / 2;
-    const int mask = (1 << P.pool.page_shift) - 1, pair_page = P.pool.n_kv_heads << P.pool.page_shift + 2;
-    // position r of 32 is row 8 (r % 4) + r / 4 of theirs
-    constexpr int SIDE = PER_COPY / 4, IN_BLOCK = 32 / PER_COPY;
-    const uint32_t lane_row = ((lane / CHUNKS & 3) * 8 + (lane / CHUNKS >> 2)) * S::ROW, lane_chunk = 16 * (lane % CHUNKS);
-    static_assert(SIDE * S::ROW == 128, "the rows of a copy behind those of the one in front");
-    auto look_up = [&](int first) {  // the entries that some row sees, as they are (nothing waits for them before they are needed); -2: none of these
-        const int i = first + lane;
-        if (i > walk.q.view.hi >> P.pool.page_shift || (P.window && !walk.q.view.any(i << P.pool.page_shift, 1 << P.pool.page_shift, P.window, P.sinks))) return -2;
-        return P.step.table[(size_t)walk.b * P.step.width + i];
-    };
-    auto issue = [&]() {  // whether there was a step to bring
-        if (t >= walk.t1) {
-            if (over || begun - ended == 2) return false;  // (a piece's record is kept until its products are done)
-            if (!walk.next(P, lim, shift, units)) { over = true; return false; }
-            t = walk.t0;
-            k = 0;
+    // (registers: 128 x (72 + 184) of the 256 x 128 that the launch has; 56 + 200 leaves more of the copies' addresses in memory: 80.3 us instead of 79.1)
+    if (tid >= 32 * R4_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ================= copies ==========================================================================================================
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // (rows, lengths and the cache may come from the kernel in front)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        R4Walk walk(P, lim, shift, units);
+        const bool first_warp = tid == 32 * R4_WARPS;
+        if (first_warp) kv_cuts(P.work)[blockIdx.x].pieces = 0;  // (no unit that begins here goes on, until one does)
+        int pages = 0, next_pages = 0, page0 = 0, next0 = -1;  // a lane has entry page0 + lane of the table
+        uint32_t there = 0;                                    // which of them are pages
+        // Of K, where the lane's 16 bytes of the head's first position are, and its row of a copy from there on; and of the pairs.  V lies as far behind K everywhere.
+        const char *k_lane = nullptr, *pair_lane = nullptr;
+        const int64_t to_v = P.pool.v - P.pool.k, page_bytes = P.pool.page_stride / 2, pos_bytes = P.pool.pos_stride / 2;
+        const int mask = (1 << P.pool.page_shift) - 1, pair_page = P.pool.n_kv_heads << P.pool.page_shift + 2;
+        // position r of 32 is row 8 (r % 4) + r / 4 of theirs
+        constexpr int SIDE = PER_COPY / 4, IN_BLOCK = 32 / PER_COPY;
+        const uint32_t lane_row = ((lane / CHUNKS & 3) * 8 + (lane / CHUNKS >> 2)) * S::ROW, lane_chunk = 16 * (lane % CHUNKS);
+        static_assert(SIDE * S::ROW == 128, "the rows of a copy behind those of the one in front");
+        auto look_up = [&](int first) {  // the entries that some row sees, as they are (nothing waits for them before they are needed); -2: none of these
+            const int i = first + lane;
+            if (i > walk.q.view.hi >> P.pool.page_shift || (P.window && !walk.q.view.any(i << P.pool.page_shift, 1 << P.pool.page_shift, P.window, P.sinks))) return -2;
+            return P.step.table[(size_t)walk.b * P.step.width + i];
+        };
+        uint32_t put = 0, ph = 1;
+        auto give = [&](int first, int flags) {  // the slot's copies and what it is, to the warp of products
+            kv_copy16_arrive(&full[warp][put]);
+            if (lane == 0) {
+                marks[warp][put] = make_int2(first, flags);
+                kv_bar_arrive(&full[warp][put]);
+            }
+            if (++put == slots) { put = 0; ph ^= 1u; }
+        };
+        bool over = false;
+#pragma unroll 1
+        for (int begun = 0; !over && walk.next(P, lim, shift, units); begun++) {
             const int head = walk.unit * split.heads + of_head;
             const bool done = walk.t0 == 0 && walk.t1 == walk.q.view.tiles;
-            if (lane == 0) pieces[warp][begun & 1] = R4Piece{walk.q.s.row0, walk.q.rows, head, walk.q.view.lo, done ? -1 : walk.first ? 0 : 1};
-            if (tid == 0 && walk.t0 == 0 && !done)  // what the kernel behind this one has to know of the CTA's last piece
+            if (first_warp && walk.t0 == 0 && !done)  // what the kernel behind this one has to know of the CTA's last piece
                 kv_cuts(P.work)[blockIdx.x] = KvCut{(int)((uint32_t)(walk.w - walk.t1 + walk.q.view.tiles - 1) / (uint32_t)walk.per) - (int)blockIdx.x + 1, walk.first ? 0 : 1, walk.q.rows,
                                                     walk.unit * split.heads, walk.q.s.row0, walk.q.view.lo, 0};
             k_lane = P.pool.k + (int64_t)head * (P.pool.head_stride / 2) + lane_chunk + (PER_COPY <= 8 || mask >= PER_COPY - 1 ? lane / CHUNKS : lane / CHUNKS & mask) * pos_bytes;
             pair_lane = reinterpret_cast<const char*>(lane < PAIR_LANES ? P.pool.ks : P.pool.vs) + (((int64_t)head << P.pool.page_shift) + (4 * (lane % PAIR_LANES) & mask)) * 4;
             page0 = next0 = -1 << 20;
-            begun++;
-        }
-        const R4View& view = walk.q.view;
-        const int j0 = view.base(t, shift) + (k * split.wph + share) * S::STEP;
-        bool some = j0 <= view.hi, whole = j0 + S::STEP <= view.lo + 1;
-        if (P.window) { some = view.any(j0, S::STEP, P.window, P.sinks); whole = view.whole(j0, S::STEP, P.window, P.sinks); }
-        const uint32_t to = kv_smem(ring + put * S::SLOT);
-        if (some) {
-            const int want = j0 >> P.pool.page_shift, last = (j0 + S::STEP - 1) >> P.pool.page_shift;
-            if (want < page0 || last > page0 + 31) {
-                if (want == next0) { pages = next_pages; page0 = next0; }
-                else { page0 = want; pages = look_up(page0); }
-                next0 = page0 + 32;  // (steps go on by whole pages, or within one, and by a divisor of 32 of them)
-                next_pages = look_up(next0);
-                if (pages != -2 && (unsigned)pages >= (unsigned)P.pool.n_pages) kv_report(P.step.status, L2_KV_BAD_PAGE);
-                if ((unsigned)pages >= (unsigned)P.pool.n_pages) pages = -1;
-                there = __ballot_sync(0xffffffffu, pages >= 0);
-            }
-            // (a step begins a page or lies inside one)
-            const int in = j0 & mask, p0 = (j0 >> P.pool.page_shift) - page0;
-            const uint32_t need = (2u << (S::STEP - 1 >> P.pool.page_shift)) - 1;
-            if ((there >> p0 & need) == need) {
-                const uint32_t at = to + lane_row + lane_chunk;
-                auto copies = [&](auto n) {  // of a step with so many pages
-                    constexpr int PER_PAGE = S::STEP / decltype(n)::value;
-                    const char* from = k_lane;
-#pragma unroll
-                    for (int i = 0; i < COPIES; i++) {
-                        if (PER_COPY > PER_PAGE || i * PER_COPY % PER_PAGE == 0) {
-                            from = k_lane + r4_times(__shfl_sync(0xffffffffu, pages, p0 + i * PER_COPY / PER_PAGE + (PER_COPY > PER_PAGE ? lane / CHUNKS / PER_PAGE : 0)), page_bytes);
-                            if (PER_PAGE == S::STEP) from += r4_times(in, pos_bytes);
-                        } else {
-                            from += PER_COPY * pos_bytes;
-                        }
-                        const uint32_t off = (at ^ 16 * (i % IN_BLOCK)) + 128 * (i % IN_BLOCK) + 32 * S::ROW * (i / IN_BLOCK);
-                        r4_copy(off, from);
-                        r4_copy(off + S::KV, from + to_v);
-                    }
-                };
-                if (P.pool.page_shift == 4) copies(std::integral_constant<int, S::STEP / 16>());
-                else if (P.pool.page_shift == 5) copies(std::integral_constant<int, S::STEP / 32>());
-                else if (P.pool.page_shift == 3) copies(std::integral_constant<int, S::STEP / 8>());
-                else copies(std::integral_constant<int, 1>());
-                // the pairs: four positions a lane, of K by the first lanes, of V by the next
-                const int page = __shfl_sync(0xffffffffu, pages, p0 + (4 * (lane % PAIR_LANES) >> P.pool.page_shift));
-                if (2 * PAIR_LANES == 32 || lane < 2 * PAIR_LANES) r4_copy(to + 2 * S::KV + 16 * lane, pair_lane + (uint64_t)(uint32_t)page * (uint32_t)pair_page + 4 * in);
-            } else {  // zeros where there is no page
+            const R4View& view = walk.q.view;
 #pragma unroll 1
-                for (int i = 0; i < COPIES; i++) {
-                    const int page = __shfl_sync(0xffffffffu, pages, p0 + (i * PER_COPY >> P.pool.page_shift) + (PER_COPY <= 8 ? 0 : lane / CHUNKS >> P.pool.page_shift));
-                    const char* const from = k_lane + r4_times(max(page, 0), page_bytes) + (in + (i * PER_COPY & mask)) * pos_bytes;
-                    const uint32_t off = to + lane_row + 128 * (i % IN_BLOCK) + 32 * S::ROW * (i / IN_BLOCK) + (lane_chunk ^ (16 * (i % IN_BLOCK)));
-                    r4_copy_if(off, from, page >= 0);
-                    r4_copy_if(off + S::KV, from + to_v, page >= 0);
+            for (int t = walk.t0, k = 0; t < walk.t1;) {
+                const int j0 = view.base(t, shift) + (k * split.wph + share) * S::STEP;
+                bool some = j0 <= view.hi, whole = j0 + S::STEP <= view.lo + 1;
+                if (P.window) { some = view.any(j0, S::STEP, P.window, P.sinks); whole = view.whole(j0, S::STEP, P.window, P.sinks); }
+                wait(&empty[warp][put], ph);
+                if ((over = wait.over())) break;
+                if (t == walk.t0 && k == 0 && lane == 0) pieces[warp][begun & 3] = R4Piece{walk.q.s.row0, walk.q.rows, head, walk.q.view.lo, done ? -1 : walk.first ? 0 : 1};
+                const uint32_t to = kv_smem(ring + put * S::SLOT);
+                if (some) {
+                    const int want = j0 >> P.pool.page_shift, last = (j0 + S::STEP - 1) >> P.pool.page_shift;
+                    if (want < page0 || last > page0 + 31) {
+                        if (want == next0) { pages = next_pages; page0 = next0; }
+                        else { page0 = want; pages = look_up(page0); }
+                        next0 = page0 + 32;  // (steps go on by whole pages, or within one, and by a divisor of 32 of them)
+                        next_pages = look_up(next0);
+                        if (pages != -2 && (unsigned)pages >= (unsigned)P.pool.n_pages) kv_report(P.step.status, L2_KV_BAD_PAGE);
+                        if ((unsigned)pages >= (unsigned)P.pool.n_pages) pages = -1;
+                        there = __ballot_sync(0xffffffffu, pages >= 0);
+                    }
+                    // (a step begins a page or lies inside one)
+                    const int in = j0 & mask, p0 = (j0 >> P.pool.page_shift) - page0;
+                    const uint32_t need = (2u << (S::STEP - 1 >> P.pool.page_shift)) - 1;
+                    if ((there >> p0 & need) == need) {
+                        const uint32_t at = to + lane_row + lane_chunk;
+                        auto copies = [&](auto n) {  // of a step with so many pages
+                            constexpr int PER_PAGE = S::STEP / decltype(n)::value;
+                            const char* from = k_lane;
+#pragma unroll
+                            for (int i = 0; i < COPIES; i++) {
+                                if (PER_COPY > PER_PAGE || i * PER_COPY % PER_PAGE == 0) {
+                                    from = k_lane + r4_times(__shfl_sync(0xffffffffu, pages, p0 + i * PER_COPY / PER_PAGE + (PER_COPY > PER_PAGE ? lane / CHUNKS / PER_PAGE : 0)), page_bytes);
+                                    if (PER_PAGE == S::STEP) from += r4_times(in, pos_bytes);
+                                } else {
+                                    from += PER_COPY * pos_bytes;
+                                }
+                                const uint32_t off = (at ^ 16 * (i % IN_BLOCK)) + 128 * (i % IN_BLOCK) + 32 * S::ROW * (i / IN_BLOCK);
+                                r4_copy(off, from);
+                                r4_copy(off + S::KV, from + to_v);
+                            }
+                        };
+                        if (P.pool.page_shift == 4) copies(std::integral_constant<int, S::STEP / 16>());
+                        else if (P.pool.page_shift == 5) copies(std::integral_constant<int, S::STEP / 32>());
+                        else if (P.pool.page_shift == 3) copies(std::integral_constant<int, S::STEP / 8>());
+                        else copies(std::integral_constant<int, 1>());
+                        // the pairs: four positions a lane, of K by the first lanes, of V by the next
+                        const int page = __shfl_sync(0xffffffffu, pages, p0 + (4 * (lane % PAIR_LANES) >> P.pool.page_shift));
+                        if (2 * PAIR_LANES == 32 || lane < 2 * PAIR_LANES) r4_copy(to + 2 * S::KV + 16 * lane, pair_lane + (uint64_t)(uint32_t)page * (uint32_t)pair_page + 4 * in);
+                    } else {  // zeros where there is no page
+#pragma unroll 1
+                        for (int i = 0; i < COPIES; i++) {
+                            const int page = __shfl_sync(0xffffffffu, pages, p0 + (i * PER_COPY >> P.pool.page_shift) + (PER_COPY <= 8 ? 0 : lane / CHUNKS >> P.pool.page_shift));
+                            const char* const from = k_lane + r4_times(max(page, 0), page_bytes) + (in + (i * PER_COPY & mask)) * pos_bytes;
+                            const uint32_t off = to + lane_row + 128 * (i % IN_BLOCK) + 32 * S::ROW * (i / IN_BLOCK) + (lane_chunk ^ (16 * (i % IN_BLOCK)));
+                            r4_copy_if(off, from, page >= 0);
+                            r4_copy_if(off + S::KV, from + to_v, page >= 0);
+                        }
+                        const int page = __shfl_sync(0xffffffffu, pages, p0 + (4 * (lane % PAIR_LANES) >> P.pool.page_shift));
+                        if (2 * PAIR_LANES == 32 || lane < 2 * PAIR_LANES) r4_copy_if(to + 2 * S::KV + 16 * lane, pair_lane + (uint64_t)(uint32_t)max(page, 0) * (uint32_t)pair_page + 4 * in, page >= 0);
+                    }
                 }
-                const int page = __shfl_sync(0xffffffffu, pages, p0 + (4 * (lane % PAIR_LANES) >> P.pool.page_shift));
-                if (2 * PAIR_LANES == 32 || lane < 2 * PAIR_LANES) r4_copy_if(to + 2 * S::KV + 16 * lane, pair_lane + (uint64_t)(uint32_t)max(page, 0) * (uint32_t)pair_page + 4 * in, page >= 0);
+                if (++k == steps) { k = 0; t++; }
+                give(j0, (int)whole | (int)some << 1 | (int)(t >= walk.t1) << 2);
             }
         }
-        r4_commit();
-        if (++k == steps) { k = 0; t++; }
-        if (lane == 0) marks[warp][put] = make_int2(j0, (int)whole | (int)some << 1 | (int)(t >= walk.t1) << 2);
-        if (++put == slots) put = 0;
-        return true;
-    };
+        if (!over) {
+            wait(&empty[warp][put], ph);
+            give(0, 8);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (lane == 0 && failed) kv_report(P.step.status, L2_KV_TIMEOUT);
+        return;
+    }
 
     // ================= products ========================================================================================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     R4Rows<HD, NT> r;
     const R4Lane at{r4_offset<S::ROW>(lane & 15, lane >> 4), r4_offset<S::ROW>((lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1)};
     R4Piece piece{};
     bool fresh = true;
-    int get = 0, under_way = 0;
+    int ended = 0;
+    uint32_t get = 0, ph = 0, met_ph = 0;
 #pragma unroll 1
     while (true) {
-        while (under_way < slots && issue()) under_way++;
-        if (under_way == 0) break;
-        __syncwarp();
+        wait(&full[warp][get], ph);
+        if (wait.over()) break;
+        const int2 mark = marks[warp][get];
+        if (mark.y & 8) break;
         if (fresh) {  // a new piece: Q, in f16, of eight elements the words (0, 4), (2, 6), (1, 5), (3, 7), as the numbers of a word of K come out
-            piece = pieces[warp][ended & 1];
+            piece = pieces[warp][ended & 3];
             fresh = false;
             r.unset = true;
 #pragma unroll
@@ -587,13 +609,10 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
                 for (int mt = 0; mt < HD / 16; mt++) r.o[mt][nt][0] = r.o[mt][nt][1] = r.o[mt][nt][2] = r.o[mt][nt][3] = 0.0f;
             }
         }
-        r4_wait(under_way - 1);
-        __syncwarp();  // (everybody's copies are there)
-        const int2 mark = marks[warp][get];
         if (mark.y & 2) r4_step<HD, NT>(P, r, at, ring + get * S::SLOT, mark.x, mark.y & 1);
-        __syncwarp();  // (the slot is free)
-        if (++get == slots) get = 0;
-        under_way--;
+        __syncwarp();
+        if (lane == 0) kv_bar_arrive(&empty[warp][get]);  // (the slot is free)
+        if (++get == slots) { get = 0; ph ^= 1u; }
         if (!(mark.y & 4)) continue;
 
         // ---- the piece's end: sums over the lanes that have the row, in units of 2^-m, with what the zeros give every element
@@ -616,7 +635,13 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
             }
         if (split.wph > 1) {  // the warps of a head meet: the upper half leaves its results for the lower, and again
             uint8_t* const room = r4_smem + R4_WARPS * slots * S::SLOT;
-            auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + of_head), "r"(32 * split.wph) : "memory"); };
+            auto meet = [&]() {
+                __syncwarp();
+                if (lane == 0) kv_bar_arrive(&met[of_head]);
+                wait(&met[of_head], met_ph);
+                met_ph ^= 1u;
+                __syncwarp();
+            };
 #pragma unroll 1
             for (int half = split.wph / 2; half; half >>= 1) {
                 float4* const o = reinterpret_cast<float4*>(room + (split.wph == 2 ? of_head : share % half) * (S::O_BYTES + S::ROWS * 8));
@@ -682,6 +707,7 @@ __global__ void __launch_bounds__(R4_THREADS, R4Shape<HD, NT>::ctas(1)) kv_rows4
                 }
         }
     }
+    if (lane == 0 && failed) kv_report(P.step.status, L2_KV_TIMEOUT);
 }
 
 // Adds the pieces of the unit that begins in CTA x of the launch in front and goes on in the next; blockIdx.y has one of its heads.
@@ -749,7 +775,7 @@ R4Grid r4_grid(const KvStep& s, const KvPool& p, int nt, int sms) {
     for (int shift = r4_least_shift(split.wph, nt);; shift++) {
         const int64_t most = (int64_t)s.n_seqs * (p.n_kv_heads / split.heads) * (((((int64_t)s.width << p.page_shift) + (1 << shift) - 1) >> shift) + 1 + R4_SETUP);
         if (most < ((int64_t)1 << 31) - 65536 || shift == 30)
-            return {shift, (int)std::min<int64_t>((nt == 1 ? R4Shape<128, 1>::ctas(split.wph) : R4Shape<128, 2>::ctas(split.wph)) * sms, most)};
+            return {shift, (int)std::min<int64_t>(R4_CTAS * sms, most)};
     }
 }
 
