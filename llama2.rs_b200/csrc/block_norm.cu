@@ -2,6 +2,7 @@
 //   t = y / sqrt(mean(y^2) + eps) w,   r = x + s g t,   out = r / sqrt(mean(r^2) + eps) v
 // A row is read once and stays in registers between the two sums; x is on its way while y's sum is formed.  Bound by memory where rows are many, else by the trip to
 // memory and the two meetings of a row's threads.
+// 8191 rows of 8192, bf16 beside an f32 residual (805 MB): 126 us, 6.4 TB/s (a plain copy 6.5; with the next row on its way into shared memory meanwhile, two CTAs an SM, 130, and rows of 2048 55 us instead of 36).  A row of 4096 with 200 of them or one: 4 us, which is latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -79,24 +80,6 @@ __device__ __forceinline__ void bn_store(const BnRows& a, int64_t row, int e, co
     } else {
         reinterpret_cast<__nv_bfloat16*>(a.data)[at] = __float2bfloat16_rn(x[0]);
     }
-}
-
-// Four elements on their way into shared memory, and from there.
-__device__ __forceinline__ void bn_fetch(uint32_t to, const BnRows& a, int64_t row, int e) {
-    const int64_t at = row * a.stride + e;
-    if (a.type == L2_F32) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(a.data + 4 * at) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(a.data + 2 * at) : "memory");
-}
-__device__ __forceinline__ BnRaw<4> bn_fetched(const uint8_t* at, int type) {
-    BnRaw<4> r;
-    if (type == L2_F32) {
-        const uint4 x = *reinterpret_cast<const uint4*>(at);
-        r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
-    } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(at);
-        r.w[0] = x.x; r.w[1] = x.y; r.w[2] = r.w[3] = 0u;
-    }
-    return r;
 }
 
 // The sum over a row's threads: a warp, or the CTA (scratch: a word a warp, used in turn with another).
@@ -239,94 +222,6 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const __g
     }
 }
 
-// Many rows: a CTA's next row is on its way into shared memory, where every thread finds its own elements again (nobody waits for another's), while a row is summed and written.
-template <int E>
-__global__ void __launch_bounds__(512, 2) block_norm_rows_kernel(const __grid_constant__ BnParams P, const int block_bytes, const int residual_bytes, const int gate_bytes) {
-    constexpr int N = E / 4;  // fours of a thread
-    extern __shared__ __align__(16) uint8_t bn_smem[];
-    __shared__ float scratch[2][32];
-    const int threads = blockDim.x, t = threadIdx.x, four = block_bytes + residual_bytes + gate_bytes;  // (bytes of four elements; 0: absent, or one row for all)
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    auto place = [&](int stage, int n) { return bn_smem + (stage * N + n) * threads * four; };
-    auto fetch = [&](int64_t row, int stage) {
-        if (row < P.rows) {
-#pragma unroll
-            for (int n = 0; n < N; n++) {
-                const int e = (n * threads + t) * 4;
-                if (e >= P.dim) break;
-                const uint32_t to = kv_smem(place(stage, n));
-                if (block_bytes) bn_fetch(to + t * block_bytes, P.block, row, e);
-                if (residual_bytes) bn_fetch(to + threads * block_bytes + t * residual_bytes, P.residual, row, e);
-                if (gate_bytes) bn_fetch(to + threads * (block_bytes + residual_bytes) + t * gate_bytes, P.gate, row, e);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    fetch(blockIdx.x, 0);
-    int stage = 0;
-    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x, stage ^= 1) {
-        fetch(row + gridDim.x, stage ^ 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        float r[E];
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            r[4 * n] = r[4 * n + 1] = r[4 * n + 2] = r[4 * n + 3] = 0.0f;
-            if (block_bytes && (n * threads + t) * 4 < P.dim) bn_values<4>(bn_fetched(place(stage, n) + t * block_bytes, P.block.type), P.block.type, r + 4 * n);
-        }
-        float f = 1.0f;
-        if (P.post) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < E; i++) sum = fmaf(r[i], r[i], sum);
-            sum = bn_sum<false>(sum, scratch[0]);
-            f = 1.0f / sqrtf(sum / (float)P.dim + P.eps);
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int e = (n * threads + t) * 4;
-            if (e >= P.dim) break;
-            if (P.post) {
-                const float4 w = *reinterpret_cast<const float4*>(P.post + e);
-                r[4 * n] = r[4 * n] * f * w.x; r[4 * n + 1] = r[4 * n + 1] * f * w.y; r[4 * n + 2] = r[4 * n + 2] * f * w.z; r[4 * n + 3] = r[4 * n + 3] * f * w.w;
-            }
-            float v[4];
-            if (P.gate.data) {
-                bn_values<4>(gate_bytes ? bn_fetched(place(stage, n) + threads * (block_bytes + residual_bytes) + t * gate_bytes, P.gate.type) : bn_load<4>(P.gate, row, e), P.gate.type, v);
-#pragma unroll
-                for (int i = 0; i < 4; i++) r[4 * n + i] *= v[i];
-            }
-            v[0] = v[1] = v[2] = v[3] = 0.0f;
-            if (residual_bytes) bn_values<4>(bn_fetched(place(stage, n) + threads * block_bytes + t * residual_bytes, P.residual.type), P.residual.type, v);
-            else if (P.residual.data) bn_values<4>(bn_load<4>(P.residual, row, e), P.residual.type, v);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                r[4 * n + i] = fmaf(P.scale, r[4 * n + i], v[i]);
-                sum = fmaf(r[4 * n + i], r[4 * n + i], sum);
-            }
-            if (P.residual_out.data) bn_store<4>(P.residual_out, row, e, r + 4 * n);
-        }
-        if (!P.out.data) {
-            if (P.post) __syncthreads();  // (the scratch of this row's sum, before the next row's)
-            continue;
-        }
-        sum = bn_sum<false>(sum, scratch[1]);
-        f = 1.0f / sqrtf(sum / (float)P.dim + P.eps);
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int e = (n * threads + t) * 4;
-            if (e >= P.dim) break;
-            float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (P.pre) { const float4 q = *reinterpret_cast<const float4*>(P.pre + e); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = r[4 * n + i] * f * w[i];
-            bn_store<4>(P.out, row, e, w);
-        }
-        if (!P.post) __syncthreads();  // (the scratch of one row's second sum, before the next row's)
-    }
-}
-
 int bn_bytes(int type) { return type == L2_F32 ? 4 : 2; }
 
 // `quads`: whether all arrays can be taken four elements at a time
@@ -394,32 +289,20 @@ extern "C" int l2_block_norm(const l2_block_norm_args* a, void* cuda_stream) {
     int sms;
     if (int rc = kv_device(&sms)) return rc;
     if (!a->rows) return L2_OK;
-    // Many rows of some length: by the kernel that has the next row under way.
-    if (quads && a->rows >= 8 * sms && a->dim >= 1024 && a->dim <= 16384 && (P.block.data || P.residual.data)) {
-        auto bytes = [](const BnRows& r) { return r.data && r.stride ? 4 * bn_bytes(r.type) : 0; };  // (one row for all: from the caches)
-        const int of[3] = {P.block.data ? 4 * bn_bytes(P.block.type) : 0, bytes(P.residual), bytes(P.gate)};
-        const int elements = a->dim > 8192 ? 32 : 16, threads = (a->dim + 32 * elements - 1) / (32 * elements) * 32;
-        const int smem = 2 * (elements / 4) * threads * (of[0] + of[1] + of[2]);
-        if (smem <= 200 * 1024) {
-            static KvOnce once[2];
-            const int per_sm = std::max(1, std::min({1024 / threads, 220 * 1024 / (smem + 2048), 6}));
-            auto go = [&](auto kernel, KvOnce& o) {
-                if (cudaError_t e = o.shared_memory(reinterpret_cast<const void*>(kernel), 200 * 1024)) return e;
-                return kv_launch(kernel, dim3((unsigned)std::min<int64_t>(a->rows, (int64_t)per_sm * sms)), threads, smem, static_cast<cudaStream_t>(cuda_stream), P, of[0], of[1], of[2]);
-            };
-            L2_CUDA(elements == 16 ? go(block_norm_rows_kernel<16>, once[0]) : go(block_norm_rows_kernel<32>, once[1]));
-            return L2_OK;
-        }
-    }
-    // A row in a warp where there are many rows that 32 threads hold; else threads enough that each has few elements where rows are few (latency), and 16 or 32 where they are many.
+    // A row in a warp where there are many rows that 32 threads hold (5000 rows of 512: 6.7 us, with a CTA a row 9.6; 148 rows: 3.1 and 2.5).  Else a CTA a row.  With four elements a
+    // thread, or eight of rows longer than 4096, as long as an SM gets no more than 1024 threads that way (592 rows of 1024: 3.3 us, with 16 elements 4.5; 148 of 4096: 3.8 and 4.6;
+    // 200 of 5120: 4.7 and 5.1); else with 16, or 32 of rows longer than 16384 (740 of 1024: 4.6 us, with four 5.2; 222 of 4096: 4.9 and 6.6).
     const bool warp = a->dim <= 512 && a->rows >= 4 * sms;
     int elements = 4, threads = 32;
+    auto widen = [&]() {
+        while (elements < 32 && 1024 * elements < a->dim) elements *= 2;
+        threads = std::min(1024, (a->dim + 32 * elements - 1) / (32 * elements) * 32);
+    };
     if (warp) {
         while (elements < 16 && 32 * elements < a->dim) elements *= 2;
     } else {
-        elements = a->rows >= 2 * sms ? 16 : 4;
-        while (elements < 32 && 1024 * elements < a->dim) elements *= 2;
-        threads = std::min(1024, (a->dim + 32 * elements - 1) / (32 * elements) * 32);
+        widen();
+        if (elements < 16 && (int64_t)a->rows * threads > 1024 * sms) { elements = 16; widen(); }
     }
     auto go = [&](auto e, auto v, auto w) {
         constexpr bool W = decltype(w)::value;
