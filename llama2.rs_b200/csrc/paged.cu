@@ -151,6 +151,7 @@ __device__ __forceinline__ float max_abs(float a, float x) {  // NaN if one of t
 // elements each of its first half and the same of its second: whole lines, and the pairs that RoPE turns in one thread.
 // Latency of loads and instructions, then bandwidth, bound it: 7900 rows of 2 x 40 heads of 128, bf16 to int8 (242 MB), take 51 us (4.8 TB/s).  A row a CTA,
 // whose look-ups nothing hid, took 76; so did 16 elements of one run a thread with conversion instructions and 110 registers (18 instructions an element).
+// To 4 bits (213 MB) 53 us: instructions bound it, 17 an element for two extremes, a rounding and the packing.
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_constant__ KvCopyParams P) {
     constexpr bool I8 = T == L2_I8, U4 = T == L2_U4;
@@ -280,6 +281,7 @@ __global__ void __launch_bounds__(KV_THREADS, 4) kv_append_kernel(const __grid_c
 
 // Bound by memory.  190,000 rows of 2 x 8 heads of 128, int8 to bf16 (1.2 GB): 210 us, 5.6 TB/s (a plain copy of as much: 6.0).  Five CTAs an SM at 48
 // registers, although the int8 forms then spill 13 words: with four and ordinary stores it took 218 us, with six 233.
+// 7900 rows of 2 x 40 heads of 128, 4 bits to bf16 (207 MB): 42 us, 4.9 TB/s; issue slots are 63 % busy.
 template <int T, int HD>
 __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const __grid_constant__ KvCopyParams P) {
     constexpr bool I8 = T == L2_I8, U4 = T == L2_U4;

@@ -32,6 +32,8 @@
 //                   reached by what it does not see.  They are taken out before the product and added to the rows that see them at the end.
 //                   int8 caches: they turn the bytes into 16-bit numbers (K q's type, V bf16, exact); scales are applied to the scores and to the
 //                   probabilities.
+//                   4 bits: they make values of 16 bits (zero + scale u, rounded once), so that the softmax has nothing to scale.  512 tokens of 64 heads behind 14,488
+//                   positions: 286 us on one input, 306 between others; 250 with the values left out of it.
 #include <cuda_runtime.h>
 
 #include <algorithm>
