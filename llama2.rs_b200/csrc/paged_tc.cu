@@ -55,7 +55,7 @@ constexpr int KT_SCALE_SLOTS = 4;
 constexpr int KT_SETUP = 4;
 constexpr int KT_RAISE = 8;  // powers of two that a score may exceed m by
 
-// WIDE, of a cache in 4 bits: see kt_held
+// WIDE, of a cache in 4 bits: see kt_values
 template <int CT, int HD>
 struct KtShape {
     static constexpr bool I8 = CT == L2_I8, U4 = CT == L2_U4, WIDEN = I8 || U4;  // WIDEN: tiles come as bytes, and helpers make numbers of 16 bits of them
@@ -146,9 +146,10 @@ __device__ __forceinline__ uint32_t kt_offset64(int r, int c) { return r * 64 + 
 __device__ __forceinline__ uint32_t kt_offset32(int r, int c) { return r * 32 + ((c ^ ((r >> 2) & 1)) << 4); }
 
 // ---- numbers of 4 bits as values of 16 ------------------------------------------------------------------------------------------
-// zero + scale u, rounded once, to f16: K, V, Q (a row of bf16 times a power of two) and the probabilities all go through the products in it.  Where some row sees
-// a pair that f16 does not hold, the CTA says so, and the launch behind this one, which else returns at once, does the call again in bf16 (WIDE): three bits less, and
-// f32's range.  (All of them in bf16 in the first place: errors of 0.0046 relative to the result where f16 has 0.0018.)
+// zero + scale u, rounded once, to f16: K, V, Q (a row of bf16 times a power of two) and the probabilities all go through the products in it.  A pair that f16 does not
+// hold is left out (0); a CTA says which of its pieces have some, and the launch behind this one, which else returns at once, does these again in bf16 (WIDE: three bits
+// less, and f32's range).  It keeps the results of the rows that see such a pair; the others have theirs from f16, so that a row goes by what it sees alone.
+// (All of them in bf16 in the first place: errors of 0.0046 relative to the result where f16 has 0.0018.)
 // A word's eight elements come out as (0, 4), (1, 5), (2, 6), (3, 7): Q is brought in that order, and O is read in it.
 __device__ __forceinline__ uint4 kt_order(uint4 w) {
     return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
@@ -178,6 +179,7 @@ __device__ __forceinline__ bool kt_held(float scale, float zero) {
     const float s = fabsf(scale), z = fabsf(zero);
     return z + 15.0f * s <= 65504.0f && (s >= 0x1p-16f || (s == 0.0f && (z == 0.0f || z >= 0x1p-14f)));
 }
+__device__ __forceinline__ bool kt_apart(uint32_t pair) { return !kv_pair_not_finite(pair) && !kt_held(kv_pair_scale(pair), kv_pair_zero(pair)); }
 // Eight elements of Q in f16 (BF: a row of bf16, times `up`) or, WIDE, in bf16.
 template <bool BF, bool WIDE>
 __device__ __forceinline__ uint4 kt_query(uint4 x, float up) {
@@ -332,12 +334,13 @@ struct KtPiece {
 };
 constexpr int KT_PIECES = 4;
 
-// QB: q is bf16, else f16.  gate: of a WIDE launch, what the CTAs of the launch in front say (see kt_held); else where they say it
+// QB: q is bf16, else f16.  gate, of a cache in 4 bits: a bit for each of a CTA's pieces (the last for all from the 32nd on), whether some row of it sees a pair that
+// f16 does not hold (see above); written here, or, WIDE, by the launch in front
 template <int CT, bool QB, int HD, bool WIDE>
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
                                                               const __grid_constant__ CUtensorMap map_v, int* const gate) {
     using S = KtShape<CT, HD>;
-    constexpr bool I8 = S::I8, U4 = S::U4, WIDEN = S::WIDEN;
+    constexpr bool I8 = S::I8, U4 = S::U4, WIDEN = S::WIDEN, REDO = U4 && WIDE, SCALED = I8 || REDO;  // SCALED: the softmax looks at the scales of a tile
     constexpr bool KB = U4 ? WIDE : QB, PB = U4 ? WIDE : I8 || QB;  // K and Q, V and the probabilities go through the products in bf16
     constexpr int LANES = HD / 8;
     constexpr uint32_t S_COL = 0, O_COL = 256;                   // tensor memory: S0 S1 O0 O1, 128 columns each; P over S
@@ -351,23 +354,25 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     __shared__ KtPiece pieces[KT_PIECES];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
-    __shared__ volatile int not_held;  // 4 bits: some row sees a pair that f16 does not hold
-    __shared__ float q_by[U4 ? KT_ROWS : 1];  // 4 bits: of a row of Q, the inverse of its power of two
-    __shared__ volatile int odd[8];  // by piece: values that are not finite have been taken out of a V tile
+    __shared__ int not_held;                  // 4 bits: what goes to `gate`
+    __shared__ float q_by[U4 ? KT_ROWS : 1];  // 4 bits: of a row of Q, the inverse of its power of two; REDO: whether the row's result is kept
+    __shared__ volatile int odd[8];  // by piece (of those done): values that are not finite have been taken out of a V tile
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem) + 1023) & ~(uintptr_t)1023);  // Q0, Q1
     uint8_t* ring = sq + S::Q_BYTES;
     uint8_t* raw = ring + S::SLOTS * S::SLOT;
     float* scales = reinterpret_cast<float*>(raw + S::RAWS * S::RAW);  // [slot][k, v][position]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    if constexpr (U4 && WIDE) {  // (nearly always there is nothing to do)
+    uint32_t again = 0;
+    if constexpr (REDO) {  // (nearly always there is nothing to do)
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        if (!__syncthreads_or(tid < gridDim.x && gate[tid] != 0)) return;
+        again = gate[blockIdx.x];
+        if (!again) return;
     }
     // (Code that runs once comes from far away, 100 clocks and more for eight instructions: every warp prepares a little.)
     if (warp == 4 && lane < S::SLOTS) { kv_bar_init(&full[lane], WIDEN ? 4 : 1); kv_bar_init(&empty[lane], WIDEN ? 2 : 6); kv_bar_init(&ready[lane], 4); }
     if (WIDEN && warp == 5 && lane < S::RAWS) { kv_bar_init(&raw_full[lane], 1); kv_bar_init(&raw_empty[lane], 4); }
-    if (WIDEN && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], I8 ? 8 : 4); }  // (read by the softmax; by the helpers)
+    if (WIDEN && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], I8 ? 8 : REDO ? 12 : 4); }  // (read by the softmax; by the helpers; by both)
     if (warp == 7 && lane < KT_PIECES) { kv_bar_init(&piece_full[lane], 1); kv_bar_init(&piece_empty[lane], 15); }
     if (warp == 8 && lane < 2) { kv_bar_init(&q_full[lane], 128); kv_bar_init(&drained[lane], 1); kv_bar_init(&row_meet[lane], 4); }
     if (warp == 9 && lane < 4) { kv_bar_init(&s_full[0][0] + lane, 1); kv_bar_init(&p_full[0][0] + lane, 4); kv_bar_init(&pv_done[0][0] + lane, 1); }
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                             for (int x = 1; x < LANES; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                             kv_q_factors(top, &up, &by);
                         }
-                        if (tid % LANES == 0) q_by[128 * i + (tid & 127) / LANES + n * Q_ROWS] = by;
+                        if (!REDO && tid % LANES == 0) q_by[128 * i + (tid & 127) / LANES + n * Q_ROWS] = by;
                         qx[n] = kt_query<QB, WIDE>(qx[n], up);
                     }
                     *reinterpret_cast<uint4*>(sq + i * S::SLOT + kt_offset((tid & 127) / LANES + n * Q_ROWS, tid % LANES)) = qx[n];
@@ -462,6 +467,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             }
             float m = -INFINITY, l = 0.0f;
             int seen = 0;      // halves of tiles seen
+            bool redo = false; // REDO: the row sees a pair that f16 does not hold
             uint32_t on = 0, all = 0;  // by tile of positions: seen by some row; by every row
 #pragma unroll 1
             for (int t = t0; t < t1; t++, on >>= 1, all >>= 1) {
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     all = walk.bits(t, [&](int base) { return mine.whole(base, P.window, P.sinks); });
                 }
                 if (!(on & 1u)) {
-                    if constexpr (I8) {
+                    if constexpr (SCALED) {
                         wait(&sc_full[sc], sc_ph);
                         __syncwarp();
                         if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     continue;
                 }
                 const bool whole = all & 1u;
-                if constexpr (I8) wait(&sc_full[sc], sc_ph);
+                if constexpr (SCALED) wait(&sc_full[sc], sc_ph);
 #pragma unroll 1
                 for (int h = 0; h < 2; h++, seen++) {
                     const float* ks = scales + sc * 2 * KT_TILE + KT_SUB * h;
@@ -505,6 +511,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
                         return below(pos - base + 1) & (P.window ? ~below(pos - P.window - base + 1) | below(P.sinks - base) : ~0ull);
                     };
+                    if constexpr (REDO) {
+                        auto apart = [&](int j) { return kt_apart(__float_as_uint(ks[j])) || kt_apart(__float_as_uint(ks[KT_TILE + j])); };
+                        __syncwarp();
+                        const uint32_t lo = __ballot_sync(0xffffffffu, apart(lane)), hi = __ballot_sync(0xffffffffu, apart(lane + 32));
+                        redo |= (visible() & ((unsigned long long)hi << 32 | lo)) != 0;
+                    }
                     if (!whole) {
                         const unsigned long long bits = visible();
 #pragma unroll
@@ -570,7 +582,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     if (lane == 0) kv_bar_arrive(&p_full[i][h]);
                 }
                 s_ph ^= 1u;
-                if constexpr (I8) {
+                if constexpr (SCALED) {
                     if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
                     if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
                 }
@@ -585,7 +597,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 fence_after();
             }
             if (128 * i >= walk.rows) { give_back(n); continue; }  // (this tile has no rows)
-            const bool fix = !I8 && started && odd[walk.index & 7];
+            if constexpr (REDO) q_by[row] = redo;
+            const bool fix = !I8 && started && odd[n & 7];
             bool none = false;  // 4 bits: the row sees a position of V that is taken as NaN
             if (U4 && fix) {
 #pragma unroll 1
@@ -647,6 +660,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     }
                 }
                 if (!done) {  // partial results: [4 columns][row][4], so that a warp's rows are side by side
+                    if (REDO && !redo) continue;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * KT_ROWS + row) * 4) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     continue;
@@ -678,12 +692,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
 #pragma unroll
                     for (int n = 0; n < 4; n++) {
                         const int fl = 128 * i + (tid & 127) / LANES + (n0 + n) * Q_ROWS, k = kt_token(P, fl);
-                        if (fl < walk.rows) *reinterpret_cast<uint4*>(out + (k * P.out.row_stride + (int64_t)(fl - k * P.group) * P.out.head_stride) * wide) = w[n];
+                        if (fl < walk.rows && (!REDO || q_by[REDO ? fl : 0] != 0.0f)) *reinterpret_cast<uint4*>(out + (k * P.out.row_stride + (int64_t)(fl - k * P.group) * P.out.head_stride) * wide) = w[n];
                     }
                 }
                 meet();
             }
-            if (!done) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
+            if (!done && (!REDO || redo)) *reinterpret_cast<float2*>(part + KT_ROWS * HD + 2 * row) = make_float2(m, l);
             fence_before();
             give_back(n);
         }
@@ -852,7 +866,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
             KvCut cut{0, 0, 0, 0, 0, 0, 0};
             bool more = true;
             for (uint32_t n = 0; more; n++) {
-                more = walk.next(P, lim);
+                do more = walk.next(P, lim); while (REDO && more && !(again >> min(walk.index, 31) & 1u));
                 const int64_t row0 = (int64_t)walk.k.s.row0 + walk.block * walk.k.tokens;
                 if (more && walk.t0 == 0 && walk.t1 < walk.view.tiles)
                     cut = KvCut{(int)kv_quotient(walk.w - walk.t1 + walk.view.tiles - 1, walk.per) - (int)blockIdx.x + 1, walk.index ? 1 : 0, walk.rows, walk.head, row0, walk.view.lo_pos, 0};
@@ -876,7 +890,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 }
                 __syncwarp();
             }
-            if (lane == 0) kv_cuts(P.work)[blockIdx.x] = cut;
+            if (!REDO && lane == 0) kv_cuts(P.work)[blockIdx.x] = cut;
         } else if (warp >= KT_HELP_WARP) {
             const int r = tid & 127;
             if constexpr (I8) {
@@ -917,7 +931,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 for (uint32_t n = 0;; n++) {
                     const KtPiece& walk = piece_at(n);
                     if (!is_one(walk)) break;
-                    if (tid == KT_HELP_WARP * 32) odd[(walk.index + 4) & 7] = 0;  // (a piece to come)
+                    if (tid == KT_HELP_WARP * 32) odd[(n + 4) & 7] = 0;  // (a piece to come)
                     uint32_t pair = 0;
                     int t = walk.t0;
                     bool seen = false;  // some row of the block sees the position.  (The rest of a page may hold anything.)
@@ -951,15 +965,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         if (!seen) pair = 0;
                         if (kv && kt_bad_pair(pair)) {  // rare: 0 x NaN is NaN, and a row must not be reached by what it does not see; rows that see it are mended at the end
                             pair = 0;
-                            odd[walk.index & 7] = 1;
+                            odd[n & 7] = 1;
                             __threadfence_block();
                         }
                         if constexpr (WIDE) {
                             const uint32_t scale = __byte_perm(pair, 0, 0x1010), zero = __byte_perm(pair, 0, 0x3232);
                             turn([&](uint32_t w) { return kt_values<true>(w, scale, zero); });
                         } else {
+                            if (kt_apart(pair)) {
+                                atomicOr(&not_held, 1 << min(walk.index, 31));
+                                pair = 0;
+                            }
                             const float s = kv_pair_scale(pair), z = kv_pair_zero(pair);
-                            if (!kt_held(s, z) && !(kv_pair_not_finite(pair))) not_held = 1;
                             const uint32_t scale = pack16<false>(s, s), zero = pack16<false>(z, z);
                             turn([&](uint32_t w) { return kt_values<false>(w, scale, zero); });
                         }
@@ -985,7 +1002,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     if (!is_one(walk)) break;
                     const KvView<KT_TILE> see[2] = {walk.part(0), walk.part(1)};
                     const int t0 = walk.t0, t1 = walk.t1;
-                    if (tid == KT_HELP_WARP * 32) odd[(walk.index + 4) & 7] = 0;  // (a piece to come)
+                    if (tid == KT_HELP_WARP * 32) odd[(n + 4) & 7] = 0;  // (a piece to come)
 #pragma unroll 1
                     for (int t = t0; t < t1; t++) {
                         const int base = walk.base(t);
@@ -1007,7 +1024,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                                     *at = make_uint4(only_finite<QB>(w.x), only_finite<QB>(w.y), only_finite<QB>(w.z), only_finite<QB>(w.w));
                                 }
                             }
-                            if (found) { odd[walk.index & 7] = 1; __threadfence_block(); }
+                            if (found) { odd[n & 7] = 1; __threadfence_block(); }
                             fence_async();
                             __syncwarp();
                             if (lane == 0) kv_bar_arrive(&ready[slot]);
@@ -1082,7 +1099,7 @@ bool kt_needed(const KvStep& s, int group) { return (int64_t)s.max_rows * group 
 
 }  // namespace
 
-// behind the cuts and the pieces: a word a CTA, see kt_held
+// behind the cuts and the pieces: a word a CTA, see kv_tc_kernel
 static size_t kt_gate_offset(int grid, int head_size) { return kv_cut_bytes(grid) + (size_t)grid * 2 * KT_ROWS * (head_size + 2) * sizeof(float); }
 
 size_t kv_tc_work(const KvStep& s, const KvPool& p, int group, int head_size, int sms) {
