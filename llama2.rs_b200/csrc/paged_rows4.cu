@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(R4_THREADS, R4_CTAS) kv_rows4_kernel(const __g
                 for (int e = 0; e < 2; e++) {
                     r.by[nt][e] = __shfl_sync(0xffffffffu, by, 4 * (2 * c + e)) * (P.scale_log2 * 0x1p24f);
                     r.sum[nt][e] = __shfl_sync(0xffffffffu, sum, 4 * (2 * c + e)) * 0x1p-24f;
-                    r.pos[nt][e] = piece.lo_pos + (8 * nt + 2 * c + e) / P.group;
+                    r.pos[nt][e] = piece.lo_pos + min(8 * nt + 2 * c + e, piece.rows - 1) / P.group;  // (rows that there are not see no more than the last)
                     r.m[nt][e] = -INFINITY;
                     r.l[nt][e] = r.y[nt][e] = 0.0f;
                     r.h[nt][e] = 1.0f;
