@@ -226,14 +226,14 @@ struct R4Rows {
     int pos[NT][2];
     float m[NT][2], l[NT][2], y[NT][2], h[NT][2];
     float o[HD / 16][NT][4];
-    bool unset;                  // (of the warp) some row has no m yet
+    int state;                   // (of the warp) 0: no row has an m yet, 1: some have none, 2: all have one
 };
 struct R4Lane { uint32_t k, v; };  // a lane's places in a slot for the fragments of K and of V
 
 // slot: the step's in shared memory (K, V, pairs of K, of V); first: its first position.  Position 4 i + 2 mb + half is row 16 mb + 8 half + i of the products, so that a thread's four
 // positions, i = g8, lie side by side; 32 more for every two mb more.
-// Nothing looks for a score above m in front of the exponentials: f32 has room for 2^100 in the sums and f16 for 2^15 in p t h, and a step that passes either, or has rows without an m,
-// is done again with a larger m and a smaller h.
+// Nothing looks for a score above m in front of the exponentials: f32 has room for 2^100 in the sums and f16 for 2^15 in p t h, and a step with rows that pass either, or have no m yet,
+// is done again with a larger m and a smaller h for these rows.
 template <int HD, int NT>
 __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>& r, const R4Lane& at, const uint8_t* slot, int first, bool whole) {
     using S = R4Shape<HD, NT>;
@@ -323,11 +323,29 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
         top &= 0x7fff7fffu;
         return most >= 0x1p100f || (top & 0xffffu) >= R4_LIMIT || (top >> 16) >= R4_LIMIT;
     };
-    bool again = r.unset;
-    if (!again) again = __any_sync(0xffffffffu, whole ? probabilities(std::true_type()) : probabilities(std::false_type()));
-    if (again) {
-        // seldom: a row's m is raised, or its h lowered, and what was summed is scaled.  (A row's result does not depend on the others.)
+    // (A loop, so that the probabilities are in the code once: one token of one sequence 13.5 -> 13.0 us, a window of 13B heads 55.7 -> 54.8)
+    bool ready = false;  // m and h hold for this step
+#pragma unroll 1
+    for (bool first = r.state == 0;; first = false) {
+        if (!first) {
+            const bool over = whole ? probabilities(std::true_type()) : probabilities(std::false_type());
+            if (ready || !(__any_sync(0xffffffffu, over) || r.state != 2)) break;
+        }
+        // seldom: a row's m is raised, or its h lowered, and what was summed is scaled.  Only of rows that need it: a row's result does not depend on the others.
         bool none = false;
+        uint32_t needs = ~0u;  // a bit a row
+        if (r.state) {
+            needs = 0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    bool mine = r.m[nt][e] == -INFINITY || l[nt][e] >= 0x1p100f;
+#pragma unroll
+                    for (int mb = 0; mb < MB; mb++) mine |= (pb[mb][nt][0] >> (16 * e) & 0x7fffu) >= R4_LIMIT || (pb[mb][nt][1] >> (16 * e) & 0x7fffu) >= R4_LIMIT;
+                    if (__ballot_sync(0xffffffffu, mine) & 0x11111111u << (threadIdx.x & 3)) needs |= 1u << (2 * nt + e);
+                }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -337,13 +355,14 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 };
+                const bool row_needs = needs >> (2 * nt + e) & 1u;
                 float x = -INFINITY, w = 0.0f;
 #pragma unroll
                 for (int mb = 0; mb < MB; mb++)
 #pragma unroll
                     for (int half = 0; half < 2; half++) x = fmaxf(x, s[mb][nt][2 * half + e]);
                 x = over_lanes(x) * r.by[nt][e] - R4_BIAS;
-                const bool up = x > r.m[nt][e] + R4_RAISE;
+                const bool up = row_needs && x > r.m[nt][e] + R4_RAISE;
                 const float m1 = up ? x : r.m[nt][e];
                 const KvScale f(m1 == -INFINITY ? 0.0f : r.m[nt][e] - m1);
                 r.m[nt][e] = m1;
@@ -357,7 +376,7 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
                         if (whole || sees(nt, mb, 2 * half + e))
                             w = fmaxf(w, fabsf(kv_exp2(fmaf(s[mb][nt][2 * half + e], r.by[nt][e], m1 == -INFINITY ? 0.0f : -m1)) * kv_pair_scale(vw[2 * mb + half])));
                 w = over_lanes(w);
-                const float h1 = up || w * r.h[nt][e] >= 32768.0f * 0.99f ? r4_factor(w, r.h[nt][e]) : r.h[nt][e];
+                const float h1 = row_needs && (up || w * r.h[nt][e] >= 32768.0f * 0.99f) ? r4_factor(w, r.h[nt][e]) : r.h[nt][e];
                 // (in two steps: the power of two between the two h may be beyond f32)
                 const int k = (int)(__float_as_uint(h1) >> 23) - (int)(__float_as_uint(r.h[nt][e]) >> 23);
                 const float a = __uint_as_float((uint32_t)(127 + k / 2) << 23), b = __uint_as_float((uint32_t)(127 + k - k / 2) << 23);
@@ -368,9 +387,8 @@ __device__ __forceinline__ void r4_step(const KvAttendParams& P, R4Rows<HD, NT>&
                     r.o[mt][nt][e + 2] = f(r.o[mt][nt][e + 2]) * a * b;
                 }
             }
-        r.unset = __any_sync(0xffffffffu, none);
-        if (whole) probabilities(std::true_type());
-        else probabilities(std::false_type());
+        r.state = __any_sync(0xffffffffu, none) ? 1 : 2;
+        ready = true;
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
@@ -559,7 +577,7 @@ __global__ void __launch_bounds__(R4_THREADS, R4_CTAS) kv_rows4_kernel(const __g
         if (fresh) {  // a new piece: Q, in f16, of eight elements the words (0, 4), (2, 6), (1, 5), (3, 7), as the numbers of a word of K come out
             piece = pieces[warp][ended & 3];
             fresh = false;
-            r.unset = true;
+            r.state = 0;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const int row = 8 * nt + g8, tok = row / P.group;

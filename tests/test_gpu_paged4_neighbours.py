@@ -4,8 +4,10 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from paged4_reference import Case4  # noqa: E402
-from test_gpu_paged4 import BF16, F32, run_attend  # noqa: E402
+from paged4_reference import Case4, attend4  # noqa: E402
+from paged_reference import check  # noqa: E402
+from test_gpu_paged4 import BF16, F16, F32, run_attend  # noqa: E402
+from test_gpu_paged4_rows import only  # noqa: E402
 
 
 def stairs(tokens, group, kv_heads, value=None):
@@ -35,3 +37,23 @@ def test_the_rest_of_the_last_page_does_not_matter(l2, tokens, group, kv_heads, 
     _, clean = run_attend(l2, c, BF16, scale=1.0, q=q, out_type=F32)
     _, out = run_attend(l2, stairs(tokens, group, kv_heads, value), BF16, scale=1.0, q=q, out_type=F32)
     assert torch.equal(out, clean) and out.isfinite().all()
+
+
+# kv heads: four warps to a head, two, and one
+@pytest.mark.parametrize("kv_heads", [1, 2, 4])
+@pytest.mark.parametrize("group", [2, 7, 12])
+@pytest.mark.parametrize("io", [F16, BF16])
+def test_a_row_does_not_follow_its_neighbours_scores(l2, io, group, kv_heads):
+    """Few rows: one row's scores rise so far that what it has summed is scaled; the rows beside it rise less, and keep their bits whether it does or not."""
+    c = stairs(1, group, kv_heads)
+    q = torch.zeros((c.n, c.heads, 128), dtype=io, device="cuda")
+    q[:, :, 0] = 1
+    rising = q.clone()
+    rising[:, ::group, 0] = 16
+    outs = [run_attend(l2, c, io, scale=1.0, q=x, out_type=F32)[1] for x in (q, rising)]
+    keep = torch.arange(c.heads) % group != 0
+    assert torch.equal(outs[0][:, keep], outs[1][:, keep])
+    part = only(c, range(7))
+    for x, out in zip((q, rising), outs):
+        want, bound = attend4(part, x, 1.0)
+        check(out[:7], want[:7], bound[:7])
