@@ -306,7 +306,7 @@ extern "C" int l2_block_norm(const l2_block_norm_args* a, void* cuda_stream) {
     }
     auto go = [&](auto e, auto v, auto w) {
         constexpr bool W = decltype(w)::value;
-        const int64_t ctas = W ? (a->rows + 7) / 8 : a->rows, most = (int64_t)sms * (W ? 8 : std::max(1, 2048 / threads));
+        const int64_t ctas = W ? ((int64_t)a->rows + 7) / 8 : a->rows, most = (int64_t)sms * (W ? 8 : std::max(1, 2048 / threads));
         return kv_launch(block_norm_kernel<decltype(e)::value, decltype(v)::value, W>, dim3((unsigned)std::min(ctas, most)), W ? 256 : threads, 0, static_cast<cudaStream_t>(cuda_stream), P);
     };
     auto by_e = [&](auto v, auto w) {
