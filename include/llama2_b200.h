@@ -347,7 +347,8 @@ int l2_kv_release(const l2_kv_tables* tables, const int32_t* keep, int window, i
  *   r = residual + scale * gate * t     (residual NULL: 0; gate NULL: 1; block NULL: r = residual)
  *   residual_out = r,  out = norm(r) * pre_weight     (pre_weight NULL: 1)
  * in f32, each result rounded once to its array's type; out goes by r before it is rounded.  residual_out may be residual itself and out may be block itself (same data, strides
- * and type); results otherwise overlap nothing.  A row stride of 0 in block, residual or gate: one row for all.  One of residual_out and out may be absent. */
+ * and type); results otherwise overlap nothing: an array ends in front of another, or its rows lie between the other's, both with the same stride in bytes (or one
+ * with a single row).  A row stride of 0 in block, residual or gate: one row for all.  One of residual_out and out may be absent. */
 typedef struct l2_rows {
     void* data;          /* element e of row i at i * row_stride + e; NULL: absent */
     int64_t row_stride;  /* in elements */

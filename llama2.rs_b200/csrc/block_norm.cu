@@ -236,12 +236,7 @@ int check_rows(const char* who, const char* what, const l2_rows& a, const l2_blo
     if (reinterpret_cast<uintptr_t>(a.data) % (4 * size) || (args->rows > 1 && a.row_stride % 4)) *quads = false;
     return L2_OK;
 }
-struct BnRange { uintptr_t lo, hi; };
-BnRange range(const BnRows& a, int rows, int dim) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(a.data);
-    return {lo, a.data ? lo + ((uintptr_t)(rows - 1) * a.stride + dim) * bn_bytes(a.type) : lo};
-}
-bool apart(BnRange a, BnRange b) { return a.lo >= b.hi || b.lo >= a.hi; }
+RowSpan span(const BnRows& a, int rows, int dim) { return {reinterpret_cast<uintptr_t>(a.data), a.stride * bn_bytes(a.type), a.data ? rows : 0, (int64_t)dim * bn_bytes(a.type)}; }
 bool same(const BnRows& a, const BnRows& b, int rows) { return a.data && a.data == b.data && a.type == b.type && (rows < 2 || a.stride == b.stride); }
 
 }  // namespace
@@ -275,13 +270,13 @@ extern "C" int l2_block_norm(const l2_block_norm_args* a, void* cuda_stream) {
     }
     if (a->rows) {
         // (in place: every element is written by the thread that has read it, or, of out, after its row has been read)
-        const BnRange w[2] = {range(P.residual_out, a->rows, a->dim), range(P.out, a->rows, a->dim)};
+        const RowSpan w[2] = {span(P.residual_out, a->rows, a->dim), span(P.out, a->rows, a->dim)};
         const BnRows* read[3] = {&P.block, &P.residual, &P.gate};
-        bool fine = apart(w[0], w[1]);
+        bool fine = rows_apart(w[0], w[1]);
         for (int i = 0; i < 2; i++) {
             for (int k = 0; k < 3; k++)
-                fine &= apart(w[i], range(*read[k], a->rows, a->dim)) || (i == 0 && k == 1 && same(P.residual_out, P.residual, a->rows)) || (i == 1 && k == 0 && same(P.out, P.block, a->rows));
-            for (const float* v : weights) fine &= !v || apart(w[i], {reinterpret_cast<uintptr_t>(v), reinterpret_cast<uintptr_t>(v + a->dim)});
+                fine &= rows_apart(w[i], span(*read[k], a->rows, a->dim)) || (i == 0 && k == 1 && same(P.residual_out, P.residual, a->rows)) || (i == 1 && k == 0 && same(P.out, P.block, a->rows));
+            for (const float* v : weights) fine &= !v || rows_apart(w[i], {reinterpret_cast<uintptr_t>(v), 0, 1, 4 * (int64_t)a->dim});
         }
         if (!fine) return fail(L2_EINVAL, "%s: results overlap one another or what is read", who);
     }

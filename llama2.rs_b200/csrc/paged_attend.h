@@ -14,6 +14,22 @@ namespace l2 {
 // SM count of the current device; L2_ECUDA where there is none that this library runs on (paged.cu).
 int kv_device(int* sms);
 
+// Rows of `width` bytes, `stride` bytes from one to the next (0: one row for all).
+struct RowSpan { uintptr_t at; int64_t stride, rows, width; };
+// Whether two arrays have no byte in common: one ends in front of the other, or the rows of one lie between those of the other all the way.  (With strides that differ
+// only the first is looked at.)
+inline bool rows_apart(RowSpan a, RowSpan b) {
+    if (a.rows < 1 || b.rows < 1) return true;
+    for (RowSpan* x : {&a, &b})
+        if (x->rows == 1 || x->stride == 0) { x->rows = 1; x->stride = 0; }
+    auto end = [](const RowSpan& x) { return (__int128)x.at + (__int128)(x.rows - 1) * x.stride + x.width; };
+    if (end(a) <= (__int128)b.at || end(b) <= (__int128)a.at) return true;
+    const int64_t s = a.stride ? a.stride : b.stride;
+    if (!s || (a.stride && b.stride && a.stride != b.stride)) return false;
+    const int64_t d = (int64_t)((((__int128)b.at - (__int128)a.at) % s + s) % s);  // from a row of a to the next of b
+    return d >= a.width && (__int128)d + b.width <= s;
+}
+
 // Sets a kernel's opt-in shared memory once per device (a static of the launch).
 struct KvOnce {
     std::atomic<uint64_t> done{0};
