@@ -306,7 +306,7 @@ int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_r
  * cache's type or either with an int8 cache; out: q's type or f32.  Products of q and k are exact and all sums are f32; the probabilities
  * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16), whatever out's type.  Sums are of probabilities
  * times up to 2^32, divided at the end: values of V up to 2^64 cannot overflow them, however many positions there are.
- * Pages that no row of the call sees are not read: with a window they can be given back. */
+ * Pages that no row of the call sees are not read: with a window they can be given back.  With a cache in 4 bits q and out have no byte in common. */
 int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* q, const l2_kv_rows* out, float scale, int window, int sinks,
                  void* workspace, size_t workspace_bytes, void* cuda_stream);
 /* Bytes of device scratch that l2_kv_attend needs for such a batch (contents need not be kept between calls; calls that may overlap

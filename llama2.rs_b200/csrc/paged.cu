@@ -410,6 +410,14 @@ int check_rows(const char* who, const char* what, const l2_kv_rows* r, const l2_
     return L2_OK;
 }
 
+// Rows and heads as rows for rows_apart: the wider of the two strides is that of rows, the other belongs to their width.
+RowSpan span(const KvRows& r, int n_rows, int head_size) {
+    const int64_t size = elem_bits(r.type) / 8;
+    int64_t rows = n_rows, row = rows > 1 ? r.row_stride : 0, heads = r.heads, head = heads > 1 ? r.head_stride : 0;
+    if (row && row < head) { std::swap(row, head); std::swap(rows, heads); }
+    return {reinterpret_cast<uintptr_t>(r.data), row * size, rows, ((heads - 1) * head + head_size) * size};
+}
+
 // What attention asks of the heads and sizes, before anything divides by them: query heads per kv head, and tiles that are counted in 31 bits.
 int check_heads(const char* who, const l2_kv_pages* p, const l2_kv_batch* b, int n_heads) {
     if (n_heads < 1 || n_heads % p->n_kv_heads || n_heads / p->n_kv_heads > 64)
@@ -529,6 +537,9 @@ extern "C" int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, 
     if (q->type == L2_F32 || (pages->type != L2_I8 && pages->type != L2_U4 && q->type != pages->type))
         return fail(L2_EINVAL, "%s: q must be of the cache's type (f16 or bf16 with an int8 or u4 cache)", who);
     if (out->type != L2_F32 && out->type != q->type) return fail(L2_EINVAL, "%s: out must be of q's type or f32", who);
+    // (of 4 bits some rows may be taken again behind the first results: see paged_tc.cu)
+    if (pages->type == L2_U4 && batch->n_rows && !rows_apart(span(P.out, batch->n_rows, pages->head_size), span(P.q, batch->n_rows, pages->head_size)))
+        return fail(L2_EINVAL, "%s: out overlaps q, which a u4 cache does not allow", who);
     if (window < 0 || sinks < 0 || !(scale > 0.0f) || !(scale < 1e30f)) return fail(L2_EINVAL, "%s: window %d, sinks %d, scale %g", who, window, sinks, scale);
     int sms;
     if (int rc = kv_device(&sms)) return rc;
