@@ -129,7 +129,8 @@ class PlannedLayer(PagedLayer):
 
 
 def serve_planned(layer, prompts, tokens, budget):
-    """As serve, by a PlannedLayer."""
+    """As serve, by a PlannedLayer.  The status word is looked at where sequences end, before their outputs count for anything: a RuntimeError says what it
+    holds (pages that ran out, ..), and the pages of all sequences have gone back."""
     torch = layer.torch
     seqs = [{"todo": p, "out": [], "left": tokens} for p in prompts]
     steps = total = 0
@@ -153,7 +154,10 @@ def serve_planned(layer, prompts, tokens, budget):
             if not len(seqs[b]["todo"]) and seqs[b]["left"] <= 0:
                 ended.append(b)
         if ended:
-            layer.end(ended)
+            status = int(layer.status)
+            layer.end(range(len(seqs)) if status else ended)
+            if status:
+                raise RuntimeError("a step went wrong: status %d" % status)
         steps, total = steps + 1, total + sum(rows)
     return [torch.cat(s["out"]) for s in seqs], steps, total
 
