@@ -75,7 +75,7 @@ class PagedLayer:
         kv_len = torch.tensor([s["length"] for s in sequences], dtype=torch.int32).cuda()
         start = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32).cuda()
         batch = self.l2.KvBatch(table, kv_len, start, n, max(rows), status=self.status)
-        out = self._attention(batch, x)
+        out = self._attention(batch, x, torch.empty)
         if self.window:  # pages that no later row sees
             for s in sequences:
                 for i in range(-(-self.sinks // self.page_size), max(0, s["length"] - self.window + 1) // self.page_size):
@@ -84,12 +84,13 @@ class PagedLayer:
                         s["table"][i] = -1
         return self._project("o", out)
 
-    def _attention(self, batch, x):
-        n, torch = x.shape[0], self.torch
+    def _attention(self, batch, x, room):
+        """room: torch.empty where every row is a sequence's, else torch.zeros."""
+        n = x.shape[0]
         q, k, v = (self._project(name, x) for name in "qkv")
-        q16 = torch.zeros((n, self.heads, 128), dtype=self.q_type, device="cuda")
+        q16 = room((n, self.heads, 128), dtype=self.q_type, device="cuda")
         self.pages.append(batch, k.view(n, -1, 128), v.view(n, -1, 128), rope=self.rope, rotation=self.rotation, q=q.view(n, -1, 128), q_out=q16)
-        out = self.pages.attend(batch, q16, torch.zeros((n, self.heads, 128), device="cuda"), window=self.window, sinks=self.sinks)
+        out = self.pages.attend(batch, q16, room((n, self.heads, 128), device="cuda"), window=self.window, sinks=self.sinks)
         return out.view(n, -1)
 
     def normed(self, y):
@@ -115,7 +116,7 @@ class PlannedLayer(PagedLayer):
         if n > self.budget:
             raise ValueError("%d rows, of %d" % (n, self.budget))
         self.tables.plan(torch.tensor(rows, dtype=torch.int32).cuda(), self.row_start, n, max(rows))
-        out = self._attention(self.l2.KvBatch(self.table, self.lengths, self.row_start, n, max(rows), status=self.status), x)
+        out = self._attention(self.l2.KvBatch(self.table, self.lengths, self.row_start, n, max(rows), status=self.status), x, torch.zeros)  # (a step without room leaves all rows out)
         if self.window:
             self.tables.release(window=self.window, sinks=self.sinks)
         return self._project("o", out)

@@ -17,3 +17,17 @@ def test_pages_that_run_out_are_an_error(l2):
     outs, _, _ = serving.serve_planned(layer, x[:2], 3, 90)
     _, other = planned("bf16")
     assert all(torch.equal(a, b) for a, b in zip(outs, serving.serve_planned(other, x[:2], 3, 90)[0]))
+
+
+def test_a_step_with_tables_of_the_host_fills_no_buffer(l2, monkeypatch):
+    import paged_serving
+    layer = paged_serving.PagedLayer(256, 4, 2, cache="f16", n_pages=8, page_size=16, positions=64)
+    x, = prompts(40)
+    sequence = {"length": 0, "table": []}
+
+    def zeros(*args, **kw):
+        raise AssertionError("every row is written anyway")
+
+    monkeypatch.setattr(torch, "zeros", zeros)
+    out = layer.step(x, [sequence], [40])
+    assert out.isfinite().all() and int(layer.status) == 0
