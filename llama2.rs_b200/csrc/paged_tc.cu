@@ -340,7 +340,7 @@ template <int CT, bool QB, int HD, bool WIDE>
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_constant__ KvAttendParams P, const int lim, const __grid_constant__ CUtensorMap map_k,
                                                               const __grid_constant__ CUtensorMap map_v, int* const gate) {
     using S = KtShape<CT, HD>;
-    constexpr bool I8 = S::I8, U4 = S::U4, WIDEN = S::WIDEN, REDO = U4 && WIDE, SCALED = I8 || REDO;  // SCALED: the softmax looks at the scales of a tile
+    constexpr bool I8 = S::I8, U4 = S::U4, WIDEN = S::WIDEN, REDO = U4 && WIDE, SCALED = I8 || REDO;  // SCALED: the softmax looks at the scales of a tile, or (REDO) at what the helpers say of them
     constexpr bool KB = U4 ? WIDE : QB, PB = U4 ? WIDE : I8 || QB;  // K and Q, V and the probabilities go through the products in bf16
     constexpr int LANES = HD / 8;
     constexpr uint32_t S_COL = 0, O_COL = 256;                   // tensor memory: S0 S1 O0 O1, 128 columns each; P over S
@@ -348,13 +348,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     constexpr float BIAS = PB ? 24.0f : 7.0f;
     extern __shared__ __align__(1024) uint8_t kt_smem[];
     __shared__ __align__(8) uint64_t full[S::SLOTS], empty[S::SLOTS], ready[S::SLOTS], raw_full[WIDEN ? S::RAWS : 1], raw_empty[WIDEN ? S::RAWS : 1],
-        sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
+        sc_full[KT_SCALE_SLOTS], sc_empty[KT_SCALE_SLOTS], apart_full[KT_SCALE_SLOTS], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
     __shared__ int64_t scratch[KT_THREADS / 32 + 2];
     __shared__ __align__(8) uint64_t piece_full[KT_PIECES], piece_empty[KT_PIECES], row_meet[2];
     __shared__ KtPiece pieces[KT_PIECES];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
     __shared__ int not_held;                  // 4 bits: what goes to `gate`
+    __shared__ uint4 apart[KT_SCALE_SLOTS];   // REDO: a bit for each position of a tile, K or V there has a pair that f16 does not hold
     __shared__ float q_by[U4 ? KT_ROWS : 1];  // 4 bits: of a row of Q, the inverse of its power of two; REDO: whether the row's result is kept
     __shared__ volatile int odd[8];  // by piece (of those done): values that are not finite have been taken out of a V tile
     uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem) + 1023) & ~(uintptr_t)1023);  // Q0, Q1
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
     // (Code that runs once comes from far away, 100 clocks and more for eight instructions: every warp prepares a little.)
     if (warp == 4 && lane < S::SLOTS) { kv_bar_init(&full[lane], WIDEN ? 4 : 1); kv_bar_init(&empty[lane], WIDEN ? 2 : 6); kv_bar_init(&ready[lane], 4); }
     if (WIDEN && warp == 5 && lane < S::RAWS) { kv_bar_init(&raw_full[lane], 1); kv_bar_init(&raw_empty[lane], 4); }
-    if (WIDEN && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], I8 ? 8 : REDO ? 12 : 4); }  // (read by the softmax; by the helpers; by both)
+    if (WIDEN && warp == 6 && lane < KT_SCALE_SLOTS) { kv_bar_init(&sc_full[lane], 32); kv_bar_init(&sc_empty[lane], I8 ? 8 : REDO ? 12 : 4); kv_bar_init(&apart_full[lane], 4); }  // (read by the softmax; by the helpers; by both)
     if (warp == 7 && lane < KT_PIECES) { kv_bar_init(&piece_full[lane], 1); kv_bar_init(&piece_empty[lane], 15); }
     if (warp == 8 && lane < 2) { kv_bar_init(&q_full[lane], 128); kv_bar_init(&drained[lane], 1); kv_bar_init(&row_meet[lane], 4); }
     if (warp == 9 && lane < 4) { kv_bar_init(&s_full[0][0] + lane, 1); kv_bar_init(&p_full[0][0] + lane, 4); kv_bar_init(&pv_done[0][0] + lane, 1); }
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                 }
                 if (!(on & 1u)) {
                     if constexpr (SCALED) {
-                        wait(&sc_full[sc], sc_ph);
+                        wait(REDO ? &apart_full[sc] : &sc_full[sc], sc_ph);
                         __syncwarp();
                         if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
                         if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
@@ -485,7 +486,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     continue;
                 }
                 const bool whole = all & 1u;
-                if constexpr (SCALED) wait(&sc_full[sc], sc_ph);
+                auto visible_of = [&](int h) {  // a bit for each of the 64 positions: j <= hi and (j > lo or j < sinks)
+                    const int base = walk.base(t) + KT_SUB * h;
+                    auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+                    return below(pos - base + 1) & (P.window ? ~below(pos - P.window - base + 1) | below(P.sinks - base) : ~0ull);
+                };
+                if constexpr (I8) wait(&sc_full[sc], sc_ph);
 #pragma unroll 1
                 for (int h = 0; h < 2; h++, seen++) {
                     const float* ks = scales + sc * 2 * KT_TILE + KT_SUB * h;
@@ -506,17 +512,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                             x[j] = __float_as_uint(a.x); x[j + 1] = __float_as_uint(a.y); x[j + 2] = __float_as_uint(b.x); x[j + 3] = __float_as_uint(b.y);
                         }
                     }
-                    auto visible = [&]() {  // a bit for each of the 64 positions: j <= hi and (j > lo or j < sinks)
-                        const int base = walk.base(t) + KT_SUB * h;
-                        auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
-                        return below(pos - base + 1) & (P.window ? ~below(pos - P.window - base + 1) | below(P.sinks - base) : ~0ull);
-                    };
-                    if constexpr (REDO) {
-                        auto apart = [&](int j) { return kt_apart(__float_as_uint(ks[j])) || kt_apart(__float_as_uint(ks[KT_TILE + j])); };
-                        __syncwarp();
-                        const uint32_t lo = __ballot_sync(0xffffffffu, apart(lane)), hi = __ballot_sync(0xffffffffu, apart(lane + 32));
-                        redo |= (visible() & ((unsigned long long)hi << 32 | lo)) != 0;
-                    }
+                    auto visible = [&]() { return visible_of(h); };
                     if (!whole) {
                         const unsigned long long bits = visible();
 #pragma unroll
@@ -582,6 +578,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                     if (lane == 0) kv_bar_arrive(&p_full[i][h]);
                 }
                 s_ph ^= 1u;
+                if constexpr (REDO) {
+                    wait(&apart_full[sc], sc_ph);
+                    const uint4 w = apart[sc];
+                    __syncwarp();
+                    if (!redo && (w.x | w.y | w.z | w.w)) redo = (visible_of(0) & ((unsigned long long)w.y << 32 | w.x)) || (visible_of(1) & ((unsigned long long)w.w << 32 | w.z));
+                }
                 if constexpr (SCALED) {
                     if (lane == 0) kv_bar_arrive(&sc_empty[sc]);
                     if (++sc == KT_SCALE_SLOTS) { sc = 0; sc_ph ^= 1u; }
@@ -940,6 +942,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tc_kernel(const __grid_const
                         if (!kv) {
                             wait(&sc_full[sc], sc_ph);
                             seen = walk.view(walk.lo_pos, walk.hi_pos).any(walk.base(t++) + r, 1, P.window, P.sinks);
+                            if constexpr (REDO) {
+                                const uint32_t* const of = reinterpret_cast<const uint32_t*>(scales) + 2 * sc * KT_TILE + r;
+                                const uint32_t bits = __ballot_sync(0xffffffffu, kt_apart(of[0]) || kt_apart(of[KT_TILE]));
+                                if (lane == 0) {
+                                    reinterpret_cast<uint32_t*>(&apart[sc])[warp - KT_HELP_WARP] = bits;
+                                    kv_bar_arrive(&apart_full[sc]);
+                                }
+                            }
                         }
                         wait(&raw_full[rs], rph);
                         wait(&empty[slot], ph);
