@@ -292,7 +292,8 @@ typedef struct l2_kv_rows {
  * nearest even.  One that holds a NaN or an infinity gets a scale of NaN (it reads back as NaN); below 2^-100 it is stored as zeros.
  * 4 bits: of a row and head, zero = the bf16 number at or below its least element, span = its largest less zero, scale = the least bf16 number s with
  * 15 s >= span, u = (x - zero) * (1 / scale), differences and reciprocal rounded to 32 bits, their product rounded once, to a whole number (nearest
- * even).  A span below 2^-100: scale and u 0.  A NaN, an infinity or a span beyond f32: scale and zero NaN. */
+ * even).  A span below 2^-100: scale and u 0.  A NaN, an infinity or a span beyond f32: scale and zero NaN.  (zero + 15 scale may lie
+ * above the largest element by up to 2^-7 of the span; beyond f32 it reads as an infinity.) */
 int l2_kv_append_rope(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* k, const l2_kv_rows* v, const l2_kv_rows* q,
                       const l2_kv_rows* q_out, const float* rope_cos, const float* rope_sin, int rope_len, int rotation, void* cuda_stream);
 /* The same with L2_ROPE_PAIRS. */
@@ -303,9 +304,15 @@ int l2_kv_read(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_r
 /* Attention of the batch's rows over the cache (their own K and V appended before).  A row at position p sees position j when j <= p and,
  * where window > 0, p - j < window or j < sinks.  out = softmax(scale * q k) v over what it sees; 0 where it sees nothing.  What a row does not see
  * does not reach its result, NaN and infinities included.  heads of q a multiple of n_kv_heads (at most 64 times).  q: f16 or bf16, the
- * cache's type or either with an int8 cache; out: q's type or f32.  Products of q and k are exact and all sums are f32; the probabilities
- * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16), whatever out's type.  Sums are of probabilities
+ * cache's type or either with a cache in int8 or 4 bits; out: q's type or f32.  Products of q and k are exact (4 bits: see below) and all sums are f32; the probabilities
+ * are rounded to q's type (with an int8 cache to bf16: times the scale they can leave the range of f16; 4 bits: see below), whatever out's type.  Sums are of probabilities
  * times up to 2^32, divided at the end: values of V up to 2^64 cannot overflow them, however many positions there are.
+ * 4 bits.  Sequences with few rows (max_rows times the query heads of a kv head up to 16; single tokens beside longer sequences): the numbers u go through the products as they are.  An
+ * element of q is resolved to 2^-36 of its row's largest, a probability times its scale of V to 2^-11 of itself, or 2^-31 of the largest such product.  The others: zero + u * scale, q
+ * and the probabilities are rounded to f16 (2^-11 each; steps of 2^-24 below 2^-14, for q of its row's largest divided by 2^15 where it is bf16).  A row that sees a pair
+ * which f16 does not hold (|zero| + 15 |scale| > 65504; |scale| below 2^-16, unless it is 0 and zero is 0 or at least 2^-14) takes all of these as bf16 (2^-8 each) for the positions that the same
+ * CTA has of its sequence, which are then gone through twice; other rows do not change.  A pair of V with a NaN or an infinity, or (not few rows) with zero + 15 scale beyond
+ * bf16, is NaN to the rows that see it.  A row of q with an element of 2^118 or more gives NaN.
  * Pages that no row of the call sees are not read: with a window they can be given back.  With a cache in 4 bits q and out have no byte in common. */
 int l2_kv_attend(const l2_kv_pages* pages, const l2_kv_batch* batch, const l2_kv_rows* q, const l2_kv_rows* out, float scale, int window, int sinks,
                  void* workspace, size_t workspace_bytes, void* cuda_stream);

@@ -247,7 +247,7 @@ class KvPages:
 
     def attend(self, batch, q, out, scale=None, window=0, sinks=0, workspace=None, stream=None):
         """Attention of the step's rows q [rows, heads, head_size] over the cache into out; scale defaults to head_size ** -0.5.
-        `workspace`: a uint8 tensor of workspace_bytes(); one is made where none is given."""
+        `workspace`: a uint8 tensor of workspace_bytes(); one is made where none is given.  With a cache in 4 bits out does not overlap q."""
         n = batch.n_rows
         if window >> 31 or sinks >> 31:
             _int32(window=window, sinks=sinks)
