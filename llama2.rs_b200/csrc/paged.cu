@@ -3,7 +3,7 @@
 //   16 bits:  cache = round(x)
 //   8 bits:   a = max |x| over a row and head, scale = a / 127, cache = rint(x * (127 / a)), and back: value = cache * scale
 //   4 bits:   zero = bf16 at or below min x, scale = least bf16 with 15 scale >= max x - zero, cache = rint((x - zero) / scale), value = zero + scale * cache.  Both are
-//             rounded outwards, so that cache stays in 0 .. 15 and no element lies more than half a step off; bf16 because it has f32's range in half the bytes (a pair beside
+//             rounded outwards, so that cache stays in 0 .. 15 and no element lies more than half a step off, but for the roundings of x - zero and 1 / scale (15 x 2^-23 of a step); bf16 because it has f32's range in half the bytes (a pair beside
 //             the 64 bytes of a head of 128)
 //   RoPE:     (a, b) = (x[d], x[d + hd/2]) turned by the angle of the row's position, first: a' = a c - b s, b' = b c + a s, or, as the
 //             token loop of this library does it in place, b' = b c + a' s

@@ -8,8 +8,8 @@
 // gives two elements of a factor, and a shift by 8 and the same masks the others: five instructions for eight elements (eleven, where numbers are made by adding to a
 // larger one and taking that off again, or one of 128 that stays in the sums).  Products and sums are f32 and hold 2^-48.  The two kinds of numbers (u and 16 u) have sums of their own in
 // the scores and rows of their own in O^T.
-// Q is in f16 as it is, or a row of bf16 times a power of two that brings its largest element to 2^15 or more: an element is resolved to 2^-39 of the
-// row's largest, which is below what the sum g keeps of it.
+// Q is in f16, a row times a power of two that brings its largest element to 2^15 or more, the elements of odd index as a sixteenth (their numbers are 16 u): half of f16's
+// smallest step, 2^-25, is 2^-40 of the row's largest for an even element, 2^-36 for an odd one.
 // p t h is rounded to f16, with h a power of two a row: it follows the largest p t seen, so that the scales may have any size (2^-60 to 2^90) beside one another.
 //
 // Work.  A warp has one kv head of a piece of a sequence, in steps of 32 positions.  Four, two or one heads side by side (as many as divide their number) are a CTA's, so that the 64
@@ -18,7 +18,7 @@
 // (m, l, O), which kv_rows4_combine_kernel adds in order.
 //
 // Copies.  Every warp of products has a warp of copies that brings its positions, 16 bytes a lane, up to three or four steps ahead, across the ends of pieces; the two meet through
-// mbarriers only.  64 sequences of 8 kv heads and 64 query heads, up to 8192 positions (292 MB): 79 us.  By the warps of products themselves 84 (a copy waits where memory is busy, and all
+// mbarriers only.  64 sequences of 8 kv heads and 64 query heads, up to 8192 positions (292 MB): 80 us.  By the warps of products themselves 84 (a copy waits where memory is busy, and all
 // behind it); by TMA, one warp for four, 93, of which the copies alone took 84: it brings a row of 64 bytes every 4.5 clocks, where it could bring one of 128.  What bounds it now: a start of
 // some 13 us (place on the line, table, first positions, first step), then copies (alone 66 us with the start) and steps (alone 68 us) that hide each other in part.
 #include <cuda_runtime.h>
@@ -36,7 +36,7 @@ namespace {
 
 constexpr int R4_WARPS = 4, R4_THREADS = 2 * 32 * R4_WARPS;  // warps of products, and as many of copies
 constexpr int R4_CTAS = 2;   // of an SM
-constexpr int R4_SETUP = 3;  // what a piece costs besides its tiles, in tiles (79.1 us at the size above; 2: 80.6, 5: 80.2)
+constexpr int R4_SETUP = 3;  // what a piece costs besides its tiles, in tiles (at the size above 2: 1.5 us longer, 5: 1.1)
 constexpr int R4_RAISE = 8;  // powers of two that a score may exceed the running maximum by before that is raised
 constexpr float R4_BIAS = 24.0f;  // probabilities carry a factor of 2^24
 
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(R4_THREADS, R4_CTAS) kv_rows4_kernel(const __g
     __syncthreads();
     const KvWait wait{&failed};
 
-    // (registers: 128 x (72 + 184) of the 256 x 128 that the launch has; 56 + 200 leaves more of the copies' addresses in memory: 80.3 us instead of 79.1)
+    // (registers: 128 x (72 + 184) of the 256 x 128 that the launch has; 56 + 200 leaves more of the copies' addresses in memory: 1.2 us longer)
     if (tid >= 32 * R4_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ================= copies ==========================================================================================================

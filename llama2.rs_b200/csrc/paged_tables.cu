@@ -8,6 +8,7 @@
 // A few kilobytes and a chain of dependent loads: nothing but latency.  So one launch of one cluster, and work shared out by rows and by entries, not by sequences (long prompts
 // often stand side by side: with a warp for a sequence's pages, 24 of them among 500, 42,000 rows, took 79 us for a plan and a release; now 15, and 8.5 for 256 sequences with a row each).  Every CTA sums up all sequences by itself, in shared memory, which costs less than
 // asking the others; they meet once, before the first writes what another may still read.  Nothing goes through atomics, and the order of pages does not depend on who was first.
+// A release with a window looks at every entry between the sinks and the window, those given back before too: 8 sequences of 5,000 positions in pages of 16 take 4.8 us, of 60,000 123.
 #include <cuda_runtime.h>
 
 #include <algorithm>
